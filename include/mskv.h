@@ -43,6 +43,9 @@ extern "C" {
 #define MSKV_EUNSUPPORTED (-2) /* valid shape the kernels do not implement     */
 #define MSKV_EWORKSPACE (-3)   /* workspace missing or smaller than required   */
 
+/* most tensors of one call that moves pages */
+#define MSKV_MAX_POOLS 8
+
 /* Library version (major * 10000 + minor * 100 + patch). */
 int mskv_version(void);
 
@@ -389,6 +392,133 @@ int mskv_qk_norm_rope_store(const void* q, const void* k, const void* v,
                             int slot_dtype, int64_t num_tokens, int num_q_heads,
                             int num_kv_heads, int head_dim, int64_t num_slots,
                             int act_dtype, void* stream);
+
+/*
+ * The 4-bit paged cache.  A value is an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * and a sign in bit 3), two to a byte, the even dimension in the low half.
+ *   k_cache        uint8 [num_blocks, num_kv_heads, block_size / 16, 4, 16, 16]:
+ *                  16 tokens; 32-dimension block; token of the 16; its codes
+ *   k_scale_cache  uint8 [num_blocks, num_kv_heads, block_size / 64, 4, 16, 4]:
+ *                  64 tokens; 32-dimension block; token t % 16; t / 16 % 4.
+ *                  The byte e + 127 of the block's scale 2^e; 255: NaN
+ *   v_cache        uint8 [num_blocks, num_kv_heads, block_size, 64]
+ *   v_scale_cache  float32 [num_blocks, num_kv_heads, block_size]
+ * head_dim == 128 and block_size a multiple of 128 (and below 2^25 tokens),
+ * else MSKV_EUNSUPPORTED.  k_cache and v_cache start on 16 bytes,
+ * k_scale_cache and v_scale_cache on four.
+ */
+
+/*
+ * Quantize K/V rows into the 4-bit cache through slot_mapping (slot s is
+ * token s % block_size of block s / block_size).
+ * K, per 32 dimensions: e = floor(log2 amax) - 2, one more where amax >=
+ * 1.75 * 2^floor(log2 amax), at least -126.  V, per row: scale =
+ * max(amax, 1e-8) / 6 in fp32.  code = e2m1(x / scale), nearest, ties to the
+ * even code, the sign kept on zero; for V x / scale is (0.75 x) / (0.125
+ * max(amax, 1e-8)) in fp32, which decides 16-bit rows as exact arithmetic on
+ * 6 x / amax does.  A block of K or a row of V that holds an infinity or a
+ * NaN gets the scale NaN.
+ * key/value: [num_tokens, num_kv_heads, 128] in act_dtype (MSKV_FLOAT16,
+ * MSKV_BFLOAT16 or MSKV_FLOAT32), key_stride / value_stride elements from
+ * token to token as in mskv_store_fp8_kvcache_strided, on 16 bytes.  Slots
+ * outside the cache are skipped; a slot is named at most once.
+ */
+int mskv_store_fp4_kvcache(const void* key, int64_t key_stride,
+                           const void* value, int64_t value_stride,
+                           void* k_cache, void* v_cache, void* k_scale_cache,
+                           float* v_scale_cache, const void* slot_mapping,
+                           int slot_dtype, int64_t num_tokens,
+                           int num_kv_heads, int head_dim, int block_size,
+                           int64_t num_blocks, int act_dtype, void* stream);
+
+/*
+ * Read tokens of the 4-bit cache back: key and value, [num_tokens,
+ * num_kv_heads, 128] in act_dtype, get the values that the slots' codes stand
+ * for, code * scale in fp32 rounded to act_dtype; zeros for slots outside the
+ * cache.
+ */
+int mskv_load_fp4_kvcache(const void* k_cache, const void* v_cache,
+                          const void* k_scale_cache, const float* v_scale_cache,
+                          const void* slot_mapping, int slot_dtype, void* key,
+                          void* value, int64_t num_tokens, int num_kv_heads,
+                          int head_dim, int block_size, int64_t num_blocks,
+                          int act_dtype, void* stream);
+
+/*
+ * mskv_fp8_decode_attention over the 4-bit cache: the same arguments, scores
+ * q . (code * 2^e) * softmax_scale, values code * v_scale.  num_splits must
+ * be what mskv_fp4_decode_num_splits returns for the shape; the workspace
+ * holds mskv_decode_workspace_bytes of it.
+ */
+int mskv_fp4_decode_num_splits(int batch, int num_q_heads, int num_kv_heads,
+                               int max_blocks_per_seq, int block_size);
+int mskv_fp4_decode_attention(const void* query, const void* k_cache,
+                              const void* v_cache, const void* k_scale_cache,
+                              const float* v_scale_cache,
+                              const int32_t* cache_seqlens,
+                              const int32_t* block_tables, void* out,
+                              int batch, int num_q_heads, int num_kv_heads,
+                              int head_dim, int block_size, int64_t num_blocks,
+                              int max_blocks_per_seq, float softmax_scale,
+                              int act_dtype, int num_splits, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/*
+ * mskv_fp8_prefill_attention_bounded over the 4-bit cache: the same
+ * arguments, refusals and workspace
+ * (mskv_fp8_prefill_bounded_workspace_bytes).
+ */
+int mskv_fp4_prefill_attention(
+    const void* query, const void* k_cache, const void* v_cache,
+    const void* k_scale_cache, const float* v_scale_cache,
+    const int32_t* block_tables, const int32_t* cu_seqlens_q,
+    const int32_t* cu_seqlens_k, int prefix_len, void* out, int num_seqs,
+    int64_t total_q, int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads,
+    int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
+    int max_blocks_per_seq, float softmax_scale, int act_dtype, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/*
+ * Copy pages of a paged pool to other pages: page dst_blocks[i] of every
+ * plane of every tensor becomes page src_blocks[i]'s bytes.
+ * A pool is num_pools (1 to MSKV_MAX_POOLS) device tensors whose pages are
+ * numbered alike: tensor t starts at bases[t] and has planes[t] stacks of
+ * num_blocks pages, plane_strides[t] bytes apart, of page_bytes[t] bytes each
+ * (the runner's [2, layers, num_blocks, ...] caches have 2 * layers planes).
+ * These four arrays and the pairs are HOST memory, read before the call
+ * returns.  Bytes, strides and bases are multiples of 16, else
+ * MSKV_EUNSUPPORTED.  Block ids lie in [0, num_blocks), no destination is
+ * named twice and none is also a source, else MSKV_EINVAL before any launch.
+ */
+int mskv_copy_kv_blocks(int num_pools, void* const* bases,
+                        const int64_t* planes, const int64_t* plane_strides,
+                        const int64_t* page_bytes, int64_t num_blocks,
+                        const int32_t* src_blocks, const int32_t* dst_blocks,
+                        int64_t num_pairs, void* stream);
+
+/*
+ * Compact a paged pool (described as in mskv_copy_kv_blocks): the n pages
+ * that block_tables names move to places 0 .. n - 1.  A named page below n
+ * stays; the i-th one from n up (ascending) takes the i-th free place below
+ * n.  Pages that no entry names are free, and their contents afterwards are
+ * unspecified.
+ * block_tables: int32 [num_entries]; entries outside [0, num_blocks) (-1
+ * padding, a garbage page behind the pool) are kept as they are, and
+ * several entries may name one page.  new_tables [num_entries]: the entries
+ * renamed (may be block_tables itself).  remap [num_blocks]: each page's new
+ * place, -1 for a free one.  num_live [1]: n.  All on the device; nothing is
+ * read on the host.  num_blocks here is the number of pages that may move,
+ * at most 2^18; plane_strides may leave room for more behind them.
+ * workspace: mskv_compact_workspace_bytes(num_blocks), on four bytes.
+ */
+size_t mskv_compact_workspace_bytes(int64_t num_blocks);
+int mskv_compact_kv_blocks(int num_pools, void* const* bases,
+                           const int64_t* planes, const int64_t* plane_strides,
+                           const int64_t* page_bytes, int64_t num_blocks,
+                           const int32_t* block_tables, int64_t num_entries,
+                           int32_t* new_tables, int32_t* remap,
+                           int32_t* num_live, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

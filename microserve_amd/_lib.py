@@ -113,6 +113,26 @@ _PROTOS = {
         _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _c_f32, _vp, _vp, _c_i64,
         _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_i64,
         _c_int, _vp]),
+    "mskv_store_fp4_kvcache": (_c_int, [
+        _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_int,
+        _c_i64, _c_int, _c_int, _c_int, _c_i64, _c_int, _vp]),
+    "mskv_load_fp4_kvcache": (_c_int, [
+        _vp, _vp, _vp, _vp, _vp, _c_int, _vp, _vp,
+        _c_i64, _c_int, _c_int, _c_int, _c_i64, _c_int, _vp]),
+    "mskv_fp4_decode_num_splits": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "mskv_fp4_decode_attention": (_c_int, [
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_int, _c_f32,
+        _c_int, _c_int, _vp, _c_size, _vp]),
+    "mskv_fp4_prefill_attention": (_c_int, [
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _vp,
+        _c_int, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64,
+        _c_int, _c_f32, _c_int, _vp, _c_size, _vp]),
+    "mskv_copy_kv_blocks": (_c_int, [
+        _c_int, _vp, _vp, _vp, _vp, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "mskv_compact_workspace_bytes": (_c_size, [_c_i64]),
+    "mskv_compact_kv_blocks": (_c_int, [
+        _c_int, _vp, _vp, _vp, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _c_size, _vp]),
 }
 
 EXPORTED = tuple(_PROTOS)
@@ -209,3 +229,10 @@ def on_device(what: str, ref, *tensors) -> None:
 def stream_of(t) -> int:
     import torch
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def current(t):
+    """``t``'s GPU as the current device: a launch goes to the device that is
+    current, and its stream must be that device's."""
+    import torch
+    return torch.cuda.device(t.device)

@@ -64,6 +64,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "mskv_device.h"
 #include "../../include/mskv.h"
@@ -163,17 +164,20 @@ __device__ __forceinline__ int wave_max_u31(int v) {  // of values >= 0
   return max((int)r32[0], (int)r32[1]);
 }
 
+// (kUnit: tokens of one step of the kernel that the rule is for)
+template <int kUnit>
 __device__ __forceinline__ int steps_of_length(int len, const SplitRule& r) {
-  return (max(0, min(len, r.max_tokens)) + kStep - 1) / kStep;
+  return (max(0, min(len, r.max_tokens)) + kUnit - 1) / kUnit;
 }
 // (Where longest / splits is not whole, it lies at least 1 / splits above the
 // whole number q below it; q * splits <= longest <= 2^17 with max_tokens <=
 // 2^22, so the float product's error, q * 2^-23, never rounds it down to q.)
+template <int kUnit>
 __device__ __forceinline__ int split_tokens_from(int steps, int longest, const SplitRule& r) {
   const int per = max((int)ceilf(fmaxf((float)steps * r.inv_slots, (float)longest * r.inv_splits)),
                       kMinSplitSteps);
-  const bool whole = longest * kStep <= r.fixed && longest - per < r.min_gain;
-  return min((whole ? max(longest, per) : per) * kStep, r.fixed);
+  const bool whole = longest * kUnit <= r.fixed && longest - per < r.min_gain;
+  return min((whole ? max(longest, per) : per) * kUnit, r.fixed);
 }
 
 // The tokens per split of this step, from the lengths on the device: a
@@ -207,13 +211,14 @@ __device__ __forceinline__ int lane_length(const int32_t* __restrict__ seqlens,
   const int lane = threadIdx.x & 63;
   return r.adapt && !r.info && r.batch > 1 && lane < r.batch ? seqlens[lane] : 0;
 }
+template <int kUnit>
 __device__ __forceinline__ int split_tokens_of(int own, int len,
                                                const int32_t* __restrict__ seqlens,
                                                const SplitRule& r) {
   if (r.info) return __builtin_amdgcn_readfirstlane(r.info[1]);
   if (!r.adapt) return r.fixed;
   int steps, longest;
-  auto steps_of = [&](int len) { return steps_of_length(len, r); };
+  auto steps_of = [&](int len) { return steps_of_length<kUnit>(len, r); };
   if (r.batch == 1) {
     steps = longest = steps_of(len);
   } else {
@@ -226,7 +231,7 @@ __device__ __forceinline__ int split_tokens_of(int own, int len,
     steps = __builtin_amdgcn_readfirstlane(wave_sum_i32(steps));
     longest = __builtin_amdgcn_readfirstlane(wave_max_u31(longest));
   }
-  return split_tokens_from(steps, longest, r);
+  return split_tokens_from<kUnit>(steps, longest, r);
 }
 
 struct StepLoads {
@@ -456,6 +461,30 @@ __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh
   }
 }
 
+// What the split kernel needs of a cache: the tokens of a step, a wave's LDS,
+// and the walk over a range of tokens.  This one is the FP8 cache.
+struct Fp8Cache {
+  static constexpr int kUnit = kStep;
+  static constexpr int kPageUnit = kStep;  // a page is a multiple of it
+  typedef uint8_t Tiles[2][2][kStep * kHeadDim];  // K and V, double-buffered
+  typedef float Scales[2][2 * kStep];
+  template <typename T>
+  static __device__ __forceinline__ void attend(const DecodeArgs& a, int b, int kvh, int qh,
+                                                bool head_ok, int t_begin, int t_end,
+                                                int blk_first, int lane, Tiles& tiles,
+                                                Scales& scales, f32x4 (&acc)[8], float& m,
+                                                float& l) {
+    attend_range<T>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane, tiles, scales, acc,
+                    m, l);
+  }
+};
+
+}  // namespace mskv
+
+#include "fp4_decode.h"
+
+namespace mskv {
+
 // out[b, qh, :] = acc / l in the activation type (zeros when l == 0)
 template <typename T>
 __device__ __forceinline__ void write_output(uint16_t* op, const f32x4 (&acc)[8], float l,
@@ -496,14 +525,12 @@ __device__ __forceinline__ void write_partial(float* po, float* plse, const f32x
 // against 124 us.)
 // kFollow: the splits follow the lengths; kFixed: they are the shape's.
 enum DecodeMode { kFixed, kFollow, kItems };
-template <typename T, int W, DecodeMode kMode>
-__global__ __launch_bounds__(64 * W)
-__attribute__((amdgpu_waves_per_eu(2, 8)))
-void decode_fp8_kernel(DecodeArgs a) {
-  // per wave: two K/V tile pairs and their scales; step i is read from
+template <typename T, int W, DecodeMode kMode, typename Cache>
+__device__ __forceinline__ void decode_split(const DecodeArgs& a) {
+  // per wave: two buffers of tiles and their scales; step i is read from
   // buffer i&1 while step i+1 is staged into the other one
-  __shared__ __attribute__((aligned(16))) uint8_t kv_lds_all[W][2][2][kStep * kHeadDim];
-  __shared__ __attribute__((aligned(16))) float s_lds_all[W][2][2 * kStep];
+  __shared__ __attribute__((aligned(16))) typename Cache::Tiles kv_lds_all[W];
+  __shared__ __attribute__((aligned(16))) typename Cache::Scales s_lds_all[W];
 
   const int wave = threadIdx.x >> 6;
   const int lane = threadIdx.x & 63;
@@ -540,7 +567,7 @@ void decode_fp8_kernel(DecodeArgs a) {
     blk_first = __builtin_amdgcn_readfirstlane(
         a.bt[(int64_t)b * a.w + min(split * a.pages_per_split, a.w - 1)]);
     if (unit >= a.hk * a.qgroups) return;
-    split_tokens = split_tokens_of(own, len_raw, a.seqlens, a.rule);
+    split_tokens = split_tokens_of<Cache::kUnit>(own, len_raw, a.seqlens, a.rule);
   } else {
     // (the split's first page is inside the table: split * pages_per_split <
     // w for every split count of these shapes)
@@ -576,8 +603,8 @@ void decode_fp8_kernel(DecodeArgs a) {
 
   f32x4 acc[8];
   float m, l;
-  attend_range<T>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane, kv_lds_all[wave],
-                  s_lds_all[wave], acc, m, l);
+  Cache::template attend<T>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane,
+                            kv_lds_all[wave], s_lds_all[wave], acc, m, l);
 
   // splits that hold tokens of this sequence; a sequence that fits in one
   // split is written here directly
@@ -590,6 +617,26 @@ void decode_fp8_kernel(DecodeArgs a) {
   // this split's partial, merged by a combine kernel
   const int64_t row = ((int64_t)b * a.hq + qh) * a.splits + split;
   write_partial(a.part_o + row * kHeadDim, a.part_lse + row, acc, m, l, g);
+}
+
+template <typename T, int W, DecodeMode kMode>
+__global__ __launch_bounds__(64 * W)
+__attribute__((amdgpu_waves_per_eu(2, 8)))
+void decode_fp8_kernel(DecodeArgs a) {
+  decode_split<T, W, kMode, Fp8Cache>(a);
+}
+template <typename T, int W, DecodeMode kMode>
+__global__ __launch_bounds__(64 * W)
+__attribute__((amdgpu_waves_per_eu(2, 8)))
+void decode_fp4_kernel(DecodeArgs a) {
+  decode_split<T, W, kMode, Fp4Cache>(a);
+}
+template <typename T, int W, DecodeMode kMode, typename Cache>
+static auto split_kernel() {
+  if constexpr (std::is_same<Cache, Fp4Cache>::value)
+    return decode_fp4_kernel<T, W, kMode>;
+  else
+    return decode_fp8_kernel<T, W, kMode>;
 }
 
 // A merge state over some splits of one row, held in plain registers: the
@@ -724,7 +771,7 @@ __device__ __forceinline__ void write_merged(uint16_t* op, float den, f32x4 o) {
 // kRule (all merges): the tokens per split may follow the lengths.
 constexpr int kLoopK = 16;
 
-template <typename T, bool kRule>
+template <typename T, bool kRule, int kUnit>
 __global__ __launch_bounds__(64) void decode_combine_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_lse,
     const int32_t* __restrict__ seqlens, uint16_t* __restrict__ out, int hq,
@@ -736,7 +783,7 @@ __global__ __launch_bounds__(64) void decode_combine_kernel(
   const int lane = threadIdx.x;
   const int j = lane >> 5, i = lane & 31;
   const int L = min(seqlens[b], rule.max_tokens);
-  const int split_tokens = kRule ? split_tokens_of(own, L, seqlens, rule) : rule.fixed;
+  const int split_tokens = kRule ? split_tokens_of<kUnit>(own, L, seqlens, rule) : rule.fixed;
   const int nvalid = L <= 0 ? 0 : min(splits, (L + split_tokens - 1) / split_tokens);
   if (nvalid == 1) return;
   const float* lse = part_lse + (int64_t)row * splits;
@@ -756,7 +803,7 @@ __global__ __launch_bounds__(64) void decode_combine_kernel(
 // batches), the reads of unused rows cost more than the round trip, so
 // those keep decode_combine_kernel.  M is the largest valid lse value and
 // the weighted sum runs in split order.
-template <typename T, int S, bool kRule>
+template <typename T, int S, bool kRule, int kUnit>
 __global__ __launch_bounds__(64) void decode_combine_small_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_lse,
     const int32_t* __restrict__ seqlens, uint16_t* __restrict__ out, int hq,
@@ -779,7 +826,7 @@ __global__ __launch_bounds__(64) void decode_combine_small_kernel(
                          : float2{0.0f, 0.0f};
   }
   const int L = min(seqlens[b], rule.max_tokens);
-  const int split_tokens = kRule ? split_tokens_of(own, L, seqlens, rule) : rule.fixed;
+  const int split_tokens = kRule ? split_tokens_of<kUnit>(own, L, seqlens, rule) : rule.fixed;
   const int nvalid = L <= 0 ? 0 : min(splits, (L + split_tokens - 1) / split_tokens);
   if (nvalid == 1) return;
   float M = -INFINITY;
@@ -813,7 +860,7 @@ constexpr int kWideWaves = 4;
 constexpr int kWideK = 8;
 constexpr int kWideThreshold = 64;  // splits above this use the wide merge
 
-template <typename T, bool kRule>
+template <typename T, bool kRule, int kUnit>
 __global__ __launch_bounds__(64 * kWideWaves) void decode_combine_wide_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_lse,
     const int32_t* __restrict__ seqlens, uint16_t* __restrict__ out, int hq,
@@ -839,7 +886,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void decode_combine_wide_kernel(
   SplitLoads<kWideK> first;
   load_splits(first, lse, po, 8 * wave + j, 8 * kWideWaves, min(splits, kPass));
   const int L = min(seqlens[b], rule.max_tokens);
-  const int split_tokens = kRule ? split_tokens_of(own, L, seqlens, rule) : rule.fixed;
+  const int split_tokens = kRule ? split_tokens_of<kUnit>(own, L, seqlens, rule) : rule.fixed;
   const int nvalid = L <= 0 ? 0 : min(splits, (L + split_tokens - 1) / split_tokens);
   if (nvalid == 1) return;  // written by the split kernel
   float m = -INFINITY, den = 0.0f;
@@ -876,6 +923,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void decode_combine_wide_kernel(
 constexpr int kOrderThreads = 256;
 constexpr int kOrderMaxBatch = 4096;
 
+template <int kUnit>
 __global__ __launch_bounds__(kOrderThreads) void decode_order_kernel(
     const int32_t* __restrict__ seqlens, const int32_t* __restrict__ bt, int4* __restrict__ items,
     int bs, int w, int pages_per_split, SplitRule rule) {
@@ -892,9 +940,9 @@ __global__ __launch_bounds__(kOrderThreads) void decode_order_kernel(
   const int blk_fixed = tid < rule.splits && fixed_page < w ? bt[(int64_t)b * w + fixed_page] : 0;
   int split_tokens = rule.fixed;
   if (rule.adapt) {
-    int steps = steps_of_length(len_own, rule), longest = steps;
+    int steps = steps_of_length<kUnit>(len_own, rule), longest = steps;
     for (int j = tid + kOrderThreads; j < rule.batch; j += kOrderThreads) {
-      const int n = steps_of_length(seqlens[j], rule);
+      const int n = steps_of_length<kUnit>(seqlens[j], rule);
       steps += n;
       longest = max(longest, n);
     }
@@ -911,7 +959,7 @@ __global__ __launch_bounds__(kOrderThreads) void decode_order_kernel(
       steps += s_steps[i];
       longest = max(longest, s_long[i]);
     }
-    split_tokens = split_tokens_from(steps, longest, rule);
+    split_tokens = split_tokens_from<kUnit>(steps, longest, rule);
   }
   // A sequence's full splits come in the order of its index, ahead of every
   // partial split; its partial one, if any, by the tokens in it (ties by
@@ -981,7 +1029,7 @@ static size_t partials_bytes(int batch, int hq, int splits) {
   return (raw + 255) & ~(size_t)255;
 }
 
-template <typename T>
+template <typename T, typename Cache>
 static hipError_t launch_decode(const DecodeArgs& a, int batch, hipStream_t stream) {
   // One 8-wave workgroup (128 KB of LDS) fills a CU.  A grid of at most
   // kWideGridMax of those runs in about two rounds; a larger grid runs in
@@ -1001,32 +1049,32 @@ static hipError_t launch_decode(const DecodeArgs& a, int batch, hipStream_t stre
     const int per_wg = wide ? kWavesPerWG : kNarrowWaves;
     const dim3 grid((unsigned)((units + per_wg - 1) / per_wg), (unsigned)a.splits,
                     (unsigned)batch);
-    hipLaunchKernelGGL(decode_order_kernel, dim3((unsigned)batch), dim3(kOrderThreads), 0, stream,
+    hipLaunchKernelGGL(decode_order_kernel<Cache::kUnit>, dim3((unsigned)batch), dim3(kOrderThreads), 0, stream,
                        a.seqlens, a.bt, const_cast<int4*>(a.items), a.bs, a.w, a.pages_per_split,
                        a.rule);
     const hipError_t eo = hipGetLastError();
     if (eo != hipSuccess) return eo;
     if (wide)
-      hipLaunchKernelGGL((decode_fp8_kernel<T, kWavesPerWG, kItems>), grid, dim3(64 * kWavesPerWG),
+      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kItems, Cache>()), grid, dim3(64 * kWavesPerWG),
                          0, stream, a);
     else
-      hipLaunchKernelGGL((decode_fp8_kernel<T, kNarrowWaves, kItems>), grid,
+      hipLaunchKernelGGL((split_kernel<T, kNarrowWaves, kItems, Cache>()), grid,
                          dim3(64 * kNarrowWaves), 0, stream, a);
   } else if (wide_wgs <= kWideGridMax) {
     dim3 grid((unsigned)((units + kWavesPerWG - 1) / kWavesPerWG), (unsigned)a.splits,
               (unsigned)batch);
     if (a.rule.adapt) {
       std::swap(grid.y, grid.z);
-      hipLaunchKernelGGL((decode_fp8_kernel<T, kWavesPerWG, kFollow>), grid,
+      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFollow, Cache>()), grid,
                          dim3(64 * kWavesPerWG), 0, stream, a);
     } else {
-      hipLaunchKernelGGL((decode_fp8_kernel<T, kWavesPerWG, kFixed>), grid,
+      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFixed, Cache>()), grid,
                          dim3(64 * kWavesPerWG), 0, stream, a);
     }
   } else {
     const dim3 grid((unsigned)((units + kNarrowWaves - 1) / kNarrowWaves), (unsigned)a.splits,
                     (unsigned)batch);
-    hipLaunchKernelGGL((decode_fp8_kernel<T, kNarrowWaves, kFixed>), grid,
+    hipLaunchKernelGGL((split_kernel<T, kNarrowWaves, kFixed, Cache>()), grid,
                        dim3(64 * kNarrowWaves), 0, stream, a);
   }
   hipError_t e = hipGetLastError();
@@ -1038,13 +1086,17 @@ static hipError_t launch_decode(const DecodeArgs& a, int batch, hipStream_t stre
   };
   const unsigned rows = (unsigned)(batch * a.hq);
   if (a.splits > kWideThreshold)
-    merge(rule ? decode_combine_wide_kernel<T, true> : decode_combine_wide_kernel<T, false>,
+    merge(rule ? decode_combine_wide_kernel<T, true, Cache::kUnit>
+               : decode_combine_wide_kernel<T, false, kStep>,
           dim3(rows, 4u), 64 * kWideWaves);
   else if (a.splits <= 8)
-    merge(rule ? decode_combine_small_kernel<T, 8, true> : decode_combine_small_kernel<T, 8, false>,
+    merge(rule ? decode_combine_small_kernel<T, 8, true, Cache::kUnit>
+               : decode_combine_small_kernel<T, 8, false, kStep>,
           dim3(rows), 64);
   else
-    merge(rule ? decode_combine_kernel<T, true> : decode_combine_kernel<T, false>, dim3(rows), 64);
+    merge(rule ? decode_combine_kernel<T, true, Cache::kUnit>
+               : decode_combine_kernel<T, false, kStep>,
+          dim3(rows), 64);
   return hipGetLastError();
 }
 
@@ -1052,20 +1104,19 @@ static int pages_per_split_of(int splits, int w) {
   return splits <= 1 ? w : (w + splits - 1) / splits;
 }
 
-}  // namespace mskv
-
-extern "C" int mskv_decode_num_splits(int batch, int num_q_heads,
-                                      int num_kv_heads, int max_blocks_per_seq,
-                                      int block_size) {
+// `step`: tokens of one step of the kernel, kMinSplitSteps of which are the
+// least of a split
+static int num_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_blocks_per_seq,
+                         int block_size, int step) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
       max_blocks_per_seq <= 0)
     return 1;
   const int group = num_q_heads / num_kv_heads;
-  const int64_t base = (int64_t)batch * num_kv_heads * mskv::qgroups_of(group);
+  const int64_t base = (int64_t)batch * num_kv_heads * qgroups_of(group);
   const int w = max_blocks_per_seq;
-  int64_t pps = (w * base + mskv::kTargetWaves - 1) / mskv::kTargetWaves;
+  int64_t pps = (w * base + kTargetWaves - 1) / kTargetWaves;
   if (pps < 1) pps = 1;
-  if (pps > mskv::kMaxPagesPerSplit) pps = mskv::kMaxPagesPerSplit;
+  if (pps > kMaxPagesPerSplit) pps = kMaxPagesPerSplit;
   int64_t splits = (w + pps - 1) / pps;
   // A page per split leaves half the waves idle: finer splits, of two steps at
   // least, as long as the partials stay small and the grid is one workgroup
@@ -1079,16 +1130,31 @@ extern "C" int mskv_decode_num_splits(int batch, int num_q_heads,
   // Only where they follow the lengths: at the shape's own split a page each,
   // more splits than table entries would start past an int's tokens at the
   // largest pages (512 splits of 2^23 tokens).
-  if (splits > 1 && 2 * w * base <= mskv::kTargetWaves && block_size > 0 &&
-      (int64_t)w * block_size <= mskv::kFollowMaxTokens) {
-    const int64_t per = (base / batch + mskv::kWavesPerWG - 1) / mskv::kWavesPerWG * batch;
-    int64_t fine = (int64_t)w * block_size / (mskv::kMinSplitSteps * mskv::kStep);
-    fine = std::min(fine, mskv::kWideGridMax / 2 / per);
-    fine = std::min(fine, (int64_t)(mskv::kFinePartialBytes /
-                                    ((int64_t)batch * num_q_heads * (mskv::kHeadDim + 1) * 4)));
+  if (splits > 1 && 2 * w * base <= kTargetWaves && block_size > 0 &&
+      (int64_t)w * block_size <= kFollowMaxTokens) {
+    const int64_t per = (base / batch + kWavesPerWG - 1) / kWavesPerWG * batch;
+    int64_t fine = (int64_t)w * block_size / (kMinSplitSteps * step);
+    fine = std::min(fine, kWideGridMax / 2 / per);
+    fine = std::min(fine, (int64_t)(kFinePartialBytes /
+                                    ((int64_t)batch * num_q_heads * (kHeadDim + 1) * 4)));
     if (2 * fine >= 3 * splits) splits = fine;
   }
   return (int)splits;
+}
+
+}  // namespace mskv
+
+extern "C" int mskv_decode_num_splits(int batch, int num_q_heads,
+                                      int num_kv_heads, int max_blocks_per_seq,
+                                      int block_size) {
+  return mskv::num_splits_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size,
+                             mskv::Fp8Cache::kUnit);
+}
+
+extern "C" int mskv_fp4_decode_num_splits(int batch, int num_q_heads, int num_kv_heads,
+                                          int max_blocks_per_seq, int block_size) {
+  return mskv::num_splits_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size,
+                             mskv::Fp4Cache::kUnit);
 }
 
 extern "C" size_t mskv_decode_workspace_bytes(int batch, int num_q_heads,
@@ -1111,8 +1177,9 @@ namespace mskv {
 // Validates a decode call and launches it with `workspace` as the split
 // partials ([batch, hq, splits, 128] outputs, then [batch, hq, splits]
 // lse values); `workspace_bytes` is what the caller's buffer holds.
+template <typename Cache>
 static int decode_checked(const void* query, const void* k_cache, const void* v_cache,
-                          const float* k_scale_cache, const float* v_scale_cache,
+                          const void* k_scale_cache, const float* v_scale_cache,
                           const int32_t* cache_seqlens, const int32_t* block_tables, void* out,
                           int batch, int num_q_heads, int num_kv_heads, int head_dim,
                           int block_size, int64_t num_blocks, int max_blocks_per_seq,
@@ -1124,13 +1191,13 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
   if (act_dtype != MSKV_FLOAT16 && act_dtype != MSKV_BFLOAT16) return MSKV_EINVAL;
   if (num_q_heads % num_kv_heads != 0) return MSKV_EINVAL;
   const int group = num_q_heads / num_kv_heads;
-  if (head_dim != kHeadDim || block_size % kStep != 0) return MSKV_EUNSUPPORTED;
+  if (head_dim != kHeadDim || block_size % Cache::kPageUnit != 0) return MSKV_EUNSUPPORTED;
   // page offsets are 32-bit buffer offsets, and token counts up to twice a
   // table's width (w * block_size + split_tokens) stay within int
   if ((int64_t)block_size * num_kv_heads * head_dim > 0x7FFFFFFFLL) return MSKV_EUNSUPPORTED;
   if ((int64_t)max_blocks_per_seq * block_size >= (1LL << 30)) return MSKV_EUNSUPPORTED;
-  if (num_splits != mskv_decode_num_splits(batch, num_q_heads, num_kv_heads,
-                                           max_blocks_per_seq, block_size))
+  if (num_splits != num_splits_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size,
+                                  Cache::kUnit))
     return MSKV_EINVAL;
   if (batch == 0) return MSKV_OK;
   if (!query || !k_cache || !v_cache || !k_scale_cache || !v_scale_cache ||
@@ -1144,7 +1211,7 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
   a.q = (const uint16_t*)query;
   a.kc = (const uint8_t*)k_cache;
   a.vc = (const uint8_t*)v_cache;
-  a.ks = k_scale_cache;
+  a.ks = (const float*)k_scale_cache;
   a.vs = v_scale_cache;
   a.seqlens = cache_seqlens;
   a.bt = block_tables;
@@ -1198,8 +1265,8 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
   a.num_blocks = num_blocks;
   a.scale_log2 = softmax_scale * kLog2e;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipError_t e = act_dtype == MSKV_BFLOAT16 ? launch_decode<__bf16>(a, batch, s)
-                                            : launch_decode<_Float16>(a, batch, s);
+  hipError_t e = act_dtype == MSKV_BFLOAT16 ? launch_decode<__bf16, Cache>(a, batch, s)
+                                            : launch_decode<_Float16, Cache>(a, batch, s);
   return (int)e;
 }
 
@@ -1242,7 +1309,7 @@ extern "C" int mskv_fp8_decode_attention(
     int64_t num_blocks, int max_blocks_per_seq, float softmax_scale,
     int act_dtype, int num_splits, void* workspace, size_t workspace_bytes,
     void* stream) {
-  return mskv::decode_checked(query, k_cache, v_cache, k_scale_cache, v_scale_cache,
+  return mskv::decode_checked<mskv::Fp8Cache>(query, k_cache, v_cache, k_scale_cache, v_scale_cache,
                               cache_seqlens, block_tables, out, batch, num_q_heads,
                               num_kv_heads, head_dim, block_size, num_blocks,
                               max_blocks_per_seq, softmax_scale, act_dtype, num_splits,
@@ -1264,9 +1331,21 @@ extern "C" int mskv_fp8_decode_attention_noalloc(
     const hipError_t e = mskv::scratch_for_current_device(&ws);
     if (e != hipSuccess) return (int)e;
   }
-  return mskv::decode_checked(query, k_cache, v_cache, k_scale_cache, v_scale_cache,
+  return mskv::decode_checked<mskv::Fp8Cache>(query, k_cache, v_cache, k_scale_cache, v_scale_cache,
                               cache_seqlens, block_tables, out, batch, num_q_heads,
                               num_kv_heads, head_dim, block_size, num_blocks,
                               max_blocks_per_seq, softmax_scale, act_dtype, num_splits, ws,
                               need, stream);
+}
+
+extern "C" int mskv_fp4_decode_attention(
+    const void* query, const void* k_cache, const void* v_cache, const void* k_scale_cache,
+    const float* v_scale_cache, const int32_t* cache_seqlens, const int32_t* block_tables,
+    void* out, int batch, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+    int64_t num_blocks, int max_blocks_per_seq, float softmax_scale, int act_dtype, int num_splits,
+    void* workspace, size_t workspace_bytes, void* stream) {
+  return mskv::decode_checked<mskv::Fp4Cache>(
+      query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens, block_tables, out, batch,
+      num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,
+      softmax_scale, act_dtype, num_splits, workspace, workspace_bytes, stream);
 }

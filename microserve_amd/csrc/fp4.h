@@ -1,0 +1,136 @@
+// The 4-bit paged KV cache shared by its store, load, decode and prefill.
+//
+// A value is an e2m1 code: 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign in bit 3,
+// two to a byte, the even dimension in the low half.
+//
+// K: a power-of-two scale for each 32 dimensions of a (token, kv head) row,
+// held as the byte e + 127 (E8M0; 255 marks a block that held an infinity or
+// a NaN).  Those blocks run along the contraction of QK^T, where
+// v_mfma_scale_f32_16x16x128_f8f6f4 applies them: no instruction dequantizes
+// K.  Pages are laid out in that MFMA's operand order, so lane (g, n) of a
+// wave reads its operand from memory with one 16-byte load, 1 KB contiguous
+// over the wave:
+//   k_cache  [num_blocks, H, BS / 16, 4, 16, 16]: 16 tokens; 32-dimension
+//            block g; token n of the 16; its 32 codes
+//   k_scale  [num_blocks, H, BS / 64, 4, 16, 4]: 64 tokens; block g; n; the
+//            bytes of tokens n, 16 + n, 32 + n and 48 + n, which the MFMA's
+//            byte select takes one after the other
+// V: one fp32 scale per row, as the FP8 cache has.  PV contracts over tokens,
+// so a row's scale belongs to the token's softmax weight; a scale per 32
+// dimensions would need four weights per token.  (On normal values the two
+// cost the same precision: the largest of 128 is about 2.7 sigma, a unit of
+// 0.45 sigma with an exact scale; the largest of 32 about 2.1 sigma, a unit
+// of 0.43 sigma on average under a power of two.)
+//   v_cache  [num_blocks, H, BS, 64], v_scale [num_blocks, H, BS]
+#pragma once
+
+#include "mskv_device.h"
+
+namespace mskv {
+
+constexpr float kFp4Max = 6.0f;
+constexpr int kFp4Row = kHeadDim / 2;  // bytes of a row's codes
+constexpr int kE8M0Nan = 255;
+
+// e4m3 parts the query is split into against 4-bit keys: bf16's 8
+// significant bits take two, fp16's 11 take three
+template <typename T> struct Fp4Query { static constexpr int parts = 3; };
+template <> struct Fp4Query<__bf16> { static constexpr int parts = 2; };
+
+// S^T += K . Q^T for 16 tokens: A the codes under their block scales (byte
+// kByte of `ks`), B a part of the query
+template <int kByte>
+__device__ __forceinline__ f32x4 mfma_fp4(const u32x4& k, uint32_t ks, const i32x8& q, f32x4 c) {
+  const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, c, 4 /* fp4 */, 0 /* e4m3 */,
+                                                          kByte, (int)ks, 0, 127);
+}
+
+// The query row of lane (g, n) as the B operand: e4m3 parts of q * f, f the
+// power of two that brings the row's largest magnitude near e4m3's (q * f is
+// exact).  The e4m3 operand's bytes 0-15 meet the dimensions [16g, 16g + 16)
+// and its bytes 16-31 [64 + 16g, 80 + 16g).  Returns f; NaNs for a
+// row that holds an infinity or a NaN, zeros where !ok.
+template <typename T>
+__device__ __forceinline__ float fp4_query(const uint16_t* row, bool ok, int g,
+                                           i32x8 (&qp)[Fp4Query<T>::parts]) {
+  using A = Act<T>;
+  float x[32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (ok) v = *reinterpret_cast<const u32x4*>(row + 64 * (c >> 1) + 16 * g + 8 * (c & 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[8 * c + 2 * i] = A::to_f32((uint16_t)(v[i] & 0xFFFFu));
+      x[8 * c + 2 * i + 1] = A::to_f32((uint16_t)(v[i] >> 16));
+    }
+  }
+  // the largest magnitude, as bits: a NaN is above infinity
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  const auto r16 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+  top = max((uint32_t)r16[0], (uint32_t)r16[1]);
+  const auto r32 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+  top = max((uint32_t)r32[0], (uint32_t)r32[1]);
+  // The clamp below would make a NaN finite: its row gets e4m3 NaNs, set by
+  // their bits, since -fno-honor-nans lets the compiler drop a NaN that it
+  // sees made.
+  const bool finite = top < 0x7F800000u;
+  const uint32_t nan = finite ? 0u : 0x7F7F7F7Fu;
+  const float amax = finite ? __uint_as_float(top) : 0.0f;
+  const float f = amax > 1e-30f ? pow2_floor(kFp8Max / amax) : 1.0f;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = fminf(fmaxf(x[4 * c + i] * f, -kFp8Max), kFp8Max);
+    uint32_t h, mi, lo;
+    if constexpr (Fp4Query<T>::parts == 2) {
+      split_fp8x4(y[0], y[1], y[2], y[3], h, lo);
+      qp[0][c] = (int)(h | nan);
+      qp[1][c] = (int)lo;
+    } else {
+      split3_fp8x4(y[0], y[1], y[2], y[3], h, mi, lo);
+      qp[0][c] = (int)(h | nan);
+      qp[1][c] = (int)mi;
+      qp[2][c] = (int)lo;
+    }
+  }
+  return f;
+}
+
+// eight codes (a dword) -> eight exact fp16 values
+__device__ __forceinline__ f16x8 fp4x8_to_f16(uint32_t w) {
+  f16x8 r;
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3);
+  r[0] = a[0]; r[1] = a[1]; r[2] = b[0]; r[3] = b[1];
+  r[4] = c[0]; r[5] = c[1]; r[6] = d[0]; r[7] = d[1];
+  return r;
+}
+
+// V tiles in LDS hold 64-byte rows whose 16-byte chunks are XOR-swizzled by
+// (row / 16) % 4.  ds_read_b64_tr_b4 hands lane i of each 16 the nibble i of
+// the 8 bytes that the 16 lanes name, lane j's as the j-th: lane (g, j) names
+// row 16 * (j / 4) + 4g + j % 4, so its result holds, at one dimension, the
+// tokens that S^T's accumulators leave in lane group g (tile j / 4, register
+// j % 4).  The swizzle gives the 16 rows of a group distinct banks.
+__device__ __forceinline__ uint32_t fp4_v_row(int lane) {
+  const int g = lane >> 4, j = lane & 15;
+  return (uint32_t)(16 * (j >> 2) + 4 * g + (j & 3)) * kFp4Row;
+}
+// byte offset of dimension tile dt (16 dimensions) inside lane's row
+__device__ __forceinline__ uint32_t fp4_v_col(int lane, int dt) {
+  return 16u * (uint32_t)((dt >> 1) ^ ((lane >> 2) & 3)) + 8u * (dt & 1);
+}
+__device__ __forceinline__ i32x2 fp4_v_read(const uint8_t* tile, uint32_t off) {
+  return __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+      reinterpret_cast<__attribute__((address_space(3))) i32x2*>(
+          (__attribute__((address_space(3))) uint8_t*)tile + off));
+}
+
+}  // namespace mskv

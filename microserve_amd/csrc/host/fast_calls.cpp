@@ -13,10 +13,12 @@
 // converted and checked, runs as if this module did not exist.  A launch
 // that failed (a positive status) raises here: the runtime forgets an error
 // once it has been read, so a second try could pass in silence.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../../include/mskv.h"
@@ -32,6 +34,11 @@ struct Api {
   decltype(&mskv_fp8_prefill_attention_bounded) prefill = nullptr;
   decltype(&mskv_prefill_attention_strided) fresh = nullptr;
   decltype(&mskv_qk_norm_rope_store) prologue = nullptr;
+  decltype(&mskv_store_fp4_kvcache) store4 = nullptr;
+  decltype(&mskv_load_fp4_kvcache) load4 = nullptr;
+  decltype(&mskv_fp4_decode_num_splits) num_splits4 = nullptr;
+  decltype(&mskv_fp4_decode_attention) decode4 = nullptr;
+  decltype(&mskv_fp4_prefill_attention) prefill4 = nullptr;
   decltype(&mskv_status_string) text = nullptr;
   bool bound = false;
 } api;
@@ -95,6 +102,24 @@ bool caches_match(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& 
                   const at::Tensor& vs, int64_t hk, int64_t d) {
   return kc.size(2) == hk && kc.size(3) == d && vc.sizes() == kc.sizes() &&
          ks.sizes() == kc.sizes().slice(0, 3) && vs.sizes() == ks.sizes();
+}
+
+struct Dims {
+  int64_t blocks, block, heads, d;
+};
+// the FP8 cache's, from k_cache (the others are checked by the caller)
+Dims dims_of(const at::Tensor& kc) { return {kc.size(0), kc.size(1), kc.size(2), kc.size(3)}; }
+// the four 4-bit caches, as fp4_kv_cache.check_fp4_caches asserts them
+bool fp4_caches(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                const at::Tensor& vs, Dims& m) {
+  if (!dense_of(kc, at::kByte) || !dense_of(vc, at::kByte) || !dense_of(ks, at::kByte) ||
+      !dense_of(vs, at::kFloat) || vc.dim() != 4 || vc.size(3) != 64)
+    return false;
+  const int64_t nb = vc.size(0), h = vc.size(1), bs = vc.size(2);
+  m = {nb, bs, h, 128};
+  return bs > 0 && bs % 128 == 0 && kc.sizes() == at::IntArrayRef({nb, h, bs / 16, 4, 16, 16}) &&
+         ks.sizes() == at::IntArrayRef({nb, h, bs / 64, 4, 16, 4}) &&
+         vs.sizes() == at::IntArrayRef({nb, h, bs});
 }
 
 // the kernels' vector and direct-to-LDS loads start on 16 bytes
@@ -205,10 +230,80 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// store4: store's arguments over the 4-bit caches
+PyObject* store4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 7) return nullptr;
+    Args in;
+    const at::Tensor *key = in.first(a[0]), *value = in.next(a[1]), *kc = in.next(a[2]),
+                     *vc = in.next(a[3]), *ks = in.next(a[4]), *vs = in.next(a[5]),
+                     *sl = in.next(a[6]);
+    Dims m;
+    if (!in.ok || key->dim() != 3 || value->sizes() != key->sizes() ||
+        value->scalar_type() != key->scalar_type() || !fp4_caches(*kc, *vc, *ks, *vs, m) ||
+        key->size(1) != m.heads || key->size(2) != m.d || !fits({key->size(0), m.heads, m.block}))
+      return nullptr;
+    int dt = MSKV_FLOAT32, st;
+    int64_t k_stride, v_stride;
+    if (key->scalar_type() != at::kFloat && !act(*key, dt)) return nullptr;
+    if (!slots_of(*sl, key->size(0), st) || !token_rows(*key, k_stride) ||
+        !token_rows(*value, v_stride))
+      return nullptr;
+    int status;
+    {
+      NoGil no_gil;
+      const c10::DeviceGuard guard(in.device);
+      status = api.store4(key->data_ptr(), k_stride, value->data_ptr(), v_stride, kc->data_ptr(),
+                          vc->data_ptr(), ks->data_ptr(), (float*)vs->data_ptr(), sl->data_ptr(),
+                          st, key->size(0), (int)m.heads, (int)m.d, (int)m.block, m.blocks, dt,
+                          stream_of(in.device));
+    }
+    if (status != MSKV_OK) return failed("store_fp4_kvcache", status);
+    Py_RETURN_TRUE;
+  });
+}
+
+// load4(k_cache, v_cache, k_scale, v_scale, slots, dtype) -> (key, value) | None
+PyObject* load4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 6 || !THPDtype_Check(a[5])) return nullptr;
+    Args in;
+    const at::Tensor *kc = in.first(a[0]), *vc = in.next(a[1]), *ks = in.next(a[2]),
+                     *vs = in.next(a[3]), *sl = in.next(a[4]);
+    Dims m;
+    if (!in.ok || !fp4_caches(*kc, *vc, *ks, *vs, m)) return nullptr;
+    const auto type = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+    const int dt = type == at::kHalf       ? MSKV_FLOAT16
+                   : type == at::kBFloat16 ? MSKV_BFLOAT16
+                   : type == at::kFloat    ? MSKV_FLOAT32
+                                           : -1;
+    const int64_t tokens = sl->numel();
+    int st;
+    if (dt < 0 || !slots_of(*sl, tokens, st) || !fits({tokens, m.heads, m.block})) return nullptr;
+    at::Tensor key, value;
+    int status;
+    {
+      NoGil no_gil;
+      const c10::DeviceGuard guard(in.device);
+      const auto opts = vs->options().dtype(type).requires_grad(false);
+      key = at::empty({tokens, m.heads, m.d}, opts);
+      value = at::empty({tokens, m.heads, m.d}, opts);
+      status = api.load4(kc->data_ptr(), vc->data_ptr(), ks->data_ptr(), (float*)vs->data_ptr(),
+                         sl->data_ptr(), st, key.data_ptr(), value.data_ptr(), tokens,
+                         (int)m.heads, (int)m.d, (int)m.block, m.blocks, dt,
+                         stream_of(in.device));
+    }
+    if (status != MSKV_OK) return failed("load_fp4_kvcache", status);
+    PyObject* k = THPVariable_Wrap(std::move(key));
+    return Py_BuildValue("(NN)", k, THPVariable_Wrap(std::move(value)));
+  });
+}
+
 // decode(query, k_cache, v_cache, k_scale, v_scale, seqlens, tables, scale,
 //        out | None, scratch) -> out | None;
 // scratch(device, stream, bytes) -> the stream's split-partials tensor
-PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+template <bool kFp4>
+PyObject* decode_call(PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 10) return nullptr;
     Args in;
@@ -219,19 +314,22 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     double scale;
     int dt;
     if (!in.ok || q->dim() != 3 || !q->is_contiguous() || !aligned(*q) || !act(*q, dt) || !number(a[7], scale) ||
-        !caches_ok(*kc, *vc, *ks, *vs) || !dense_of(*len, at::kInt) || bt->dim() != 2 ||
-        !dense_of(*bt, at::kInt))
+        !dense_of(*len, at::kInt) || bt->dim() != 2 || !dense_of(*bt, at::kInt))
       return nullptr;
-    const int64_t b = q->size(0), hq = q->size(1), d = q->size(2), hk = kc->size(2),
-                  bs = kc->size(1), w = bt->size(1);
-    if (!fits({b, hq, d, hk, bs, w}) || hq % hk != 0 || d != kc->size(3) || bt->size(0) != b ||
+    Dims m;
+    if (kFp4 ? !fp4_caches(*kc, *vc, *ks, *vs, m) : !caches_ok(*kc, *vc, *ks, *vs)) return nullptr;
+    if (!kFp4) m = dims_of(*kc);
+    const int64_t b = q->size(0), hq = q->size(1), d = q->size(2), hk = m.heads, bs = m.block,
+                  w = bt->size(1);
+    if (!fits({b, hq, d, hk, bs, w}) || hq % hk != 0 || d != m.d || bt->size(0) != b ||
         len->numel() != b)
       return nullptr;
     if (given && (given->sizes() != q->sizes() || given->scalar_type() != q->scalar_type() ||
                   !given->is_contiguous()))
       return nullptr;
     void* stream = stream_of(in.device);
-    const int splits = api.num_splits((int)b, (int)hq, (int)hk, (int)w, (int)bs);
+    const int splits =
+        (kFp4 ? api.num_splits4 : api.num_splits)((int)b, (int)hq, (int)hk, (int)w, (int)bs);
     const size_t bytes = api.decode_bytes((int)b, (int)hq, (int)hk, (int)d, splits);
     void* ws = nullptr;
     if (bytes) {
@@ -249,14 +347,22 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int status;
     {
       NoGil no_gil;
+      const c10::DeviceGuard guard(in.device);
       if (!given) fresh = at::empty(q->sizes(), q->options().requires_grad(false));
       const at::Tensor& out = given ? *given : fresh;
-      status = api.decode(q->data_ptr(), kc->data_ptr(), vc->data_ptr(), (float*)ks->data_ptr(),
-                   (float*)vs->data_ptr(), (int32_t*)len->data_ptr(), (int32_t*)bt->data_ptr(),
-                   out.data_ptr(), (int)b, (int)hq, (int)hk, (int)d, (int)bs, kc->size(0), (int)w,
-                   (float)scale, dt, splits, ws, bytes, stream);
+      auto call = [&](auto f) {
+        return f(q->data_ptr(), kc->data_ptr(), vc->data_ptr(), (float*)ks->data_ptr(),
+                 (float*)vs->data_ptr(), (int32_t*)len->data_ptr(), (int32_t*)bt->data_ptr(),
+                 out.data_ptr(), (int)b, (int)hq, (int)hk, (int)d, (int)bs, m.blocks, (int)w,
+                 (float)scale, dt, splits, ws, bytes, stream);
+      };
+      if constexpr (kFp4)
+        status = call(api.decode4);
+      else
+        status = call(api.decode);
     }
-    if (status != MSKV_OK) return failed("fp8_decode_attention", status);
+    if (status != MSKV_OK)
+      return failed(kFp4 ? "fp4_decode_attention" : "fp8_decode_attention", status);
     if (given) {
       Py_INCREF(a[8]);
       return a[8];
@@ -265,11 +371,15 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) { return decode_call<false>(a, n); }
+PyObject* decode4(PyObject*, PyObject* const* a, Py_ssize_t n) { return decode_call<true>(a, n); }
+
 // prefill(query, k_cache, v_cache, k_scale, v_scale, tables, cu_q | None,
 //         cu_k | None, prefix_len, max_seqlen_q, max_seqlen_k, scale)
 //   -> out | None
 // (without cu_q, one sequence: max_seqlen_q and max_seqlen_k are not read)
-PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+template <bool kFp4>
+PyObject* prefill_call(PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 12) return nullptr;
     Args in;
@@ -281,11 +391,13 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     double scale;
     int dt, prefix, max_q, bound;
     if (!in.ok || q->dim() != 3 || !q->is_contiguous() || !aligned(*q) || !act(*q, dt) || !whole(a[8], prefix) ||
-        !whole(a[9], max_q) || !whole(a[10], bound) || !number(a[11], scale) || !caches_ok(*kc, *vc, *ks, *vs) ||
+        !whole(a[9], max_q) || !whole(a[10], bound) || !number(a[11], scale) ||
         !dense_of(*bt, at::kInt))
       return nullptr;
-    const int64_t nq = q->size(0), hq = q->size(1), d = q->size(2), hk = kc->size(2),
-                  bs = kc->size(1);
+    Dims m;
+    if (kFp4 ? !fp4_caches(*kc, *vc, *ks, *vs, m) : !caches_ok(*kc, *vc, *ks, *vs)) return nullptr;
+    if (!kFp4) m = dims_of(*kc);
+    const int64_t nq = q->size(0), hq = q->size(1), d = q->size(2), hk = m.heads, bs = m.block;
     int64_t seqs = 1, w = bt->numel();
     if (varlen) {
       if (bt->dim() != 2 || !dense_of(*cq, at::kInt) || !dense_of(*ck, at::kInt)) return nullptr;
@@ -293,7 +405,7 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
       w = bt->size(1);
       if (ck->numel() != seqs + 1 || bt->size(0) != seqs) return nullptr;
     }
-    if (!fits({nq, hq, d, hk, bs, w, seqs}) || hq % hk != 0 || d != kc->size(3)) return nullptr;
+    if (!fits({nq, hq, d, hk, bs, w, seqs}) || hq % hk != 0 || d != m.d) return nullptr;
     int64_t max_k = bound;
     if (!varlen) {
       max_q = (int)nq;
@@ -305,21 +417,37 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int status;
     {
       NoGil no_gil;
+      const c10::DeviceGuard guard(in.device);
       if (bytes) ws = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte).requires_grad(false));
       out = at::empty(q->sizes(), q->options().requires_grad(false));
-      status = api.prefill(q->data_ptr(), kc->data_ptr(), vc->data_ptr(), (float*)ks->data_ptr(),
-                    (float*)vs->data_ptr(), (int32_t*)bt->data_ptr(),
-                    varlen ? (int32_t*)cq->data_ptr() : nullptr,
-                    varlen ? (int32_t*)ck->data_ptr() : nullptr, prefix, out.data_ptr(), (int)seqs,
-                    nq, max_q, max_k, (int)hq, (int)hk, (int)d, (int)bs, kc->size(0), (int)w,
-                    (float)scale, dt, bytes ? ws.data_ptr() : nullptr, bytes,
-                    stream_of(in.device));
+      auto call = [&](auto f) {
+        return f(q->data_ptr(), kc->data_ptr(), vc->data_ptr(), (float*)ks->data_ptr(),
+                 (float*)vs->data_ptr(), (int32_t*)bt->data_ptr(),
+                 varlen ? (int32_t*)cq->data_ptr() : nullptr,
+                 varlen ? (int32_t*)ck->data_ptr() : nullptr, prefix, out.data_ptr(), (int)seqs,
+                 nq, max_q, max_k, (int)hq, (int)hk, (int)d, (int)bs, m.blocks, (int)w,
+                 (float)scale, dt, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(in.device));
+      };
+      if constexpr (kFp4)
+        status = call(api.prefill4);
+      else
+        status = call(api.prefill);
     }
-    if (status != MSKV_OK)
+    if (status != MSKV_OK) {
+      if (kFp4)
+        return failed(varlen ? "fp4_varlen_prefill_attention" : "fp4_chunk_prefill_attention",
+                      status);
       return failed(varlen ? "fp8_varlen_prefill_attention" : "fp8_chunk_prefill_attention",
                     status);
+    }
     return THPVariable_Wrap(std::move(out));
   });
+}
+PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return prefill_call<false>(a, n);
+}
+PyObject* prefill4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return prefill_call<true>(a, n);
 }
 
 // fresh(q, k, v, cu_q, cu_k, max_seqlen_q, scale) -> out | None
@@ -433,7 +561,11 @@ PyObject* bind(PyObject*, PyObject* table) {
             get("mskv_fp8_prefill_bounded_workspace_bytes", f.prefill_bytes) &&
             get("mskv_fp8_prefill_attention_bounded", f.prefill) &&
             get("mskv_prefill_attention_strided", f.fresh) &&
-            get("mskv_qk_norm_rope_store", f.prologue) && get("mskv_status_string", f.text);
+            get("mskv_qk_norm_rope_store", f.prologue) &&
+            get("mskv_store_fp4_kvcache", f.store4) && get("mskv_load_fp4_kvcache", f.load4) &&
+            get("mskv_fp4_decode_num_splits", f.num_splits4) &&
+            get("mskv_fp4_decode_attention", f.decode4) &&
+            get("mskv_fp4_prefill_attention", f.prefill4) && get("mskv_status_string", f.text);
   if (!f.bound) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "an entry point has no address");
     return nullptr;
@@ -444,6 +576,7 @@ PyObject* bind(PyObject*, PyObject* table) {
 
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FAST(store), FAST(decode), FAST(prefill), FAST(fresh), FAST(prologue),
+                          FAST(store4), FAST(load4), FAST(decode4), FAST(prefill4),
                           {"bind", bind, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 

@@ -1,0 +1,289 @@
+// Moving whole pages of a paged KV pool: copies (a forked sequence's last
+// page) and compaction (the live pages to the lowest places).
+//
+// A pool is up to kMaxPools tensors whose pages are numbered alike (codes and
+// scales, FP8 or 4-bit, one layer's or all layers'): `planes` stacks of pages
+// `plane_stride` bytes apart, pages of `page_bytes` back to back.  All of a
+// call's bytes move in one launch: workgroups take segments of a page, 16
+// bytes a lane and load, several loads in flight.  HBM-bound, 2 bytes moved
+// per byte of the pages.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "mskv_device.h"
+#include "../../include/mskv.h"
+
+namespace mskv {
+
+constexpr int kMaxPools = MSKV_MAX_POOLS;
+constexpr int kMoveThreads = 256;
+constexpr int kMoveLoads = 4;  // 16-byte pieces a lane has in flight
+constexpr int kSegBytes = kMoveThreads * kMoveLoads * 16;
+// pairs that travel as arguments of one launch
+constexpr int kMaxPairs = 256;
+
+struct Pools {
+  uint8_t* base[kMaxPools];
+  int64_t plane_stride[kMaxPools], page_bytes[kMaxPools];
+  int segs[kMaxPools];       // segments per page
+  int first[kMaxPools + 1];  // of a pool's planes, among a page's segments
+  int count;
+};
+
+struct PagePairs {
+  int32_t src[kMaxPairs], dst[kMaxPairs];
+};
+
+// Copies segment `seg` (of all the pools' planes) of page src to page dst.
+__device__ __forceinline__ void copy_segment(const Pools& p, int seg, int64_t src, int64_t dst) {
+  int t = 0;
+  while (t + 1 < p.count && seg >= p.first[t + 1]) ++t;
+  const int s = seg - p.first[t];
+  const int plane = s / p.segs[t], part = s - plane * p.segs[t];
+  const int64_t page = p.page_bytes[t], begin = (int64_t)part * kSegBytes;
+  uint8_t* stack = p.base[t] + plane * p.plane_stride[t] + begin;
+  const u32x4* from = reinterpret_cast<const u32x4*>(stack + src * page);
+  u32x4* to = reinterpret_cast<u32x4*>(stack + dst * page);
+  const int n = (int)min((int64_t)kSegBytes, page - begin) / 16;
+  u32x4 v[kMoveLoads];
+#pragma unroll
+  for (int i = 0; i < kMoveLoads; ++i) {
+    const int at = i * kMoveThreads + threadIdx.x;
+    if (at < n) v[i] = __builtin_nontemporal_load(from + at);
+  }
+#pragma unroll
+  for (int i = 0; i < kMoveLoads; ++i) {
+    const int at = i * kMoveThreads + threadIdx.x;
+    if (at < n) __builtin_nontemporal_store(v[i], to + at);
+  }
+}
+
+// grid (segments of a page in all pools, pairs)
+__global__ __launch_bounds__(kMoveThreads) void copy_kv_blocks_kernel(Pools p, PagePairs pairs) {
+  copy_segment(p, blockIdx.x, pairs.src[blockIdx.y], pairs.dst[blockIdx.y]);
+}
+
+// The plan of a compaction: n pages are named by the tables; the i-th named
+// page at or above n (ascending) goes to the i-th free page below n, so no
+// page is both read and written.  One workgroup: the pages' flags are a
+// bitmap in LDS, each thread ranks a run of its words.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanMaxBlocks = 1 << 18;  // 32 KB of flags
+
+// sums of v over the threads before this one, and over all
+__device__ __forceinline__ int2 block_scan(int v, int* s_wave) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 63) s_wave[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    before += w < wave ? s_wave[w] : 0;
+    all += s_wave[w];
+  }
+  __syncthreads();
+  return int2{before + x - v, all};
+}
+
+struct CompactArgs {
+  const int32_t* tables;
+  int32_t *new_tables, *remap, *num_live;
+  int32_t *moves, *src, *dst;  // workspace: their number, then the pages
+  int64_t entries;
+  int num_blocks, segs;
+};
+
+__global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactArgs a) {
+  extern __shared__ uint32_t flags[];
+  __shared__ int s_wave[kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  const int words = (a.num_blocks + 31) / 32;
+  for (int w = tid; w < words; w += kPlanThreads) flags[w] = 0;
+  __syncthreads();
+  for (int64_t i = tid; i < a.entries; i += kPlanThreads) {
+    const int32_t page = a.tables[i];
+    if (page >= 0 && page < a.num_blocks) atomicOr(&flags[page >> 5], 1u << (page & 31));
+  }
+  __syncthreads();
+  const int per = (words + kPlanThreads - 1) / kPlanThreads;
+  const int w0 = min(tid * per, words), w1 = min(w0 + per, words);
+  int own = 0;
+  for (int w = w0; w < w1; ++w) own += __popc(flags[w]);
+  const int n = block_scan(own, s_wave).y;
+  // of this thread's pages: the free ones below n, and the named ones from n
+  int holes = 0, movers = 0;
+  for (int w = w0; w < w1; ++w) {
+    const int below = min(max(n - 32 * w, 0), 32);
+    const uint32_t low = below == 32 ? ~0u : (1u << below) - 1u;
+    holes += __popc(~flags[w] & low);
+    movers += __popc(flags[w] & ~low);
+  }
+  const int2 h = block_scan(holes, s_wave), m = block_scan(movers, s_wave);
+  int hi = h.x, mi = m.x;
+  for (int w = w0; w < w1; ++w) {
+    const uint32_t f = flags[w];
+    for (int b = 0; b < 32 && 32 * w + b < a.num_blocks; ++b) {
+      const int page = 32 * w + b;
+      const bool named = (f >> b) & 1u;
+      if (page < n && !named) a.dst[hi++] = page;
+      if (page >= n && named) a.src[mi++] = page;
+      a.remap[page] = named && page < n ? page : -1;
+    }
+  }
+  if (tid == 0) {
+    *a.moves = h.y;
+    *a.num_live = n;
+  }
+  __syncthreads();  // (the pages above were written by this workgroup)
+  for (int i = tid; i < h.y; i += kPlanThreads) a.remap[a.src[i]] = a.dst[i];
+}
+
+// Moves the pages and renames the tables' entries, both from the plan.
+__global__ __launch_bounds__(kMoveThreads) void compact_move_kernel(Pools p, CompactArgs a) {
+  const int moves = __builtin_amdgcn_readfirstlane(*a.moves);
+  for (int64_t i = (int64_t)blockIdx.x * kMoveThreads + threadIdx.x; i < a.entries;
+       i += (int64_t)gridDim.x * kMoveThreads) {
+    const int32_t page = a.tables[i];
+    a.new_tables[i] = page >= 0 && page < a.num_blocks ? a.remap[page] : page;
+  }
+  const int64_t total = (int64_t)moves * a.segs;
+  for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+    const int pair = (int)(i / a.segs);
+    copy_segment(p, (int)(i - (int64_t)pair * a.segs),
+                 __builtin_amdgcn_readfirstlane(a.src[pair]),
+                 __builtin_amdgcn_readfirstlane(a.dst[pair]));
+  }
+}
+
+// Checks a call's pools and lays their segments out.
+static int pools_of(Pools& p, int count, void* const* bases, const int64_t* planes,
+                    const int64_t* plane_strides, const int64_t* page_bytes, int64_t num_blocks) {
+  if (count <= 0 || count > kMaxPools || !bases || !planes || !plane_strides || !page_bytes)
+    return MSKV_EINVAL;
+  if (num_blocks < 0 || num_blocks > 0x7FFFFFFFLL) return MSKV_EINVAL;
+  int64_t first = 0;
+  p.count = count;
+  for (int t = 0; t < count; ++t) {
+    if (!bases[t] || planes[t] <= 0 || page_bytes[t] <= 0 || plane_strides[t] < 0)
+      return MSKV_EINVAL;
+    if (misaligned({bases[t]}) || page_bytes[t] % 16 != 0 || plane_strides[t] % 16 != 0)
+      return MSKV_EUNSUPPORTED;
+    // every byte offset fits an int64, and the planes do not overlap
+    if (num_blocks > 0 && page_bytes[t] > (INT64_MAX >> 1) / num_blocks) return MSKV_EINVAL;
+    if (planes[t] > 1 && plane_strides[t] < page_bytes[t] * num_blocks) return MSKV_EINVAL;
+    if (planes[t] > 1 && plane_strides[t] > (INT64_MAX >> 1) / planes[t]) return MSKV_EINVAL;
+    const int64_t segs = (page_bytes[t] + kSegBytes - 1) / kSegBytes;
+    if (segs > 0x3FFFFFFF || planes[t] > 0x3FFFFFFF / segs) return MSKV_EUNSUPPORTED;
+    p.base[t] = (uint8_t*)bases[t];
+    p.plane_stride[t] = plane_strides[t];
+    p.page_bytes[t] = page_bytes[t];
+    p.segs[t] = (int)segs;
+    p.first[t] = (int)first;
+    first += segs * planes[t];
+    if (first > 0xFFFFFF) return MSKV_EUNSUPPORTED;  // a grid's threads fit 32 bits
+  }
+  p.first[count] = (int)first;
+  return MSKV_OK;
+}
+
+}  // namespace mskv
+
+extern "C" int mskv_copy_kv_blocks(int num_pools, void* const* bases, const int64_t* planes,
+                                   const int64_t* plane_strides, const int64_t* page_bytes,
+                                   int64_t num_blocks, const int32_t* src_blocks,
+                                   const int32_t* dst_blocks, int64_t num_pairs, void* stream) {
+  using namespace mskv;
+  Pools p;
+  const int status = pools_of(p, num_pools, bases, planes, plane_strides, page_bytes, num_blocks);
+  if (status != MSKV_OK) return status;
+  if (num_pairs < 0) return MSKV_EINVAL;
+  if (num_pairs == 0) return MSKV_OK;
+  if (!src_blocks || !dst_blocks || num_pairs > num_blocks) return MSKV_EINVAL;
+  // Pages are read and written side by side: each is written once, and none
+  // that is written is read.
+  try {
+    std::vector<int32_t> from(src_blocks, src_blocks + num_pairs),
+        to(dst_blocks, dst_blocks + num_pairs);
+    std::sort(from.begin(), from.end());
+    std::sort(to.begin(), to.end());
+    if (from.front() < 0 || to.front() < 0 || from.back() >= num_blocks ||
+        to.back() >= num_blocks)
+      return MSKV_EINVAL;
+    if (std::adjacent_find(to.begin(), to.end()) != to.end()) return MSKV_EINVAL;
+    for (int32_t d : to)
+      if (std::binary_search(from.begin(), from.end(), d)) return MSKV_EINVAL;
+  } catch (...) {
+    return MSKV_EINVAL;
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  for (int64_t at = 0; at < num_pairs; at += kMaxPairs) {
+    const int n = (int)std::min<int64_t>(kMaxPairs, num_pairs - at);
+    PagePairs pairs = {};
+    std::copy_n(src_blocks + at, n, pairs.src);
+    std::copy_n(dst_blocks + at, n, pairs.dst);
+    hipLaunchKernelGGL(copy_kv_blocks_kernel, dim3((unsigned)p.first[p.count], (unsigned)n),
+                       dim3(kMoveThreads), 0, s, p, pairs);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return MSKV_OK;
+}
+
+extern "C" size_t mskv_compact_workspace_bytes(int64_t num_blocks) {
+  if (num_blocks <= 0 || num_blocks > mskv::kPlanMaxBlocks) return 0;
+  // the number of moves (16 bytes), then as many sources and destinations as
+  // there can be: a page moves only if another one is free
+  return 16 + 2 * sizeof(int32_t) * (size_t)(num_blocks / 2 + 1);
+}
+
+extern "C" int mskv_compact_kv_blocks(int num_pools, void* const* bases, const int64_t* planes,
+                                      const int64_t* plane_strides, const int64_t* page_bytes,
+                                      int64_t num_blocks, const int32_t* block_tables,
+                                      int64_t num_entries, int32_t* new_tables, int32_t* remap,
+                                      int32_t* num_live, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  using namespace mskv;
+  Pools p;
+  const int status = pools_of(p, num_pools, bases, planes, plane_strides, page_bytes, num_blocks);
+  if (status != MSKV_OK) return status;
+  if (num_entries < 0 || num_blocks <= 0) return MSKV_EINVAL;
+  if (num_blocks > kPlanMaxBlocks || num_entries > (int64_t)1 << 40) return MSKV_EUNSUPPORTED;
+  if (!remap || !num_live || (num_entries > 0 && (!block_tables || !new_tables)))
+    return MSKV_EINVAL;
+  if (!workspace || workspace_bytes < mskv_compact_workspace_bytes(num_blocks))
+    return MSKV_EWORKSPACE;
+  CompactArgs a;
+  a.tables = block_tables;
+  a.new_tables = new_tables;
+  a.remap = remap;
+  a.num_live = num_live;
+  a.moves = (int32_t*)workspace;
+  a.src = a.moves + 4;
+  a.dst = a.src + num_blocks / 2 + 1;
+  a.entries = num_entries;
+  a.num_blocks = (int)num_blocks;
+  a.segs = p.first[p.count];
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const unsigned lds = (unsigned)((num_blocks + 31) / 32 * 4);
+  hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), lds, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return (int)e;
+  // a grid that fills the chip walks the moves, whose number only the device
+  // knows
+  const int64_t most = std::max<int64_t>(num_blocks / 2 * a.segs,
+                                         (num_entries + kMoveThreads - 1) / kMoveThreads);
+  const unsigned grid = (unsigned)std::min<int64_t>(std::max<int64_t>(most, 1), 2048);
+  hipLaunchKernelGGL(compact_move_kernel, dim3(grid), dim3(kMoveThreads), 0, s, p, a);
+  return (int)hipGetLastError();
+}

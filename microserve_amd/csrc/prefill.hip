@@ -50,6 +50,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mskv_device.h"
 #include "../../include/mskv.h"
@@ -606,6 +607,12 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp8_kernel(Prefill
   }
 }
 
+}  // namespace mskv
+
+#include "fp4_prefill.h"
+
+namespace mskv {
+
 // out[row] = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M) over the splits
 // that saw keys of the row (zeros if none did).  32 lanes per row, four d
 // each; every split's partial is loaded at once.  HBM-bound: it reads what
@@ -665,16 +672,23 @@ static void launch_merge(const PrefillArgs& a, int num_seqs, int tokens, hipStre
                      a.total_q, tokens);
 }
 
-template <typename T>
+template <typename T, bool kFp4>
 static hipError_t launch_prefill(const PrefillArgs& a, int num_seqs, int64_t qblocks,
                                  hipStream_t st) {
   dim3 grid((unsigned)(a.hk * a.qgroups), (unsigned)num_seqs, (unsigned)qblocks);
+  auto rows = [&](auto split) {
+    constexpr bool kSplit = decltype(split)::value;
+    if constexpr (kFp4)
+      hipLaunchKernelGGL((prefill_fp4_kernel<T, kSplit>), grid, dim3(PShape::threads), 0, st, a);
+    else
+      hipLaunchKernelGGL((prefill_fp8_kernel<T, kSplit>), grid, dim3(PShape::threads), 0, st, a);
+  };
   if (a.splits <= 1) {
-    hipLaunchKernelGGL((prefill_fp8_kernel<T, false>), grid, dim3(PShape::threads), 0, st, a);
+    rows(std::false_type());
     return hipGetLastError();
   }
   grid.z *= (unsigned)a.splits;
-  hipLaunchKernelGGL((prefill_fp8_kernel<T, true>), grid, dim3(PShape::threads), 0, st, a);
+  rows(std::true_type());
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   // the tokens of a sequence that the grid covers
@@ -761,9 +775,13 @@ extern "C" size_t mskv_fp8_prefill_workspace_bytes(int num_seqs, int64_t total_q
                                                   max_blocks_per_seq);
 }
 
-extern "C" int mskv_fp8_prefill_attention_bounded(
+namespace mskv {
+
+// Validates a prefill call over either cache and launches it.
+template <bool kFp4>
+static int prefill_checked(
     const void* query, const void* k_cache, const void* v_cache,
-    const float* k_scale_cache, const float* v_scale_cache,
+    const void* k_scale_cache, const float* v_scale_cache,
     const int32_t* block_tables, const int32_t* cu_seqlens_q,
     const int32_t* cu_seqlens_k, int prefix_len, void* out, int num_seqs,
     int64_t total_q, int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads, int num_kv_heads,
@@ -780,9 +798,9 @@ extern "C" int mskv_fp8_prefill_attention_bounded(
   if (cu_seqlens_q == nullptr && num_seqs != 1) return MSKV_EINVAL;
   if (cu_seqlens_q == nullptr && total_q > 0x7FFFFFFFLL - prefix_len) return MSKV_EINVAL;
   const int group = num_q_heads / num_kv_heads;
-  if (head_dim != mskv::kHeadDim || block_size % mskv::kPStep != 0) return MSKV_EUNSUPPORTED;
+  if (head_dim != kHeadDim || block_size % kPStep != 0) return MSKV_EUNSUPPORTED;
   // the row maxima are taken before the scale, which must keep their order
-  const float scale_log2 = softmax_scale * mskv::kLog2e;
+  const float scale_log2 = softmax_scale * kLog2e;
   if (!(scale_log2 > 0.0f && scale_log2 < INFINITY)) return MSKV_EUNSUPPORTED;
   if ((int64_t)block_size * num_kv_heads * head_dim > 0x7FFFFFFFLL) return MSKV_EUNSUPPORTED;
   if (num_seqs == 0 || total_q == 0 || max_seqlen_q == 0) return MSKV_OK;
@@ -790,11 +808,11 @@ extern "C" int mskv_fp8_prefill_attention_bounded(
       !block_tables || !out)
     return MSKV_EINVAL;
 
-  mskv::PrefillArgs a;
+  PrefillArgs a;
   a.q = (const uint16_t*)query;
   a.kc = (const uint8_t*)k_cache;
   a.vc = (const uint8_t*)v_cache;
-  a.ks = k_scale_cache;
+  a.ks = (const float*)k_scale_cache;
   a.vs = v_scale_cache;
   a.bt = block_tables;
   a.cu_q = cu_seqlens_q;
@@ -817,8 +835,9 @@ extern "C" int mskv_fp8_prefill_attention_bounded(
   // grid y and z are limited to 65535
   const int64_t qblocks = ((int64_t)max_seqlen_q + per_wg - 1) / per_wg;
   if (num_seqs > 65535 || qblocks > 65535) return MSKV_EUNSUPPORTED;
-  // rows go to LDS directly, 16 bytes a lane
-  if (mskv::misaligned({query, k_cache, v_cache, out, workspace})) return MSKV_EINVAL;
+  // rows go to LDS directly, 16 bytes a lane (scales four)
+  if (misaligned({query, k_cache, v_cache, out, workspace})) return MSKV_EINVAL;
+  if (kFp4 && ((uintptr_t)k_scale_cache | (uintptr_t)v_scale_cache) % 4) return MSKV_EINVAL;
   // without a workspace, one workgroup walks all the keys of its rows
   a.splits = 1;
   a.part_o = a.part_lse = nullptr;
@@ -828,7 +847,7 @@ extern "C" int mskv_fp8_prefill_attention_bounded(
         block_size, max_blocks_per_seq);
     if (workspace_bytes < need) return MSKV_EWORKSPACE;
     if (need > 0) {
-      a.splits = mskv::prefill_splits(num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads,
+      a.splits = prefill_splits(num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads,
                                       num_kv_heads, block_size, max_blocks_per_seq);
       a.part_o = (float*)workspace;
       a.part_lse = a.part_o + (size_t)total_q * num_q_heads * a.splits * head_dim;
@@ -836,8 +855,42 @@ extern "C" int mskv_fp8_prefill_attention_bounded(
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (act_dtype == MSKV_BFLOAT16)
-    return (int)mskv::launch_prefill<__bf16>(a, num_seqs, qblocks, s);
-  return (int)mskv::launch_prefill<_Float16>(a, num_seqs, qblocks, s);
+    return (int)launch_prefill<__bf16, kFp4>(a, num_seqs, qblocks, s);
+  return (int)launch_prefill<_Float16, kFp4>(a, num_seqs, qblocks, s);
+}
+
+}  // namespace mskv
+
+extern "C" int mskv_fp8_prefill_attention_bounded(
+    const void* query, const void* k_cache, const void* v_cache,
+    const float* k_scale_cache, const float* v_scale_cache,
+    const int32_t* block_tables, const int32_t* cu_seqlens_q,
+    const int32_t* cu_seqlens_k, int prefix_len, void* out, int num_seqs,
+    int64_t total_q, int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads, int num_kv_heads,
+    int head_dim, int block_size, int64_t num_blocks, int max_blocks_per_seq,
+    float softmax_scale, int act_dtype, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  return mskv::prefill_checked<false>(
+      query, k_cache, v_cache, k_scale_cache, v_scale_cache, block_tables, cu_seqlens_q,
+      cu_seqlens_k, prefix_len, out, num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads,
+      num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq, softmax_scale, act_dtype,
+      workspace, workspace_bytes, stream);
+}
+
+extern "C" int mskv_fp4_prefill_attention(
+    const void* query, const void* k_cache, const void* v_cache,
+    const void* k_scale_cache, const float* v_scale_cache,
+    const int32_t* block_tables, const int32_t* cu_seqlens_q,
+    const int32_t* cu_seqlens_k, int prefix_len, void* out, int num_seqs,
+    int64_t total_q, int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads, int num_kv_heads,
+    int head_dim, int block_size, int64_t num_blocks, int max_blocks_per_seq,
+    float softmax_scale, int act_dtype, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  return mskv::prefill_checked<true>(
+      query, k_cache, v_cache, k_scale_cache, v_scale_cache, block_tables, cu_seqlens_q,
+      cu_seqlens_k, prefix_len, out, num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads,
+      num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq, softmax_scale, act_dtype,
+      workspace, workspace_bytes, stream);
 }
 
 extern "C" int mskv_fp8_prefill_attention_ws(

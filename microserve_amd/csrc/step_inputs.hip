@@ -110,3 +110,5 @@ extern "C" int mskv_build_step_inputs(
                      reinterpret_cast<hipStream_t>(stream), a);
   return (int)hipGetLastError();
 }
+
+#include "kv_blocks.h"

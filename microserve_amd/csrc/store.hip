@@ -169,3 +169,5 @@ extern "C" int mskv_store_fp8_kvcache(const void* key, const void* value,
                                         v_scale_cache, slot_mapping, slot_dtype, num_tokens,
                                         num_kv_heads, head_dim, num_slots, act_dtype, stream);
 }
+
+#include "fp4_store.h"
