@@ -46,20 +46,32 @@ __device__ __forceinline__ f32x4 mfma_fp4(const u32x4& k, uint32_t ks, const i32
                                                           kByte, (int)ks, 0, 127);
 }
 
+// The pieces of a query row that lane (g, n) holds in the B operand: the e4m3
+// operand's bytes 0-15 meet the dimensions [16g, 16g + 16) and its bytes 16-31
+// [64 + 16g, 80 + 16g).
+struct QueryRow {
+  u32x4 v[4];
+};
+__device__ __forceinline__ QueryRow load_query(const uint16_t* row, int g) {
+  QueryRow q;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    q.v[c] = *reinterpret_cast<const u32x4*>(row + 64 * (c >> 1) + 16 * g + 8 * (c & 1));
+  return q;
+}
+
 // The query row of lane (g, n) as the B operand: e4m3 parts of q * f, f the
 // power of two that brings the row's largest magnitude near e4m3's (q * f is
-// exact).  The e4m3 operand's bytes 0-15 meet the dimensions [16g, 16g + 16)
-// and its bytes 16-31 [64 + 16g, 80 + 16g).  Returns f; NaNs for a
-// row that holds an infinity or a NaN, zeros where !ok.
+// exact).  Returns f; NaNs for a row that holds an infinity or a NaN, zeros
+// where !ok.
 template <typename T>
-__device__ __forceinline__ float fp4_query(const uint16_t* row, bool ok, int g,
+__device__ __forceinline__ float fp4_query(const QueryRow& row, bool ok,
                                            i32x8 (&qp)[Fp4Query<T>::parts]) {
   using A = Act<T>;
   float x[32];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (ok) v = *reinterpret_cast<const u32x4*>(row + 64 * (c >> 1) + 16 * g + 8 * (c & 1));
+    const u32x4 v = ok ? row.v[c] : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[8 * c + 2 * i] = A::to_f32((uint16_t)(v[i] & 0xFFFFu));

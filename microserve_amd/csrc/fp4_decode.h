@@ -28,30 +28,27 @@ struct Fp4Loads {
 struct Fp4Cache {
   static constexpr int kUnit = 64;
   static constexpr int kPageUnit = 128;  // as the prefill's tiles
+  // a token whose bytes (64 a token, 31 bits) lie past the end of any page
+  static constexpr uint32_t kPastEnd = (1u << 25) - kUnit;
   typedef uint8_t Tiles[2][kUnit * kFp4Row];  // V, double-buffered
   typedef float Scales[2][kUnit];             // v_scale * f
 
-  // Issues the loads of the step at token t0, whose page holds block `blk`.
-  // An invalid block is read through zero-length resources.
-  static __device__ __forceinline__ void load(const DecodeArgs& a, int blk, int kvh, int t0,
-                                              int t_end, int lane, Fp4Loads& s) {
-    const int off = t0 % a.bs;
-    const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
-    const int64_t row = ((ok ? (int64_t)blk : 0) * a.hk + kvh) * a.bs;
-    const uint32_t bytes = ok ? (uint32_t)a.bs * kFp4Row : 0u;
-    const uint32_t sbytes = ok ? (uint32_t)a.bs * 4u : 0u;
-    const auto kr = make_rsrc(a.kc + row * kFp4Row, bytes);
-    const auto vr = make_rsrc(a.vc + row * kFp4Row, bytes);
-    const auto ksr = make_rsrc(a.ks + row, sbytes);
-    const auto vsr = make_rsrc(a.vs + row, sbytes);
-    const uint32_t o = (uint32_t)off * kFp4Row + 16u * lane;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) s.k[c] = buf_load16_nt(kr, o + 1024u * c);
-    s.kscale = __float_as_uint(buf_load_f32(ksr, ((uint32_t)off + lane) * 4u));
-#pragma unroll
-    for (int c = 0; c < 4; ++c) s.v[c] = buf_load16_nt(vr, o + 1024u * c);
-    s.vscale = buf_load_f32(vsr, ((uint32_t)off + lane) * 4u);
-    s.valid = ok ? min(kUnit, t_end - t0) : 0;
+  // The page that loads are issued from: four resources of one kv head's rows
+  // (zero-length for an invalid block), and the next step's place in it.
+  struct Page {
+    __amdgpu_buffer_rsrc_t k, v, ks, vs;
+    bool ok;
+    int off, index;
+  };
+  static __device__ __forceinline__ void open(const DecodeArgs& a, int blk, int kvh, Page& p) {
+    p.ok = blk >= 0 && (int64_t)blk < a.num_blocks;
+    const int64_t row = ((p.ok ? (int64_t)blk : 0) * a.hk + kvh) * a.bs;
+    const uint32_t bytes = p.ok ? (uint32_t)a.bs * kFp4Row : 0u;
+    const uint32_t sbytes = p.ok ? (uint32_t)a.bs * 4u : 0u;
+    p.k = make_rsrc(a.kc + row * kFp4Row, bytes);
+    p.v = make_rsrc(a.vc + row * kFp4Row, bytes);
+    p.ks = make_rsrc(a.ks + row, sbytes);
+    p.vs = make_rsrc(a.vs + row, sbytes);
   }
 
   template <typename T>
@@ -62,10 +59,52 @@ struct Fp4Cache {
                                                 float& l) {
     constexpr int NQ = Fp4Query<T>::parts;
     const int g = lane >> 4;
+    // (a wave's own: the compiler takes it to differ from lane to lane)
+    kvh = __builtin_amdgcn_readfirstlane(kvh);
+    // the block table is read-only: the constant address space keeps its
+    // loads scalar
+    const auto* table = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
+        reinterpret_cast<uintptr_t>(a.bt + (int64_t)b * a.w));
+    Page page;
+    page.index = t_begin / a.bs;
+    page.off = t_begin - page.index * a.bs;
+    open(a, blk_first, kvh, page);
+    // the block after it, read a page ahead
+    int blk_next = table[min(page.index + 1, a.w - 1)];
+    // Issues the loads of the step at token t0; steps come in order.  Past the
+    // end every offset is out of range: the loads read nothing, but they are
+    // always issued, so that the waits for the loads before them can be counted.
+    auto issue = [&](int t0, Fp4Loads& s) {
+      const bool more = t0 < t_end;
+      if (more && page.off == a.bs) {
+        page.off = 0;
+        open(a, blk_next, kvh, page);
+        blk_next = table[min(++page.index + 1, a.w - 1)];
+      }
+      const uint32_t at = more ? (uint32_t)page.off : kPastEnd;
+      const uint32_t o = at * kFp4Row + 16u * lane;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s.k[c] = buf_load16_nt(page.k, o + 1024u * c);
+      const uint32_t so = (at + lane) * 4u;
+      s.kscale = __float_as_uint(buf_load_f32(page.ks, so));
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s.v[c] = buf_load16_nt(page.v, o + 1024u * c);
+      s.vscale = buf_load_f32(page.vs, so);
+      s.valid = page.ok ? max(min(kUnit, t_end - t0), 0) : 0;
+      page.off += kUnit;
+    };
+    // (the query's row first: waiting for it is then no wait for the steps')
+    const QueryRow row = load_query(
+        a.q + ((int64_t)b * a.hq + (head_ok ? qh : kvh * a.group)) * kHeadDim, g);
+    // Two steps are in flight: the loads of step i + 2 go into the registers
+    // of step i once its products are issued (its V lies in LDS by then).
+    Fp4Loads even, odd;
+    issue(t_begin, even);
+    issue(t_begin + kUnit, odd);
+
     i32x8 qp[NQ];
     // scores in log2 units: S^T * qs
-    const float qs =
-        a.scale_log2 / fp4_query<T>(a.q + ((int64_t)b * a.hq + qh) * kHeadDim, head_ok, g, qp);
+    const float qs = a.scale_log2 / fp4_query<T>(row, head_ok, qp);
 
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -100,17 +139,9 @@ struct Fp4Cache {
     };
 
     const uint32_t vrow = fp4_v_row(lane);
-    Fp4Loads cur, nxt;
-    load(a, blk_first, kvh, t_begin, t_end, lane, cur);
-    stage(cur, 0);
-    wave_lds_sync();
-    int buf = 0;
-    for (int t0 = t_begin; t0 < t_end; t0 += kUnit, buf ^= 1) {
+    // step i, whose V is in buffer `buf`; `cur` holds its K, `nxt` step i + 1
+    auto step = [&](int t0, int buf, Fp4Loads& cur, Fp4Loads& nxt, auto last) {
       const int valid = cur.valid;
-      const bool more = t0 + kUnit < t_end;
-      if (more)
-        load(a, a.bt[(int64_t)b * a.w + (t0 + kUnit) / a.bs], kvh, t0 + kUnit, t_end, lane, nxt);
-
       // lane (g, n): scores of tokens 16c + 4g + r of head n
       f32x4 s[4];
       const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -124,6 +155,12 @@ struct Fp4Cache {
         s[1] = mfma_fp4<1>(cur.k[1], cur.kscale, qp[p], s[1]);
         s[2] = mfma_fp4<2>(cur.k[2], cur.kscale, qp[p], s[2]);
         s[3] = mfma_fp4<3>(cur.k[3], cur.kscale, qp[p], s[3]);
+      }
+      // (not before the products: the loads would take other registers, and
+      // moving those at the loop's end would wait for them)
+      if constexpr (!decltype(last)::value) {
+        __builtin_amdgcn_sched_barrier(0);
+        issue(t0 + 2 * kUnit, cur);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) s[c] *= qs;
@@ -175,12 +212,22 @@ struct Fp4Cache {
         acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp4x8_to_f16((uint32_t)raw[1]), pt[1],
                                                          acc[dt], 0, 0, 0);
       }
-      if (more) {
-        stage(nxt, buf ^ 1);
-        cur = nxt;
+      if constexpr (!decltype(last)::value) {
+        stage(nxt, buf ^ 1);  // (past the end: nothing, as it was loaded)
+        wave_lds_sync();
       }
-      wave_lds_sync();
+    };
+
+    stage(even, 0);
+    wave_lds_sync();
+    // (the last step of an odd number after the loop: a way out of its middle
+    // would also lose the count of the loads in flight)
+    int t0 = t_begin;
+    for (; t0 + kUnit < t_end; t0 += 2 * kUnit) {
+      step(t0, 0, even, odd, std::false_type());
+      step(t0 + kUnit, 1, odd, even, std::false_type());
     }
+    if (t0 < t_end) step(t0, 0, even, odd, std::true_type());
     l = sum_xor32(sum_xor16(l));
     if (f != 0.0f) {
       const float inv_f = 1.0f / f;  // a power of two: exact

@@ -120,8 +120,8 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
     row_ok[b] = n < a.tpr * a.gc && qi < lq && qgi * 16 + n - nq * a.gc < a.group;
     qh[b] = kvh * a.group + qgi * 16 + n - nq * a.gc;
     lim[b] = row_ok[b] ? prefix + qi + 1 : 0;
-    qs[b] = a.scale_log2 / fp4_query<T>(
-        a.q + ((int64_t)(q_begin + qi) * a.hq + qh[b]) * kHeadDim, row_ok[b], g, qp[b]);
+    const int64_t row = row_ok[b] ? (int64_t)(q_begin + qi) * a.hq + qh[b] : 0;
+    qs[b] = a.scale_log2 / fp4_query<T>(load_query(a.q + row * kHeadDim, g), row_ok[b], qp[b]);
   }
 
   // acc: O^T in units of fw, the power-of-two scale applied to v_scale (0
