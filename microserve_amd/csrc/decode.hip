@@ -164,7 +164,8 @@ __device__ __forceinline__ int wave_max_u31(int v) {  // of values >= 0
   return max((int)r32[0], (int)r32[1]);
 }
 
-// (kUnit: tokens of one step of the kernel that the rule is for)
+// (kUnit: tokens of one step of the kernel that the rule is for, 32 or the
+// 4-bit walk's 64, of which a split may hold one)
 template <int kUnit>
 __device__ __forceinline__ int steps_of_length(int len, const SplitRule& r) {
   return (max(0, min(len, r.max_tokens)) + kUnit - 1) / kUnit;
@@ -175,7 +176,7 @@ __device__ __forceinline__ int steps_of_length(int len, const SplitRule& r) {
 template <int kUnit>
 __device__ __forceinline__ int split_tokens_from(int steps, int longest, const SplitRule& r) {
   const int per = max((int)ceilf(fmaxf((float)steps * r.inv_slots, (float)longest * r.inv_splits)),
-                      kMinSplitSteps);
+                      kUnit == kStep ? kMinSplitSteps : 1);
   const bool whole = longest * kUnit <= r.fixed && longest - per < r.min_gain;
   return min((whole ? max(longest, per) : per) * kUnit, r.fixed);
 }
@@ -466,6 +467,9 @@ __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh
 struct Fp8Cache {
   static constexpr int kUnit = kStep;
   static constexpr int kPageUnit = kStep;  // a page is a multiple of it
+  static constexpr int kMaxPages = kMaxPagesPerSplit;
+  static constexpr int kMinSteps = kMinSplitSteps;
+  static constexpr int kItemWaves = kWavesPerWG;  // of a workgroup that takes work items
   typedef uint8_t Tiles[2][2][kStep * kHeadDim];  // K and V, double-buffered
   typedef float Scales[2][2 * kStep];
   template <typename T>
@@ -1045,7 +1049,7 @@ static hipError_t launch_decode(const DecodeArgs& a, int batch, hipStream_t stre
     // 8-wave workgroups also run the work items when every wave has a unit:
     // with the short sequences last, their longer units no longer lengthen
     // the tail (ragged batch 256: 425-426 against 433-435 us with 4 waves).
-    const bool wide = units >= kWavesPerWG;
+    const bool wide = Cache::kItemWaves == kWavesPerWG && units >= kWavesPerWG;
     const int per_wg = wide ? kWavesPerWG : kNarrowWaves;
     const dim3 grid((unsigned)((units + per_wg - 1) / per_wg), (unsigned)a.splits,
                     (unsigned)batch);
@@ -1054,12 +1058,13 @@ static hipError_t launch_decode(const DecodeArgs& a, int batch, hipStream_t stre
                        a.rule);
     const hipError_t eo = hipGetLastError();
     if (eo != hipSuccess) return eo;
-    if (wide)
-      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kItems, Cache>()), grid, dim3(64 * kWavesPerWG),
-                         0, stream, a);
-    else
-      hipLaunchKernelGGL((split_kernel<T, kNarrowWaves, kItems, Cache>()), grid,
-                         dim3(64 * kNarrowWaves), 0, stream, a);
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(64 * per_wg), 0, stream, a);
+    };
+    if constexpr (Cache::kItemWaves == kWavesPerWG) {
+      if (wide) run(split_kernel<T, kWavesPerWG, kItems, Cache>());
+    }
+    if (!wide) run(split_kernel<T, kNarrowWaves, kItems, Cache>());
   } else if (wide_wgs <= kWideGridMax) {
     dim3 grid((unsigned)((units + kWavesPerWG - 1) / kWavesPerWG), (unsigned)a.splits,
               (unsigned)batch);
@@ -1104,10 +1109,9 @@ static int pages_per_split_of(int splits, int w) {
   return splits <= 1 ? w : (w + splits - 1) / splits;
 }
 
-// `step`: tokens of one step of the kernel, kMinSplitSteps of which are the
-// least of a split
+template <typename Cache>
 static int num_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_blocks_per_seq,
-                         int block_size, int step) {
+                         int block_size) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
       max_blocks_per_seq <= 0)
     return 1;
@@ -1116,7 +1120,7 @@ static int num_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_b
   const int w = max_blocks_per_seq;
   int64_t pps = (w * base + kTargetWaves - 1) / kTargetWaves;
   if (pps < 1) pps = 1;
-  if (pps > kMaxPagesPerSplit) pps = kMaxPagesPerSplit;
+  if (pps > Cache::kMaxPages) pps = Cache::kMaxPages;
   int64_t splits = (w + pps - 1) / pps;
   // A page per split leaves half the waves idle: finer splits, of two steps at
   // least, as long as the partials stay small and the grid is one workgroup
@@ -1133,7 +1137,7 @@ static int num_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_b
   if (splits > 1 && 2 * w * base <= kTargetWaves && block_size > 0 &&
       (int64_t)w * block_size <= kFollowMaxTokens) {
     const int64_t per = (base / batch + kWavesPerWG - 1) / kWavesPerWG * batch;
-    int64_t fine = (int64_t)w * block_size / (kMinSplitSteps * step);
+    int64_t fine = (int64_t)w * block_size / (Cache::kMinSteps * Cache::kUnit);
     fine = std::min(fine, kWideGridMax / 2 / per);
     fine = std::min(fine, (int64_t)(kFinePartialBytes /
                                     ((int64_t)batch * num_q_heads * (kHeadDim + 1) * 4)));
@@ -1147,14 +1151,14 @@ static int num_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_b
 extern "C" int mskv_decode_num_splits(int batch, int num_q_heads,
                                       int num_kv_heads, int max_blocks_per_seq,
                                       int block_size) {
-  return mskv::num_splits_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size,
-                             mskv::Fp8Cache::kUnit);
+  return mskv::num_splits_of<mskv::Fp8Cache>(batch, num_q_heads, num_kv_heads,
+                                             max_blocks_per_seq, block_size);
 }
 
 extern "C" int mskv_fp4_decode_num_splits(int batch, int num_q_heads, int num_kv_heads,
                                           int max_blocks_per_seq, int block_size) {
-  return mskv::num_splits_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size,
-                             mskv::Fp4Cache::kUnit);
+  return mskv::num_splits_of<mskv::Fp4Cache>(batch, num_q_heads, num_kv_heads,
+                                             max_blocks_per_seq, block_size);
 }
 
 extern "C" size_t mskv_decode_workspace_bytes(int batch, int num_q_heads,
@@ -1196,8 +1200,8 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
   // table's width (w * block_size + split_tokens) stay within int
   if ((int64_t)block_size * num_kv_heads * head_dim > 0x7FFFFFFFLL) return MSKV_EUNSUPPORTED;
   if ((int64_t)max_blocks_per_seq * block_size >= (1LL << 30)) return MSKV_EUNSUPPORTED;
-  if (num_splits != num_splits_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size,
-                                  Cache::kUnit))
+  if (num_splits != num_splits_of<Cache>(batch, num_q_heads, num_kv_heads, max_blocks_per_seq,
+                                         block_size))
     return MSKV_EINVAL;
   if (batch == 0) return MSKV_OK;
   if (!query || !k_cache || !v_cache || !k_scale_cache || !v_scale_cache ||

@@ -28,6 +28,16 @@ struct Fp4Loads {
 struct Fp4Cache {
   static constexpr int kUnit = 64;
   static constexpr int kPageUnit = 128;  // as the prefill's tiles
+  // A split of a grid of many rounds holds twice the FP8 cache's pages, its
+  // bytes, and a workgroup of work items half the waves (two workgroups a CU,
+  // whose starts and ends overlap).  At 4 pages and 8 waves / 8 and 8 / 8 and
+  // 4 / 16 and 4, us: 256 x 16 to 32768 tokens 217 / 215 / 208 / 209, 128 x
+  // 8192 200 / 190 / 192 / 186, 256 x 16 to 8192 76 to 82 / 80 / 75 / 160.
+  static constexpr int kMaxPages = 8;
+  // one step is the least of a split: 1 x 700 tokens 10.0 us (two steps 11.8),
+  // 8 x 1000 10.4 (12.1)
+  static constexpr int kMinSteps = 1;
+  static constexpr int kItemWaves = kNarrowWaves;
   // a token whose bytes (64 a token, 31 bits) lie past the end of any page
   static constexpr uint32_t kPastEnd = (1u << 25) - kUnit;
   typedef uint8_t Tiles[2][kUnit * kFp4Row];  // V, double-buffered
