@@ -113,6 +113,86 @@ __device__ __forceinline__ float fp4_query(const QueryRow& row, bool ok,
   return f;
 }
 
+// The query in e2m3 parts, for the prefill: against codes, a 6-bit operand runs
+// at 1.6 times e4m3's rate (9.5 and 15.2 ns an MFMA and SIMD), and three of its
+// 4 significant bits hold fp16's 11 as three of e4m3 do.
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+constexpr int kQ6Parts = 3;
+
+template <int kByte, int kPart>
+__device__ __forceinline__ f32x4 mfma_fp4_q6(const u32x4& k, uint32_t ks, const u32x6& q,
+                                             uint32_t qscale, f32x4 c) {
+  const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+  const i32x8 b = {(int)q[0], (int)q[1], (int)q[2], (int)q[3], (int)q[4], (int)q[5], 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4 /* fp4 */, 2 /* e2m3 */,
+                                                          kByte, (int)ks, kPart, (int)qscale);
+}
+
+// The pieces of a query row that lane (g, n) holds in the e2m3 operand: the
+// dimensions [32g, 32g + 32), K's own blocks.
+__device__ __forceinline__ QueryRow load_query6(const uint16_t* row, int g) {
+  QueryRow q;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) q.v[c] = *reinterpret_cast<const u32x4*>(row + 32 * g + 8 * c);
+  return q;
+}
+
+// e2m3 parts of the lane's block under scales 2^e, 2^(e-4) and 2^(e-9) (bytes 0, 1
+// and 2 of the returned word), e the smallest with every magnitude at most 7.5 *
+// 2^e.  A part leaves at most a quarter of 2^e, then 2^(e-7); the third's step
+// is 2^(e-12) at most, and finer where the rest is small: only elements below
+// 2^-5 of the block's largest binade lose bits of fp16, at most 2^(e-13).
+// Blocks with an infinity or a NaN get a NaN scale, zeros come out where !ok.
+template <typename T>
+__device__ __forceinline__ uint32_t fp4_query6(const QueryRow& row, bool ok,
+                                               u32x6 (&qp)[kQ6Parts]) {
+  typedef T x32 __attribute__((ext_vector_type(32)));
+  typedef float f32x16 __attribute__((ext_vector_type(16)));
+  typedef float f32x32 __attribute__((ext_vector_type(32)));
+  typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
+  u32x16 w;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    w[i] = ok ? row.v[i >> 2][i & 3] : 0u;
+    // (fp16 and bf16 both order as their bits; a NaN is above infinity)
+    top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+  }
+  const uint32_t bits = __float_as_uint(Act<T>::to_f32((uint16_t)top));
+  // 1.875 * 2^floor and up start the next power of two
+  const uint32_t e = (uint32_t)max((int)((bits + 0x100000u) >> 23) - 2, 16);
+  const float s0 = __uint_as_float(e << 23), s1 = __uint_as_float((e - 4) << 23),
+              s2 = __uint_as_float((e - 9) << 23);
+  const x32 x = __builtin_bit_cast(x32, w);
+  // (The wide converts write their result while they still read: keeping the
+  // sources live past them keeps the result out of the sources' registers.)
+  if constexpr (Act<T>::kId == 1)
+    qp[0] = __builtin_amdgcn_cvt_scalef32_pk32_fp6_bf16(x, s0);
+  else
+    qp[0] = __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(x, s0);
+  asm volatile("" ::"v"(x), "v"(qp[0]));
+  f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(qp[0], s0);
+  asm volatile("" ::"v"(qp[0]), "v"(back));
+  f32x16 even, odd;  // (the fp32 convert interleaves its two sources)
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    even[i] = Act<T>::to_f32((uint16_t)(w[i] & 0xFFFFu)) - back[2 * i];
+    odd[i] = Act<T>::to_f32((uint16_t)(w[i] >> 16)) - back[2 * i + 1];
+  }
+  qp[1] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s1);
+  asm volatile("" ::"v"(even), "v"(odd), "v"(qp[1]));
+  back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(qp[1], s1);
+  asm volatile("" ::"v"(qp[1]), "v"(back));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    even[i] -= back[2 * i];
+    odd[i] -= back[2 * i + 1];
+  }
+  qp[2] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s2);
+  asm volatile("" ::"v"(even), "v"(odd), "v"(qp[2]));
+  return bits >= 0x7F800000u ? 0xFFFFFFu : e | (e - 4) << 8 | (e - 9) << 16;
+}
+
 // eight codes (a dword) -> eight exact fp16 values
 __device__ __forceinline__ f16x8 fp4x8_to_f16(uint32_t w) {
   f16x8 r;

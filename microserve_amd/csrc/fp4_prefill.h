@@ -10,8 +10,9 @@
 //    order that it has in memory and read back 16 bytes a lane, free of
 //    bank conflicts.
 //  * QK^T: v_mfma_scale_f32_16x16x128_f8f6f4 takes the codes and their block
-//    scales as stored, and the query in e4m3 parts; the scores need no
-//    scaling by key.
+//    scales as stored, and the query in three e2m3 parts under scales of their
+//    own; the scores need no scaling by key.  (Two e4m3 parts of a bf16 query
+//    took the same time, three of an fp16 one 9% more of the whole kernel.)
 //  * PV: v_mfma_f32_16x16x32_f16; V^T from ds_read_b64_tr_b4 converts to fp16
 //    exactly; weights fp16(p) * fp16(v_scale * fw) as in the FP8 kernel.
 #pragma once
@@ -27,7 +28,6 @@ template <int N> using Int = std::integral_constant<int, N>;
 template <typename T, bool kSplit>
 __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(PrefillArgs a) {
   using A = Act<T>;
-  constexpr int NQ = Fp4Query<T>::parts;
   constexpr int kPBlocks = PShape::blocks;
   constexpr int kPWaves = PShape::waves;
   // two tile buffers as separate objects, and a loop unrolled by two, as in
@@ -109,8 +109,8 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
   int lim[kPBlocks];
   bool row_ok[kPBlocks];
   int qh[kPBlocks];
-  i32x8 qp[kPBlocks][NQ];
-  float qs[kPBlocks];
+  u32x6 qp[kPBlocks][kQ6Parts];
+  uint32_t qe[kPBlocks];  // the parts' scale bytes
 #pragma unroll
   for (int b = 0; b < kPBlocks; ++b) {
     const int nq = (n * a.gc_magic) >> 8;  // n / gc
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
     qh[b] = kvh * a.group + qgi * 16 + n - nq * a.gc;
     lim[b] = row_ok[b] ? prefix + qi + 1 : 0;
     const int64_t row = row_ok[b] ? (int64_t)(q_begin + qi) * a.hq + qh[b] : 0;
-    qs[b] = a.scale_log2 / fp4_query<T>(load_query(a.q + row * kHeadDim, g), row_ok[b], qp[b]);
+    qe[b] = fp4_query6<T>(load_query6(a.q + row * kHeadDim, g), row_ok[b], qp[b]);
   }
 
   // acc: O^T in units of fw, the power-of-two scale applied to v_scale (0
@@ -196,10 +196,11 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
         const u32x4 ka = *reinterpret_cast<const u32x4*>(kt + 1024 * tt + 16 * lane);
 #pragma unroll
         for (int b = 0; b < kPBlocks; ++b) {
+          const uint32_t ks = tt < 4 ? ks0 : ks1;
           f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int p = 0; p < NQ; ++p) c = mfma_fp4<tt & 3>(ka, tt < 4 ? ks0 : ks1, qp[b][p], c);
-          st[b][tt] = c;
+          c = mfma_fp4_q6<tt & 3, 0>(ka, ks, qp[b][0], qe[b], c);
+          c = mfma_fp4_q6<tt & 3, 1>(ka, ks, qp[b][1], qe[b], c);
+          st[b][tt] = mfma_fp4_q6<tt & 3, 2>(ka, ks, qp[b][2], qe[b], c);
         }
       };
       qk(Int<0>()), qk(Int<1>()), qk(Int<2>()), qk(Int<3>());
@@ -238,12 +239,12 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
         for (int tt = 1; tt < 8; ++tt)
           v = fmaxf(fmaxf(v, st[b][tt][0]), fmaxf(fmaxf(st[b][tt][1], st[b][tt][2]), st[b][tt][3]));
         lm[b] = v;
-        grow |= v * qs[b] > m[b] + kPSlack;
+        grow |= v * a.scale_log2 > m[b] + kPSlack;
       }
       if (__any(grow)) {
 #pragma unroll
         for (int b = 0; b < kPBlocks; ++b) {
-          const float m_new = fmaxf(m[b], max_xor32(max_xor16(lm[b])) * qs[b]);
+          const float m_new = fmaxf(m[b], max_xor32(max_xor16(lm[b])) * a.scale_log2);
           const float alpha = exp2_fast(m[b] - m_new);
           lacc[b] *= alpha;
 #pragma unroll
@@ -313,7 +314,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
           for (int b = 0; b < kPBlocks; ++b) {
             float pf[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) pf[r] = exp2_fast(fmaf(st[b][tt][r], qs[b], -m[b]));
+            for (int r = 0; r < 4; ++r) pf[r] = exp2_fast(fmaf(st[b][tt][r], a.scale_log2, -m[b]));
             const f16x2 p01 = {(_Float16)pf[0], (_Float16)pf[1]};
             const f16x2 p23 = {(_Float16)pf[2], (_Float16)pf[3]};
             const f16x2 w01 = p01 * f16x2{vf[0], vf[1]};

@@ -64,13 +64,15 @@ def check(got, want, weight, reach, dtype, keys, vmax, weights):
       (prefill, twice: the sum and the denominator) or of a unit in which the
       largest v_scale is at least 64 (decode), times a code of at most 6: no
       more than 6 vmax 2^-24 a key;
-    * the scores: the e4m3 parts of the query leave at most 2^-10 of a unit in
-      which its largest element is at least 224, 2^-17.8 of it a dimension;
-      the product's fp32 sum of 128 x 3 terms at most 384 x 2^-24: together
-      2^-15 of reach; the scale and the maximum's subtraction 2^-22 of reach.
-      Each moves a weight, and the denominator, by that much relatively;
+    * the scores: the query's parts leave at most 2^-10 of a unit in which its
+      largest element is at least 224, 2^-17.8 of it a dimension (decode,
+      e4m3), or 2^-13 of one in which its block's largest is at least 3.75,
+      2^-14.9 (prefill, e2m3); the product's fp32 sum of 128 x 3 terms at most
+      384 x 2^-24: together 2^-14 of reach; the scale and the maximum's
+      subtraction 2^-22 of reach.  Each moves a weight, and the denominator,
+      by that much relatively;
     * exp2, the sums over the keys and the merge of the splits: 2^-18."""
-    rel = weights * 2.0 ** -11 + 2 * reach * (2.0 ** -15 + 2.0 ** -22) + 2.0 ** -18
+    rel = weights * 2.0 ** -11 + 2 * reach * (2.0 ** -14 + 2.0 ** -22) + 2.0 ** -18
     tol = rel[..., None] * weight + keys * 6 * vmax * 2.0 ** -24
     tol = tol + torch.finfo(dtype).eps / 2 * (np.abs(want) + tol) + 1e-30
     err = np.abs(got.double().cpu().numpy() - want)
