@@ -23,23 +23,39 @@ namespace mskv {
 
 template <int N> using Int = std::integral_constant<int, N>;
 
+#ifndef FB
+#define FB 2
+#define FK 128
+#define FO 2
+#endif
+struct Fp4Shape {
+  static constexpr int blocks = FB;     // 16-row blocks per wave
+  static constexpr int keys = FK;     // per tile
+  static constexpr int occupancy = FO;  // waves per SIMD
+};
+
 // kSplit: the workgroup takes one of a.splits ranges of the keys (whole
 // tiles, from the actual key count) and leaves partials for the merge.
-template <typename T, bool kSplit>
-__global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(PrefillArgs a) {
+template <typename T, bool kSplit, typename Shape>
+__global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4_kernel(
+    PrefillArgs a) {
   using A = Act<T>;
-  constexpr int kPBlocks = PShape::blocks;
+  constexpr int kPBlocks = Shape::blocks;
   constexpr int kPWaves = PShape::waves;
+  constexpr int kKeys = Shape::keys;         // of a tile
+  constexpr int kGroups = kKeys / 16;        // S^T tiles
+  constexpr int kChunks = kKeys / 32;        // P^T chunks
+  constexpr int kHalves = kKeys / 64;        // V^T reads
   // two tile buffers as separate objects, and a loop unrolled by two, as in
   // the FP8 kernel: direct loads into one then never alias the other's reads
-  __shared__ __attribute__((aligned(16))) uint8_t k_lds0[kPStep * kFp4Row];
-  __shared__ __attribute__((aligned(16))) uint8_t v_lds0[kPStep * kFp4Row];
-  __shared__ __attribute__((aligned(16))) uint8_t k_lds1[kPStep * kFp4Row];
-  __shared__ __attribute__((aligned(16))) uint8_t v_lds1[kPStep * kFp4Row];
-  __shared__ __attribute__((aligned(16))) uint32_t sc_lds0[2][kPStep];
-  __shared__ __attribute__((aligned(16))) uint32_t sc_lds1[2][kPStep];
+  __shared__ __attribute__((aligned(16))) uint8_t k_lds0[kKeys * kFp4Row];
+  __shared__ __attribute__((aligned(16))) uint8_t v_lds0[kKeys * kFp4Row];
+  __shared__ __attribute__((aligned(16))) uint8_t k_lds1[kKeys * kFp4Row];
+  __shared__ __attribute__((aligned(16))) uint8_t v_lds1[kKeys * kFp4Row];
+  __shared__ __attribute__((aligned(16))) uint32_t sc_lds0[2][kKeys];
+  __shared__ __attribute__((aligned(16))) uint32_t sc_lds1[2][kKeys];
   // each wave's fp16 v_scale * fw of the current tile's keys
-  __shared__ __attribute__((aligned(16))) _Float16 vsf_lds[kPWaves][kPStep];
+  __shared__ __attribute__((aligned(16))) _Float16 vsf_lds[kPWaves][kKeys];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -160,53 +176,68 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
   // Keys past the last valid one keep whatever the page holds: every code is
   // a finite value and their scores are masked.  Their v_scale reads as zero,
   // since 0 * NaN would not.
-  auto stage_tile = [&](int t0, uint8_t* kt, uint8_t* vt, uint32_t (*sct)[kPStep]) {
+  auto stage_tile = [&](int t0, uint8_t* kt, uint8_t* vt, uint32_t (*sct)[kKeys]) {
     const int page = t0 / a.bs;
     const int off = t0 - page * a.bs;
     const int blk = btc[(int64_t)s * a.w + page];
     const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
-    const int valid = ok ? min(kPStep, lk - t0) : 0;
+    const int valid = ok ? min(kKeys, lk - t0) : 0;
     const int64_t row = ((ok ? (int64_t)blk : 0) * a.hk + kvh) * a.bs + off;
-    const uint32_t bytes = valid > 0 ? kPStep * kFp4Row : 0u;
+    const uint32_t bytes = valid > 0 ? kKeys * kFp4Row : 0u;
     const auto kr = make_rsrc(a.kc + row * kFp4Row, bytes);
     const auto vr = make_rsrc(a.vc + row * kFp4Row, bytes);
-    const auto sr = make_rsrc((wave < 2 ? a.ks : a.vs) + row,
-                              valid > 0 ? (wave < 2 ? kPStep : valid) * 4u : 0u);
+    // waves 0 to kHalves - 1 load the block scales of K, the next the v_scales
+    const bool of_k = wave < kHalves;
+    const int half = of_k ? wave : wave - kHalves;
+    const auto sr = make_rsrc((of_k ? a.ks : a.vs) + row,
+                              valid > 0 ? (of_k ? kKeys : valid) * 4u : 0u);
 #pragma unroll
-    for (int j = 0; j < 8 / kPWaves; ++j) {
+    for (int j = 0; j < kKeys / 16 / kPWaves; ++j) {
       const int kb = kPWaves * j + wave;
       lds_load16(kr, kt + 1024 * kb, 1024u * kb + 16u * lane);
       lds_load16(vr, vt + 1024 * kb, 1024u * kb + 16u * (lane ^ (kb & 3)));
     }
-    // waves 0-1 load the block scales of K, waves 2-3 the v_scales
-    lds_load4(sr, &sct[wave >> 1][64 * (wave & 1)], 256u * (wave & 1) + 4u * lane);
+    if (wave < 2 * kHalves)
+      lds_load4(sr, &sct[of_k ? 0 : 1][64 * half], 256u * half + 4u * lane);
     return valid;
   };
 
   // one tile of work for this wave: QK^T, softmax, PV
   auto compute_tile = [&](int t0, int valid, const uint8_t* kt, const uint8_t* vt,
-                          const uint32_t (*sct)[kPStep]) {
+                          const uint32_t (*sct)[kKeys]) {
     if (t0 < w_none) {
       const float* vss = reinterpret_cast<const float*>(sct[1]);
       // S^T = K . Q^T: lane (g, n) gets keys 16tt + 4g + r of row n
-      f32x4 st[kPBlocks][8];
-      const uint32_t ks0 = sct[0][lane], ks1 = sct[0][64 + lane];
-      auto qk = [&](auto tile) {
-        constexpr int tt = decltype(tile)::value;
-        const u32x4 ka = *reinterpret_cast<const u32x4*>(kt + 1024 * tt + 16 * lane);
+      f32x4 st[kPBlocks][kGroups];
+      uint32_t ksw[kHalves];
+#pragma unroll
+      for (int i = 0; i < kHalves; ++i) ksw[i] = sct[0][64 * i + lane];
+      u32x4 ka[kGroups];
+#pragma unroll
+      for (int tt = 0; tt < kGroups; ++tt)
+        ka[tt] = *reinterpret_cast<const u32x4*>(kt + 1024 * tt + 16 * lane);
+      // One part of the query at a time over 64 keys: an MFMA follows the one
+      // whose sum it continues at a distance of eight.
+      auto qk = [&](auto half, auto part) {
+        constexpr int h = decltype(half)::value, p = decltype(part)::value;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int b = 0; b < kPBlocks; ++b) {
-          const uint32_t ks = tt < 4 ? ks0 : ks1;
-          f32x4 c = {0.f, 0.f, 0.f, 0.f};
-          c = mfma_fp4_q6<tt & 3, 0>(ka, ks, qp[b][0], qe[b], c);
-          c = mfma_fp4_q6<tt & 3, 1>(ka, ks, qp[b][1], qe[b], c);
-          st[b][tt] = mfma_fp4_q6<tt & 3, 2>(ka, ks, qp[b][2], qe[b], c);
+          auto one = [&](auto tile) {
+            constexpr int t = decltype(tile)::value;
+            const f32x4 c = p == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : st[b][4 * h + t];
+            st[b][4 * h + t] =
+                mfma_fp4_q6<t, p>(ka[4 * h + t], ksw[h], qp[b][p], qe[b], c);
+          };
+          one(Int<0>()), one(Int<1>()), one(Int<2>()), one(Int<3>());
         }
       };
-      qk(Int<0>()), qk(Int<1>()), qk(Int<2>()), qk(Int<3>());
-      qk(Int<4>()), qk(Int<5>()), qk(Int<6>()), qk(Int<7>());
+      qk(Int<0>(), Int<0>()), qk(Int<0>(), Int<1>()), qk(Int<0>(), Int<2>());
+      if constexpr (kHalves == 2)
+        qk(Int<1>(), Int<0>()), qk(Int<1>(), Int<1>()), qk(Int<1>(), Int<2>());
+      __builtin_amdgcn_sched_barrier(0);
       // masked keys -> -inf on tiles that need masks
-      const bool full = t0 + kPStep <= w_all && valid == kPStep;
+      const bool full = t0 + kKeys <= w_all && valid == kKeys;
       // The barrier after each row of keys keeps the scheduler from hoisting
       // all 64 lane-mask compares ahead of their selects.  Hoisted, their
       // SGPR pairs overflow the SGPR file, and the allocator then spills
@@ -214,7 +245,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
       // v_readlane/v_writelane per full tile): 4.7-4.9% of kernel time.
       if (!full) {
 #pragma unroll
-        for (int tt = 0; tt < 8; ++tt) {
+        for (int tt = 0; tt < kGroups; ++tt) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int key = 16 * tt + 4 * g + r;
@@ -236,7 +267,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
       for (int b = 0; b < kPBlocks; ++b) {
         float v = fmaxf(fmaxf(st[b][0][0], st[b][0][1]), fmaxf(st[b][0][2], st[b][0][3]));
 #pragma unroll
-        for (int tt = 1; tt < 8; ++tt)
+        for (int tt = 1; tt < kGroups; ++tt)
           v = fmaxf(fmaxf(v, st[b][tt][0]), fmaxf(fmaxf(st[b][tt][1], st[b][tt][2]), st[b][tt][3]));
         lm[b] = v;
         grow |= v * a.scale_log2 > m[b] + kPSlack;
@@ -264,7 +295,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
       // while every key fits under fw (a NaN scale fails the test and takes
       // the exact path, whose maximum ignores it).
       {
-        const float v0 = vss[lane], v1 = vss[64 + lane];
+        const float v0 = vss[lane], v1 = kHalves == 2 ? vss[64 + lane] : v0;
         if (__any(!(v0 * fw <= kPVScaleMax) || !(v1 * fw <= kPVScaleMax)) || fw == 0.0f) {
           const float vm = max_xor32(max_xor16(max16_dpp(fmaxf(v0, v1))));
           if (vm > 0.0f && (fw == 0.0f || vm * fw > kPVScaleMax)) {
@@ -286,7 +317,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
       // orders them
       _Float16* vsw = vsf_lds[wave];
       vsw[lane] = (_Float16)(vss[lane] * fw);
-      vsw[64 + lane] = (_Float16)(vss[64 + lane] * fw);
+      if constexpr (kHalves == 2) vsw[64 + lane] = (_Float16)(vss[64 + lane] * fw);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -300,16 +331,16 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
       // ahead: read per block and group, every read's LDS latency was
       // exposed.  The denominator's MFMA for a chunk follows its probabilities.
       typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-      f16x8 pw[kPBlocks][4];
+      f16x8 pw[kPBlocks][kChunks];
       f16x4 vsf_next = *reinterpret_cast<const f16x4*>(vsw + 4 * g);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kChunks; ++c) {
         f16x8 pc[kPBlocks];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int tt = 2 * c + h;
           const f16x4 vf = vsf_next;
-          if (tt < 7) vsf_next = *reinterpret_cast<const f16x4*>(vsw + 16 * (tt + 1) + 4 * g);
+          if (tt < kGroups - 1) vsf_next = *reinterpret_cast<const f16x4*>(vsw + 16 * (tt + 1) + 4 * g);
 #pragma unroll
           for (int b = 0; b < kPBlocks; ++b) {
             float pf[4];
@@ -336,7 +367,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
       // A masked key's p is 0, but its v_scale may be no number: where a tile
       // that needs masks holds such a scale, the masked weights are set to 0.
       if (!full) {
-        const uint32_t v0 = sct[1][lane], v1 = sct[1][64 + lane];
+        const uint32_t v0 = sct[1][lane], v1 = kHalves == 2 ? sct[1][64 + lane] : v0;
         if (__any((v0 & 0x7F800000u) == 0x7F800000u || (v1 & 0x7F800000u) == 0x7F800000u)) {
           // (the rows' ends again from the lane id: kept live so far, they spill)
           int ln = lane;
@@ -344,7 +375,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
           const int first = 4 * (ln >> 4);
           const int end0 = prefix + w_q0 + (((ln & 15) * a.gc_magic) >> 8) + 1 - t0;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < kKeys / 4; ++i) {
             const int key = 16 * (i >> 2) + (i & 3) + first;
 #pragma unroll
             for (int b = 0; b < kPBlocks; ++b)
@@ -356,24 +387,24 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
       // O^T += V^T . P^T, one 16-wide d tile and 32-key chunk per MFMA; a read
       // brings a lane 16 tokens of 64, two chunks.  The reads of d tile dt + 1
       // are issued before the MFMAs of tile dt.
-      i32x2 raw[2];
+      i32x2 raw[kHalves];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) raw[c] = fp4_v_read(vt + 64 * kFp4Row * c, vrow + fp4_v_col(lane, 0));
+      for (int c = 0; c < kHalves; ++c) raw[c] = fp4_v_read(vt + 64 * kFp4Row * c, vrow + fp4_v_col(lane, 0));
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) {
-        i32x2 nxt[2];
+        i32x2 nxt[kHalves];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < kHalves; ++c)
           nxt[c] = fp4_v_read(vt + 64 * kFp4Row * c, vrow + fp4_v_col(lane, dt < 7 ? dt + 1 : dt));
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           const f16x8 va = fp4x8_to_f16((uint32_t)raw[c >> 1][c & 1]);
 #pragma unroll
           for (int b = 0; b < kPBlocks; ++b)
             acc[b][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pw[b][c], acc[b][dt], 0, 0, 0);
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) raw[c] = nxt[c];
+        for (int c = 0; c < kHalves; ++c) raw[c] = nxt[c];
       }
       __builtin_amdgcn_s_setprio(0);
     }
@@ -381,19 +412,19 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
 
   int valid = stage_tile(kv_begin, k_lds0, v_lds0, sc_lds0);
   __syncthreads();
-  for (int t0 = kv_begin; t0 < kv_end; t0 += 2 * kPStep) {
+  for (int t0 = kv_begin; t0 < kv_end; t0 += 2 * kKeys) {
     {
-      const bool more = t0 + kPStep < kv_end;
-      const int valid_next = more ? stage_tile(t0 + kPStep, k_lds1, v_lds1, sc_lds1) : 0;
+      const bool more = t0 + kKeys < kv_end;
+      const int valid_next = more ? stage_tile(t0 + kKeys, k_lds1, v_lds1, sc_lds1) : 0;
       compute_tile(t0, valid, k_lds0, v_lds0, sc_lds0);
       __syncthreads();  // also waits for this wave's direct loads
       valid = valid_next;
       if (!more) break;
     }
     {
-      const int t1 = t0 + kPStep;
-      const bool more = t1 + kPStep < kv_end;
-      const int valid_next = more ? stage_tile(t1 + kPStep, k_lds0, v_lds0, sc_lds0) : 0;
+      const int t1 = t0 + kKeys;
+      const bool more = t1 + kKeys < kv_end;
+      const int valid_next = more ? stage_tile(t1 + kKeys, k_lds0, v_lds0, sc_lds0) : 0;
       compute_tile(t1, valid, k_lds1, v_lds1, sc_lds1);
       __syncthreads();
       valid = valid_next;
