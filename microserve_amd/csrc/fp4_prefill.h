@@ -23,29 +23,17 @@ namespace mskv {
 
 template <int N> using Int = std::integral_constant<int, N>;
 
-#ifndef FB
-#define FB 2
-#define FK 128
-#define FO 2
-#endif
-struct Fp4Shape {
-  static constexpr int blocks = FB;     // 16-row blocks per wave
-  static constexpr int keys = FK;     // per tile
-  static constexpr int occupancy = FO;  // waves per SIMD
-};
-
 // kSplit: the workgroup takes one of a.splits ranges of the keys (whole
 // tiles, from the actual key count) and leaves partials for the merge.
-template <typename T, bool kSplit, typename Shape>
-__global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4_kernel(
-    PrefillArgs a) {
+template <typename T, bool kSplit>
+__global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(PrefillArgs a) {
   using A = Act<T>;
-  constexpr int kPBlocks = Shape::blocks;
+  constexpr int kPBlocks = PShape::blocks;
   constexpr int kPWaves = PShape::waves;
-  constexpr int kKeys = Shape::keys;         // of a tile
-  constexpr int kGroups = kKeys / 16;        // S^T tiles
-  constexpr int kChunks = kKeys / 32;        // P^T chunks
-  constexpr int kHalves = kKeys / 64;        // V^T reads
+  constexpr int kKeys = kPStep;  // of a tile
+  constexpr int kGroups = kKeys / 16;  // S^T tiles
+  constexpr int kChunks = kKeys / 32;  // P^T chunks
+  constexpr int kHalves = kKeys / 64;  // V^T reads
   // two tile buffers as separate objects, and a loop unrolled by two, as in
   // the FP8 kernel: direct loads into one then never alias the other's reads
   __shared__ __attribute__((aligned(16))) uint8_t k_lds0[kKeys * kFp4Row];
@@ -54,8 +42,11 @@ __global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4
   __shared__ __attribute__((aligned(16))) uint8_t v_lds1[kKeys * kFp4Row];
   __shared__ __attribute__((aligned(16))) uint32_t sc_lds0[2][kKeys];
   __shared__ __attribute__((aligned(16))) uint32_t sc_lds1[2][kKeys];
-  // each wave's fp16 v_scale * fw of the current tile's keys
-  __shared__ __attribute__((aligned(16))) _Float16 vsf_lds[kPWaves][kKeys];
+  // each wave's v_scale * fw of the current tile's keys
+  constexpr bool kFp16 = A::kId == 0;
+  typedef typename std::conditional<kFp16, float, _Float16>::type VScale;
+  typedef VScale vscale4 __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(16))) VScale vsf_lds[kPWaves][kKeys];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -233,8 +224,7 @@ __global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4
         }
       };
       qk(Int<0>(), Int<0>()), qk(Int<0>(), Int<1>()), qk(Int<0>(), Int<2>());
-      if constexpr (kHalves == 2)
-        qk(Int<1>(), Int<0>()), qk(Int<1>(), Int<1>()), qk(Int<1>(), Int<2>());
+      qk(Int<1>(), Int<0>()), qk(Int<1>(), Int<1>()), qk(Int<1>(), Int<2>());
       __builtin_amdgcn_sched_barrier(0);
       // masked keys -> -inf on tiles that need masks
       const bool full = t0 + kKeys <= w_all && valid == kKeys;
@@ -295,7 +285,7 @@ __global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4
       // while every key fits under fw (a NaN scale fails the test and takes
       // the exact path, whose maximum ignores it).
       {
-        const float v0 = vss[lane], v1 = kHalves == 2 ? vss[64 + lane] : v0;
+        const float v0 = vss[lane], v1 = vss[64 + lane];
         if (__any(!(v0 * fw <= kPVScaleMax) || !(v1 * fw <= kPVScaleMax)) || fw == 0.0f) {
           const float vm = max_xor32(max_xor16(max16_dpp(fmaxf(v0, v1))));
           if (vm > 0.0f && (fw == 0.0f || vm * fw > kPVScaleMax)) {
@@ -311,13 +301,13 @@ __global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4
           }
         }
       }
-      // fp16(v_scale * fw) of the tile's keys, computed once per key by
+      // v_scale * fw of the tile's keys, computed once per key by
       // this wave (lane i: keys i and 64 + i) and read back in groups of
       // four; the wave reads only its own writes, so a wave-level barrier
       // orders them
-      _Float16* vsw = vsf_lds[wave];
-      vsw[lane] = (_Float16)(vss[lane] * fw);
-      if constexpr (kHalves == 2) vsw[64 + lane] = (_Float16)(vss[64 + lane] * fw);
+      VScale* vsw = vsf_lds[wave];
+      vsw[lane] = (VScale)(vss[lane] * fw);
+      vsw[64 + lane] = (VScale)(vss[64 + lane] * fw);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -330,17 +320,20 @@ __global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4
       // Each 16-key group's scales are read once for both blocks, one group
       // ahead: read per block and group, every read's LDS latency was
       // exposed.  The denominator's MFMA for a chunk follows its probabilities.
-      typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+      // An fp16 output sees the weights' roundings: there the scale stays in
+      // 32 bits and a weight is rounded once, as in the decode (error against
+      // 64 bits 2.9e-4 instead of 3.7e-4, of which the output's own rounding
+      // is 2.1e-4).
       f16x8 pw[kPBlocks][kChunks];
-      f16x4 vsf_next = *reinterpret_cast<const f16x4*>(vsw + 4 * g);
+      vscale4 vsf_next = *reinterpret_cast<const vscale4*>(vsw + 4 * g);
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         f16x8 pc[kPBlocks];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int tt = 2 * c + h;
-          const f16x4 vf = vsf_next;
-          if (tt < kGroups - 1) vsf_next = *reinterpret_cast<const f16x4*>(vsw + 16 * (tt + 1) + 4 * g);
+          const vscale4 vf = vsf_next;
+          if (tt < kGroups - 1) vsf_next = *reinterpret_cast<const vscale4*>(vsw + 16 * (tt + 1) + 4 * g);
 #pragma unroll
           for (int b = 0; b < kPBlocks; ++b) {
             float pf[4];
@@ -348,8 +341,14 @@ __global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4
             for (int r = 0; r < 4; ++r) pf[r] = exp2_fast(fmaf(st[b][tt][r], a.scale_log2, -m[b]));
             const f16x2 p01 = {(_Float16)pf[0], (_Float16)pf[1]};
             const f16x2 p23 = {(_Float16)pf[2], (_Float16)pf[3]};
-            const f16x2 w01 = p01 * f16x2{vf[0], vf[1]};
-            const f16x2 w23 = p23 * f16x2{vf[2], vf[3]};
+            f16x2 w01, w23;
+            if constexpr (kFp16) {
+              w01 = f16x2{(_Float16)(pf[0] * vf[0]), (_Float16)(pf[1] * vf[1])};
+              w23 = f16x2{(_Float16)(pf[2] * vf[2]), (_Float16)(pf[3] * vf[3])};
+            } else {
+              w01 = p01 * f16x2{vf[0], vf[1]};
+              w23 = p23 * f16x2{vf[2], vf[3]};
+            }
             pc[b][4 * h + 0] = p01[0];
             pc[b][4 * h + 1] = p01[1];
             pc[b][4 * h + 2] = p23[0];
@@ -367,7 +366,7 @@ __global__ __launch_bounds__(PShape::threads, Shape::occupancy) void prefill_fp4
       // A masked key's p is 0, but its v_scale may be no number: where a tile
       // that needs masks holds such a scale, the masked weights are set to 0.
       if (!full) {
-        const uint32_t v0 = sct[1][lane], v1 = kHalves == 2 ? sct[1][64 + lane] : v0;
+        const uint32_t v0 = sct[1][lane], v1 = sct[1][64 + lane];
         if (__any((v0 & 0x7F800000u) == 0x7F800000u || (v1 & 0x7F800000u) == 0x7F800000u)) {
           // (the rows' ends again from the lane id: kept live so far, they spill)
           int ln = lane;

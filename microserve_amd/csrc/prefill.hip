@@ -679,7 +679,7 @@ static hipError_t launch_prefill(const PrefillArgs& a, int num_seqs, int64_t qbl
   auto rows = [&](auto split) {
     constexpr bool kSplit = decltype(split)::value;
     if constexpr (kFp4)
-      hipLaunchKernelGGL((prefill_fp4_kernel<T, kSplit, Fp4Shape>), grid, dim3(PShape::threads), 0, st, a);
+      hipLaunchKernelGGL((prefill_fp4_kernel<T, kSplit>), grid, dim3(PShape::threads), 0, st, a);
     else
       hipLaunchKernelGGL((prefill_fp8_kernel<T, kSplit>), grid, dim3(PShape::threads), 0, st, a);
   };
