@@ -505,20 +505,18 @@ int mskv_copy_kv_blocks(int num_pools, void* const* bases,
  * block_tables: int32 [num_entries]; entries outside [0, num_blocks) (-1
  * padding, a garbage page behind the pool) are kept as they are, and
  * several entries may name one page.  new_tables [num_entries]: the entries
- * renamed (may be block_tables itself).  remap [num_blocks]: each page's new
- * place, -1 for a free one.  num_live [1]: n.  All on the device; nothing is
- * read on the host.  num_blocks here is the number of pages that may move,
- * at most 2^18; plane_strides may leave room for more behind them.
- * workspace: mskv_compact_workspace_bytes(num_blocks), on four bytes.
+ * renamed; it may not overlap block_tables (MSKV_EINVAL).  remap
+ * [num_blocks]: each page's new place, -1 for a free one.  num_live [1]: n.
+ * All on the device; nothing is read on the host.  num_blocks here is the
+ * number of pages that may move, at most 2^18 (else MSKV_EUNSUPPORTED);
+ * plane_strides may leave room for more behind them.
  */
-size_t mskv_compact_workspace_bytes(int64_t num_blocks);
 int mskv_compact_kv_blocks(int num_pools, void* const* bases,
                            const int64_t* planes, const int64_t* plane_strides,
                            const int64_t* page_bytes, int64_t num_blocks,
                            const int32_t* block_tables, int64_t num_entries,
                            int32_t* new_tables, int32_t* remap,
-                           int32_t* num_live, void* workspace,
-                           size_t workspace_bytes, void* stream);
+                           int32_t* num_live, void* stream);
 
 #ifdef __cplusplus
 }

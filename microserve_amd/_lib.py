@@ -130,9 +130,8 @@ _PROTOS = {
         _c_int, _c_f32, _c_int, _vp, _c_size, _vp]),
     "mskv_copy_kv_blocks": (_c_int, [
         _c_int, _vp, _vp, _vp, _vp, _c_i64, _vp, _vp, _c_i64, _vp]),
-    "mskv_compact_workspace_bytes": (_c_size, [_c_i64]),
     "mskv_compact_kv_blocks": (_c_int, [
-        _c_int, _vp, _vp, _vp, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _c_size, _vp]),
+        _c_int, _vp, _vp, _vp, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp]),
 }
 
 EXPORTED = tuple(_PROTOS)

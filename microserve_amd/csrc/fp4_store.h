@@ -125,47 +125,39 @@ __global__ __launch_bounds__(64 * kFp4Waves) void store_fp4_kernel(Fp4StoreArgs 
   if (sub == 0) a.vs[p.vs] = vscale;
 }
 
-// this lane's 16 elements, rounded once to the row's type
+// eight elements, rounded once to the row's type
 template <typename T>
-__device__ __forceinline__ void store16(void* base, int64_t at, int sub, const float* x) {
+__device__ __forceinline__ void store8(void* base, int64_t at, const float* x) {
   if constexpr (sizeof(T) == 4) {
-    u32x4* p = reinterpret_cast<u32x4*>(reinterpret_cast<float*>(base) + at + sub * 16);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      u32x4 v;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(x[4 * c + i]);
-      __builtin_nontemporal_store(v, p + c);
-    }
+    f32x4* p = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(base) + at);
+    p[0] = f32x4{x[0], x[1], x[2], x[3]};
+    p[1] = f32x4{x[4], x[5], x[6], x[7]};
   } else {
-    u32x4* p = reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(base) + at + sub * 16);
+    u32x4 v;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      u32x4 v;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = (uint32_t)Act<T>::from_f32(x[8 * c + 2 * i]) |
-               ((uint32_t)Act<T>::from_f32(x[8 * c + 2 * i + 1]) << 16);
-      __builtin_nontemporal_store(v, p + c);
-    }
+    for (int i = 0; i < 4; ++i)
+      v[i] = (uint32_t)Act<T>::from_f32(x[2 * i]) |
+             ((uint32_t)Act<T>::from_f32(x[2 * i + 1]) << 16);
+    __builtin_nontemporal_store(
+        v, reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(base) + at));
   }
 }
 
-__device__ __forceinline__ void fp4_unpack16(u32x2 w, float scale, float* x) {
+__device__ __forceinline__ void fp4_unpack8(uint32_t w, float scale, float* x) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[h], 1.0f, 0);
-    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[h], 1.0f, 1);
-    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[h], 1.0f, 2);
-    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[h], 1.0f, 3);
-    x[8 * h + 0] = a[0] * scale; x[8 * h + 1] = a[1] * scale;
-    x[8 * h + 2] = b[0] * scale; x[8 * h + 3] = b[1] * scale;
-    x[8 * h + 4] = c[0] * scale; x[8 * h + 5] = c[1] * scale;
-    x[8 * h + 6] = d[0] * scale; x[8 * h + 7] = d[1] * scale;
-  }
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0);
+  const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+  const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2);
+  const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+  x[0] = a[0] * scale; x[1] = a[1] * scale;
+  x[2] = b[0] * scale; x[3] = b[1] * scale;
+  x[4] = c[0] * scale; x[5] = c[1] * scale;
+  x[6] = d[0] * scale; x[7] = d[1] * scale;
 }
 
+// The eight lanes of a row write whole 128-byte lines: lane l the dimensions
+// [8l, 8l + 8) and [64 + 8l, 72 + 8l).  (16 in one run, as the store reads
+// them, leave half of every 32 bytes to a second store: 65,536 tokens 134 us.)
 template <typename T, typename SlotT>
 __global__ __launch_bounds__(64 * kFp4Waves) void load_fp4_kernel(Fp4StoreArgs a) {
   const int lane = threadIdx.x & 63;
@@ -176,24 +168,33 @@ __global__ __launch_bounds__(64 * kFp4Waves) void load_fp4_kernel(Fp4StoreArgs a
   const int64_t tok = tb * kFp4Tokens + (lane >> 3);
   if (tok >= a.tokens) return;
   const int64_t slot = (int64_t)static_cast<const SlotT*>(a.slots)[tok];
-  float x[16], y[16];
+  float x[2][8], y[2][8];
   if (slot >= 0 && slot < a.num_slots) {
-    const Fp4Place p = fp4_place(slot, head, sub, a.hk, a.bs);
-    const u32x2 kq = *reinterpret_cast<const u32x2*>(a.kc + p.k);
-    const u32x2 vq = *reinterpret_cast<const u32x2*>(a.vc + p.v);
-    const uint32_t e = a.ks[p.ks];
+    const Fp4Place p = fp4_place(slot, head, 0, a.hk, a.bs);
     const float vscale = a.vs[p.vs];
-    // (2^-127 is a subnormal float)
-    const uint32_t bits = e == (uint32_t)kE8M0Nan ? 0x7FC00000u : e == 0 ? 0x00400000u : e << 23;
-    fp4_unpack16(kq, __uint_as_float(bits), x);
-    fp4_unpack16(vq, vscale, y);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int block = 2 * h + (sub >> 2);
+      const uint32_t kq =
+          *reinterpret_cast<const uint32_t*>(a.kc + p.k + 256 * block + 4 * (sub & 3));
+      const uint32_t vq = *reinterpret_cast<const uint32_t*>(a.vc + p.v + 32 * h + 4 * sub);
+      const uint32_t e = a.ks[p.ks + 64 * block];
+      // (2^-127 is a subnormal float)
+      const uint32_t bits =
+          e == (uint32_t)kE8M0Nan ? 0x7FC00000u : e == 0 ? 0x00400000u : e << 23;
+      fp4_unpack8(kq, __uint_as_float(bits), x[h]);
+      fp4_unpack8(vq, vscale, y[h]);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = y[i] = 0.0f;
+    for (int i = 0; i < 8; ++i) x[0][i] = x[1][i] = y[0][i] = y[1][i] = 0.0f;
   }
-  const int64_t at = (tok * a.hk + head) * kHeadDim;
-  store16<T>(a.key_out, at, sub, x);
-  store16<T>(a.value_out, at, sub, y);
+  const int64_t at = (tok * a.hk + head) * kHeadDim + 8 * sub;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    store8<T>(a.key_out, at + 64 * h, x[h]);
+    store8<T>(a.value_out, at + 64 * h, y[h]);
+  }
 }
 
 template <bool kStore, typename T, typename SlotT>

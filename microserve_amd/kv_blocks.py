@@ -121,13 +121,10 @@ def compact_kv_blocks(caches, block_tables: torch.Tensor, num_blocks: int | None
         ints = dict(dtype=torch.int32, device=tables.device)
         renamed = torch.empty(tables.shape, **ints)
         remap, live = torch.empty(num_blocks, **ints), torch.empty(1, **ints)
-        ws_bytes = lib.mskv_compact_workspace_bytes(num_blocks)
-        ws = torch.empty(max(ws_bytes, 4), dtype=torch.uint8, device=tables.device)
         stream = _lib.stream_of(tables)
         for count, *described in groups:
             # (a later group's plan is the first one's: the tables are kept)
             _lib.check(lib.mskv_compact_kv_blocks(
                 count, *described, num_blocks, tables.data_ptr(), tables.numel(),
-                renamed.data_ptr(), remap.data_ptr(), live.data_ptr(), ws.data_ptr(), ws_bytes,
-                stream), what)
+                renamed.data_ptr(), remap.data_ptr(), live.data_ptr(), stream), what)
     return renamed, remap, live

@@ -214,7 +214,7 @@ def _i32(x):
 
 def test_page_moves_refuse_before_any_launch():
     lib = _lib.load()
-    E, U, W = -1, -2, -3
+    E, U = -1, -2
 
     def copy(src=(0,), dst=(1,), n=None, **pool):
         return lib.mskv_copy_kv_blocks(*_pool(**pool), _i32(src), _i32(dst),
@@ -235,16 +235,12 @@ def test_page_moves_refuse_before_any_launch():
                                    None) == E
     assert lib.mskv_copy_kv_blocks(*_pool(n=9), _i32((0,)), _i32((1,)), 1, None) == E
 
-    ws = lib.mskv_compact_workspace_bytes(8)
-    assert ws == 16 + 8 * 5
-    assert lib.mskv_compact_workspace_bytes(0) == lib.mskv_compact_workspace_bytes(1 << 19) == 0
-
-    def compact(tables=FAKE, n=4, remap=FAKE, space=FAKE, size=ws, **pool):
-        return lib.mskv_compact_kv_blocks(*_pool(**pool), tables, n, FAKE, remap, FAKE, space, size,
-                                          None)
+    def compact(tables=FAKE, n=4, new=2 * FAKE, remap=FAKE, **pool):
+        return lib.mskv_compact_kv_blocks(*_pool(**pool), tables, n, new, remap, FAKE, None)
 
     assert compact(n=-1) == E and compact(tables=None) == E and compact(remap=None) == E
-    assert compact(space=None) == W and compact(size=ws - 1) == W
+    assert compact(new=None) == E and compact(new=FAKE) == E  # tables that others still read
+    assert compact(new=FAKE + 12) == E and compact(new=FAKE - 12) == E
     assert compact(blocks=0) == E and compact(blocks=1 << 19) == U
     assert compact(page=8) == U
 

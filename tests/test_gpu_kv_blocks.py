@@ -111,7 +111,7 @@ def _check_compact(pools, tables, num_blocks, block_dim):
 
 @pytest.mark.parametrize("pages,live,width", [
     (1, 1, 1), (1, 0, 1), (2, 1, 1), (31, 9, 4), (32, 32, 8), (33, 16, 5), (64, 1, 1),
-    (65, 64, 9), (1000, 500, 40), (5000, 77, 100), (5000, 4999, 130)])
+    (65, 64, 9), (1000, 500, 40), (5000, 77, 100), (5000, 4999, 130), (70000, 30000, 200)])
 def test_compaction_follows_the_rule(pages, live, width):
     gen = torch.Generator().manual_seed(pages + live)
     pool = torch.randint(0, 1 << 30, (2, pages, 8), generator=gen, dtype=torch.int32).to(DEV)
