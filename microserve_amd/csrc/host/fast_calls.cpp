@@ -21,6 +21,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <vector>
+
 #include "../../../include/mskv.h"
 
 namespace {
@@ -39,6 +41,8 @@ struct Api {
   decltype(&mskv_fp4_decode_num_splits) num_splits4 = nullptr;
   decltype(&mskv_fp4_decode_attention) decode4 = nullptr;
   decltype(&mskv_fp4_prefill_attention) prefill4 = nullptr;
+  decltype(&mskv_copy_kv_blocks) copy = nullptr;
+  decltype(&mskv_compact_kv_blocks) compact = nullptr;
   decltype(&mskv_status_string) text = nullptr;
   bool bound = false;
 } api;
@@ -544,6 +548,104 @@ PyObject* prologue(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// The caches of a call that moves pages, as kv_blocks._pools describes them:
+// a tensor or a tuple or list of up to MSKV_MAX_POOLS, dimension `dim` of each
+// numbering the same blocks.
+struct PoolArgs {
+  int count = 0;
+  void* bases[MSKV_MAX_POOLS];
+  int64_t planes[MSKV_MAX_POOLS], strides[MSKV_MAX_POOLS], pages[MSKV_MAX_POOLS], blocks = -1;
+  bool add(Args& in, PyObject* o, int dim) {
+    const at::Tensor* t = count ? in.next(o) : in.first(o);
+    if (!in.ok || count == MSKV_MAX_POOLS || !t->is_contiguous() || t->dim() <= dim ||
+        t->numel() <= 0 || (blocks >= 0 && t->size(dim) != blocks))
+      return false;
+    blocks = t->size(dim);
+    int64_t n = 1;
+    for (int i = 0; i < dim; ++i) n *= t->size(i);
+    bases[count] = t->data_ptr();
+    planes[count] = n;
+    pages[count] = t->numel() / (n * blocks) * t->element_size();
+    strides[count] = blocks * pages[count];
+    ++count;
+    return true;
+  }
+  bool take(Args& in, PyObject* caches, int dim) {
+    if (!PyTuple_CheckExact(caches) && !PyList_CheckExact(caches)) return add(in, caches, dim);
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(caches);
+    if (n < 1 || n > MSKV_MAX_POOLS) return false;
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (!add(in, PySequence_Fast_GET_ITEM(caches, i), dim)) return false;
+    return true;
+  }
+};
+
+// a list or tuple of whole numbers that fit an int
+bool ids_of(PyObject* o, std::vector<int32_t>& v) {
+  if (!PyTuple_CheckExact(o) && !PyList_CheckExact(o)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  v.resize((size_t)n);
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (!whole(PySequence_Fast_GET_ITEM(o, i), v[(size_t)i])) return false;
+  return true;
+}
+
+// copy_blocks(caches, src, dst, block_dim) -> True | None
+PyObject* copy_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int dim;
+    std::vector<int32_t> src, dst;
+    if (n != 4 || !whole(a[3], dim) || !ids_of(a[1], src) || !ids_of(a[2], dst) ||
+        src.size() != dst.size())
+      return nullptr;
+    Args in;
+    PoolArgs p;
+    if (!p.take(in, a[0], dim)) return nullptr;
+    int status;
+    {
+      NoGil no_gil;
+      const c10::DeviceGuard guard(in.device);
+      status = api.copy(p.count, p.bases, p.planes, p.strides, p.pages, p.blocks, src.data(),
+                        dst.data(), (int64_t)src.size(), stream_of(in.device));
+    }
+    if (status != MSKV_OK) return failed("copy_kv_blocks", status);
+    Py_RETURN_TRUE;
+  });
+}
+
+// compact_blocks(caches, tables, num_blocks | None, block_dim)
+//   -> (tables, remap, num_live) | None
+PyObject* compact_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int dim, given = 0;
+    if (n != 4 || !whole(a[3], dim) || (a[2] != Py_None && !whole(a[2], given))) return nullptr;
+    Args in;
+    PoolArgs p;
+    if (!p.take(in, a[0], dim)) return nullptr;
+    const at::Tensor* tables = in.next(a[1]);
+    const int64_t blocks = a[2] == Py_None ? p.blocks : given;
+    if (!in.ok || !dense_of(*tables, at::kInt) || blocks < 1 || blocks > p.blocks) return nullptr;
+    at::Tensor renamed, remap, live;
+    int status;
+    {
+      NoGil no_gil;
+      const c10::DeviceGuard guard(in.device);
+      const auto opts = tables->options().requires_grad(false);
+      renamed = at::empty(tables->sizes(), opts);
+      remap = at::empty({blocks}, opts);
+      live = at::empty({1}, opts);
+      status = api.compact(p.count, p.bases, p.planes, p.strides, p.pages, blocks,
+                           (const int32_t*)tables->data_ptr(), tables->numel(),
+                           (int32_t*)renamed.data_ptr(), (int32_t*)remap.data_ptr(),
+                           (int32_t*)live.data_ptr(), stream_of(in.device));
+    }
+    if (status != MSKV_OK) return failed("compact_kv_blocks", status);
+    PyObject* t = THPVariable_Wrap(std::move(renamed));
+    PyObject* r = THPVariable_Wrap(std::move(remap));
+    return Py_BuildValue("(NNN)", t, r, THPVariable_Wrap(std::move(live)));
+  });
+}
+
 // bind({name: address}): the entry points of the loaded library
 PyObject* bind(PyObject*, PyObject* table) {
   auto get = [&](const char* name, auto& fn) {
@@ -565,7 +667,8 @@ PyObject* bind(PyObject*, PyObject* table) {
             get("mskv_store_fp4_kvcache", f.store4) && get("mskv_load_fp4_kvcache", f.load4) &&
             get("mskv_fp4_decode_num_splits", f.num_splits4) &&
             get("mskv_fp4_decode_attention", f.decode4) &&
-            get("mskv_fp4_prefill_attention", f.prefill4) && get("mskv_status_string", f.text);
+            get("mskv_fp4_prefill_attention", f.prefill4) &&
+            get("mskv_copy_kv_blocks", f.copy) && get("mskv_compact_kv_blocks", f.compact) && get("mskv_status_string", f.text);
   if (!f.bound) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "an entry point has no address");
     return nullptr;
@@ -577,6 +680,7 @@ PyObject* bind(PyObject*, PyObject* table) {
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FAST(store), FAST(decode), FAST(prefill), FAST(fresh), FAST(prologue),
                           FAST(store4), FAST(load4), FAST(decode4), FAST(prefill4),
+                          FAST(copy_blocks), FAST(compact_blocks),
                           {"bind", bind, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 

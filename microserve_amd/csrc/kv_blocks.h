@@ -5,7 +5,7 @@
 // scales, FP8 or 4-bit, one layer's or all layers'): `planes` stacks of pages
 // `plane_stride` bytes apart, pages of `page_bytes` back to back.  All of a
 // call's bytes move in one launch: workgroups take segments of a page, 16
-// bytes a lane and load, several loads in flight.  HBM-bound, 2 bytes moved
+// bytes a lane and load, copied through registers.  HBM-bound, 2 bytes moved
 // per byte of the pages.
 #pragma once
 
@@ -22,8 +22,13 @@ namespace mskv {
 
 constexpr int kMaxPools = MSKV_MAX_POOLS;
 constexpr int kMoveThreads = 256;
-constexpr int kMoveLoads = 4;  // 16-byte pieces a lane has in flight
-constexpr int kSegBytes = kMoveThreads * kMoveLoads * 16;
+// 16-byte pieces of a lane's turn.  A copy's workgroups come and go with one
+// each: 1.2 GB in 206 us (226 with two, 236 with four).  A compaction's walk the
+// moves, two pieces at a time: 122 of 512 pages in 212 us (265 with one, 214
+// with four; the same pages as a copy 174).  Asking for a workgroup's next
+// segment before it stores one gained nothing (216 to 227).
+constexpr int kCopyLoads = 1, kCompactLoads = 2;
+constexpr int seg_bytes(int loads) { return kMoveThreads * loads * 16; }
 // pairs that travel as arguments of one launch
 constexpr int kMaxPairs = 256;
 
@@ -40,24 +45,25 @@ struct PagePairs {
 };
 
 // Copies segment `seg` (of all the pools' planes) of page src to page dst.
+template <int kLoads>
 __device__ __forceinline__ void copy_segment(const Pools& p, int seg, int64_t src, int64_t dst) {
   int t = 0;
   while (t + 1 < p.count && seg >= p.first[t + 1]) ++t;
   const int s = seg - p.first[t];
   const int plane = s / p.segs[t], part = s - plane * p.segs[t];
-  const int64_t page = p.page_bytes[t], begin = (int64_t)part * kSegBytes;
+  const int64_t page = p.page_bytes[t], begin = (int64_t)part * seg_bytes(kLoads);
   uint8_t* stack = p.base[t] + plane * p.plane_stride[t] + begin;
   const u32x4* from = reinterpret_cast<const u32x4*>(stack + src * page);
   u32x4* to = reinterpret_cast<u32x4*>(stack + dst * page);
-  const int n = (int)min((int64_t)kSegBytes, page - begin) / 16;
-  u32x4 v[kMoveLoads];
+  const int n = (int)min((int64_t)seg_bytes(kLoads), page - begin) / 16;
+  u32x4 v[kLoads];
 #pragma unroll
-  for (int i = 0; i < kMoveLoads; ++i) {
+  for (int i = 0; i < kLoads; ++i) {
     const int at = i * kMoveThreads + threadIdx.x;
     if (at < n) v[i] = __builtin_nontemporal_load(from + at);
   }
 #pragma unroll
-  for (int i = 0; i < kMoveLoads; ++i) {
+  for (int i = 0; i < kLoads; ++i) {
     const int at = i * kMoveThreads + threadIdx.x;
     if (at < n) __builtin_nontemporal_store(v[i], to + at);
   }
@@ -65,7 +71,7 @@ __device__ __forceinline__ void copy_segment(const Pools& p, int seg, int64_t sr
 
 // grid (segments of a page in all pools, pairs)
 __global__ __launch_bounds__(kMoveThreads) void copy_kv_blocks_kernel(Pools p, PagePairs pairs) {
-  copy_segment(p, blockIdx.x, pairs.src[blockIdx.y], pairs.dst[blockIdx.y]);
+  copy_segment<kCopyLoads>(p, blockIdx.x, pairs.src[blockIdx.y], pairs.dst[blockIdx.y]);
 }
 
 // A compaction: n pages are named by the tables; the i-th named page at or
@@ -177,9 +183,10 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kv_blocks_kernel(Pools p
   const int64_t total = (int64_t)moves * a.segs;
   for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
     const int pair = (int)(i / a.segs);
-    copy_segment(p, (int)(i - (int64_t)pair * a.segs),
-                 __builtin_amdgcn_readfirstlane(find_bit(movers_at, words, pair, movers)),
-                 __builtin_amdgcn_readfirstlane(find_bit(holes_at, words, pair, holes)));
+    copy_segment<kCompactLoads>(
+        p, (int)(i - (int64_t)pair * a.segs),
+        __builtin_amdgcn_readfirstlane(find_bit(movers_at, words, pair, movers)),
+        __builtin_amdgcn_readfirstlane(find_bit(holes_at, words, pair, holes)));
   }
   for (int64_t i = first; i < a.entries; i += step) {
     const int32_t page = a.tables[i];
@@ -189,7 +196,8 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kv_blocks_kernel(Pools p
 
 // Checks a call's pools and lays their segments out.
 static int pools_of(Pools& p, int count, void* const* bases, const int64_t* planes,
-                    const int64_t* plane_strides, const int64_t* page_bytes, int64_t num_blocks) {
+                    const int64_t* plane_strides, const int64_t* page_bytes, int64_t num_blocks,
+                    int loads) {
   if (count <= 0 || count > kMaxPools || !bases || !planes || !plane_strides || !page_bytes)
     return MSKV_EINVAL;
   if (num_blocks < 0 || num_blocks > 0x7FFFFFFFLL) return MSKV_EINVAL;
@@ -204,7 +212,7 @@ static int pools_of(Pools& p, int count, void* const* bases, const int64_t* plan
     if (num_blocks > 0 && page_bytes[t] > (INT64_MAX >> 1) / num_blocks) return MSKV_EINVAL;
     if (planes[t] > 1 && plane_strides[t] < page_bytes[t] * num_blocks) return MSKV_EINVAL;
     if (planes[t] > 1 && plane_strides[t] > (INT64_MAX >> 1) / planes[t]) return MSKV_EINVAL;
-    const int64_t segs = (page_bytes[t] + kSegBytes - 1) / kSegBytes;
+    const int64_t segs = (page_bytes[t] + seg_bytes(loads) - 1) / seg_bytes(loads);
     if (segs > 0x3FFFFFFF || planes[t] > 0x3FFFFFFF / segs) return MSKV_EUNSUPPORTED;
     p.base[t] = (uint8_t*)bases[t];
     p.plane_stride[t] = plane_strides[t];
@@ -226,7 +234,8 @@ extern "C" int mskv_copy_kv_blocks(int num_pools, void* const* bases, const int6
                                    const int32_t* dst_blocks, int64_t num_pairs, void* stream) {
   using namespace mskv;
   Pools p;
-  const int status = pools_of(p, num_pools, bases, planes, plane_strides, page_bytes, num_blocks);
+  const int status = pools_of(p, num_pools, bases, planes, plane_strides, page_bytes, num_blocks,
+                              kCopyLoads);
   if (status != MSKV_OK) return status;
   if (num_pairs < 0) return MSKV_EINVAL;
   if (num_pairs == 0) return MSKV_OK;
@@ -268,16 +277,20 @@ extern "C" int mskv_compact_kv_blocks(int num_pools, void* const* bases, const i
                                       int32_t* num_live, void* stream) {
   using namespace mskv;
   Pools p;
-  const int status = pools_of(p, num_pools, bases, planes, plane_strides, page_bytes, num_blocks);
+  const int status = pools_of(p, num_pools, bases, planes, plane_strides, page_bytes, num_blocks,
+                              kCompactLoads);
   if (status != MSKV_OK) return status;
   if (num_entries < 0 || num_blocks <= 0) return MSKV_EINVAL;
   if (num_blocks > kPlanMaxBlocks || num_entries > (int64_t)1 << 40) return MSKV_EUNSUPPORTED;
   if (!remap || !num_live || (num_entries > 0 && (!block_tables || !new_tables)))
     return MSKV_EINVAL;
   // every workgroup reads the tables while others write the renamed ones
-  const uintptr_t from = (uintptr_t)block_tables, to = (uintptr_t)new_tables;
-  const uintptr_t size = (uintptr_t)num_entries * sizeof(int32_t);
-  if (from < to + size && to < from + size) return MSKV_EINVAL;
+  const uintptr_t from = (uintptr_t)block_tables, end = from + (uintptr_t)num_entries * 4;
+  auto overlaps = [&](const int32_t* to, int64_t n) {
+    return from < (uintptr_t)to + (uintptr_t)n * 4 && (uintptr_t)to < end;
+  };
+  if (overlaps(new_tables, num_entries) || overlaps(remap, num_blocks) || overlaps(num_live, 1))
+    return MSKV_EINVAL;
   CompactArgs a;
   a.tables = block_tables;
   a.new_tables = new_tables;

@@ -71,6 +71,8 @@ def copy_kv_blocks(caches, src_blocks, dst_blocks, block_dim: int = 0) -> None:
     To fork a sequence, give the child the parent's full pages and copy the
     partly filled one to a page of its own.
     """
+    if _lib.fast.copy_blocks(caches, src_blocks, dst_blocks, block_dim):
+        return
     what = "copy_kv_blocks"
     src, dst = _ids(what, src_blocks), _ids(what, dst_blocks)
     assert len(src) == len(dst), f"{what}: as many destinations as sources"
@@ -108,6 +110,9 @@ def compact_kv_blocks(caches, block_tables: torch.Tensor, num_blocks: int | None
     the runner's garbage page behind the pool) are kept as they are.  Nothing
     is read on the host, and the call may be captured in a HIP graph.
     """
+    res = _lib.fast.compact_blocks(caches, block_tables, num_blocks, block_dim)
+    if res is not None:
+        return res
     what = "compact_kv_blocks"
     tensors = _tensors(caches)
     groups, pool = _pools(what, tensors, block_dim)

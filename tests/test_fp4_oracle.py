@@ -283,6 +283,12 @@ def test_native_paths_leave_other_calls_to_the_wrappers():
     assert f.load4(*caches, i32, torch.float16) is None
     assert f.decode4(q, *caches, i32, i32.view(-1, 1), 0.1, None, None) is None
     assert f.prefill4(q, *caches, i32, None, None, 0, 2, 0, 0.1) is None
+    pool = torch.zeros(3, 64)
+    assert f.copy_blocks(pool, [0], [1], 0) is None and f.copy_blocks((pool,), [0], [1], 0) is None
+    assert f.compact_blocks([pool], i32, None, 0) is None
+    for fn in (f.copy_blocks, f.compact_blocks):
+        assert fn() is None and fn(*[None] * 4) is None and fn(*["x"] * 4) is None
+        assert fn((), [], [], 0) is None and fn((3, "y"), (1 << 40,), [1.5], -1) is None
     for fn in (f.store4, f.load4, f.decode4, f.prefill4):
         assert fn() is None
         assert fn(*[None] * 6) is None and fn(*[None] * 7) is None and fn(*["x"] * 12) is None

@@ -178,3 +178,32 @@ def test_fork_of_both_formats():
         a = M.load_fp4_kvcache(*layer, slots)
         b = M.load_fp4_kvcache(*layer, slots + 3 * 128)
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and a[0].abs().sum() > 0
+
+
+def test_native_paths_and_wrappers_agree(monkeypatch):
+    """Every call above ran natively where it could; here the wrappers'."""
+    from microserve_amd import _lib
+
+    class Off:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    gen = torch.Generator().manual_seed(14)
+    first = list(_runner_pool(gen, 2, 30, 128, 2))
+    other = [t.clone() for t in first]
+    tables = torch.tensor([[29, 4, -1], [17, 28, 30]], dtype=torch.int32, device=DEV)
+    assert _lib.fast.copy_blocks(tuple(first), [1, 2], (3, 4), 2) is True
+    native = M.compact_kv_blocks(first, tables, 29, block_dim=2)
+    assert _lib.fast.compact_blocks(first, tables, 29, 2) is not None
+    for bad in (dict(src=[0, 1], dst=[2, 2]), dict(src=[3], dst=[3]), dict(src=[0], dst=[30])):
+        with pytest.raises(AssertionError):
+            M.copy_kv_blocks(first, bad["src"], bad["dst"], block_dim=2)
+    with pytest.raises(AssertionError):
+        M.compact_kv_blocks(first, tables, 31, block_dim=2)
+    monkeypatch.setattr(_lib, "fast", Off())
+    M.copy_kv_blocks(tuple(other), [1, 2], (3, 4), block_dim=2)
+    for a, b in zip(native, M.compact_kv_blocks(other, tables, 29, block_dim=2)):
+        assert torch.equal(a, b)
+    M.compact_kv_blocks(other, tables, 29, block_dim=2)
+    for a, b in zip(first, other):
+        assert torch.equal(_bytes(a), _bytes(b))
