@@ -421,7 +421,8 @@ int mskv_qk_norm_rope_store(const void* q, const void* k, const void* v,
  * key/value: [num_tokens, num_kv_heads, 128] in act_dtype (MSKV_FLOAT16,
  * MSKV_BFLOAT16 or MSKV_FLOAT32), key_stride / value_stride elements from
  * token to token as in mskv_store_fp8_kvcache_strided, on 16 bytes.  Slots
- * outside the cache are skipped; a slot is named at most once.
+ * outside the cache are skipped; one that several tokens name holds
+ * unspecified bytes.
  */
 int mskv_store_fp4_kvcache(const void* key, int64_t key_stride,
                            const void* value, int64_t value_stride,

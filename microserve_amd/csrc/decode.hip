@@ -1207,6 +1207,11 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
   if (!query || !k_cache || !v_cache || !k_scale_cache || !v_scale_cache ||
       !cache_seqlens || !block_tables || !out)
     return MSKV_EINVAL;
+  // (buffer loads take the address's last bits for zero)
+  if (std::is_same<Cache, Fp4Cache>::value &&
+      (misaligned({query, k_cache, v_cache}) ||
+       (((uintptr_t)k_scale_cache | (uintptr_t)v_scale_cache) & 3)))
+    return MSKV_EINVAL;
   const size_t need =
       mskv_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_splits);
   if (need > 0 && (!workspace || workspace_bytes < need)) return MSKV_EWORKSPACE;

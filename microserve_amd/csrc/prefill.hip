@@ -837,6 +837,9 @@ static int prefill_checked(
   if (num_seqs > 65535 || qblocks > 65535) return MSKV_EUNSUPPORTED;
   // rows go to LDS directly, 16 bytes a lane (scales four)
   if (misaligned({query, k_cache, v_cache, out, workspace})) return MSKV_EINVAL;
+  // positions up to a table's width stay within int
+  if (kFp4 && (int64_t)max_blocks_per_seq * block_size > 0x7FFFFFFFLL - kPStep)
+    return MSKV_EUNSUPPORTED;
   if (kFp4 && ((uintptr_t)k_scale_cache | (uintptr_t)v_scale_cache) % 4) return MSKV_EINVAL;
   // without a workspace, one workgroup walks all the keys of its rows
   a.splits = 1;

@@ -30,7 +30,8 @@ def fp4_decode_attention(
     ``fp8_decode_attention``'s arguments and rules: rows of length 0 are
     zeros, block ids outside the pool read as empty, the split count depends
     on shapes only and the split partials live in the persistent scratch of
-    the (device, stream), so the call may be captured in a HIP graph.
+    the (device, stream), so the call may be captured in a HIP graph; graphs
+    captured on one stream share that scratch and replay one after the other.
     """
     res = _lib.fast.decode4(query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens,
                             block_tables, softmax_scale, out, _scratch)

@@ -77,7 +77,8 @@ def store_fp4_kvcache(
 
     ``store_fp8_kvcache``'s arguments over the 4-bit cache.  Token ``t`` lands
     in slot ``slot_mapping[t]``: token ``slot % BS`` of block ``slot // BS``;
-    slots outside the cache are skipped, and a slot may be named once.  K's
+    slots outside the cache are skipped, and one that several tokens name (as
+    the runner's padding does its garbage slot) holds unspecified bytes.  K's
     scale is the power of two, for each 32 dimensions, that brings the largest
     magnitude to at most 7 (a 7 rounds to 6, half of the last step); V's is
     ``max(amax, 1e-8) / 6``.  Codes are nearest, ties to even.  32 dimensions

@@ -202,6 +202,19 @@ def test_the_c_entries_refuse_before_any_launch():
     assert prefill(bs=64) == U and prefill(d=64) == U and prefill(seqs=70000, cu=FAKE) == U
 
 
+def test_attention_refuses_other_alignments_and_tables_past_an_int():
+    lib = _lib.load()
+    splits = lib.mskv_fp4_decode_num_splits(2, 4, 2, 1, 128)
+    for at in range(5):  # query, K, V and the two scales
+        ptrs = [FAKE + (2 if i == at else 0) for i in range(5)]
+        assert lib.mskv_fp4_decode_attention(*ptrs, FAKE, FAKE, FAKE, 2, 4, 2, 128, 128, 8, 1, 0.1,
+                                             0, splits, FAKE, 1 << 20, None) == -1
+        assert lib.mskv_fp4_prefill_attention(*ptrs, FAKE, None, None, 0, FAKE, 1, 4, 4, 0, 4, 2,
+                                              128, 128, 8, 4, 0.1, 0, None, 0, None) == -1
+    assert lib.mskv_fp4_prefill_attention(*[FAKE] * 6, None, None, 0, FAKE, 1, 4, 4, 0, 4, 2, 128,
+                                          128, 8, 1 << 24, 0.1, 0, None, 0, None) == -2
+
+
 def _pool(n=1, base=FAKE, planes=2, stride=None, page=256, blocks=8):
     stride = blocks * page if stride is None else stride
     return (n, (ctypes.c_void_p * n)(*[base] * n), (ctypes.c_int64 * n)(*[planes] * n),
@@ -241,6 +254,7 @@ def test_page_moves_refuse_before_any_launch():
     assert compact(n=-1) == E and compact(tables=None) == E and compact(remap=None) == E
     assert compact(new=None) == E and compact(new=FAKE) == E  # tables that others still read
     assert compact(new=FAKE + 12) == E and compact(new=FAKE - 12) == E
+    assert compact(remap=FAKE + 12) == E  # written over the tables
     assert compact(blocks=0) == E and compact(blocks=1 << 19) == U
     assert compact(page=8) == U
 

@@ -198,6 +198,21 @@ def test_calls_on_two_streams_at_once():
         assert all(torch.equal(o, want[i]) for o in outs[i])
 
 
+def test_no_sequences_and_caches_that_start_on_an_odd_byte():
+    host, dev, tables, q = _decode(31, [200, 130], 8, 2, 128, FP16)
+    none = M.fp4_decode_attention(q[:0].to(H.DEV), *dev, _i32([]), _i32(tables[:0]), SCALE)
+    assert none.shape == (0, 8, 128)
+    none = M.fp4_varlen_prefill_attention(q[:0].to(H.DEV), *dev, _i32(tables[:0]), _i32([0]),
+                                          _i32([0]), 0, SCALE)
+    assert none.shape == (0, 8, 128)
+    flat = torch.zeros(dev[0].numel() + 4, dtype=torch.uint8, device=H.DEV)
+    odd = flat[1:1 + dev[0].numel()].view(dev[0].shape)
+    with pytest.raises(Exception, match="status -1"):
+        M.fp4_decode_attention(q.to(H.DEV), odd, *dev[1:], _i32([200, 130]), _i32(tables), SCALE)
+    with pytest.raises(Exception, match="status -1"):
+        M.fp4_chunk_prefill_attention(q.to(H.DEV), odd, *dev[1:], _i32(tables[0]), 3, SCALE)
+
+
 def test_out_and_views():
     lens = [100, 90]
     host, dev, tables, q = _decode(22, lens, 8, 2, 128, FP16)

@@ -78,9 +78,9 @@ def test_copies_of_a_pool_past_32_bits_of_bytes():
 
 def _plan(tables, n):
     """(remap, live, renamed tables, moves) of the documented rule."""
-    named = sorted({p for p in tables.flatten().tolist() if 0 <= p < n})
-    live = len(named)
-    holes = [p for p in range(live) if p not in set(named)]
+    used = {p for p in tables.flatten().tolist() if 0 <= p < n}
+    named, live = sorted(used), len(used)
+    holes = [p for p in range(live) if p not in used]
     remap = np.full(n, -1, np.int32)
     moves = []
     for p in named:
@@ -104,8 +104,9 @@ def _check_compact(pools, tables, num_blocks, block_dim):
     for p, b in zip(pools, before):
         b = b.movedim(block_dim, 0)
         want = b.clone()
-        for src, dst in moves:
-            want[dst] = b[src]
+        if moves:
+            src, dst = zip(*moves)
+            want[list(dst)] = b[list(src)]
         assert torch.equal(_bytes(p).movedim(block_dim, 0), want)
 
 
@@ -121,6 +122,15 @@ def test_compaction_follows_the_rule(pages, live, width):
         tables.reshape(-1)[:live] = order[:live].numpy()
         tables[-1, 0] = tables[0, 0]  # a shared page
         _check_compact([pool], tables, None, 1)
+
+
+def test_compaction_of_the_most_pages():
+    """2^18 pages: the plan takes 98 KB of a workgroup's memory."""
+    pages = 1 << 18
+    gen = torch.Generator().manual_seed(15)
+    pool = torch.randint(0, 1 << 30, (pages, 4), generator=gen, dtype=torch.int32).to(DEV)
+    _check_compact([pool], torch.randperm(pages, generator=gen)[:90000].to(torch.int32).numpy()
+                   .reshape(300, 300), None, 0)
 
 
 def test_compaction_of_the_runners_pool_keeps_the_garbage_page():
