@@ -1034,7 +1034,7 @@ static size_t partials_bytes(int batch, int hq, int splits) {
 }
 
 template <typename T, typename Cache>
-static hipError_t launch_decode(const DecodeArgs& a, int batch, hipStream_t stream) {
+static hipError_t launch_decode(const DecodeArgs& a, int batch, bool joined, hipStream_t stream) {
   // One 8-wave workgroup (128 KB of LDS) fills a CU.  A grid of at most
   // kWideGridMax of those runs in about two rounds; a larger grid runs in
   // many, over the work items of the pre-pass.  Beyond the
@@ -1044,6 +1044,13 @@ static hipError_t launch_decode(const DecodeArgs& a, int batch, hipStream_t stre
   // 64 x 4096 step prefers 8 waves, 88.3 against 90.5 us.  Shapes only, so
   // the choice is the same on every call of a captured graph.
   const int units = a.hk * a.qgroups;
+  if constexpr (std::is_same<Cache, Fp4Cache>::value) {
+    if (joined) {
+      hipLaunchKernelGGL(decode_fp4_joined_kernel<T>, dim3((unsigned)units, 1, (unsigned)batch),
+                         dim3(64 * kJoinWaves), 0, stream, a);
+      return hipGetLastError();
+    }
+  }
   const int64_t wide_wgs = (int64_t)((units + kWavesPerWG - 1) / kWavesPerWG) * a.splits * batch;
   if (a.items) {
     // 8-wave workgroups also run the work items when every wave has a unit:
@@ -1110,7 +1117,7 @@ static int pages_per_split_of(int splits, int w) {
 }
 
 template <typename Cache>
-static int num_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_blocks_per_seq,
+static int shape_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_blocks_per_seq,
                          int block_size) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
       max_blocks_per_seq <= 0)
@@ -1144,6 +1151,44 @@ static int num_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_b
     if (2 * fine >= 3 * splits) splits = fine;
   }
   return (int)splits;
+}
+
+// Whether a workgroup takes the whole of each (sequence, kv head): from the
+// shapes, and only for the 4-bit cache, whose pages hold a head's rows in one
+// piece.  It saves the merge's launch and the partials, and the runs follow the
+// lengths; a wave's chain of steps, 0.9 us each where the chip is not full, is
+// a quarter of the sequence, so few sequences with long tables stay split, and
+// so do those whose work items run long ones first, and one-round shapes of
+// many short tables.  Split against joined, 32 q / 8 kv heads, us (full
+// tables; lengths spread over the logarithm from 16):
+//   1 x 512 8.6, 5.8; 1 x 1024 9.1, 7.5; 1 x 2048 9.7, 11.4
+//   8 x 1024 10.6, 8.2 (9.9, 8.0); 8 x 2048 13.0, 11.9 (10.5, 11.6); 8 x 4096
+//   15.6, 19.4 (12.7, 18.8); 24 x 4096 25.3, 21.8 (20.3, 19.1); 32 x 8192 52,
+//   47 (33, 34); 64 x 300 13.9, 9.0
+//   64 x 4096 51.5, 47.5 (32.7, 23.7); 128 x 4096 95, 90 (55, 32); 192 x 1024
+//   49, 39 (33, 22); 256 x 4096 188, 181 (91, 54)
+//   256 x 512 27, 33 (19, 23); 512 x 512 53, 61 (33, 41); with work items 256 x
+//   8192 385, 369 (73, 85), 512 x 4096 388, 371 (80, 94)
+static bool joined_of(int batch, int num_q_heads, int num_kv_heads, int w, int block_size) {
+  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || w <= 0 || block_size <= 0)
+    return false;
+  const int qgroups = qgroups_of(num_q_heads / num_kv_heads);
+  const int64_t pairs = (int64_t)batch * num_kv_heads * qgroups;
+  const int64_t tokens = (int64_t)w * block_size;
+  if (tokens > kJoinMaxTokens) return false;
+  if (tokens > 1024 && pairs <= tokens / 32) return false;
+  if (pairs > 1024 && tokens <= std::max<int64_t>(512, pairs / 4)) return false;
+  return !ordered_of(batch, num_kv_heads, qgroups,
+                     shape_splits_of<Fp4Cache>(batch, num_q_heads, num_kv_heads, w, block_size));
+}
+
+template <typename Cache>
+static int num_splits_of(int batch, int num_q_heads, int num_kv_heads, int max_blocks_per_seq,
+                         int block_size) {
+  if (std::is_same<Cache, Fp4Cache>::value &&
+      joined_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size))
+    return 1;
+  return shape_splits_of<Cache>(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size);
 }
 
 }  // namespace mskv
@@ -1274,8 +1319,11 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
   a.num_blocks = num_blocks;
   a.scale_log2 = softmax_scale * kLog2e;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipError_t e = act_dtype == MSKV_BFLOAT16 ? launch_decode<__bf16, Cache>(a, batch, s)
-                                            : launch_decode<_Float16, Cache>(a, batch, s);
+  const bool joined = std::is_same<Cache, Fp4Cache>::value &&
+                      joined_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size);
+  hipError_t e = act_dtype == MSKV_BFLOAT16
+                     ? launch_decode<__bf16, Cache>(a, batch, joined, s)
+                     : launch_decode<_Float16, Cache>(a, batch, joined, s);
   return (int)e;
 }
 

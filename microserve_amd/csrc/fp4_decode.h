@@ -247,4 +247,86 @@ struct Fp4Cache {
   }
 };
 
+// The whole of a (sequence, kv head) in one workgroup: its four waves take
+// equal runs of the sequence's steps and join their results in LDS, in one
+// launch and without partials in memory.  Two such workgroups run on a CU at
+// once, 512 on the chip, and start and end apart from each other.  Which
+// shapes take it, and what it measured, stands at joined_of.  (Eight waves of
+// half the steps were no faster up to 2048 tokens: 64 x 4096 51.8 against 47
+// us, 32 x 2048 16.4 against 14.8, 8 x 4096 17.9 against 19.4.)
+constexpr int kJoinWaves = 4;
+constexpr int64_t kJoinMaxTokens = 8192;
+static_assert(kJoinMaxTokens / Fp4Cache::kPageUnit <= 64, "a table's entries fit a wave's lanes");
+
+template <typename T>
+__global__ __launch_bounds__(64 * kJoinWaves)
+__attribute__((amdgpu_waves_per_eu(2, 8)))
+void decode_fp4_joined_kernel(DecodeArgs a) {
+  using A = Act<T>;
+  constexpr int W = kJoinWaves;
+  // a wave's tiles, then its output: 16 heads of 128 dimensions, 16-byte chunks
+  // XOR-swizzled by the head
+  __shared__ __attribute__((aligned(16))) Fp4Cache::Tiles tiles[W];
+  __shared__ __attribute__((aligned(16))) Fp4Cache::Scales scales[W];
+  __shared__ float s_m[W][16], s_l[W][16];
+  static_assert(sizeof(Fp4Cache::Tiles) >= 16 * kHeadDim * sizeof(float), "");
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int g = lane >> 4, n = lane & 15;
+  const int unit = blockIdx.x, b = blockIdx.z;
+  // (the length and the block ids, 64 at most, in one round trip)
+  const int32_t* row = a.bt + (int64_t)b * a.w;
+  const int entry = row[min(lane, a.w - 1)];
+  const int L = min(__builtin_amdgcn_readfirstlane(a.seqlens[b]), a.w * a.bs);
+  const int kvh = unit / a.qgroups;
+  const int first = (unit - kvh * a.qgroups) * 16;  // head within the group
+  const int heads = min(16, a.group - first);
+  const int qh0 = kvh * a.group + first;
+  const int steps = (max(L, 0) + Fp4Cache::kUnit - 1) / Fp4Cache::kUnit;
+  const int per = (steps + W - 1) / W * Fp4Cache::kUnit;
+  const int t_begin = wave * per, t_end = min(L, t_begin + per);
+  f32x4 acc[8];
+  float m = -INFINITY, l = 0.0f;
+  if (t_begin < t_end) {
+    const int blk = __builtin_amdgcn_readlane(entry, t_begin / a.bs);
+    Fp4Cache::attend<T>(a, b, kvh, qh0 + n, n < heads, t_begin, t_end, blk, lane, tiles[wave],
+                        scales[wave], acc, m, l);
+  } else {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  wave_lds_sync();
+  auto* part = reinterpret_cast<f32x4(*)[16][kHeadDim / 4]>(&tiles[0][0][0]);
+  if (n < heads) {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) part[wave][n][(4 * dt + g) ^ n] = acc[dt];
+  }
+  if (g == 0) {
+    s_m[wave][n] = m;
+    s_l[wave][n] = l;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * (kHeadDim / 4); i += 64 * W) {
+    const int h = i / (kHeadDim / 4), c = i % (kHeadDim / 4);
+    float top = s_m[0][h];
+#pragma unroll
+    for (int w = 1; w < W; ++w) top = fmaxf(top, s_m[w][h]);
+    // (no token seen: every weight 2^-inf, of zeros or of NaNs)
+    if (top == -INFINITY) top = 0.0f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float p = exp2_fast(s_m[w][h] - top);
+      sum += part[w][h][c ^ h] * p;
+      den += s_l[w][h] * p;
+    }
+    sum *= den > 0.0f ? 1.0f / den : 0.0f;
+    const uint32_t lo = (uint32_t)A::from_f32(sum[0]) | ((uint32_t)A::from_f32(sum[1]) << 16);
+    const uint32_t hi = (uint32_t)A::from_f32(sum[2]) | ((uint32_t)A::from_f32(sum[3]) << 16);
+    *reinterpret_cast<u32x2*>(a.out + ((int64_t)b * a.hq + qh0 + h) * kHeadDim + 4 * c) =
+        u32x2{lo, hi};
+  }
+}
+
 }  // namespace mskv

@@ -185,7 +185,8 @@ def test_the_c_entries_refuse_before_any_launch():
     assert decode(d=64) == U and decode(bs=64) == U and decode(bs=192) == U
     assert decode(w=1 << 23) == U
     assert decode(splits=999) == E and decode(w=1, kc=None) == E
-    assert lib.mskv_fp4_decode_num_splits(2, 4, 2, 4, 128) > 1 and decode() == W
+    assert lib.mskv_fp4_decode_num_splits(2, 4, 2, 90, 128) > 1 and decode(w=90) == W
+    assert lib.mskv_fp4_decode_num_splits(2, 4, 2, 4, 128) == 1  # (no workspace)
 
     def prefill(seqs=1, total=4, cu=None, scale=0.1, bs=128, d=128, hq=4, prefix=0, kc=FAKE,
                 ks=FAKE, dt=0):

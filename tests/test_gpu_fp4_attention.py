@@ -59,14 +59,20 @@ def test_decode_matches_the_oracle(dtype, lens, hq, hk, block, width):
     _check_decode(*_decode(1 + len(lens), lens, hq, hk, block, dtype, width), lens)
 
 
-@pytest.mark.parametrize("lens,hq,hk,width,kind", [
-    ([320] * 70, 8, 8, 0, "one launch of four splits at most"),
-    ([40, 900, 3, 0, 260] * 10, 4, 4, 48, "work items of few heads"),
-    ([60, 1500, 2, 0, 128, 700] * 12, 8, 8, 24, "work items"),
-    ([5000, 70, 1, 0], 8, 1, 64, "splits that follow the lengths"),
-    ([9000], 2, 2, 70, "the wide merge")])
-def test_decode_of_every_launch_form(lens, hq, hk, width, kind):
-    _check_decode(*_decode(41, lens, hq, hk, 128, BF16, width), lens)
+@pytest.mark.parametrize("lens,hq,hk,block,width,kind", [
+    ([1, 64, 65, 128, 129, 0, 255, 256, 257, 511, 512, 513, 1000, 1024], 34, 2, 128, 8,
+     "joined, with idle lanes"),
+    ([1, 320, 64] * 23, 8, 8, 128, 0, "joined"),
+    ([8192, 70] + [300] * 15, 16, 16, 256, 0, "joined, the longest"),
+    ([90, 128, 1] * 40, 32, 32, 128, 0, "a wave each"),
+    ([100, 0, 128] * 400, 8, 8, 128, 0, "a wave each, of more workgroups"),
+    ([130] * 63 + [5000], 8, 8, 256, 64, "splits of the shape"),
+    ([40, 900, 3, 0, 260] * 24, 4, 4, 128, 66, "work items of few heads"),
+    ([60, 1500, 2, 0, 128, 700] * 24, 8, 8, 128, 65, "work items"),
+    ([5000, 70, 1, 0], 8, 1, 128, 64, "splits that follow the lengths"),
+    ([9000], 2, 2, 128, 70, "the wide merge")])
+def test_decode_of_every_launch_form(lens, hq, hk, block, width, kind):
+    _check_decode(*_decode(41, lens, hq, hk, block, BF16, width), lens)
 
 
 def test_decode_lengths_past_the_table_are_cut():
@@ -74,28 +80,37 @@ def test_decode_lengths_past_the_table_are_cut():
     _check_decode(host, dev, tables, q, [5000, 300])
 
 
-def test_decode_skips_blocks_outside_the_pool():
-    host, dev, tables, q = _decode(6, [300, 400, 100], 8, 2, 128, BF16)
+# tables of a few pages: a workgroup takes a head's whole sequence; of many: the
+# sequences are split and merged
+WIDTHS = pytest.mark.parametrize("width", [8, 60])
+
+
+@WIDTHS
+def test_decode_skips_blocks_outside_the_pool(width):
+    host, dev, tables, q = _decode(6, [300, 400, 100], 8, 2, 128, BF16, width)
     tables[0, 0], tables[1, 2], tables[2, 0] = 999, -7, -1
     got = _check_decode(host, dev, tables, q, [300, 400, 100])
     assert (got[2] == 0).all()
 
 
+@WIDTHS
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
-def test_decode_of_any_scale(scale):
-    host, dev, tables, q = _decode(7, [200, 70], 8, 2, 128, FP16)
+def test_decode_of_any_scale(scale, width):
+    host, dev, tables, q = _decode(7, [200, 70], 8, 2, 128, FP16, width)
     _check_decode(host, dev, tables, q, [200, 70], scale)
 
 
+@WIDTHS
 @pytest.mark.parametrize("ratio", [1e3, 1e5, 1e-5])
-def test_values_of_very_different_sizes(ratio):
+def test_values_of_very_different_sizes(ratio, width):
     """One key a step whose V is `ratio` times the others', with a low score:
     the others keep their precision."""
     gen = torch.Generator().manual_seed(14)
     host, dev = H.filled(gen, 4, 2, 128, v_gain=0.01 if ratio > 1 else 10.0)
-    tables = np.array([[2, 0, 3]], np.int32)
+    tables = np.full((1, width), -1, np.int32)
+    tables[0, :3] = 2, 0, 3
     q = torch.randn(1, 8, 128, generator=gen).to(BF16)
-    for page in tables[0]:
+    for page in tables[0, :3]:
         host[3][page, :, 5::64] *= np.float32(ratio)
         host[0][page, :, 0::4, :, 5] = 0  # score 0 by codes of 0
     dev = H.to_gpu(host)
@@ -106,10 +121,11 @@ def test_values_of_very_different_sizes(ratio):
     H.check(row, *want, BF16, 380, host[3].max(), 4)
 
 
+@WIDTHS
 @pytest.mark.parametrize("where", ["query", "key", "value"])
-def test_a_nan_reaches_the_rows_that_see_it_and_no_other(where):
+def test_a_nan_reaches_the_rows_that_see_it_and_no_other(where, width):
     lens = [200, 500, 70]
-    host, dev, tables, q = _decode(8, lens, 8, 2, 128, FP16, width=40)
+    host, dev, tables, q = _decode(8, lens, 8, 2, 128, FP16, width)
     page = tables[1, 2]
     if where == "query":
         q[1, 4, 100] = float("nan")
@@ -130,11 +146,12 @@ def test_a_nan_reaches_the_rows_that_see_it_and_no_other(where):
     assert bad[first:, 4:].all() and not bad[:first].any() and not bad[:, :4].any()
 
 
-def test_garbage_behind_the_last_token_is_not_seen():
+@WIDTHS
+def test_garbage_behind_the_last_token_is_not_seen(width):
     """Scales of NaN and infinity, and any codes, behind the sequence's end
     and in its unused pages."""
     for n in (1, 60, 64, 100, 128, 190):
-        host, dev, tables, q = _decode(15, [n], 8, 2, 128, BF16, width=3, extra=2)
+        host, dev, tables, q = _decode(15, [n], 8, 2, 128, BF16, width, extra=2)
         want = _decode_want(q, host, [n], tables, SCALE)
         pages = -(-n // 128)
         used = np.zeros((host[1].shape[0], 128), bool)
@@ -153,9 +170,10 @@ def test_garbage_behind_the_last_token_is_not_seen():
         H.check(got, *want, BF16, n, 1.0, 4)
 
 
-def test_decode_graph_replays_with_new_lengths_beside_eager_calls():
+@WIDTHS
+def test_decode_graph_replays_with_new_lengths_beside_eager_calls(width):
     lens = [300, 900, 0, 64]
-    host, dev, tables, q = _decode(16, lens, 8, 2, 128, BF16, width=12)
+    host, dev, tables, q = _decode(16, lens, 8, 2, 128, BF16, width)
     q, lens_t, tables_t = q.to(H.DEV), _i32(lens), _i32(tables)
     out = torch.empty_like(q)
 
