@@ -506,8 +506,8 @@ int mskv_copy_kv_blocks(int num_pools, void* const* bases,
  * block_tables: int32 [num_entries]; entries outside [0, num_blocks) (-1
  * padding, a garbage page behind the pool) are kept as they are, and
  * several entries may name one page.  new_tables [num_entries]: the entries
- * renamed; it may not overlap block_tables (MSKV_EINVAL).  remap
- * [num_blocks]: each page's new place, -1 for a free one.  num_live [1]: n.
+ * renamed.  remap [num_blocks]: each page's new place, -1 for a free one.
+ * num_live [1]: n.  None of the three may overlap block_tables (MSKV_EINVAL).
  * All on the device; nothing is read on the host.  num_blocks here is the
  * number of pages that may move, at most 2^18 (else MSKV_EUNSUPPORTED);
  * plane_strides may leave room for more behind them.
