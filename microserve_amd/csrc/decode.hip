@@ -60,6 +60,9 @@
 //  * Every page is read through a buffer resource sized to that page; an
 //    invalid block id gives a zero-length resource (loads return 0) and its
 //    tokens are masked, so a bad table entry cannot fault.
+//
+// The split kernel, the merges and the pre-pass are templates over the cache:
+// fp4_decode.h holds the walk over the 4-bit one, and its form of one launch.
 #include <math.h>
 
 #include <algorithm>

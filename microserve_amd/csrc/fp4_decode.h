@@ -31,11 +31,11 @@ struct Fp4Cache {
   // A split of a grid of many rounds holds twice the FP8 cache's pages, its
   // bytes, and a workgroup of work items half the waves (two workgroups a CU,
   // whose starts and ends overlap).  At 4 pages and 8 waves / 8 and 8 / 8 and
-  // 4 / 16 and 4, us: 256 x 16 to 32768 tokens 217 / 215 / 208 / 209, 128 x
+  // 4 / 16 and 4, all split, us: 256 x 16 to 32768 tokens 217 / 215 / 208 / 209, 128 x
   // 8192 200 / 190 / 192 / 186, 256 x 16 to 8192 76 to 82 / 80 / 75 / 160.
   static constexpr int kMaxPages = 8;
-  // one step is the least of a split: 1 x 700 tokens 10.0 us (two steps 11.8),
-  // 8 x 1000 10.4 (12.1)
+  // one step is the least of a split: under tables of 128 entries, 1 x 700
+  // tokens 10.0 us (two steps 11.8), 8 x 1000 10.4 (12.1)
   static constexpr int kMinSteps = 1;
   static constexpr int kItemWaves = kNarrowWaves;
   // a token whose bytes (64 a token, 31 bits) lie past the end of any page
