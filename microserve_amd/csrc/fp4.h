@@ -38,12 +38,13 @@ template <typename T> struct Fp4Query { static constexpr int parts = 3; };
 template <> struct Fp4Query<__bf16> { static constexpr int parts = 2; };
 
 // S^T += K . Q^T for 16 tokens: A the codes under their block scales (byte
-// kByte of `ks`), B a part of the query
+// kByte of `ks`), B a part of the query under its row's scale byte
 template <int kByte>
-__device__ __forceinline__ f32x4 mfma_fp4(const u32x4& k, uint32_t ks, const i32x8& q, f32x4 c) {
+__device__ __forceinline__ f32x4 mfma_fp4(const u32x4& k, uint32_t ks, const i32x8& q,
+                                          uint32_t qscale, f32x4 c) {
   const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, c, 4 /* fp4 */, 0 /* e4m3 */,
-                                                          kByte, (int)ks, 0, 127);
+                                                          kByte, (int)ks, 0, (int)qscale);
 }
 
 // The pieces of a query row that lane (g, n) holds in the B operand: the e4m3
@@ -60,13 +61,24 @@ __device__ __forceinline__ QueryRow load_query(const uint16_t* row, int g) {
   return q;
 }
 
+// What the products of a query row's parts come in: the scale byte they are
+// multiplied under, and what takes them to q . k.
+struct QueryScale {
+  uint32_t byte;
+  float unit;
+};
+
 // The query row of lane (g, n) as the B operand: e4m3 parts of q * f, f the
 // power of two that brings the row's largest magnitude near e4m3's (q * f is
-// exact).  Returns f; NaNs for a row that holds an infinity or a NaN, zeros
-// where !ok.
+// exact; below 2^-117 f stays 2^126).  NaNs for a row that holds an infinity or
+// a NaN, zeros where !ok.
+// Where f is above 1, the scale byte takes it back out inside the MFMA: keys
+// large enough to meet so small a query would overflow the products else (a
+// key of 10^34 times 448).  Below 1 the products stay in units of 1 / f, as
+// large queries times ordinary keys would overflow without.
 template <typename T>
-__device__ __forceinline__ float fp4_query(const QueryRow& row, bool ok,
-                                           i32x8 (&qp)[Fp4Query<T>::parts]) {
+__device__ __forceinline__ QueryScale fp4_query(const QueryRow& row, bool ok,
+                                                i32x8 (&qp)[Fp4Query<T>::parts]) {
   using A = Act<T>;
   float x[32];
 #pragma unroll
@@ -92,7 +104,7 @@ __device__ __forceinline__ float fp4_query(const QueryRow& row, bool ok,
   const bool finite = top < 0x7F800000u;
   const uint32_t nan = finite ? 0u : 0x7F7F7F7Fu;
   const float amax = finite ? __uint_as_float(top) : 0.0f;
-  const float f = amax > 1e-30f ? pow2_floor(kFp8Max / amax) : 1.0f;
+  const float f = fminf(amax > 0.0f ? pow2_floor(kFp8Max / amax) : 1.0f, 0x1p126f);
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
     float y[4];
@@ -110,7 +122,9 @@ __device__ __forceinline__ float fp4_query(const QueryRow& row, bool ok,
       qp[2][c] = (int)lo;
     }
   }
-  return f;
+  // (127 - log2 f, from f's exponent field)
+  const bool small = f > 1.0f;
+  return {small ? 254u - (__float_as_uint(f) >> 23) : 127u, small ? 1.0f : 1.0f / f};
 }
 
 // The query in e2m3 parts, for the prefill: against codes, a 6-bit operand runs

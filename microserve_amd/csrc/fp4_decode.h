@@ -113,8 +113,9 @@ struct Fp4Cache {
     issue(t_begin + kUnit, odd);
 
     i32x8 qp[NQ];
+    const QueryScale qu = fp4_query<T>(row, head_ok, qp);
     // scores in log2 units: S^T * qs
-    const float qs = a.scale_log2 / fp4_query<T>(row, head_ok, qp);
+    const float qs = a.scale_log2 * qu.unit;
 
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -155,16 +156,16 @@ struct Fp4Cache {
       // lane (g, n): scores of tokens 16c + 4g + r of head n
       f32x4 s[4];
       const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-      s[0] = mfma_fp4<0>(cur.k[0], cur.kscale, qp[0], zero);
-      s[1] = mfma_fp4<1>(cur.k[1], cur.kscale, qp[0], zero);
-      s[2] = mfma_fp4<2>(cur.k[2], cur.kscale, qp[0], zero);
-      s[3] = mfma_fp4<3>(cur.k[3], cur.kscale, qp[0], zero);
+      s[0] = mfma_fp4<0>(cur.k[0], cur.kscale, qp[0], qu.byte, zero);
+      s[1] = mfma_fp4<1>(cur.k[1], cur.kscale, qp[0], qu.byte, zero);
+      s[2] = mfma_fp4<2>(cur.k[2], cur.kscale, qp[0], qu.byte, zero);
+      s[3] = mfma_fp4<3>(cur.k[3], cur.kscale, qp[0], qu.byte, zero);
 #pragma unroll
       for (int p = 1; p < NQ; ++p) {
-        s[0] = mfma_fp4<0>(cur.k[0], cur.kscale, qp[p], s[0]);
-        s[1] = mfma_fp4<1>(cur.k[1], cur.kscale, qp[p], s[1]);
-        s[2] = mfma_fp4<2>(cur.k[2], cur.kscale, qp[p], s[2]);
-        s[3] = mfma_fp4<3>(cur.k[3], cur.kscale, qp[p], s[3]);
+        s[0] = mfma_fp4<0>(cur.k[0], cur.kscale, qp[p], qu.byte, s[0]);
+        s[1] = mfma_fp4<1>(cur.k[1], cur.kscale, qp[p], qu.byte, s[1]);
+        s[2] = mfma_fp4<2>(cur.k[2], cur.kscale, qp[p], qu.byte, s[2]);
+        s[3] = mfma_fp4<3>(cur.k[3], cur.kscale, qp[p], qu.byte, s[3]);
       }
       // (not before the products: the loads would take other registers, and
       // moving those at the loop's end would wait for them)
