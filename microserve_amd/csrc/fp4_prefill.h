@@ -23,6 +23,22 @@ namespace mskv {
 
 template <int N> using Int = std::integral_constant<int, N>;
 
+// What a row's exponents are taken against, from its running maximum m of the
+// unscaled scores: exponent = (score - base) * scale - log.  With base 0, log
+// is m * scale, whose rounding the row's keys share, and the exponent is one
+// fma.  Past kPFar in log2 units that rounding would show (from 2^27 up by more
+// than 2^3, and weights would leave fp16's range): such scores are
+// subtracted before the scale.  A row without a key (-FLT_MAX) is none of those.
+constexpr float kPFar = 1 << 20;
+struct Level {
+  float base, log;
+};
+__device__ __forceinline__ Level level_of(float m, float scale) {
+  const float log = fmaxf(m * scale, -FLT_MAX);
+  const bool far = fabsf(log) > kPFar && m != -FLT_MAX;
+  return {far ? m : 0.0f, far ? 0.0f : log};
+}
+
 // kSplit: the workgroup takes one of a.splits ranges of the keys (whole
 // tiles, from the actual key count) and leaves partials for the merge.
 template <typename T, bool kSplit>
@@ -136,7 +152,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
   // denominator, as the output tile of an all-ones A operand against P^T,
   // so every row of it holds its column's sum of the fp16 probabilities
   f32x4 acc[kPBlocks][8], lacc[kPBlocks];
-  float m[kPBlocks];
+  float m[kPBlocks];  // the running maxima, of the scores before the scale
 #pragma unroll
   for (int b = 0; b < kPBlocks; ++b) {
 #pragma unroll
@@ -144,8 +160,9 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
     lacc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
     // -FLT_MAX rather than -inf: a row that has seen no key yet keeps it,
     // and its masked (-inf) scores still give p = 0 with no select; the
-    // first finite score raises it like any other growth
-    m[b] = -FLT_MAX;
+    // first finite score raises it like any other growth (an idle lane's row
+    // needs none)
+    m[b] = row_ok[b] ? -FLT_MAX : 0.0f;
   }
   float fw = 0.0f;
   f16x8 ones;
@@ -246,12 +263,13 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      // Row maxima in log2 units (qs > 0 per row).  Each lane tests its own
+      // Row maxima (the scale is positive: they keep their order).  Each lane tests its own
       // 32 scores against the row's running max: a row's maximum is the
       // largest of its four lanes', and the positive scale keeps the order,
       // so the wave vote equals the test on the row maxima, and the
       // cross-lane reduction runs only when the vote passes.
-      float lm[kPBlocks];
+      // Maxima past kPFar take that way with every tile.
+      float lm[kPBlocks], ml[kPBlocks];  // (ml: of m, as the exponents below take it)
       bool grow = false;
 #pragma unroll
       for (int b = 0; b < kPBlocks; ++b) {
@@ -260,17 +278,30 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
         for (int tt = 1; tt < kGroups; ++tt)
           v = fmaxf(fmaxf(v, st[b][tt][0]), fmaxf(fmaxf(st[b][tt][1], st[b][tt][2]), st[b][tt][3]));
         lm[b] = v;
-        grow |= v * a.scale_log2 > m[b] + kPSlack;
+        ml[b] = fmaxf(m[b] * a.scale_log2, -FLT_MAX);
+        grow |= v * a.scale_log2 > ml[b] + kPSlack || fabsf(ml[b]) > kPFar;
       }
       if (__any(grow)) {
+        float base[kPBlocks];
+        bool far = false;
 #pragma unroll
         for (int b = 0; b < kPBlocks; ++b) {
-          const float m_new = fmaxf(m[b], max_xor32(max_xor16(lm[b])) * a.scale_log2);
-          const float alpha = exp2_fast(m[b] - m_new);
+          const float m_new = fmaxf(m[b], max_xor32(max_xor16(lm[b])));
+          const Level was = level_of(m[b], a.scale_log2), is = level_of(m_new, a.scale_log2);
+          const float alpha = exp2_fast(fmaf(was.base - is.base, a.scale_log2, was.log - is.log));
+          ml[b] = is.log;
+          base[b] = is.base;
+          far |= is.base != 0.0f;
           lacc[b] *= alpha;
 #pragma unroll
           for (int dt = 0; dt < 8; ++dt) acc[b][dt] *= alpha;
           m[b] = m_new;
+        }
+        if (__any(far)) {
+#pragma unroll
+          for (int b = 0; b < kPBlocks; ++b)
+#pragma unroll
+            for (int tt = 0; tt < kGroups; ++tt) st[b][tt] -= base[b];
         }
       }
       // The PV product runs on v_mfma_f32_16x16x32_f16.  V converts to fp16
@@ -338,7 +369,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
           for (int b = 0; b < kPBlocks; ++b) {
             float pf[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) pf[r] = exp2_fast(fmaf(st[b][tt][r], a.scale_log2, -m[b]));
+            for (int r = 0; r < 4; ++r) pf[r] = exp2_fast(fmaf(st[b][tt][r], a.scale_log2, -ml[b]));
             const f16x2 p01 = {(_Float16)pf[0], (_Float16)pf[1]};
             const f16x2 p23 = {(_Float16)pf[2], (_Float16)pf[3]};
             f16x2 w01, w23;
@@ -465,7 +496,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp4_kernel(Prefill
       if (g == 0)
         part_lse[row * splits + max(split, 0)] = split < 0      ? kPWritten
                                                  : is_nan(lt)   ? FLT_MAX
-                                                 : lt > 0.0f    ? m[b] + __log2f(lt)
+                                                 : lt > 0.0f    ? m[b] * a.scale_log2 + __log2f(lt)
                                                                 : -INFINITY;
       if (split >= 0) {
         float* po = part_o + (row * splits + split) * kHeadDim;

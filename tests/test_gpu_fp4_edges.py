@@ -1,11 +1,13 @@
 """The 4-bit attention where its arithmetic could give way: keys and queries
-near the ends of their types, and queries whose parts split unevenly."""
+near the ends of their types, scores of any size, and queries whose parts
+split unevenly."""
 
 import numpy as np
 import pytest
 import torch
 
 import microserve_amd as M
+from microserve_amd import _lib
 from oracle import fp4_oracle as O
 from tests import fp4_helpers as H
 
@@ -56,6 +58,82 @@ def test_keys_and_queries_near_the_ends_of_their_types(dtype, k_gain, q_gain):
     for form, weights, got in _both(q, dev, tables, lens, scale):
         assert got.isfinite().all(), form
         H.check(got, *want, dtype, max(lens), host[3].max(), weights)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_scores_of_any_size_keep_the_largest_key(dtype):
+    """Scores far beyond exp2's range: the row is its best key's value."""
+    gen = torch.Generator().manual_seed(62)
+    k_gain = 1e34 if dtype == BF16 else 1e30
+    lens = [200, 70, 3]
+    host, dev = H.filled(gen, 5, HK, BLOCK, k_gain=k_gain)
+    tables = H.tables_of(gen, lens, BLOCK, 5)
+    q = torch.randn(3, HQ, 128, generator=gen).to(dtype)
+    for form, _, got in _both(q, dev, tables, lens, 1.0):
+        got = got.double().cpu().numpy()
+        assert np.isfinite(got).all(), form
+        for i, n in enumerate(lens):
+            k, v = O.rows(host, tables[i], n)
+            for h in range(HQ):
+                kh = k[h * HK // HQ]
+                s = kh @ q[i, h].double().numpy()
+                order = np.argsort(s)
+                # (2^-14 of the reach is what a score may be off by)
+                reach = q[i, h].abs().max().item() * np.abs(kh).sum(-1).max()
+                if s[order[-1]] - s[order[-2]] < 2.0 ** -12 * reach:
+                    continue
+                best = v[h * HK // HQ, order[-1]]
+                # the value's fp16 product, the weight and the output's type round once each
+                tol = (2.0 ** -10 + torch.finfo(dtype).eps / 2) * np.abs(best) + 1e-6
+                assert (np.abs(got[i, h] - best) <= tol).all(), (form, i, h)
+
+
+@pytest.mark.parametrize("sign", [1, -1, 0])
+@pytest.mark.parametrize("splits", [False, True])
+def test_prefill_scores_that_leave_the_exponents_range_on_the_way(sign, splits):
+    """Keys of growing size, from ordinary scores to 10^14, above zero (+1) or of
+    either sign (0), or of shrinking size and all scores below zero (-1).  Rows
+    whose best key is clear are its value; the others stay finite."""
+    gen = torch.Generator().manual_seed(66)
+    lq, lc = (20, 2400) if splits else (150, 420)
+    lk = lq + lc
+    pool = -(-lk // BLOCK)
+    base = torch.randn(HK, 128, generator=gen)
+    k = base * (1 + 0.3 * torch.randn(lk, HK, 128, generator=gen)) if sign else torch.randn(
+        lk, HK, 128, generator=gen)
+    k = k * 10 ** (torch.linspace(0, 12, lk) if sign >= 0 else torch.linspace(12, 4, lk))[
+        :, None, None]
+    v = torch.randn(lk, HK, 128, generator=gen)
+    host = H.empty(pool, HK, BLOCK)
+    O.store(k.numpy(), v.numpy(), host, np.arange(lk))
+    dev, table = H.to_gpu(host), np.arange(pool)
+    q = torch.randn(lq, HQ, 128, generator=gen)
+    if sign:
+        q = sign * base.repeat_interleave(HQ // HK, 0) + 0.1 * q
+    q = q.to(BF16)
+    need = _lib.load().mskv_fp8_prefill_bounded_workspace_bytes(1, lq, lq, lk, HQ, HK, 128, BLOCK,
+                                                                pool)
+    assert (need > 0) == splits
+    got = M.fp4_chunk_prefill_attention(q.to(H.DEV), *dev, _i32(table), lc, 1.0)
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    kk, vv = O.rows(host, table, lk)
+    clear = 0
+    for h in range(HQ):
+        kh, vh = kk[h * HK // HQ], vv[h * HK // HQ]
+        s = q[:, h].double().numpy() @ kh.T
+        off = 2.0 ** -13 * q[:, h].abs().amax(-1).double().numpy()[:, None] * np.abs(kh).sum(-1)
+        for i in range(lq):
+            n = lc + i + 1
+            best = s[i, :n].argmax()
+            rest = np.delete(np.arange(n), best)
+            # (each score is off by its own key's bound, and 60 units leave nothing of the others)
+            if s[i, best] - off[i, best] < (s[i, rest] + off[i, rest]).max() + 60:
+                continue
+            clear += 1
+            tol = (2.0 ** -9 + torch.finfo(BF16).eps / 2) * np.abs(vh[best]) + 1e-6
+            assert (np.abs(got[i, h] - vh[best]) <= tol).all(), (h, i)
+    assert clear > lq * HQ // 8
 
 
 def _queries(kind, rows, dtype, gen):
