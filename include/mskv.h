@@ -498,6 +498,17 @@ int mskv_copy_kv_blocks(int num_pools, void* const* bases,
                         int64_t num_pairs, void* stream);
 
 /*
+ * What mskv_copy_kv_blocks (compact 0) or mskv_compact_kv_blocks (compact 1)
+ * would say to this pool, without a launch.  A pool of more than
+ * MSKV_MAX_POOLS tensors takes several calls: checking all of them before the
+ * first keeps a refusal from leaving the pool half moved.
+ */
+int mskv_check_kv_blocks(int num_pools, void* const* bases,
+                         const int64_t* planes, const int64_t* plane_strides,
+                         const int64_t* page_bytes, int64_t num_blocks,
+                         int compact);
+
+/*
  * Compact a paged pool (described as in mskv_copy_kv_blocks): the n pages
  * that block_tables names move to places 0 .. n - 1.  A named page below n
  * stays; the i-th one from n up (ascending) takes the i-th free place below

@@ -130,6 +130,7 @@ _PROTOS = {
         _c_int, _c_f32, _c_int, _vp, _c_size, _vp]),
     "mskv_copy_kv_blocks": (_c_int, [
         _c_int, _vp, _vp, _vp, _vp, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "mskv_check_kv_blocks": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _c_i64, _c_int]),
     "mskv_compact_kv_blocks": (_c_int, [
         _c_int, _vp, _vp, _vp, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp]),
 }

@@ -226,7 +226,29 @@ static int pools_of(Pools& p, int count, void* const* bases, const int64_t* plan
   return MSKV_OK;
 }
 
+// The same for a compaction, which numbers its pages in LDS.
+static int compact_pools_of(Pools& p, int count, void* const* bases, const int64_t* planes,
+                            const int64_t* plane_strides, const int64_t* page_bytes,
+                            int64_t num_blocks) {
+  const int status = pools_of(p, count, bases, planes, plane_strides, page_bytes, num_blocks,
+                              kCompactLoads);
+  if (status != MSKV_OK) return status;
+  if (num_blocks <= 0) return MSKV_EINVAL;
+  return num_blocks > kPlanMaxBlocks ? MSKV_EUNSUPPORTED : MSKV_OK;
+}
+
 }  // namespace mskv
+
+extern "C" int mskv_check_kv_blocks(int num_pools, void* const* bases, const int64_t* planes,
+                                    const int64_t* plane_strides, const int64_t* page_bytes,
+                                    int64_t num_blocks, int compact) {
+  using namespace mskv;
+  Pools p;
+  return compact ? compact_pools_of(p, num_pools, bases, planes, plane_strides, page_bytes,
+                                    num_blocks)
+                 : pools_of(p, num_pools, bases, planes, plane_strides, page_bytes, num_blocks,
+                            kCopyLoads);
+}
 
 extern "C" int mskv_copy_kv_blocks(int num_pools, void* const* bases, const int64_t* planes,
                                    const int64_t* plane_strides, const int64_t* page_bytes,
@@ -277,11 +299,11 @@ extern "C" int mskv_compact_kv_blocks(int num_pools, void* const* bases, const i
                                       int32_t* num_live, void* stream) {
   using namespace mskv;
   Pools p;
-  const int status = pools_of(p, num_pools, bases, planes, plane_strides, page_bytes, num_blocks,
-                              kCompactLoads);
+  const int status = compact_pools_of(p, num_pools, bases, planes, plane_strides, page_bytes,
+                                      num_blocks);
   if (status != MSKV_OK) return status;
-  if (num_entries < 0 || num_blocks <= 0) return MSKV_EINVAL;
-  if (num_blocks > kPlanMaxBlocks || num_entries > (int64_t)1 << 40) return MSKV_EUNSUPPORTED;
+  if (num_entries < 0) return MSKV_EINVAL;
+  if (num_entries > (int64_t)1 << 40) return MSKV_EUNSUPPORTED;
   if (!remap || !num_live || (num_entries > 0 && (!block_tables || !new_tables)))
     return MSKV_EINVAL;
   // every workgroup reads the tables while others write the renamed ones

@@ -47,6 +47,13 @@ def _pools(what, caches, block_dim):
     return groups, num_blocks
 
 
+def _check_all(what, lib, groups, num_blocks, compact):
+    """Refuses a pool of several launches before the first of them."""
+    if len(groups) > 1:
+        for count, *described in groups:
+            _lib.check(lib.mskv_check_kv_blocks(count, *described, num_blocks, compact), what)
+
+
 def _ids(what, blocks):
     if isinstance(blocks, torch.Tensor):
         assert not blocks.is_cuda, f"{what}: block ids are host integers"
@@ -66,7 +73,9 @@ def copy_kv_blocks(caches, src_blocks, dst_blocks, block_dim: int = 0) -> None:
     with ``block_dim=2``, one layer's caches with 0.  The ids are host
     integers (the block manager's), a list or a CPU tensor, and travel with
     the launch.  No page may be written twice or be both read and written
-    (AssertionError), so the order of the pairs does not matter.
+    (AssertionError), so the order of the pairs does not matter.  Tensors start
+    and pages end on 16 bytes (RuntimeError); a call that is refused has moved
+    nothing.
 
     To fork a sequence, give the child the parent's full pages and copy the
     partly filled one to a page of its own.
@@ -87,6 +96,7 @@ def copy_kv_blocks(caches, src_blocks, dst_blocks, block_dim: int = 0) -> None:
     assert written.isdisjoint(src), f"{what}: a block is both read and written"
     src_at, dst_at = src.buffer_info()[0], dst.buffer_info()[0]
     lib = _lib.load()
+    _check_all(what, lib, groups, num_blocks, compact=0)
     with _lib.current(tensors[0]):
         stream = _lib.stream_of(tensors[0])
         for count, *described in groups:
@@ -108,7 +118,9 @@ def compact_kv_blocks(caches, block_tables: torch.Tensor, num_blocks: int | None
     ``num_blocks`` is the number of pages that take part, the first ones of
     dimension ``block_dim`` (default: all); entries outside them (-1 padding,
     the runner's garbage page behind the pool) are kept as they are.  Nothing
-    is read on the host, and the call may be captured in a HIP graph.
+    is read on the host, and the call may be captured in a HIP graph.  Refusals
+    are ``copy_kv_blocks``'s, and more than 2^18 pages; they come before any
+    page moves.
     """
     res = _lib.fast.compact_blocks(caches, block_tables, num_blocks, block_dim)
     if res is not None:
@@ -122,6 +134,7 @@ def compact_kv_blocks(caches, block_tables: torch.Tensor, num_blocks: int | None
     _lib.on_device(what, tensors[0], block_tables)
     tables = block_tables.contiguous()
     lib = _lib.load()
+    _check_all(what, lib, groups, num_blocks, compact=1)
     with _lib.current(tables):
         ints = dict(dtype=torch.int32, device=tables.device)
         renamed = torch.empty(tables.shape, **ints)
