@@ -8,6 +8,7 @@ silently take another path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib
 import os
@@ -235,4 +236,9 @@ def current(t):
     """``t``'s GPU as the current device: a launch goes to the device that is
     current, and its stream must be that device's."""
     import torch
+    if t.device.index == torch.cuda.current_device():  # (1 us less than to set it)
+        return _AS_IT_IS
     return torch.cuda.device(t.device)
+
+
+_AS_IT_IS = contextlib.nullcontext()

@@ -175,10 +175,14 @@ bool fits(std::initializer_list<int64_t> v) {
   return true;
 }
 
-// Held around allocations and launches, as torch's and ctypes' own calls do.
-struct NoGil {
+// Held around allocations and launches, as torch's and ctypes' own calls do:
+// the tensors' GPU is current (a launch goes to the current one, and its
+// stream must be that one's), and other threads may run.
+struct OnDevice {
+  const c10::DeviceGuard guard;
   PyThreadState* state = PyEval_SaveThread();
-  ~NoGil() { PyEval_RestoreThread(state); }
+  explicit OnDevice(c10::Device d) : guard(d) {}
+  ~OnDevice() { PyEval_RestoreThread(state); }
 };
 
 // The bodies run inside this: a C++ exception (an allocation that failed,
@@ -223,7 +227,7 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     int status;
     {
-      NoGil no_gil;
+      const OnDevice on(in.device);
       status = api.store(key->data_ptr(), k_stride, value->data_ptr(), v_stride, kc->data_ptr(),
                   vc->data_ptr(), (float*)ks->data_ptr(), (float*)vs->data_ptr(), sl->data_ptr(),
                   st, key->size(0), (int)key->size(1), (int)key->size(2),
@@ -255,8 +259,7 @@ PyObject* store4(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     int status;
     {
-      NoGil no_gil;
-      const c10::DeviceGuard guard(in.device);
+      const OnDevice on(in.device);
       status = api.store4(key->data_ptr(), k_stride, value->data_ptr(), v_stride, kc->data_ptr(),
                           vc->data_ptr(), ks->data_ptr(), (float*)vs->data_ptr(), sl->data_ptr(),
                           st, key->size(0), (int)m.heads, (int)m.d, (int)m.block, m.blocks, dt,
@@ -287,8 +290,7 @@ PyObject* load4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor key, value;
     int status;
     {
-      NoGil no_gil;
-      const c10::DeviceGuard guard(in.device);
+      const OnDevice on(in.device);
       const auto opts = vs->options().dtype(type).requires_grad(false);
       key = at::empty({tokens, m.heads, m.d}, opts);
       value = at::empty({tokens, m.heads, m.d}, opts);
@@ -350,8 +352,7 @@ PyObject* decode_call(PyObject* const* a, Py_ssize_t n) {
     at::Tensor fresh;
     int status;
     {
-      NoGil no_gil;
-      const c10::DeviceGuard guard(in.device);
+      const OnDevice on(in.device);
       if (!given) fresh = at::empty(q->sizes(), q->options().requires_grad(false));
       const at::Tensor& out = given ? *given : fresh;
       auto call = [&](auto f) {
@@ -420,8 +421,7 @@ PyObject* prefill_call(PyObject* const* a, Py_ssize_t n) {
     at::Tensor ws, out;
     int status;
     {
-      NoGil no_gil;
-      const c10::DeviceGuard guard(in.device);
+      const OnDevice on(in.device);
       if (bytes) ws = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte).requires_grad(false));
       out = at::empty(q->sizes(), q->options().requires_grad(false));
       auto call = [&](auto f) {
@@ -477,7 +477,7 @@ PyObject* fresh(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor out;
     int status;
     {
-      NoGil no_gil;
+      const OnDevice on(in.device);
       out = at::empty(q->sizes(), q->options().requires_grad(false));
       status = api.fresh(q->data_ptr(), k->data_ptr(), k_stride, v->data_ptr(), v_stride, out.data_ptr(),
                   (int32_t*)cq->data_ptr(), (int32_t*)ck->data_ptr(), (int)seqs, nq, nk, max_q,
@@ -526,7 +526,7 @@ PyObject* prologue(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool with_k = a[14] == Py_True;
     int status;
     {
-      NoGil no_gil;
+      const OnDevice on(in.device);
       q_out = at::empty({t, hq, d}, opts);
       if (with_k) k_out = at::empty({t, hk, d}, opts);
       status = api.prologue(q->data_ptr(), k->data_ptr(), v->data_ptr(), q->stride(0), k->stride(0),
@@ -603,8 +603,7 @@ PyObject* copy_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!p.take(in, a[0], dim)) return nullptr;
     int status;
     {
-      NoGil no_gil;
-      const c10::DeviceGuard guard(in.device);
+      const OnDevice on(in.device);
       status = api.copy(p.count, p.bases, p.planes, p.strides, p.pages, p.blocks, src.data(),
                         dst.data(), (int64_t)src.size(), stream_of(in.device));
     }
@@ -628,8 +627,7 @@ PyObject* compact_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor renamed, remap, live;
     int status;
     {
-      NoGil no_gil;
-      const c10::DeviceGuard guard(in.device);
+      const OnDevice on(in.device);
       const auto opts = tables->options().requires_grad(false);
       renamed = at::empty(tables->sizes(), opts);
       remap = at::empty({blocks}, opts);

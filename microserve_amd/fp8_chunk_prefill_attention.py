@@ -35,16 +35,17 @@ def _launch(lib, what, query, caches, tables, cu_q, cu_k, prefix_len, output, nu
     ws_bytes = lib.mskv_fp8_prefill_bounded_workspace_bytes(
         num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim,
         block_size, max_blocks)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
-    status = lib.mskv_fp8_prefill_attention_bounded(
-        query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        k_scale_cache.data_ptr(), v_scale_cache.data_ptr(), tables.data_ptr(),
-        None if cu_q is None else cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(),
-        prefix_len, output.data_ptr(), num_seqs, total_q, max_seqlen_q, max_seqlen_k,
-        num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks,
-        float(softmax_scale),
-        _lib.act_dtype(query), None if ws is None else ws.data_ptr(), ws_bytes,
-        _lib.stream_of(query))
+    with _lib.current(query):
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
+        status = lib.mskv_fp8_prefill_attention_bounded(
+            query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale_cache.data_ptr(), v_scale_cache.data_ptr(), tables.data_ptr(),
+            None if cu_q is None else cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(),
+            prefix_len, output.data_ptr(), num_seqs, total_q, max_seqlen_q, max_seqlen_k,
+            num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks,
+            float(softmax_scale),
+            _lib.act_dtype(query), None if ws is None else ws.data_ptr(), ws_bytes,
+            _lib.stream_of(query))
     _lib.check(status, what)
 
 

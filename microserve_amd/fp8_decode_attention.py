@@ -109,15 +109,16 @@ def fp8_decode_attention(
     lib = _lib.load()
     splits, ws_bytes = _plan(batch_size, num_q_heads, num_kv_heads, head_dim,
                              max_num_blocks, block_size)
-    stream = _lib.stream_of(query)
-    ws = _scratch(query.device, stream, ws_bytes) if ws_bytes else None
-    status = lib.mskv_fp8_decode_attention(
-        query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        k_scale_cache.data_ptr(), v_scale_cache.data_ptr(),
-        cache_seqlens.data_ptr(), block_tables.data_ptr(), out.data_ptr(),
-        batch_size, num_q_heads, num_kv_heads, head_dim, block_size,
-        k_cache.shape[0], max_num_blocks, float(softmax_scale),
-        _lib.act_dtype(query), splits,
-        ws.data_ptr() if ws is not None else None, ws_bytes, stream)
+    with _lib.current(query):
+        stream = _lib.stream_of(query)
+        ws = _scratch(query.device, stream, ws_bytes) if ws_bytes else None
+        status = lib.mskv_fp8_decode_attention(
+            query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale_cache.data_ptr(), v_scale_cache.data_ptr(),
+            cache_seqlens.data_ptr(), block_tables.data_ptr(), out.data_ptr(),
+            batch_size, num_q_heads, num_kv_heads, head_dim, block_size,
+            k_cache.shape[0], max_num_blocks, float(softmax_scale),
+            _lib.act_dtype(query), splits,
+            ws.data_ptr() if ws is not None else None, ws_bytes, stream)
     _lib.check(status, "fp8_decode_attention")
     return out

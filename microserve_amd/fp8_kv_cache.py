@@ -48,11 +48,12 @@ def store_fp8_kvcache(
     value, value_stride = _lib.token_rows(value)
     num_slots = k_cache.shape[0] * k_cache.shape[1]
     lib = _lib.load()
-    status = lib.mskv_store_fp8_kvcache_strided(
-        key.data_ptr(), key_stride, value.data_ptr(), value_stride, k_cache.data_ptr(),
-        v_cache.data_ptr(), k_scale_cache.data_ptr(), v_scale_cache.data_ptr(),
-        slot_mapping.data_ptr(),
-        _lib.INT64 if slot_mapping.dtype == torch.int64 else _lib.INT32,
-        num_tokens, num_kv_heads, head_dim, num_slots, _lib.store_dtype(key),
-        _lib.stream_of(key))
+    with _lib.current(key):
+        status = lib.mskv_store_fp8_kvcache_strided(
+            key.data_ptr(), key_stride, value.data_ptr(), value_stride, k_cache.data_ptr(),
+            v_cache.data_ptr(), k_scale_cache.data_ptr(), v_scale_cache.data_ptr(),
+            slot_mapping.data_ptr(),
+            _lib.INT64 if slot_mapping.dtype == torch.int64 else _lib.INT32,
+            num_tokens, num_kv_heads, head_dim, num_slots, _lib.store_dtype(key),
+            _lib.stream_of(key))
     _lib.check(status, "store_fp8_kvcache")

@@ -74,15 +74,16 @@ def qk_norm_rope_store(positions, q, k, v, q_norm_weight, k_norm_weight, eps,
     q_out = torch.empty(n, hq, d, dtype=q.dtype, device=q.device)
     k_out = torch.empty(n, hk, d, dtype=q.dtype, device=q.device) if return_k else None
     lib = _lib.load()
-    _lib.check(lib.mskv_qk_norm_rope_store(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
-        positions.data_ptr(),
-        None if q_norm_weight is None else q_norm_weight.data_ptr(),
-        None if k_norm_weight is None else k_norm_weight.data_ptr(), float(eps),
-        cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_out.data_ptr(),
-        None if k_out is None else k_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        k_scale_cache.data_ptr(), v_scale_cache.data_ptr(), slot_mapping.data_ptr(),
-        _lib.INT64 if slot_mapping.dtype == torch.int64 else _lib.INT32,
-        n, hq, hk, d, k_cache.shape[0] * k_cache.shape[1], dt, _lib.stream_of(q)),
-        "mskv_qk_norm_rope_store")
+    with _lib.current(q):
+        _lib.check(lib.mskv_qk_norm_rope_store(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
+            positions.data_ptr(),
+            None if q_norm_weight is None else q_norm_weight.data_ptr(),
+            None if k_norm_weight is None else k_norm_weight.data_ptr(), float(eps),
+            cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_out.data_ptr(),
+            None if k_out is None else k_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale_cache.data_ptr(), v_scale_cache.data_ptr(), slot_mapping.data_ptr(),
+            _lib.INT64 if slot_mapping.dtype == torch.int64 else _lib.INT32,
+            n, hq, hk, d, k_cache.shape[0] * k_cache.shape[1], dt, _lib.stream_of(q)),
+            "mskv_qk_norm_rope_store")
     return q_out, k_out

@@ -55,11 +55,12 @@ def varlen_attention(
     if total_q == 0 or num_seqs == 0:
         return out
     lib = _lib.load()
-    status = lib.mskv_prefill_attention_strided(
-        q.data_ptr(), k.data_ptr(), k_stride, v.data_ptr(), v_stride, out.data_ptr(),
-        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), num_seqs,
-        total_q, total_k, int(max_seqlen_q), num_q_heads, num_kv_heads,
-        head_dim, float(softmax_scale), _lib.act_dtype(q), _lib.stream_of(q))
+    with _lib.current(q):
+        status = lib.mskv_prefill_attention_strided(
+            q.data_ptr(), k.data_ptr(), k_stride, v.data_ptr(), v_stride, out.data_ptr(),
+            cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), num_seqs,
+            total_q, total_k, int(max_seqlen_q), num_q_heads, num_kv_heads,
+            head_dim, float(softmax_scale), _lib.act_dtype(q), _lib.stream_of(q))
     _lib.check(status, "varlen_attention")
     return out
 
