@@ -513,7 +513,8 @@ int mskv_check_kv_blocks(int num_pools, void* const* bases,
  * that block_tables names move to places 0 .. n - 1.  A named page below n
  * stays; the i-th one from n up (ascending) takes the i-th free place below
  * n.  Pages that no entry names are free, and their contents afterwards are
- * unspecified.
+ * unspecified: pages cached without a sequence (a prefix cache's) must be named
+ * too, and all that holds page numbers outside the tables renamed by remap.
  * block_tables: int32 [num_entries]; entries outside [0, num_blocks) (-1
  * padding, a garbage page behind the pool) are kept as they are, and
  * several entries may name one page.  new_tables [num_entries]: the entries

@@ -3,8 +3,11 @@
 //
 //  * K goes from memory to the matrix unit: the page's layout is the A
 //    operand's (fp4.h), the block scales are applied by the MFMA, and the
-//    e4m3 parts of the query are the B operand: exact for bf16, fp16 with a
-//    2^-12 residual.  No K byte passes through LDS or a conversion.
+//    e4m3 parts of the query are the B operand.  In units in which the row's
+//    largest element lies in [224, 448], a bf16 element from 1/4 up is exact and
+//    an fp16 one from 2 up; smaller ones are off by at most 2^-10, half of
+//    e4m3's last step, which is 2^-17.8 of the largest.  No K byte passes
+//    through LDS or a conversion.
 //  * V rows pass through a per-wave LDS tile and come back transposed
 //    (ds_read_b64_tr_b4), 16 tokens a lane at one dimension, and convert to
 //    fp16 exactly.

@@ -21,8 +21,10 @@
 //  * QK^T: S^T = K . Q8^T with v_mfma_f32_16x16x128_f8f6f4 -- the whole
 //    head_dim is one MFMA.  K bytes are used as stored.  The query row is
 //    scaled by a power of two (exact) and split into e4m3 parts: hi + lo
-//    represent a bf16 query exactly (4 + 4 significant bits), fp16 needs
-//    hi + mid + lo; one MFMA per part into the same accumulator.
+//    hold bf16's 8 significant bits, fp16's 11 need hi + mid + lo; one MFMA
+//    per part into the same accumulator.  (Elements below 2^-9 of the row's
+//    largest, fp16 2^-6, meet e4m3's last step: off by up to 2^-17.8 of the
+//    largest.)
 //  * PV: O^T = V^T . P^T with v_mfma_f32_16x16x32_f16, which runs at the
 //    same rate per key as two FP8 parts would.  S^T's accumulator leaves
 //    lane (g, n) holding 32 keys of row n, exactly the B-operand layout of
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(PShape::threads, 2) void prefill_fp8_kernel(Prefill
 #pragma unroll
     for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
     amax = max_xor32(max_xor16(amax));
-    // power-of-two scale: x * f is exact, so the parts carry every bit
+    // power-of-two scale: x * f is exact
     const float f = amax > 1e-30f ? pow2_floor(kFp8Max / amax) : 1.0f;
     qs[b] = a.scale_log2 / f;
 #pragma unroll
@@ -705,7 +707,8 @@ static hipError_t launch_prefill(const PrefillArgs& a, int num_seqs, int64_t qbl
   return hipGetLastError();
 }
 
-// Key ranges per workgroup, from what the host knows: the shapes and a bound
+// Key ranges per workgroup, for either cache (the times are the FP8 kernel's),
+// from what the host knows: the shapes and a bound
 // of a sequence's keys (the call's own, or the table's width).  Two
 // workgroups are resident per CU, 512 on the chip, and a second one costs the
 // first little (a tile takes 3.0 us unsplit, 3.2 us beside other ranges, 3.9
@@ -851,7 +854,7 @@ static int prefill_checked(
     if (workspace_bytes < need) return MSKV_EWORKSPACE;
     if (need > 0) {
       a.splits = prefill_splits(num_seqs, total_q, max_seqlen_q, max_seqlen_k, num_q_heads,
-                                      num_kv_heads, block_size, max_blocks_per_seq);
+                                num_kv_heads, block_size, max_blocks_per_seq);
       a.part_o = (float*)workspace;
       a.part_lse = a.part_o + (size_t)total_q * num_q_heads * a.splits * head_dim;
     }

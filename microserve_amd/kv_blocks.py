@@ -113,7 +113,13 @@ def compact_kv_blocks(caches, block_tables: torch.Tensor, num_blocks: int | None
     ``[num_blocks]``, -1 for a page that no entry names) and the number of
     live pages (int32 ``[1]``), which fill places ``0 .. num_live - 1``.  A
     live page below ``num_live`` stays; the others take the free places in
-    ascending order.  The contents of free pages are unspecified afterwards.
+    ascending order.
+
+    A page that no entry names is free to this call and may be overwritten.
+    Pages that are cached without a running sequence (a prefix cache's) must
+    be named too, in rows of their own, and whatever else holds page numbers
+    (the hash table of cached pages, reference counts, the free list, the
+    sequences' own tables) must be renamed by ``remap`` before it is used again.
 
     ``num_blocks`` is the number of pages that take part, the first ones of
     dimension ``block_dim`` (default: all); entries outside them (-1 padding,
