@@ -531,6 +531,95 @@ int mskv_compact_kv_blocks(int num_pools, void* const* bases,
                            int32_t* new_tables, int32_t* remap,
                            int32_t* num_live, void* stream);
 
+/*
+ * Attention weights of cached tokens.  `weights` is float32 [num_blocks,
+ * num_kv_heads, block_size] beside the FP8 caches: the entry of a token and
+ * kv head is a sum of softmax probabilities (of the q heads that read the kv
+ * head, over queries).  Only positions from starts[b] (int32 [batch], or
+ * `start` for all where starts is NULL) on are written: pages that several
+ * sequences of a call name must lie before it, else their entries are
+ * unspecified.  Entries of tokens in invalid blocks are not written.  Nothing is
+ * added by atomics: results do not depend on timing.
+ *
+ * mskv_fp8_decode_attention_weights: mskv_fp8_decode_attention, which also
+ * adds the step's probabilities to the entries of positions below
+ * cache_seqlens[b] - 1 and sets that of the newest token, at
+ * cache_seqlens[b] - 1 (the entry of a reused page needs no clearing).
+ * weights starts on 16 bytes.  The workspace holds
+ * mskv_decode_weights_workspace_bytes: the split partials and, up to 1 GiB,
+ * every score of the step (batch * num_q_heads * max_blocks_per_seq *
+ * block_size floats); past that K is read again instead, and block_size must
+ * be a multiple of 128.
+ */
+size_t mskv_decode_weights_workspace_bytes(int batch, int num_q_heads,
+                                           int num_kv_heads, int block_size,
+                                           int max_blocks_per_seq);
+int mskv_fp8_decode_attention_weights(
+    const void* query, const void* k_cache, const void* v_cache,
+    const float* k_scale_cache, const float* v_scale_cache,
+    const int32_t* cache_seqlens, const int32_t* block_tables, float* weights,
+    const int32_t* starts, int start, void* out, int batch, int num_q_heads,
+    int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
+    int max_blocks_per_seq, float softmax_scale, int act_dtype,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The probabilities that a varlen batch's queries (the last ones of each
+ * sequence, described as in mskv_fp8_prefill_attention) give the sequences'
+ * tokens: query i of a sequence with Lq queries and Lk tokens sees positions
+ * p < Lk - Lq + i + 1.  The entries of positions [start, Lk) are set, or added
+ * to where accumulate is not 0.  max_seqlen_q and max_seqlen_k (0: the tables'
+ * width) bound every sequence's queries and tokens: rows past them are not
+ * counted.  block_size % 128 == 0, head_dim == 128.
+ */
+size_t mskv_window_weights_workspace_bytes(int64_t total_q,
+                                           int64_t max_seqlen_k,
+                                           int num_q_heads, int block_size,
+                                           int max_blocks_per_seq);
+int mskv_fp8_window_attention_weights(
+    const void* query, const void* k_cache, const float* k_scale_cache,
+    const int32_t* block_tables, const int32_t* cu_seqlens_q,
+    const int32_t* cu_seqlens_k, float* weights, const int32_t* starts,
+    int start, int accumulate, int num_seqs, int64_t total_q,
+    int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads, int num_kv_heads,
+    int head_dim, int block_size, int64_t num_blocks, int max_blocks_per_seq,
+    float softmax_scale, int act_dtype, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/*
+ * The tokens that stay of every (sequence, kv head): of L = cache_seqlens[b]
+ * tokens n = min(L, budget), namely the first starts[b] (or `start`), the last
+ * `recent` and the heaviest of those between.  Where they do not all fit, the
+ * first ones go before the last ones.  Of equal weights the earlier position
+ * stays; a NaN, and a token in an invalid block, counts as the lightest.
+ * kept: int32 [batch, num_kv_heads, budget], the positions that stay in
+ * ascending order, -1 behind them; new_seqlens: int32 [batch], n.
+ */
+int mskv_select_kv_tokens(const float* weights, const int32_t* cache_seqlens,
+                          const int32_t* block_tables, const int32_t* starts,
+                          int start, int recent, int budget, int32_t* kept,
+                          int32_t* new_seqlens, int batch, int num_kv_heads,
+                          int block_size, int64_t num_blocks,
+                          int max_blocks_per_seq, void* stream);
+
+/*
+ * Move the kept tokens' rows together: position i < new_seqlens[b] of every
+ * (sequence b, kv head h) gets the K and V bytes and scales (and the entry of
+ * `weights`, unless NULL) of position kept[b, h, i].  kept ascends, as
+ * mskv_select_kv_tokens leaves it (else the rows moved are unspecified).
+ * Rows from new_seqlens[b] on are left as they are.  A page that is changed
+ * must be named by one sequence of the call only, once.  Positions outside
+ * the tables and blocks outside the cache are skipped.  k_cache and v_cache
+ * start on 16 bytes.
+ */
+int mskv_evict_kv_tokens(void* k_cache, void* v_cache, float* k_scale_cache,
+                         float* v_scale_cache, float* weights,
+                         const int32_t* kept, const int32_t* new_seqlens,
+                         const int32_t* block_tables, int batch,
+                         int num_kv_heads, int head_dim, int block_size,
+                         int64_t num_blocks, int max_blocks_per_seq,
+                         int budget, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,564 @@
+// The attention weight of each cached token: sums of softmax probabilities over
+// the queries that read its kv head, added to a tensor [num_blocks, H, BS] that
+// lies beside the caches (fp32, a head's tokens of a page in a row).
+//
+//  * A decode that tracks its weights (track_weights_kernel): the split kernel
+//    leaves each score in memory, 4 bytes a (q head, token), and the splits'
+//    log-sum-exps; this kernel adds 2^(score - lse) over a kv head's q heads.
+//    HBM-bound: the scores are 8 bytes a q head and token (written and read
+//    once), 32 at a group of four, where reading K again for them is 132.
+//  * The last queries of prompts (window_lse_kernel, window_sum_kernel): many
+//    rows a kv head, whose scores would be more bytes than K.  The scores are
+//    computed twice, first for each row's log-sum-exp, then for the sums.
+#pragma once
+
+namespace mskv {
+
+struct TrackArgs {
+  DecodeArgs d;
+  float* weights;
+  const int32_t* starts;
+  int start;
+};
+
+// The log-sum-exp of a row from those of its first n splits (+inf for a row
+// without tokens: 2^(score - lse) is then 0).
+__device__ __forceinline__ float merged_lse(const float* lse, int n, int lane) {
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, lse[i]);
+  m = max_xor32(max_xor16(max16_dpp(m)));
+  if (m == -INFINITY) return INFINITY;
+  float l = 0.0f;
+  for (int i = lane; i < n; i += 64) l += exp2_fast(lse[i] - m);
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) l += __shfl_xor(l, d);
+  l = sum_xor32(sum_xor16(l));
+  return m + __log2f(l);
+}
+
+constexpr int kTrackThreads = 256;
+constexpr int kTrackTokens = 4 * kTrackThreads;  // of a workgroup's turn
+
+// grid (turns of a sequence's tokens, kv heads, sequences).  A page is whole
+// steps of 32 tokens, so a thread's four lie in one page.
+template <bool kRule>
+__global__ __launch_bounds__(kTrackThreads) void track_weights_kernel(TrackArgs t) {
+  const DecodeArgs& a = t.d;
+  extern __shared__ float s_lse[];  // of the group's heads
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int own = kRule ? lane_length(a.seqlens, a.rule) : 0;
+  const int L = min(a.seqlens[b], a.w * a.bs);
+  if ((int)blockIdx.x * kTrackTokens >= L) return;
+  const int split_tokens =
+      kRule ? split_tokens_of<kStep>(own, L, a.seqlens, a.rule) : a.rule.fixed;
+  const int nvalid = min(a.splits, (L + split_tokens - 1) / split_tokens);
+  const int64_t row0 = (int64_t)b * a.hq + kvh * a.group;
+  for (int h = wave; h < a.group; h += kTrackThreads / 64) {
+    const float lse = merged_lse(a.part_lse + (row0 + h) * a.splits, nvalid, lane);
+    if (lane == 0) s_lse[h] = lse;
+  }
+  __syncthreads();
+  const int64_t cap = (int64_t)a.w * a.bs;
+  const int first = max(t.starts ? t.starts[b] : t.start, 0);
+  for (int at = blockIdx.x * kTrackTokens; at < L; at += gridDim.x * kTrackTokens) {
+    const int tok = at + 4 * threadIdx.x;
+    if (tok >= L || tok + 4 <= first) continue;
+    const int page = tok / a.bs;
+    const int blk = a.bt[(int64_t)b * a.w + page];
+    if (blk < 0 || (int64_t)blk >= a.num_blocks) continue;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    const float* s = a.scores + row0 * cap + tok;
+    for (int h = 0; h < a.group; ++h) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(s + h * cap);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[r] += exp2_fast(x[r] - s_lse[h]);
+    }
+    float* to = t.weights + ((int64_t)blk * a.hk + kvh) * a.bs + (tok - page * a.bs);
+    if (tok >= first && tok + 4 < L) {
+      *reinterpret_cast<f32x4*>(to) += sum;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (tok + r >= first && tok + r < L)  // the newest token's entry starts here
+          to[r] = tok + r < L - 1 ? to[r] + sum[r] : sum[r];
+    }
+  }
+}
+
+// ------------------------------------------------------- windows of queries --
+
+struct WindowArgs {
+  const uint16_t* q;
+  const uint8_t* kc;
+  const float* ks;
+  const int32_t *bt, *cu_q, *cu_k;  // cu_q null: one query a sequence, lengths in cu_k
+  const int32_t* starts;
+  float *weights, *part, *lse;
+  int64_t total_q, num_blocks;
+  float scale_log2;
+  int hq, hk, group, bs, w, start, chunks, rows;
+  bool add, set_new;
+};
+
+constexpr int kWinThreads = 256;
+constexpr int kWinKeys = 256;  // of a workgroup: 64 a wave
+constexpr int kWinRows = 128;  // (query, q head of the group), of a turn
+
+// A sequence's queries and keys, clamped to the tensors.
+struct WindowSeq {
+  int q_begin, lq, lk, rows;
+};
+__device__ __forceinline__ WindowSeq window_seq(const WindowArgs& a, int s) {
+  WindowSeq w;
+  const int64_t tq = a.total_q;
+  if (a.cu_q) {
+    w.q_begin = (int)min((int64_t)max(a.cu_q[s], 0), tq);
+    w.lq = (int)min((int64_t)max(a.cu_q[s + 1], w.q_begin), tq) - w.q_begin;
+    w.lk = a.cu_k[s + 1] - a.cu_k[s];
+  } else {
+    w.q_begin = s;
+    w.lq = 1;
+    w.lk = a.cu_k[s];
+  }
+  w.lk = max(0, min(w.lk, a.w * a.bs));
+  w.rows = (int)min((int64_t)w.lq * a.group, (int64_t)a.rows);
+  return w;
+}
+
+// The wave's 64 keys (16 kg + n of lane (g, n)) as the matrix unit's operand:
+// dimensions [16g, 16g + 16) and [64 + 16g, 64 + 16g + 16), as the decode has
+// them; zeros past the sequence's end and for an invalid page.
+template <typename T>
+__device__ __forceinline__ void window_keys(const WindowArgs& a, int s, int kvh, int t0, int lk,
+                                            int lane, typename Act<T>::x8 (&kop)[4][4],
+                                            float& scale, int& valid) {
+  const int g = lane >> 4, n = lane & 15;
+  const int page = t0 / a.bs, off = t0 - page * a.bs;
+  const int blk = t0 < lk ? a.bt[(int64_t)s * a.w + page] : -1;
+  const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
+  const int64_t bo = ok ? blk : 0;
+  valid = ok ? min(64, lk - t0) : 0;
+  const uint32_t stride = (uint32_t)a.hk * kHeadDim;
+  const auto kr = make_rsrc(a.kc + bo * a.bs * stride, (uint32_t)(off + valid) * (ok ? stride : 0u));
+  const auto sr = make_rsrc(a.ks + bo * a.bs * a.hk, ok ? (uint32_t)(off + valid) * a.hk * 4u : 0u);
+  u32x4 lo[4], hi[4];
+#pragma unroll
+  for (int kg = 0; kg < 4; ++kg) {
+    const uint32_t o = (uint32_t)(off + 16 * kg + n) * stride + (uint32_t)kvh * kHeadDim + 16u * g;
+    lo[kg] = buf_load16(kr, o);
+    hi[kg] = buf_load16(kr, o + 64u);
+  }
+  scale = buf_load_f32(sr, (((uint32_t)off + lane) * a.hk + kvh) * 4u) * a.scale_log2;
+  using A = Act<T>;
+#pragma unroll
+  for (int kg = 0; kg < 4; ++kg) {
+    A::fp8x4_to(lo[kg][0], kop[kg][0], 0); A::fp8x4_to(lo[kg][1], kop[kg][0], 4);
+    A::fp8x4_to(lo[kg][2], kop[kg][1], 0); A::fp8x4_to(lo[kg][3], kop[kg][1], 4);
+    A::fp8x4_to(hi[kg][0], kop[kg][2], 0); A::fp8x4_to(hi[kg][1], kop[kg][2], 4);
+    A::fp8x4_to(hi[kg][2], kop[kg][3], 0); A::fp8x4_to(hi[kg][3], kop[kg][3], 4);
+  }
+}
+
+// Stages rows [row0, row0 + 128) of a kv head into LDS (256-byte rows, 16-byte
+// chunks XOR-swizzled by the row; zeros past the last one), with each row's
+// number of visible keys.
+__device__ __forceinline__ void window_rows(const WindowArgs& a, const WindowSeq& w, int kvh,
+                                            int row0, uint8_t* q_lds, int* s_lim) {
+#pragma unroll
+  for (int i = 0; i < kWinRows * 16 / kWinThreads; ++i) {
+    const int r = (i * kWinThreads + threadIdx.x) >> 4, c = threadIdx.x & 15;
+    const int row = row0 + r;
+    const int qi = row / a.group, h = row - qi * a.group;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (row < w.rows)
+      v = *reinterpret_cast<const u32x4*>(
+          a.q + ((int64_t)(w.q_begin + qi) * a.hq + kvh * a.group + h) * kHeadDim + 8 * c);
+    *reinterpret_cast<u32x4*>(q_lds + r * 256 + 16 * (c ^ (r & 15))) = v;
+    if (c == 0) s_lim[r] = row < w.rows ? w.lk - w.lq + qi + 1 : 0;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void window_operand(const uint8_t* q_lds, int rb, int lane,
+                                               typename Act<T>::x8 (&qop)[4]) {
+  const int g = lane >> 4, n = lane & 15;
+  const uint8_t* row = q_lds + (16 * rb + n) * 256;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = (j & 2) * 4 + 2 * g + (j & 1);
+    qop[j] = __builtin_bit_cast(typename Act<T>::x8,
+                                *reinterpret_cast<const u32x4*>(row + 16 * (c ^ n)));
+  }
+}
+
+// The largest score and the sum of 2^(score - it) of each row over the
+// workgroup's 256 keys.  S^T = K . Q^T: a lane holds 16 keys of one row.
+// grid (key chunks, kv heads x turns of rows, sequences)
+template <typename T>
+__global__ __launch_bounds__(kWinThreads) void window_lse_kernel(WindowArgs a) {
+  using A = Act<T>;
+  __shared__ __attribute__((aligned(16))) uint8_t q_lds[kWinRows * 256];
+  __shared__ __attribute__((aligned(16))) float s_scale[kWinKeys];
+  __shared__ int s_lim[kWinRows];
+  __shared__ float s_m[4][kWinRows], s_l[4][kWinRows];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const int s = blockIdx.z;
+  const int kvh = blockIdx.y % a.hk, row0 = blockIdx.y / a.hk * kWinRows;
+  const WindowSeq w = window_seq(a, s);
+  const int t0 = blockIdx.x * kWinKeys;
+  if (row0 >= w.rows || (t0 >= w.lk && t0 > 0)) return;
+  typename A::x8 kop[4][4];
+  float scale;
+  int valid;
+  const int k0 = t0 + 64 * wave;
+  window_keys<T>(a, s, kvh, k0, w.lk, lane, kop, scale, valid);
+  s_scale[tid] = scale;
+  window_rows(a, w, kvh, row0, q_lds, s_lim);
+  __syncthreads();
+  const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;  // every row sees every key
+  f32x4 ksc[4];
+#pragma unroll
+  for (int kg = 0; kg < 4; ++kg)
+    ksc[kg] = *reinterpret_cast<const f32x4*>(&s_scale[64 * wave + 16 * kg + 4 * g]);
+  for (int rb = 0; rb < kWinRows / 16; ++rb) {
+    typename A::x8 qop[4];
+    window_operand<T>(q_lds, rb, lane, qop);
+    f32x4 x[4];
+#pragma unroll
+    for (int kg = 0; kg < 4; ++kg) {
+      x[kg] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[kg] = A::mfma(kop[kg][j], qop[j], x[kg]);
+      x[kg] *= ksc[kg];
+    }
+    if (!all) {
+      const int lim = min(s_lim[16 * rb + n] - k0, valid);
+#pragma unroll
+      for (int kg = 0; kg < 4; ++kg)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!(16 * kg + 4 * g + r < lim)) x[kg][r] = -INFINITY;
+    }
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int kg = 0; kg < 4; ++kg)
+      m = fmaxf(fmaxf(m, fmaxf(x[kg][0], x[kg][1])), fmaxf(x[kg][2], x[kg][3]));
+    m = max_xor32(max_xor16(m));
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int kg = 0; kg < 4; ++kg)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) l += exp2_fast(x[kg][r] - ref);
+    l = sum_xor32(sum_xor16(l));
+    if (g == 0) {
+      s_m[wave][16 * rb + n] = m;
+      s_l[wave][16 * rb + n] = l;
+    }
+  }
+  __syncthreads();
+  if (tid >= kWinRows || row0 + tid >= w.rows) return;
+  float m = s_m[0][tid];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = fmaxf(m, s_m[i][tid]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) l += s_l[i][tid] * exp2_fast(s_m[i][tid] - ref);
+  const float lse = partial_lse(m, l);
+  const int row = row0 + tid;
+  const int qi = row / a.group;
+  const int64_t at = (int64_t)(w.q_begin + qi) * a.hq + kvh * a.group + (row - qi * a.group);
+  a.part[at * a.chunks + blockIdx.x] = lse;
+}
+
+// lse[row] from the chunks that hold keys; +inf where no key is seen.
+// One wave a row; grid (rows of the query tensor / 4, sequences)
+constexpr int kWinMergeRows = 4;
+__global__ __launch_bounds__(64 * kWinMergeRows) void window_merge_kernel(WindowArgs a) {
+  const WindowSeq w = window_seq(a, blockIdx.y);
+  const int local = blockIdx.x * kWinMergeRows + (threadIdx.x >> 6);
+  // (row `local` of the sequence: query local / hq, q head local % hq)
+  if (local >= w.rows / a.group * a.hq) return;
+  const int64_t at = (int64_t)w.q_begin * a.hq + local;
+  const int n = max(1, min(a.chunks, (w.lk + kWinKeys - 1) / kWinKeys));
+  const float lse = merged_lse(a.part + at * a.chunks, n, threadIdx.x & 63);
+  if ((threadIdx.x & 63) == 0) a.lse[at] = lse;
+}
+
+// The sums over the rows of 2^(score - lse) at the workgroup's 256 keys.
+// S = Q . K^T: a lane holds four rows of one key, whose sum needs no exchange
+// until all the rows are in.  grid (key chunks, kv heads, sequences)
+template <typename T>
+__global__ __launch_bounds__(kWinThreads) void window_sum_kernel(WindowArgs a) {
+  using A = Act<T>;
+  __shared__ __attribute__((aligned(16))) uint8_t q_lds[kWinRows * 256];
+  __shared__ __attribute__((aligned(16))) int s_lim[kWinRows];
+  __shared__ __attribute__((aligned(16))) float s_lse[kWinRows];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const int s = blockIdx.z, kvh = blockIdx.y;
+  const WindowSeq w = window_seq(a, s);
+  const int t0 = blockIdx.x * kWinKeys;
+  if (t0 >= w.lk) return;
+  typename A::x8 kop[4][4];
+  float scale;
+  int valid;
+  const int k0 = t0 + 64 * wave;
+  window_keys<T>(a, s, kvh, k0, w.lk, lane, kop, scale, valid);
+  const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;
+  float ksc[4], sum[4];
+#pragma unroll
+  for (int kg = 0; kg < 4; ++kg) {
+    ksc[kg] = __shfl(scale, 16 * kg + n);
+    sum[kg] = 0.0f;
+  }
+  for (int row0 = 0; row0 < w.rows; row0 += kWinRows) {
+    if (row0 > 0) __syncthreads();
+    window_rows(a, w, kvh, row0, q_lds, s_lim);
+    if (tid < kWinRows) {
+      const int row = row0 + tid, qi = row / a.group;
+      const int64_t at = (int64_t)(w.q_begin + qi) * a.hq + kvh * a.group + (row - qi * a.group);
+      s_lse[tid] = row < w.rows ? a.lse[at] : INFINITY;
+    }
+    __syncthreads();
+    const int blocks = min(kWinRows, w.rows - row0 + 15) / 16;
+    for (int rb = 0; rb < blocks; ++rb) {
+      typename A::x8 qop[4];
+      window_operand<T>(q_lds, rb, lane, qop);
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[16 * rb + 4 * g]);
+#pragma unroll
+      for (int kg = 0; kg < 4; ++kg) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x = A::mfma(qop[j], kop[kg][j], x);
+        f32x4 p;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = exp2_fast(fmaf(x[r], ksc[kg], -lse[r]));
+        if (!all) {
+          const int key = 16 * kg + n;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!(key < valid && k0 + key < s_lim[16 * rb + 4 * g + r])) p[r] = 0.0f;
+        }
+        sum[kg] += (p[0] + p[1]) + (p[2] + p[3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int kg = 0; kg < 4; ++kg) sum[kg] = sum_xor32(sum_xor16(sum[kg]));
+  const float own = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
+  const int tok = k0 + lane;  // key 16 g + n of the wave's
+  if (lane >= valid || tok < max(a.starts ? a.starts[s] : a.start, 0)) return;
+  const int page = k0 / a.bs;
+  float* to = a.weights +
+              ((int64_t)a.bt[(int64_t)s * a.w + page] * a.hk + kvh) * a.bs + (tok - page * a.bs);
+  const bool add = a.add && !(a.set_new && tok >= w.lk - w.lq);
+  *to = add ? *to + own : own;
+}
+
+// [total_q * hq, chunks] partial log-sum-exps, then [total_q * hq] final ones
+static size_t window_bytes(int64_t total_q, int hq, int64_t chunks) {
+  return (size_t)total_q * hq * (chunks + 1) * sizeof(float);
+}
+
+template <typename T>
+static hipError_t launch_window(const WindowArgs& a, int num_seqs, hipStream_t st) {
+  if (a.rows > 0) {  // (without queries there are only zeros to write)
+    const unsigned turns = (unsigned)((a.rows + kWinRows - 1) / kWinRows);
+    hipLaunchKernelGGL(window_lse_kernel<T>,
+                       dim3((unsigned)a.chunks, (unsigned)a.hk * turns, (unsigned)num_seqs),
+                       dim3(kWinThreads), 0, st, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t local = (int64_t)a.rows / a.group * a.hq;
+    hipLaunchKernelGGL(window_merge_kernel,
+                       dim3((unsigned)((local + kWinMergeRows - 1) / kWinMergeRows),
+                            (unsigned)num_seqs),
+                       dim3(64 * kWinMergeRows), 0, st, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(window_sum_kernel<T>,
+                     dim3((unsigned)a.chunks, (unsigned)a.hk, (unsigned)num_seqs),
+                     dim3(kWinThreads), 0, st, a);
+  return hipGetLastError();
+}
+
+// Key chunks of a window call, by the most keys of a sequence.
+static int64_t window_chunks(int64_t max_seqlen_k, int block_size, int w) {
+  int64_t keys = (int64_t)w * block_size;
+  if (max_seqlen_k > 0) keys = std::min(keys, max_seqlen_k);
+  return (keys + kWinKeys - 1) / kWinKeys;
+}
+
+// Most bytes of scores that a tracking decode asks for; past it K is read again
+// instead.
+constexpr size_t kTrackMaxScores = (size_t)1 << 30;
+
+}  // namespace mskv
+
+extern "C" size_t mskv_window_weights_workspace_bytes(int64_t total_q, int64_t max_seqlen_k,
+                                                      int num_q_heads, int block_size,
+                                                      int max_blocks_per_seq) {
+  if (total_q <= 0 || num_q_heads <= 0 || block_size <= 0 || max_blocks_per_seq <= 0) return 0;
+  return mskv::window_bytes(total_q, num_q_heads,
+                            mskv::window_chunks(max_seqlen_k, block_size, max_blocks_per_seq));
+}
+
+namespace mskv {
+
+// Validates a window call and launches it.  Without cu_seqlens_q: one query a
+// sequence, its length in cu_seqlens_k, the newest token's entry set.
+static int window_checked(
+    const void* query, const void* k_cache, const float* k_scale_cache,
+    const int32_t* block_tables, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+    float* weights, const int32_t* starts, int start, bool accumulate, int num_seqs,
+    int64_t total_q, int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads, int num_kv_heads,
+    int head_dim, int block_size, int64_t num_blocks, int max_blocks_per_seq, float softmax_scale,
+    int act_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (num_seqs < 0 || total_q < 0 || max_seqlen_q < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      block_size <= 0 || num_blocks < 0 || max_blocks_per_seq <= 0 || start < 0)
+    return MSKV_EINVAL;
+  if (act_dtype != MSKV_FLOAT16 && act_dtype != MSKV_BFLOAT16) return MSKV_EINVAL;
+  if (num_q_heads % num_kv_heads != 0) return MSKV_EINVAL;
+  if (head_dim != kHeadDim || block_size % 128 != 0) return MSKV_EUNSUPPORTED;
+  if ((int64_t)block_size * num_kv_heads * head_dim > 0x7FFFFFFFLL) return MSKV_EUNSUPPORTED;
+  if ((int64_t)max_blocks_per_seq * block_size >= (1LL << 30)) return MSKV_EUNSUPPORTED;
+  const int group = num_q_heads / num_kv_heads;
+  const int64_t rows = (int64_t)max_seqlen_q * group;
+  const int64_t turns = (rows + kWinRows - 1) / kWinRows;
+  if (num_seqs > 65535 || turns * num_kv_heads > 65535 || total_q > 0x7FFFFFFFLL)
+    return MSKV_EUNSUPPORTED;
+  if (num_seqs == 0) return MSKV_OK;
+  if (!k_cache || !k_scale_cache || !block_tables || !cu_seqlens_k || !weights)
+    return MSKV_EINVAL;
+  if (total_q > 0 && !query) return MSKV_EINVAL;
+  if (misaligned({query, k_cache})) return MSKV_EINVAL;
+  WindowArgs a = {};
+  a.chunks = (int)window_chunks(max_seqlen_k, block_size, max_blocks_per_seq);
+  const size_t need = mskv_window_weights_workspace_bytes(total_q, max_seqlen_k, num_q_heads,
+                                                          block_size, max_blocks_per_seq);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return MSKV_EWORKSPACE;
+  a.q = (const uint16_t*)query;
+  a.kc = (const uint8_t*)k_cache;
+  a.ks = k_scale_cache;
+  a.bt = block_tables;
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.starts = starts;
+  a.start = start;
+  a.weights = weights;
+  a.part = (float*)workspace;
+  a.lse = a.part + (size_t)total_q * num_q_heads * a.chunks;
+  a.total_q = total_q;
+  a.num_blocks = num_blocks;
+  a.scale_log2 = softmax_scale * kLog2e;
+  a.hq = num_q_heads;
+  a.hk = num_kv_heads;
+  a.group = group;
+  a.bs = block_size;
+  a.w = max_blocks_per_seq;
+  a.rows = total_q > 0 ? (int)std::min<int64_t>(rows, total_q * group) : 0;
+  a.add = accumulate;
+  a.set_new = cu_seqlens_q == nullptr;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return (int)(act_dtype == MSKV_BFLOAT16 ? launch_window<__bf16>(a, num_seqs, s)
+                                          : launch_window<_Float16>(a, num_seqs, s));
+}
+
+}  // namespace mskv
+
+extern "C" int mskv_fp8_window_attention_weights(
+    const void* query, const void* k_cache, const float* k_scale_cache,
+    const int32_t* block_tables, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+    float* weights, const int32_t* starts, int start, int accumulate, int num_seqs,
+    int64_t total_q, int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads, int num_kv_heads,
+    int head_dim, int block_size, int64_t num_blocks, int max_blocks_per_seq, float softmax_scale,
+    int act_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (num_seqs > 0 && !cu_seqlens_q) return MSKV_EINVAL;
+  return mskv::window_checked(query, k_cache, k_scale_cache, block_tables, cu_seqlens_q,
+                              cu_seqlens_k, weights, starts, start, accumulate != 0, num_seqs,
+                              total_q, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads,
+                              head_dim, block_size, num_blocks, max_blocks_per_seq, softmax_scale,
+                              act_dtype, workspace, workspace_bytes, stream);
+}
+
+namespace mskv {
+
+// Whether a tracking decode of this shape leaves its scores in memory.
+static bool track_scores(int batch, int hq, int w, int block_size) {
+  return track_scores_bytes(batch, hq, w, block_size) <= kTrackMaxScores;
+}
+
+}  // namespace mskv
+
+extern "C" size_t mskv_decode_weights_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
+                                                      int block_size, int max_blocks_per_seq) {
+  using namespace mskv;
+  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
+      block_size <= 0 || max_blocks_per_seq <= 0)
+    return 0;
+  const int splits = mskv_decode_num_splits(batch, num_q_heads, num_kv_heads, max_blocks_per_seq,
+                                            block_size);
+  if (track_scores(batch, num_q_heads, max_blocks_per_seq, block_size))
+    return track_scores_at(batch, num_q_heads, num_kv_heads, splits) +
+           track_scores_bytes(batch, num_q_heads, max_blocks_per_seq, block_size);
+  // the decode's own workspace, then the window kernels' one
+  return std::max(mskv_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, kHeadDim, splits),
+                  mskv_window_weights_workspace_bytes(batch, 0, num_q_heads, block_size,
+                                                      max_blocks_per_seq));
+}
+
+extern "C" int mskv_fp8_decode_attention_weights(
+    const void* query, const void* k_cache, const void* v_cache, const float* k_scale_cache,
+    const float* v_scale_cache, const int32_t* cache_seqlens, const int32_t* block_tables,
+    float* weights, const int32_t* starts, int start, void* out, int batch, int num_q_heads,
+    int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, int max_blocks_per_seq,
+    float softmax_scale, int act_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mskv;
+  if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || block_size <= 0 ||
+      max_blocks_per_seq <= 0 || start < 0 || num_q_heads % num_kv_heads != 0)
+    return MSKV_EINVAL;
+  if (batch > 65535 || num_kv_heads > 65535 || num_q_heads / num_kv_heads > 8192)
+    return MSKV_EUNSUPPORTED;
+  if (batch > 0 && (!weights || misaligned({weights}))) return MSKV_EINVAL;
+  if (batch > 0 && (!workspace || workspace_bytes < mskv_decode_weights_workspace_bytes(
+                                                        batch, num_q_heads, num_kv_heads,
+                                                        block_size, max_blocks_per_seq)))
+    return MSKV_EWORKSPACE;
+  const int splits = mskv_decode_num_splits(batch, num_q_heads, num_kv_heads, max_blocks_per_seq,
+                                            block_size);
+  if (!track_scores(batch, num_q_heads, max_blocks_per_seq, block_size)) {
+    if (block_size % 128 != 0) return MSKV_EUNSUPPORTED;
+    const int status = decode_checked<Fp8Cache>(
+        query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens, block_tables, out,
+        batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,
+        softmax_scale, act_dtype, splits, workspace, workspace_bytes, stream);
+    if (status != MSKV_OK || batch == 0) return status;
+    return window_checked(query, k_cache, k_scale_cache, block_tables, nullptr, cache_seqlens,
+                          weights, starts, start, true, batch, batch, 1, 0, num_q_heads,
+                          num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,
+                          softmax_scale, act_dtype, workspace, workspace_bytes, stream);
+  }
+  auto track = [&](const DecodeArgs& d, hipStream_t s) -> int {
+    const TrackArgs t = {d, weights, starts, start};
+    const int64_t turns = ((int64_t)d.w * d.bs + kTrackTokens - 1) / kTrackTokens;
+    // (a table's width says little of the lengths: workgroups walk the turns
+    // past a grid of 4096)
+    const int64_t most = std::max<int64_t>(1, 4096 / ((int64_t)d.batch * d.hk));
+    const dim3 grid((unsigned)std::min(turns, most), (unsigned)d.hk, (unsigned)d.batch);
+    const unsigned lds = (unsigned)(d.group * sizeof(float));
+    if (d.rule.adapt || d.rule.info)
+      hipLaunchKernelGGL(track_weights_kernel<true>, grid, dim3(kTrackThreads), lds, s, t);
+    else
+      hipLaunchKernelGGL(track_weights_kernel<false>, grid, dim3(kTrackThreads), lds, s, t);
+    return (int)hipGetLastError();
+  };
+  return decode_checked<Fp8Cache, true>(
+      query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens, block_tables, out,
+      batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,
+      softmax_scale, act_dtype, splits, workspace, workspace_bytes, stream, track);
+}

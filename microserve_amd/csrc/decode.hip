@@ -142,6 +142,8 @@ struct DecodeArgs {
   // the sequences' last ones by length; rule.info[0] of them are valid.
   const int4* items;
   SplitRule rule;
+  // [batch, hq, w * bs] scores of a decode that tracks its weights (else null)
+  float* scores;
 };
 
 // Sum / max over the wave with DPP row shifts and the two cross-row swaps
@@ -276,13 +278,15 @@ __device__ __forceinline__ void load_step(const DecodeArgs& a, int blk, int kvh,
 // un-normalized accumulator O^T, the running max m (log2 units) and the
 // lane's share of the denominator l.  kv_lds / s_lds are this wave's own
 // double-buffered LDS tiles; blk_first is the block of t_begin's page.
-template <typename T>
+// kTrack: the scores of the lane's tokens, in log2 units (-inf: not a token),
+// are left in `scores`, the row's by position, for track_weights_kernel.
+template <typename T, bool kTrack = false>
 __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh, int qh,
                                              bool head_ok, int t_begin, int t_end,
                                              int blk_first, int lane,
                                              uint8_t (&kv_lds)[2][2][kStep * kHeadDim],
                                              float (&s_lds)[2][2 * kStep], f32x4 (&acc)[8],
-                                             float& m, float& l) {
+                                             float& m, float& l, float* scores = nullptr) {
   using A = Act<T>;
   using x8 = typename A::x8;
   const int g = lane >> 4, n = lane & 15;
@@ -411,6 +415,14 @@ __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh
         if (!(16 + 4 * g + r < valid)) x[4 + r] = -INFINITY;
       }
     }
+    if constexpr (kTrack) {
+      if (head_ok) {
+        // (a page is whole steps: the row has room for this one)
+        float* to = scores + t0 + 4 * g;
+        *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(to + 16) = f32x4{x[4], x[5], x[6], x[7]};
+      }
+    }
     float tmax = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     tmax = max_xor32(max_xor16(tmax));
@@ -511,13 +523,16 @@ __device__ __forceinline__ void write_output(uint16_t* op, const f32x4 (&acc)[8]
 // l (a NaN query, key or scale) is left as +inf: every merge weighs it with
 // 2^(inf - inf), so the row comes out NaN, as it does from a single split,
 // and is not taken for a split without tokens.
+__device__ __forceinline__ float partial_lse(float m, float l) {
+  return is_nan(l) ? INFINITY : l > 0.0f ? m + __log2f(l) : -INFINITY;
+}
 __device__ __forceinline__ void write_partial(float* po, float* plse, const f32x4 (&acc)[8],
                                               float m, float l, int g) {
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt)
     *reinterpret_cast<f32x4*>(po + 16 * dt + 4 * g) = acc[dt] * inv;
-  if (g == 0) *plse = is_nan(l) ? INFINITY : l > 0.0f ? m + __log2f(l) : -INFINITY;
+  if (g == 0) *plse = partial_lse(m, l);
 }
 
 // 2 waves per SIMD, the occupancy the LDS allows: one 8-wave workgroup
@@ -532,7 +547,9 @@ __device__ __forceinline__ void write_partial(float* po, float* plse, const f32x
 // against 124 us.)
 // kFollow: the splits follow the lengths; kFixed: they are the shape's.
 enum DecodeMode { kFixed, kFollow, kItems };
-template <typename T, int W, DecodeMode kMode, typename Cache>
+// kTrack: scores and every split's log-sum-exp are left for track_weights_kernel
+// (the FP8 cache only).
+template <typename T, int W, DecodeMode kMode, typename Cache, bool kTrack = false>
 __device__ __forceinline__ void decode_split(const DecodeArgs& a) {
   // per wave: two buffers of tiles and their scales; step i is read from
   // buffer i&1 while step i+1 is staged into the other one
@@ -610,8 +627,13 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& a) {
 
   f32x4 acc[8];
   float m, l;
-  Cache::template attend<T>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane,
-                            kv_lds_all[wave], s_lds_all[wave], acc, m, l);
+  if constexpr (kTrack)
+    attend_range<T, true>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane,
+                          kv_lds_all[wave], s_lds_all[wave], acc, m, l,
+                          a.scores + ((int64_t)b * a.hq + qh) * a.w * a.bs);
+  else
+    Cache::template attend<T>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane,
+                              kv_lds_all[wave], s_lds_all[wave], acc, m, l);
 
   // splits that hold tokens of this sequence; a sequence that fits in one
   // split is written here directly
@@ -619,6 +641,8 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& a) {
   if (!head_ok) return;
   if (nvalid == 1) {
     write_output<T>(a.out + ((int64_t)b * a.hq + qh) * kHeadDim, acc, l, g);
+    if (kTrack && g == 0)
+      a.part_lse[((int64_t)b * a.hq + qh) * a.splits] = partial_lse(m, l);
     return;
   }
   // this split's partial, merged by a combine kernel
@@ -638,9 +662,17 @@ __attribute__((amdgpu_waves_per_eu(2, 8)))
 void decode_fp4_kernel(DecodeArgs a) {
   decode_split<T, W, kMode, Fp4Cache>(a);
 }
-template <typename T, int W, DecodeMode kMode, typename Cache>
+template <typename T, int W, DecodeMode kMode>
+__global__ __launch_bounds__(64 * W)
+__attribute__((amdgpu_waves_per_eu(2, 8)))
+void decode_track_kernel(DecodeArgs a) {
+  decode_split<T, W, kMode, Fp8Cache, true>(a);
+}
+template <typename T, int W, DecodeMode kMode, typename Cache, bool kTrack>
 static auto split_kernel() {
-  if constexpr (std::is_same<Cache, Fp4Cache>::value)
+  if constexpr (kTrack)
+    return decode_track_kernel<T, W, kMode>;
+  else if constexpr (std::is_same<Cache, Fp4Cache>::value)
     return decode_fp4_kernel<T, W, kMode>;
   else
     return decode_fp8_kernel<T, W, kMode>;
@@ -1036,7 +1068,7 @@ static size_t partials_bytes(int batch, int hq, int splits) {
   return (raw + 255) & ~(size_t)255;
 }
 
-template <typename T, typename Cache>
+template <typename T, typename Cache, bool kTrack = false>
 static hipError_t launch_decode(const DecodeArgs& a, int batch, bool joined, hipStream_t stream) {
   // One 8-wave workgroup (128 KB of LDS) fills a CU.  A grid of at most
   // kWideGridMax of those runs in about two rounds; a larger grid runs in
@@ -1072,24 +1104,24 @@ static hipError_t launch_decode(const DecodeArgs& a, int batch, bool joined, hip
       hipLaunchKernelGGL(kernel, grid, dim3(64 * per_wg), 0, stream, a);
     };
     if constexpr (Cache::kItemWaves == kWavesPerWG) {
-      if (wide) run(split_kernel<T, kWavesPerWG, kItems, Cache>());
+      if (wide) run(split_kernel<T, kWavesPerWG, kItems, Cache, kTrack>());
     }
-    if (!wide) run(split_kernel<T, kNarrowWaves, kItems, Cache>());
+    if (!wide) run(split_kernel<T, kNarrowWaves, kItems, Cache, kTrack>());
   } else if (wide_wgs <= kWideGridMax) {
     dim3 grid((unsigned)((units + kWavesPerWG - 1) / kWavesPerWG), (unsigned)a.splits,
               (unsigned)batch);
     if (a.rule.adapt) {
       std::swap(grid.y, grid.z);
-      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFollow, Cache>()), grid,
+      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFollow, Cache, kTrack>()), grid,
                          dim3(64 * kWavesPerWG), 0, stream, a);
     } else {
-      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFixed, Cache>()), grid,
+      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFixed, Cache, kTrack>()), grid,
                          dim3(64 * kWavesPerWG), 0, stream, a);
     }
   } else {
     const dim3 grid((unsigned)((units + kNarrowWaves - 1) / kNarrowWaves), (unsigned)a.splits,
                     (unsigned)batch);
-    hipLaunchKernelGGL((split_kernel<T, kNarrowWaves, kFixed, Cache>()), grid,
+    hipLaunchKernelGGL((split_kernel<T, kNarrowWaves, kFixed, Cache, kTrack>()), grid,
                        dim3(64 * kNarrowWaves), 0, stream, a);
   }
   hipError_t e = hipGetLastError();
@@ -1226,17 +1258,30 @@ extern "C" size_t mskv_decode_workspace_bytes(int batch, int num_q_heads,
 
 namespace mskv {
 
+// Where the scores of a decode that tracks its weights start in its workspace,
+// behind the partials and work items, and their bytes.
+static size_t track_scores_at(int batch, int hq, int hk, int splits) {
+  const size_t items = mskv_decode_workspace_bytes(batch, hq, hk, kHeadDim, splits);
+  return (std::max(items, partials_bytes(batch, hq, splits)) + 255) & ~(size_t)255;
+}
+static size_t track_scores_bytes(int batch, int hq, int w, int block_size) {
+  return (size_t)batch * hq * w * block_size * sizeof(float);
+}
+
 // Validates a decode call and launches it with `workspace` as the split
 // partials ([batch, hq, splits, 128] outputs, then [batch, hq, splits]
 // lse values); `workspace_bytes` is what the caller's buffer holds.
-template <typename Cache>
+//
+// kTrack: the workspace holds partials whatever the splits, then the scores
+// (track_scores_at), and `track` is launched behind the decode.
+template <typename Cache, bool kTrack = false, typename Track = std::nullptr_t>
 static int decode_checked(const void* query, const void* k_cache, const void* v_cache,
                           const void* k_scale_cache, const float* v_scale_cache,
                           const int32_t* cache_seqlens, const int32_t* block_tables, void* out,
                           int batch, int num_q_heads, int num_kv_heads, int head_dim,
                           int block_size, int64_t num_blocks, int max_blocks_per_seq,
                           float softmax_scale, int act_dtype, int num_splits, void* workspace,
-                          size_t workspace_bytes, void* stream) {
+                          size_t workspace_bytes, void* stream, Track track = nullptr) {
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || block_size <= 0 ||
       num_blocks < 0 || max_blocks_per_seq <= 0 || num_splits <= 0)
     return MSKV_EINVAL;
@@ -1261,7 +1306,9 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
        (((uintptr_t)k_scale_cache | (uintptr_t)v_scale_cache) & 3)))
     return MSKV_EINVAL;
   const size_t need =
-      mskv_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_splits);
+      kTrack ? track_scores_at(batch, num_q_heads, num_kv_heads, num_splits) +
+                   track_scores_bytes(batch, num_q_heads, max_blocks_per_seq, block_size)
+             : mskv_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_splits);
   if (need > 0 && (!workspace || workspace_bytes < need)) return MSKV_EWORKSPACE;
 
   DecodeArgs a;
@@ -1321,7 +1368,16 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
                      info};
   a.num_blocks = num_blocks;
   a.scale_log2 = softmax_scale * kLog2e;
+  a.scores = nullptr;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if constexpr (kTrack) {
+    a.scores = (float*)((uint8_t*)workspace +
+                        track_scores_at(batch, num_q_heads, num_kv_heads, num_splits));
+    const hipError_t e = act_dtype == MSKV_BFLOAT16
+                             ? launch_decode<__bf16, Cache, true>(a, batch, false, s)
+                             : launch_decode<_Float16, Cache, true>(a, batch, false, s);
+    return e != hipSuccess ? (int)e : track(a, s);
+  }
   const bool joined = std::is_same<Cache, Fp4Cache>::value &&
                       joined_of(batch, num_q_heads, num_kv_heads, max_blocks_per_seq, block_size);
   hipError_t e = act_dtype == MSKV_BFLOAT16
@@ -1409,3 +1465,5 @@ extern "C" int mskv_fp4_decode_attention(
       num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,
       softmax_scale, act_dtype, num_splits, workspace, workspace_bytes, stream);
 }
+
+#include "attention_weights.h"

@@ -1,0 +1,375 @@
+// Eviction from the FP8 paged cache: the tokens of every (sequence, kv head)
+// that stay, and the moving of their rows to the front of the sequence's pages.
+//
+//  * select_kv_tokens_kernel: of L tokens n = min(L, budget) stay: the first
+//    `start`, the last `recent`, and the heaviest of those between.  The
+//    threshold weight is found by its digits, from the highest (11, 11 and 10
+//    bits of an order-preserving integer form of the weight), each by a
+//    histogram in LDS; one more pass writes the kept positions in ascending
+//    order, of the tokens at the threshold the earliest.  One workgroup a
+//    (sequence, kv head), which holds up to 32 keys a thread in registers.
+//  * evict_kv_tokens_kernel: place i of a (sequence, kv head) gets the row of
+//    position kept[i].  The positions ascend, so kept[i] >= i, and a workgroup
+//    that walks the places in order may overwrite what it has read: a run of
+//    places is loaded whole, then stored, and no later run reads below its own
+//    first place.  HBM-bound, two bytes moved per byte that changes its place.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "mskv_device.h"
+#include "../../include/mskv.h"
+
+namespace mskv {
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kSelectBins = 2048;
+
+struct SelectArgs {
+  const float* weights;
+  const int32_t *seqlens, *bt, *starts;
+  int32_t *kept, *new_lens;
+  int64_t num_blocks;
+  int hk, bs, w, start, recent, budget;
+};
+
+// An integer that orders as the weight does: NaN lowest, -0 as 0.
+__device__ __forceinline__ uint32_t weight_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
+  if ((u & 0x7FFFFFFFu) == 0u) return 0x80000000u;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// The sum of v over the threads before this one, and over all.
+__device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_wave, uint32_t& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 63) s_wave[wave] = x;
+  __syncthreads();
+  uint32_t before = x - v;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < kSelectWaves; ++i) {
+    const uint32_t t = s_wave[i];
+    if (i < wave) before += t;
+    all += t;
+  }
+  __syncthreads();
+  return before;
+}
+
+// kItems: keys that a thread holds (0: the weights are read again on every
+// pass; thread t's j-th key is that of token j * 1024 + t of the range).
+template <int kItems>
+__global__ __launch_bounds__(kSelectThreads) void select_kv_tokens_kernel(SelectArgs a) {
+  __shared__ uint32_t s_hist[kSelectBins];
+  __shared__ uint32_t s_wave[kSelectWaves];
+  __shared__ uint32_t s_found[2];
+  constexpr int kTurn = kItems > 0 && kItems < 8 ? kItems : 8;  // keys of the last pass's turn
+  constexpr int kEntries = kTurn * kSelectWaves;
+  __shared__ uint32_t s_count[kEntries];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x / a.hk, h = blockIdx.x - b * a.hk;
+  const int L = max(0, min(__builtin_amdgcn_readfirstlane(a.seqlens[b]), a.w * a.bs));
+  const int n = min(L, a.budget);
+  int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
+  if (h == 0 && tid == 0) a.new_lens[b] = n;
+  const int first =
+      min(max(a.starts ? __builtin_amdgcn_readfirstlane(a.starts[b]) : a.start, 0), n);
+  const int last = min(a.recent, n - first);
+  // what stays whatever it weighs
+  const int fixed_front = n == L ? n : first;
+  for (int i = tid; i < fixed_front; i += kSelectThreads) kept[i] = i;
+  for (int i = n + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+  if (n == L) return;
+  for (int i = tid; i < last; i += kSelectThreads) kept[n - last + i] = L - last + i;
+  const int quota = n - first - last;
+  if (quota == 0) return;
+  const int count = L - last - first;  // tokens that compete: more than quota
+
+  const int32_t* table = a.bt + (int64_t)b * a.w;
+  auto read = [&](int i) -> uint32_t {  // the key of the range's token i
+    const int t = first + i, page = t / a.bs;
+    const int blk = table[page];
+    if (blk < 0 || (int64_t)blk >= a.num_blocks) return 0u;
+    return weight_key(a.weights[((int64_t)blk * a.hk + h) * a.bs + (t - page * a.bs)]);
+  };
+  uint32_t own[kItems > 0 ? kItems : 1];
+  if constexpr (kItems > 0) {
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const int i = j * kSelectThreads + tid;
+      own[j] = i < count ? read(i) : 0u;
+    }
+  }
+  auto each = [&](auto&& f) {  // f(token of the range, key)
+    if constexpr (kItems > 0) {
+      // (the compiler would keep a mask a key from pass to pass, and spill them)
+      int n_own = count;
+      asm volatile("" : "+s"(n_own));
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        const int i = j * kSelectThreads + tid;
+        if (i < n_own) f(i, own[j]);
+      }
+    } else {
+      for (int i = tid; i < count; i += kSelectThreads) f(i, read(i));
+    }
+  };
+
+  // The threshold: the quota-th largest key, digit by digit; `need` of the
+  // tokens whose digits so far are the threshold's are still to be found.
+  uint32_t need = quota, digits = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t mask = pass == 2 ? 1023u : 2047u;
+    for (int i = tid; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
+    __syncthreads();
+    each([&](int, uint32_t key) {
+      // (the digits above: all 32 bits on the first pass have none)
+      if (pass == 0 || (key >> (pass == 1 ? 21 : 10)) == digits)
+        atomicAdd(&s_hist[(key >> shift) & mask], 1u);
+    });
+    __syncthreads();
+    // this thread's two bins, from the highest down
+    const uint32_t hi = s_hist[kSelectBins - 1 - 2 * tid], lo = s_hist[kSelectBins - 2 - 2 * tid];
+    uint32_t all;
+    const uint32_t before = scan_before(hi + lo, s_wave, all);
+    if (before < need && before + hi + lo >= need) {
+      const bool upper = before + hi >= need;
+      s_found[0] = kSelectBins - 1 - 2 * tid - (upper ? 0 : 1);
+      s_found[1] = need - before - (upper ? 0 : hi);
+    }
+    __syncthreads();
+    digits = pass == 0 ? s_found[0] : digits << (pass == 1 ? 11 : 10) | s_found[0];
+    need = s_found[1];
+    __syncthreads();
+  }
+  const uint32_t threshold = digits;
+
+  // The kept positions in order: those above the threshold, and the first
+  // `need` at it.  A wave's counts of 64 tokens of either, then their running
+  // sums over the workgroup (two counts in a word: at most 2^13 tokens a turn).
+  uint32_t above0 = 0, equal0 = 0;  // before this turn
+  int32_t* to = kept + first;
+  auto turn = [&](int at, const uint32_t (&key)[kTurn]) {
+#pragma unroll
+    for (int j = 0; j < kTurn; ++j) {
+      const bool live = at + j * kSelectThreads + tid < count;
+      const uint64_t above = __ballot(live && key[j] > threshold);
+      const uint64_t equal = __ballot(live && key[j] == threshold);
+      if (lane == 0) s_count[j * kSelectWaves + wave] = __popcll(above) | __popcll(equal) << 16;
+    }
+    __syncthreads();
+    uint32_t all;
+    const uint32_t c = tid < kEntries ? s_count[tid] : 0u;
+    const uint32_t before = scan_before(c, s_wave, all);
+    if (tid < kEntries) s_count[tid] = before;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kTurn; ++j) {
+      const int i = at + j * kSelectThreads + tid;
+      const bool is_above = i < count && key[j] > threshold;
+      const bool is_equal = i < count && key[j] == threshold;
+      const uint32_t base = s_count[j * kSelectWaves + wave];
+      const uint32_t above = above0 + (base & 0xFFFFu) + lanes_below(__ballot(is_above));
+      const uint32_t equal = equal0 + (base >> 16) + lanes_below(__ballot(is_equal));
+      if (is_above || (is_equal && equal < need)) to[above + min(equal, need)] = first + i;
+    }
+    above0 += all & 0xFFFFu;
+    equal0 += all >> 16;
+    __syncthreads();
+  };
+  if constexpr (kItems > 0) {
+#pragma unroll
+    for (int t = 0; t < kItems / kTurn; ++t) {
+      if (t * kTurn * kSelectThreads >= count) break;
+      uint32_t key[kTurn];
+#pragma unroll
+      for (int j = 0; j < kTurn; ++j) key[j] = own[t * kTurn + j];
+      turn(t * kTurn * kSelectThreads, key);
+    }
+  } else {
+    for (int at = 0; at < count; at += kTurn * kSelectThreads) {
+      uint32_t key[kTurn];
+#pragma unroll
+      for (int j = 0; j < kTurn; ++j) {
+        const int i = at + j * kSelectThreads + tid;
+        key[j] = i < count ? read(i) : 0u;
+      }
+      turn(at, key);
+    }
+  }
+}
+
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictLoads = 4;  // 16-byte pieces a lane and run
+
+struct EvictArgs {
+  uint8_t *kc, *vc;
+  float *ks, *vs, *weights;
+  const int32_t *kept, *lens, *bt;
+  int64_t num_blocks;
+  int hk, bs, w, budget;
+};
+
+// A token's slot (its row among all pages' rows), -1 if it has none.
+__device__ __forceinline__ int64_t slot_of(const EvictArgs& a, const int32_t* table, int t) {
+  if (t < 0 || t >= a.w * a.bs) return -1;
+  const int page = t / a.bs;
+  const int blk = table[page];
+  return blk < 0 || (int64_t)blk >= a.num_blocks ? -1 : (int64_t)blk * a.bs + (t - page * a.bs);
+}
+
+// grid (kv head, part, sequence); parts: columns of K's rows, columns of V's
+// rows (kParts pieces of a row each), the scales and weights.
+template <int kParts>
+__global__ __launch_bounds__(kEvictThreads) void evict_kv_tokens_kernel(EvictArgs a) {
+  const int tid = threadIdx.x;
+  const int h = blockIdx.x, part = blockIdx.y, b = blockIdx.z;
+  const int32_t* table = a.bt + (int64_t)b * a.w;
+  const int32_t* kept = a.kept + ((int64_t)b * a.hk + h) * a.budget;
+  const int n = min(a.lens[b], a.budget);
+  if (part < 2 * kParts) {
+    constexpr int kLanes = kHeadDim / 16 / kParts;  // of a piece of a row
+    constexpr int kRows = kEvictThreads / kLanes;
+    uint8_t* rows = (part < kParts ? a.kc : a.vc) + h * kHeadDim +
+                    (part % kParts) * (kHeadDim / kParts) + 16 * (tid % kLanes);
+    const int64_t stride = (int64_t)a.hk * kHeadDim;
+    for (int at = 0; at < n; at += kRows * kEvictLoads) {
+      u32x4 v[kEvictLoads];
+      int64_t dst[kEvictLoads];
+#pragma unroll
+      for (int k = 0; k < kEvictLoads; ++k) {
+        const int i = at + k * kRows + tid / kLanes;
+        const int from = i < n ? kept[i] : i;
+        dst[k] = -1;
+        if (from != i) {
+          const int64_t src = slot_of(a, table, from);
+          if (src >= 0) {
+            dst[k] = slot_of(a, table, i);
+            v[k] = *reinterpret_cast<const u32x4*>(rows + src * stride);
+          }
+        }
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();  // every row of this run is read
+#pragma unroll
+      for (int k = 0; k < kEvictLoads; ++k)
+        if (dst[k] >= 0) *reinterpret_cast<u32x4*>(rows + dst[k] * stride) = v[k];
+    }
+    return;
+  }
+  for (int at = 0; at < n; at += kEvictThreads) {
+    const int i = at + tid;
+    const int from = i < n ? kept[i] : i;
+    int64_t src = -1, dst = -1;
+    if (from != i) {
+      src = slot_of(a, table, from);
+      dst = src < 0 ? -1 : slot_of(a, table, i);
+    }
+    // a weight lies in its page's stretch of the head
+    auto place = [&](int64_t slot) {
+      const int64_t page = slot / a.bs;
+      return (page * a.hk + h) * a.bs + (slot - page * a.bs);
+    };
+    float k = 0.0f, v = 0.0f, x = 0.0f;
+    if (dst >= 0) {
+      k = a.ks[src * a.hk + h];
+      v = a.vs[src * a.hk + h];
+      if (a.weights) x = a.weights[place(src)];
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (dst >= 0) {
+      a.ks[dst * a.hk + h] = k;
+      a.vs[dst * a.hk + h] = v;
+      if (a.weights) a.weights[place(dst)] = x;
+    }
+  }
+}
+
+static int evict_shape(int batch, int num_kv_heads, int block_size, int64_t num_blocks,
+                       int max_blocks_per_seq, int budget) {
+  if (batch < 0 || num_kv_heads <= 0 || block_size <= 0 || num_blocks < 0 ||
+      max_blocks_per_seq <= 0 || budget <= 0)
+    return MSKV_EINVAL;
+  if ((int64_t)max_blocks_per_seq * block_size >= 1LL << 30 || batch > 65535 ||
+      num_kv_heads > 65535)
+    return MSKV_EUNSUPPORTED;
+  return MSKV_OK;
+}
+
+}  // namespace mskv
+
+extern "C" int mskv_select_kv_tokens(const float* weights, const int32_t* cache_seqlens,
+                                     const int32_t* block_tables, const int32_t* starts, int start,
+                                     int recent, int budget, int32_t* kept, int32_t* new_seqlens,
+                                     int batch, int num_kv_heads, int block_size,
+                                     int64_t num_blocks, int max_blocks_per_seq, void* stream) {
+  using namespace mskv;
+  const int status = evict_shape(batch, num_kv_heads, block_size, num_blocks, max_blocks_per_seq,
+                                 budget);
+  if (status != MSKV_OK) return status;
+  if (start < 0 || recent < 0) return MSKV_EINVAL;
+  if (batch == 0) return MSKV_OK;
+  if (!weights || !cache_seqlens || !block_tables || !kept || !new_seqlens) return MSKV_EINVAL;
+  const SelectArgs a = {weights, cache_seqlens, block_tables,       starts, kept,   new_seqlens,
+                        num_blocks, num_kv_heads, block_size, max_blocks_per_seq, start, recent,
+                        budget};
+  const dim3 grid((unsigned)(batch * num_kv_heads));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  // (by the most tokens that can compete)
+  const int64_t tokens = (int64_t)max_blocks_per_seq * block_size;
+  if (tokens <= 2 * kSelectThreads)
+    hipLaunchKernelGGL(select_kv_tokens_kernel<2>, grid, dim3(kSelectThreads), 0, s, a);
+  else if (tokens <= 8 * kSelectThreads)
+    hipLaunchKernelGGL(select_kv_tokens_kernel<8>, grid, dim3(kSelectThreads), 0, s, a);
+  else if (tokens <= 32 * kSelectThreads)
+    hipLaunchKernelGGL(select_kv_tokens_kernel<32>, grid, dim3(kSelectThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(select_kv_tokens_kernel<0>, grid, dim3(kSelectThreads), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+extern "C" int mskv_evict_kv_tokens(void* k_cache, void* v_cache, float* k_scale_cache,
+                                    float* v_scale_cache, float* weights, const int32_t* kept,
+                                    const int32_t* new_seqlens, const int32_t* block_tables,
+                                    int batch, int num_kv_heads, int head_dim, int block_size,
+                                    int64_t num_blocks, int max_blocks_per_seq, int budget,
+                                    void* stream) {
+  using namespace mskv;
+  const int status = evict_shape(batch, num_kv_heads, block_size, num_blocks, max_blocks_per_seq,
+                                 budget);
+  if (status != MSKV_OK) return status;
+  if (head_dim != kHeadDim) return MSKV_EUNSUPPORTED;
+  if (batch == 0) return MSKV_OK;
+  if (!k_cache || !v_cache || !k_scale_cache || !v_scale_cache || !kept || !new_seqlens ||
+      !block_tables || misaligned({k_cache, v_cache}))
+    return MSKV_EINVAL;
+  const EvictArgs a = {(uint8_t*)k_cache, (uint8_t*)v_cache, k_scale_cache, v_scale_cache, weights,
+                       kept, new_seqlens, block_tables, num_blocks, num_kv_heads, block_size,
+                       max_blocks_per_seq, budget};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  constexpr int kParts = 1;
+  hipLaunchKernelGGL(evict_kv_tokens_kernel<kParts>,
+                     dim3((unsigned)num_kv_heads, 2 * kParts + 1, (unsigned)batch),
+                     dim3(kEvictThreads), 0, s, a);
+  return (int)hipGetLastError();
+}

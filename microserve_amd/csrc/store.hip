@@ -171,3 +171,4 @@ extern "C" int mskv_store_fp8_kvcache(const void* key, const void* value,
 }
 
 #include "fp4_store.h"
+#include "evict.h"
