@@ -532,6 +532,38 @@ int mskv_compact_kv_blocks(int num_pools, void* const* bases,
                            int32_t* num_live, void* stream);
 
 /*
+ * mskv_fp8_decode_attention for sequences that share prefixes: the first
+ * prefix_lens[g] tokens of the sequences cu_groups[g] .. cu_groups[g + 1] - 1
+ * are the same pages, and are read once for all of them.  cu_groups: int32
+ * [num_groups + 1], ascending; prefix_lens: int32 [num_groups]; both on the
+ * device.  cache_seqlens counts the whole context and block_tables names all
+ * of its pages, the prefix's in every row of the group.  Sequences in no group
+ * have a prefix of their own.  What is shared ends at a multiple of 128
+ * tokens, at the shortest of the group's sequences (those without tokens
+ * aside) and at max_prefix_len, a bound known to the host that the launch is
+ * laid out by; the rest is read sequence by sequence, so that the result is
+ * mskv_fp8_decode_attention's in any case.
+ * The workspace holds mskv_shared_decode_workspace_bytes: fp32 partials, merged
+ * by a second kernel.  It belongs to one call at a time.
+ * Supported: head_dim == 128, block_size % 128 == 0, num_groups <= 1024;
+ * query, k_cache, v_cache, out and workspace on 16 bytes (MSKV_EINVAL).
+ */
+size_t mskv_shared_decode_workspace_bytes(int batch, int num_groups,
+                                          int num_q_heads, int num_kv_heads,
+                                          int block_size,
+                                          int max_blocks_per_seq,
+                                          int64_t max_prefix_len);
+int mskv_fp8_shared_prefix_decode_attention(
+    const void* query, const void* k_cache, const void* v_cache,
+    const float* k_scale_cache, const float* v_scale_cache,
+    const int32_t* cache_seqlens, const int32_t* block_tables,
+    const int32_t* cu_groups, const int32_t* prefix_lens,
+    int64_t max_prefix_len, void* out, int batch, int num_groups,
+    int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+    int64_t num_blocks, int max_blocks_per_seq, float softmax_scale,
+    int act_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Attention weights of cached tokens.  `weights` is float32 [num_blocks,
  * num_kv_heads, block_size] beside the FP8 caches: the entry of a token and
  * kv head is a sum of softmax probabilities (of the q heads that read the kv

@@ -10,7 +10,8 @@ hand-written gfx950 HIP kernels behind the C ABI in ``include/mskv.h``.
 
 Beside them, the same path over a cache held in 4 bits (``fp4_kv_cache``,
 ``fp4_attention``; the ``Attention`` layer takes either), the moving of a
-pool's pages (``kv_blocks``), and the attention weights of cached tokens with
+pool's pages (``kv_blocks``), the decode of sequences that share prefixes
+(``shared_prefix``), and the attention weights of cached tokens with
 eviction by them (``attention_weights``).
 """
 
@@ -29,6 +30,8 @@ from microserve_amd.fp4_kv_cache import (  # noqa: F401
 from microserve_amd.fp4_attention import (  # noqa: F401
     fp4_chunk_prefill_attention, fp4_decode_attention, fp4_varlen_prefill_attention)
 from microserve_amd.kv_blocks import compact_kv_blocks, copy_kv_blocks  # noqa: F401
+from microserve_amd.shared_prefix import (  # noqa: F401
+    fp8_shared_prefix_decode_attention, group_by_prefix)
 from microserve_amd.attention_weights import (  # noqa: F401
     allocate_attention_weights, evict_kv_tokens, fp8_decode_attention_weights,
     fp8_window_attention_weights, select_kv_tokens)

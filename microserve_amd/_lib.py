@@ -134,6 +134,12 @@ _PROTOS = {
     "mskv_check_kv_blocks": (_c_int, [_c_int, _vp, _vp, _vp, _vp, _c_i64, _c_int]),
     "mskv_compact_kv_blocks": (_c_int, [
         _c_int, _vp, _vp, _vp, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp]),
+    "mskv_shared_decode_workspace_bytes": (_c_size, [
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64]),
+    "mskv_fp8_shared_prefix_decode_attention": (_c_int, [
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _vp,
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_int, _c_f32, _c_int,
+        _vp, _c_size, _vp]),
     "mskv_decode_weights_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
     "mskv_fp8_decode_attention_weights": (_c_int, [
         _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _vp,

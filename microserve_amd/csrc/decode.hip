@@ -1467,3 +1467,4 @@ extern "C" int mskv_fp4_decode_attention(
 }
 
 #include "attention_weights.h"
+#include "shared_decode.h"

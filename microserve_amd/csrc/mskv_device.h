@@ -60,6 +60,17 @@ __device__ __forceinline__ float buf_load_f32(__amdgpu_buffer_rsrc_t r,
                             __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0));
 }
 
+// Direct global -> LDS loads (buffer_load ... lds): lane i of the wave
+// writes its `bytes` at lds + i * bytes, from any per-lane offset.
+__device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      r, (__attribute__((address_space(3))) void*)lds, 16, (int)off, 0, 0, 0);
+}
+__device__ __forceinline__ void lds_load4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      r, (__attribute__((address_space(3))) void*)lds, 4, (int)off, 0, 0, 0);
+}
+
 // LDS byte offset of 16-byte chunk `chunk` of row `row` in a tile of
 // 128-byte rows, XOR-swizzled by (row / 2) % 8.  Row-major writes of eight
 // chunks per row, reads of one chunk from 16 consecutive rows (MFMA operand

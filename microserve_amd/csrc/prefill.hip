@@ -111,17 +111,6 @@ __device__ __forceinline__ f32x4 mfma_fp8(const i32x8& a, const i32x8& b, f32x4 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
 
-// Direct global -> LDS loads (buffer_load ... lds): lane i of the wave
-// writes its `bytes` at lds + i * bytes, from any per-lane offset.
-__device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(
-      r, (__attribute__((address_space(3))) void*)lds, 16, (int)off, 0, 0, 0);
-}
-__device__ __forceinline__ void lds_load4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(
-      r, (__attribute__((address_space(3))) void*)lds, 4, (int)off, 0, 0, 0);
-}
-
 // kSplit: the workgroup takes one of a.splits ranges of the keys (whole
 // tiles, from the actual key count) and leaves partials for the merge.
 template <typename T, bool kSplit>
