@@ -95,78 +95,140 @@ struct WindowArgs {
   const int32_t *bt, *cu_q, *cu_k;  // cu_q null: one query a sequence, lengths in cu_k
   const int32_t* starts;
   float *weights, *part, *lse;
+  int* per;  // tiles of a range of window_lse_kernel, for the merge
   int64_t total_q, num_blocks;
   float scale_log2;
-  int hq, hk, group, bs, w, start, chunks, rows;
+  int num_seqs, hq, hk, group, bs, w, start, ranges, rows;
   bool add, set_new;
 };
 
 constexpr int kWinThreads = 256;
-constexpr int kWinKeys = 256;  // of a workgroup: 64 a wave
-constexpr int kWinRows = 128;  // (query, q head of the group), of a turn
+constexpr int kWinTile = 256;  // keys of a workgroup's turn, 64 a wave
+constexpr int kWinRows = 128;  // (query, q head of the group) rows of a turn
+// Workgroups that should run at once, two a CU
+constexpr int kWinSlots = 512;
 
 // A sequence's queries and keys, clamped to the tensors.
 struct WindowSeq {
   int q_begin, lq, lk, rows;
 };
+__device__ __forceinline__ int window_keys_of(const WindowArgs& a, int s) {
+  const int lk = a.cu_q ? a.cu_k[s + 1] - a.cu_k[s] : a.cu_k[s];
+  // (a bound that is too low drops the keys past it)
+  return max(0, (int)min((int64_t)min(lk, a.w * a.bs), (int64_t)a.ranges * kWinTile));
+}
 __device__ __forceinline__ WindowSeq window_seq(const WindowArgs& a, int s) {
   WindowSeq w;
   const int64_t tq = a.total_q;
   if (a.cu_q) {
     w.q_begin = (int)min((int64_t)max(a.cu_q[s], 0), tq);
     w.lq = (int)min((int64_t)max(a.cu_q[s + 1], w.q_begin), tq) - w.q_begin;
-    w.lk = a.cu_k[s + 1] - a.cu_k[s];
   } else {
     w.q_begin = s;
     w.lq = 1;
-    w.lk = a.cu_k[s];
   }
-  w.lk = max(0, min(w.lk, a.w * a.bs));
+  w.lk = window_keys_of(a, s);
   w.rows = (int)min((int64_t)w.lq * a.group, (int64_t)a.rows);
   return w;
 }
 
-// The wave's 64 keys (16 kg + n of lane (g, n)) as the matrix unit's operand:
-// dimensions [16g, 16g + 16) and [64 + 16g, 64 + 16g + 16), as the decode has
-// them; zeros past the sequence's end and for an invalid page.
-template <typename T>
-__device__ __forceinline__ void window_keys(const WindowArgs& a, int s, int kvh, int t0, int lk,
-                                            int lane, typename Act<T>::x8 (&kop)[4][4],
-                                            float& scale, int& valid) {
+// The workgroup's range of keys: the sequences' tiles are spread over the
+// workgroups that run at once, from the lengths (`units` workgroups take a range:
+// kv heads, turns of rows), and the ranges with keys come first in the grid.
+// (By sequence and chunk, with a grid as wide as the longest one, workgroups
+// without keys leave the others on a fraction of the CUs: 8 sequences of 20 to
+// 8192 tokens 63 us where eight of 8192 take 75.)
+struct WindowRange {
+  int s, index, per;  // the sequence (-1: none), its range, tiles of a range
+};
+__device__ __forceinline__ int wave_scan_i32(int v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(v, d);
+    if (lane >= d) v += y;
+  }
+  return v;
+}
+__device__ __forceinline__ WindowRange window_range(const WindowArgs& a, int item, int units) {
+  const int lane = threadIdx.x & 63;
+  auto tiles_of = [&](int s) {
+    return s < a.num_seqs ? (window_keys_of(a, s) + kWinTile - 1) / kWinTile : 0;
+  };
+  const int own = tiles_of(lane);
+  int64_t total = own;
+  for (int s = 64 + lane; s < a.num_seqs; s += 64) total += tiles_of(s);
+  int tiles = (int)min(total, (int64_t)1 << 24);
+  tiles = __builtin_amdgcn_readfirstlane(wave_sum_i32(tiles));
+  WindowRange r = {-1, 0, 0};
+  r.per = max(1, (int)(((int64_t)tiles * units + kWinSlots - 1) / kWinSlots));
+  for (int base = 0; base < a.num_seqs; base += 64) {
+    const int n = ((base == 0 ? own : tiles_of(base + lane)) + r.per - 1) / r.per;
+    const int upto = wave_scan_i32(n);
+    const uint64_t hit = __ballot(item < upto);
+    if (hit) {
+      const int at = __ffsll((unsigned long long)hit) - 1;
+      r.s = base + at;
+      r.index = item - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
+      return r;
+    }
+    item -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return r;
+}
+
+// The wave's 64 keys from t0 on (16 kg + n of lane (g, n)) in the decode's order
+// of dimensions: [16g, 16g + 16) and [64 + 16g, 64 + 16g + 16).  Zeros past the
+// sequence's end and for an invalid page.
+struct WindowLoads {
+  u32x4 lo[4], hi[4];
+  float scale;  // of key `lane`
+  int valid;
+};
+__device__ __forceinline__ void window_load(const WindowArgs& a, int s, int kvh, int t0, int lk,
+                                            int lane, WindowLoads& x) {
   const int g = lane >> 4, n = lane & 15;
   const int page = t0 / a.bs, off = t0 - page * a.bs;
-  const int blk = t0 < lk ? a.bt[(int64_t)s * a.w + page] : -1;
+  typedef const __attribute__((address_space(4))) int32_t* Table;  // (stays scalar)
+  const int blk =
+      t0 < lk ? ((Table)reinterpret_cast<uintptr_t>(a.bt))[(int64_t)s * a.w + page] : -1;
   const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
   const int64_t bo = ok ? blk : 0;
-  valid = ok ? min(64, lk - t0) : 0;
+  x.valid = ok ? min(64, lk - t0) : 0;
   const uint32_t stride = (uint32_t)a.hk * kHeadDim;
-  const auto kr = make_rsrc(a.kc + bo * a.bs * stride, (uint32_t)(off + valid) * (ok ? stride : 0u));
-  const auto sr = make_rsrc(a.ks + bo * a.bs * a.hk, ok ? (uint32_t)(off + valid) * a.hk * 4u : 0u);
-  u32x4 lo[4], hi[4];
+  const auto kr =
+      make_rsrc(a.kc + bo * a.bs * stride, ok ? (uint32_t)(off + x.valid) * stride : 0u);
+  const auto sr =
+      make_rsrc(a.ks + bo * a.bs * a.hk, ok ? (uint32_t)(off + x.valid) * a.hk * 4u : 0u);
 #pragma unroll
   for (int kg = 0; kg < 4; ++kg) {
     const uint32_t o = (uint32_t)(off + 16 * kg + n) * stride + (uint32_t)kvh * kHeadDim + 16u * g;
-    lo[kg] = buf_load16(kr, o);
-    hi[kg] = buf_load16(kr, o + 64u);
+    x.lo[kg] = buf_load16(kr, o);
+    x.hi[kg] = buf_load16(kr, o + 64u);
   }
-  scale = buf_load_f32(sr, (((uint32_t)off + lane) * a.hk + kvh) * 4u) * a.scale_log2;
+  x.scale = buf_load_f32(sr, (((uint32_t)off + lane) * a.hk + kvh) * 4u);
+}
+template <typename T>
+__device__ __forceinline__ void window_operand(const WindowLoads& x,
+                                               typename Act<T>::x8 (&kop)[4][4]) {
   using A = Act<T>;
 #pragma unroll
   for (int kg = 0; kg < 4; ++kg) {
-    A::fp8x4_to(lo[kg][0], kop[kg][0], 0); A::fp8x4_to(lo[kg][1], kop[kg][0], 4);
-    A::fp8x4_to(lo[kg][2], kop[kg][1], 0); A::fp8x4_to(lo[kg][3], kop[kg][1], 4);
-    A::fp8x4_to(hi[kg][0], kop[kg][2], 0); A::fp8x4_to(hi[kg][1], kop[kg][2], 4);
-    A::fp8x4_to(hi[kg][2], kop[kg][3], 0); A::fp8x4_to(hi[kg][3], kop[kg][3], 4);
+    A::fp8x4_to(x.lo[kg][0], kop[kg][0], 0); A::fp8x4_to(x.lo[kg][1], kop[kg][0], 4);
+    A::fp8x4_to(x.lo[kg][2], kop[kg][1], 0); A::fp8x4_to(x.lo[kg][3], kop[kg][1], 4);
+    A::fp8x4_to(x.hi[kg][0], kop[kg][2], 0); A::fp8x4_to(x.hi[kg][1], kop[kg][2], 4);
+    A::fp8x4_to(x.hi[kg][2], kop[kg][3], 0); A::fp8x4_to(x.hi[kg][3], kop[kg][3], 4);
   }
 }
 
-// Stages rows [row0, row0 + 128) of a kv head into LDS (256-byte rows, 16-byte
+// Stages kRows rows of a kv head from row0 on into LDS (256-byte rows, 16-byte
 // chunks XOR-swizzled by the row; zeros past the last one), with each row's
 // number of visible keys.
+template <int kRows>
 __device__ __forceinline__ void window_rows(const WindowArgs& a, const WindowSeq& w, int kvh,
                                             int row0, uint8_t* q_lds, int* s_lim) {
 #pragma unroll
-  for (int i = 0; i < kWinRows * 16 / kWinThreads; ++i) {
+  for (int i = 0; i < kRows * 16 / kWinThreads; ++i) {
     const int r = (i * kWinThreads + threadIdx.x) >> 4, c = threadIdx.x & 15;
     const int row = row0 + r;
     const int qi = row / a.group, h = row - qi * a.group;
@@ -179,8 +241,8 @@ __device__ __forceinline__ void window_rows(const WindowArgs& a, const WindowSeq
   }
 }
 template <typename T>
-__device__ __forceinline__ void window_operand(const uint8_t* q_lds, int rb, int lane,
-                                               typename Act<T>::x8 (&qop)[4]) {
+__device__ __forceinline__ void window_query(const uint8_t* q_lds, int rb, int lane,
+                                             typename Act<T>::x8 (&qop)[4]) {
   const int g = lane >> 4, n = lane & 15;
   const uint8_t* row = q_lds + (16 * rb + n) * 256;
 #pragma unroll
@@ -191,207 +253,260 @@ __device__ __forceinline__ void window_operand(const uint8_t* q_lds, int rb, int
   }
 }
 
-// The largest score and the sum of 2^(score - it) of each row over the
-// workgroup's 256 keys.  S^T = K . Q^T: a lane holds 16 keys of one row.
-// grid (key chunks, kv heads x turns of rows, sequences)
+// The log-sum-exp of each of 128 rows over the workgroup's range of keys.
+// S^T = K . Q^T: a lane holds 16 keys of one row, for which it keeps a running
+// maximum and sum of its own; they meet at the end.
+// grid: ranges x (kv heads x turns of rows)
 template <typename T>
-__global__ __launch_bounds__(kWinThreads) void window_lse_kernel(WindowArgs a) {
+__global__ __launch_bounds__(kWinThreads, 2) void window_lse_kernel(WindowArgs a, int units) {
   using A = Act<T>;
+  constexpr int kBlocks = kWinRows / 16;
   __shared__ __attribute__((aligned(16))) uint8_t q_lds[kWinRows * 256];
-  __shared__ __attribute__((aligned(16))) float s_scale[kWinKeys];
+  __shared__ __attribute__((aligned(16))) float s_scale[4][64];
   __shared__ int s_lim[kWinRows];
   __shared__ float s_m[4][kWinRows], s_l[4][kWinRows];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n = lane & 15;
-  const int s = blockIdx.z;
-  const int kvh = blockIdx.y % a.hk, row0 = blockIdx.y / a.hk * kWinRows;
+  const int unit = blockIdx.x % units;
+  const WindowRange range = window_range(a, blockIdx.x / units, units);
+  if (blockIdx.x == 0 && tid == 0) *a.per = range.per;
+  if (range.s < 0) return;
+  const int s = range.s, kvh = unit % a.hk, row0 = unit / a.hk * kWinRows;
   const WindowSeq w = window_seq(a, s);
-  const int t0 = blockIdx.x * kWinKeys;
-  if (row0 >= w.rows || (t0 >= w.lk && t0 > 0)) return;
-  typename A::x8 kop[4][4];
-  float scale;
-  int valid;
-  const int k0 = t0 + 64 * wave;
-  window_keys<T>(a, s, kvh, k0, w.lk, lane, kop, scale, valid);
-  s_scale[tid] = scale;
-  window_rows(a, w, kvh, row0, q_lds, s_lim);
+  if (row0 >= w.rows) return;
+  const int first = range.index * range.per * kWinTile;
+  const int end = min(w.lk, first + range.per * kWinTile);
+  WindowLoads next;
+  window_load(a, s, kvh, first + 64 * wave, w.lk, lane, next);
+  window_rows<kWinRows>(a, w, kvh, row0, q_lds, s_lim);
   __syncthreads();
-  const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;  // every row sees every key
-  f32x4 ksc[4];
+  const int blocks = (min(kWinRows, w.rows - row0) + 15) / 16;
+  float m[kBlocks], l[kBlocks];
 #pragma unroll
-  for (int kg = 0; kg < 4; ++kg)
-    ksc[kg] = *reinterpret_cast<const f32x4*>(&s_scale[64 * wave + 16 * kg + 4 * g]);
-  for (int rb = 0; rb < kWinRows / 16; ++rb) {
-    typename A::x8 qop[4];
-    window_operand<T>(q_lds, rb, lane, qop);
-    f32x4 x[4];
-#pragma unroll
-    for (int kg = 0; kg < 4; ++kg) {
-      x[kg] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[kg] = A::mfma(kop[kg][j], qop[j], x[kg]);
-      x[kg] *= ksc[kg];
-    }
-    if (!all) {
-      const int lim = min(s_lim[16 * rb + n] - k0, valid);
-#pragma unroll
-      for (int kg = 0; kg < 4; ++kg)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!(16 * kg + 4 * g + r < lim)) x[kg][r] = -INFINITY;
-    }
-    float m = -INFINITY, l = 0.0f;
+  for (int rb = 0; rb < kBlocks; ++rb) m[rb] = -INFINITY, l[rb] = 0.0f;
+  for (int t0 = first; t0 < end; t0 += kWinTile) {
+    const int k0 = t0 + 64 * wave;
+    typename A::x8 kop[4][4];
+    window_operand<T>(next, kop);
+    const int valid = next.valid;
+    s_scale[wave][lane] = next.scale * a.scale_log2;
+    wave_lds_sync();
+    f32x4 ksc[4];
 #pragma unroll
     for (int kg = 0; kg < 4; ++kg)
-      m = fmaxf(fmaxf(m, fmaxf(x[kg][0], x[kg][1])), fmaxf(x[kg][2], x[kg][3]));
-    m = max_xor32(max_xor16(m));
-    const float ref = m == -INFINITY ? 0.0f : m;
+      ksc[kg] = *reinterpret_cast<const f32x4*>(&s_scale[wave][16 * kg + 4 * g]);
+    if (t0 + kWinTile < end) window_load(a, s, kvh, k0 + kWinTile, w.lk, lane, next);
+    if (valid > 0) {
+      const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;  // every row sees every key
 #pragma unroll
-    for (int kg = 0; kg < 4; ++kg)
+      for (int rb = 0; rb < kBlocks; ++rb) {
+        if (rb < blocks) {
+          typename A::x8 qop[4];
+          window_query<T>(q_lds, rb, lane, qop);
+          f32x4 x[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) l += exp2_fast(x[kg][r] - ref);
-    l = sum_xor32(sum_xor16(l));
+          for (int kg = 0; kg < 4; ++kg) {
+            x[kg] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[kg] = A::mfma(kop[kg][j], qop[j], x[kg]);
+            x[kg] *= ksc[kg];
+          }
+          if (!all) {
+            const int lim = min(s_lim[16 * rb + n] - k0, valid);
+#pragma unroll
+            for (int kg = 0; kg < 4; ++kg)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (!(16 * kg + 4 * g + r < lim)) x[kg][r] = -INFINITY;
+          }
+          float top = m[rb];
+#pragma unroll
+          for (int kg = 0; kg < 4; ++kg)
+            top = fmaxf(fmaxf(top, fmaxf(x[kg][0], x[kg][1])), fmaxf(x[kg][2], x[kg][3]));
+          const float ref = top == -INFINITY ? 0.0f : top;
+          float sum = 0.0f;
+#pragma unroll
+          for (int kg = 0; kg < 4; ++kg)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum += exp2_fast(x[kg][r] - ref);
+          l[rb] = l[rb] * exp2_fast(m[rb] - ref) + sum;
+          m[rb] = top;
+        }
+      }
+    }
+    wave_lds_sync();  // (the scales are read before the next ones are written)
+  }
+#pragma unroll
+  for (int rb = 0; rb < kBlocks; ++rb) {
+    const float top = max_xor32(max_xor16(m[rb]));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    const float sum = sum_xor32(sum_xor16(l[rb] * exp2_fast(m[rb] - ref)));
     if (g == 0) {
-      s_m[wave][16 * rb + n] = m;
-      s_l[wave][16 * rb + n] = l;
+      s_m[wave][16 * rb + n] = top;
+      s_l[wave][16 * rb + n] = sum;
     }
   }
   __syncthreads();
   if (tid >= kWinRows || row0 + tid >= w.rows) return;
-  float m = s_m[0][tid];
+  float top = s_m[0][tid];
 #pragma unroll
-  for (int i = 1; i < 4; ++i) m = fmaxf(m, s_m[i][tid]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
+  for (int i = 1; i < 4; ++i) top = fmaxf(top, s_m[i][tid]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) l += s_l[i][tid] * exp2_fast(s_m[i][tid] - ref);
-  const float lse = partial_lse(m, l);
+  for (int i = 0; i < 4; ++i) sum += s_l[i][tid] * exp2_fast(s_m[i][tid] - ref);
   const int row = row0 + tid;
   const int qi = row / a.group;
   const int64_t at = (int64_t)(w.q_begin + qi) * a.hq + kvh * a.group + (row - qi * a.group);
-  a.part[at * a.chunks + blockIdx.x] = lse;
+  a.part[at * a.ranges + range.index] = partial_lse(top, sum);
 }
 
-// lse[row] from the chunks that hold keys; +inf where no key is seen.
+// lse[row] from the ranges that hold keys; +inf where no key is seen.
 // One wave a row; grid (rows of the query tensor / 4, sequences)
 constexpr int kWinMergeRows = 4;
 __global__ __launch_bounds__(64 * kWinMergeRows) void window_merge_kernel(WindowArgs a) {
   const WindowSeq w = window_seq(a, blockIdx.y);
   const int local = blockIdx.x * kWinMergeRows + (threadIdx.x >> 6);
   // (row `local` of the sequence: query local / hq, q head local % hq)
-  if (local >= w.rows / a.group * a.hq) return;
+  if (local >= w.rows / a.group * a.hq || w.lk == 0) return;
   const int64_t at = (int64_t)w.q_begin * a.hq + local;
-  const int n = max(1, min(a.chunks, (w.lk + kWinKeys - 1) / kWinKeys));
-  const float lse = merged_lse(a.part + at * a.chunks, n, threadIdx.x & 63);
+  const int keys = *a.per * kWinTile;
+  const int n = min(a.ranges, (w.lk + keys - 1) / keys);
+  const float lse = merged_lse(a.part + at * a.ranges, n, threadIdx.x & 63);
   if ((threadIdx.x & 63) == 0) a.lse[at] = lse;
 }
 
-// The sums over the rows of 2^(score - lse) at the workgroup's 256 keys.
+// The sums over the rows of 2^(score - lse) at the workgroup's range of keys.
 // S = Q . K^T: a lane holds four rows of one key, whose sum needs no exchange
-// until all the rows are in.  grid (key chunks, kv heads, sequences)
-template <typename T>
-__global__ __launch_bounds__(kWinThreads) void window_sum_kernel(WindowArgs a) {
+// until all the rows are in.  grid: ranges x kv heads.  kRows: rows in LDS at
+// once; more of them are staged again for every tile.
+template <typename T, int kRows>
+__global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a) {
   using A = Act<T>;
-  __shared__ __attribute__((aligned(16))) uint8_t q_lds[kWinRows * 256];
-  __shared__ __attribute__((aligned(16))) int s_lim[kWinRows];
-  __shared__ __attribute__((aligned(16))) float s_lse[kWinRows];
+  __shared__ __attribute__((aligned(16))) uint8_t q_lds[kRows * 256];
+  __shared__ __attribute__((aligned(16))) int s_lim[kRows];
+  __shared__ __attribute__((aligned(16))) float s_lse[kRows];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n = lane & 15;
-  const int s = blockIdx.z, kvh = blockIdx.y;
+  const int kvh = blockIdx.x % a.hk;
+  const WindowRange range = window_range(a, blockIdx.x / a.hk, a.hk);
+  if (range.s < 0) return;
+  const int s = range.s;
   const WindowSeq w = window_seq(a, s);
-  const int t0 = blockIdx.x * kWinKeys;
-  if (t0 >= w.lk) return;
-  typename A::x8 kop[4][4];
-  float scale;
-  int valid;
-  const int k0 = t0 + 64 * wave;
-  window_keys<T>(a, s, kvh, k0, w.lk, lane, kop, scale, valid);
-  const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;
-  float ksc[4], sum[4];
-#pragma unroll
-  for (int kg = 0; kg < 4; ++kg) {
-    ksc[kg] = __shfl(scale, 16 * kg + n);
-    sum[kg] = 0.0f;
-  }
-  for (int row0 = 0; row0 < w.rows; row0 += kWinRows) {
-    if (row0 > 0) __syncthreads();
-    window_rows(a, w, kvh, row0, q_lds, s_lim);
-    if (tid < kWinRows) {
+  const int from = max(a.starts ? a.starts[s] : a.start, 0);
+  auto rows = [&](int row0) {
+    window_rows<kRows>(a, w, kvh, row0, q_lds, s_lim);
+    if (tid < kRows) {
       const int row = row0 + tid, qi = row / a.group;
       const int64_t at = (int64_t)(w.q_begin + qi) * a.hq + kvh * a.group + (row - qi * a.group);
       s_lse[tid] = row < w.rows ? a.lse[at] : INFINITY;
     }
-    __syncthreads();
-    const int blocks = min(kWinRows, w.rows - row0 + 15) / 16;
-    for (int rb = 0; rb < blocks; ++rb) {
-      typename A::x8 qop[4];
-      window_operand<T>(q_lds, rb, lane, qop);
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[16 * rb + 4 * g]);
+  };
+  const int first = range.index * range.per * kWinTile;
+  const int end = min(w.lk, first + range.per * kWinTile);
+  WindowLoads next;
+  window_load(a, s, kvh, first + 64 * wave, w.lk, lane, next);
+  rows(0);
+  __syncthreads();
+  for (int t0 = first; t0 < end; t0 += kWinTile) {
+    const int k0 = t0 + 64 * wave;
+    typename A::x8 kop[4][4];
+    window_operand<T>(next, kop);
+    const int valid = next.valid;
+    float ksc[4], sum[4];
 #pragma unroll
-      for (int kg = 0; kg < 4; ++kg) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int kg = 0; kg < 4; ++kg) {
+      ksc[kg] = __shfl(next.scale, 16 * kg + n) * a.scale_log2;
+      sum[kg] = 0.0f;
+    }
+    if (t0 + kWinTile < end) window_load(a, s, kvh, k0 + kWinTile, w.lk, lane, next);
+    const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;  // every row sees every key
+    for (int row0 = 0; row0 < w.rows; row0 += kRows) {
+      if (w.rows > kRows && (row0 > 0 || t0 > first)) {
+        __syncthreads();
+        rows(row0);
+        __syncthreads();
+      }
+      if (valid == 0) continue;
+      const int blocks = (min(kRows, w.rows - row0) + 15) / 16;
+      for (int rb = 0; rb < blocks; ++rb) {
+        typename A::x8 qop[4];
+        window_query<T>(q_lds, rb, lane, qop);
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[16 * rb + 4 * g]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x = A::mfma(qop[j], kop[kg][j], x);
-        f32x4 p;
+        for (int kg = 0; kg < 4; ++kg) {
+          f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = exp2_fast(fmaf(x[r], ksc[kg], -lse[r]));
-        if (!all) {
-          const int key = 16 * kg + n;
+          for (int j = 0; j < 4; ++j) x = A::mfma(qop[j], kop[kg][j], x);
+          f32x4 p;
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!(key < valid && k0 + key < s_lim[16 * rb + 4 * g + r])) p[r] = 0.0f;
+          for (int r = 0; r < 4; ++r) p[r] = exp2_fast(fmaf(x[r], ksc[kg], -lse[r]));
+          if (!all) {
+            const int key = 16 * kg + n;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!(key < valid && k0 + key < s_lim[16 * rb + 4 * g + r])) p[r] = 0.0f;
+          }
+          sum[kg] += (p[0] + p[1]) + (p[2] + p[3]);
         }
-        sum[kg] += (p[0] + p[1]) + (p[2] + p[3]);
       }
     }
-  }
 #pragma unroll
-  for (int kg = 0; kg < 4; ++kg) sum[kg] = sum_xor32(sum_xor16(sum[kg]));
-  const float own = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
-  const int tok = k0 + lane;  // key 16 g + n of the wave's
-  if (lane >= valid || tok < max(a.starts ? a.starts[s] : a.start, 0)) return;
-  const int page = k0 / a.bs;
-  float* to = a.weights +
-              ((int64_t)a.bt[(int64_t)s * a.w + page] * a.hk + kvh) * a.bs + (tok - page * a.bs);
-  const bool add = a.add && !(a.set_new && tok >= w.lk - w.lq);
-  *to = add ? *to + own : own;
+    for (int kg = 0; kg < 4; ++kg) sum[kg] = sum_xor32(sum_xor16(sum[kg]));
+    const float own = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
+    const int tok = k0 + lane;  // key 16 g + n of the wave's
+    if (lane < valid && tok >= from) {
+      const int page = k0 / a.bs;
+      float* to = a.weights + ((int64_t)a.bt[(int64_t)s * a.w + page] * a.hk + kvh) * a.bs +
+                  (tok - page * a.bs);
+      const bool add = a.add && !(a.set_new && tok >= w.lk - w.lq);
+      *to = add ? *to + own : own;
+    }
+  }
 }
 
-// [total_q * hq, chunks] partial log-sum-exps, then [total_q * hq] final ones
-static size_t window_bytes(int64_t total_q, int hq, int64_t chunks) {
-  return (size_t)total_q * hq * (chunks + 1) * sizeof(float);
+// [total_q * hq, ranges] partial log-sum-exps, [total_q * hq] final ones, then
+// the tiles of a range
+static size_t window_bytes(int64_t total_q, int hq, int64_t ranges) {
+  return ((size_t)total_q * hq * (ranges + 1) + 1) * sizeof(float);
 }
 
 template <typename T>
-static hipError_t launch_window(const WindowArgs& a, int num_seqs, hipStream_t st) {
+static hipError_t launch_window(const WindowArgs& a, hipStream_t st) {
+  // ranges with keys: at most the workgroups that run at once over `units`, and
+  // one more a sequence
+  auto grid = [&](int64_t units) {
+    const int64_t most = (kWinSlots + units - 1) / units + a.num_seqs;
+    return dim3((unsigned)(std::min(most, (int64_t)a.ranges * a.num_seqs) * units));
+  };
   if (a.rows > 0) {  // (without queries there are only zeros to write)
-    const unsigned turns = (unsigned)((a.rows + kWinRows - 1) / kWinRows);
-    hipLaunchKernelGGL(window_lse_kernel<T>,
-                       dim3((unsigned)a.chunks, (unsigned)a.hk * turns, (unsigned)num_seqs),
-                       dim3(kWinThreads), 0, st, a);
+    const int units = a.hk * ((a.rows + kWinRows - 1) / kWinRows);
+    hipLaunchKernelGGL(window_lse_kernel<T>, grid(units), dim3(kWinThreads), 0, st, a, units);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t local = (int64_t)a.rows / a.group * a.hq;
     hipLaunchKernelGGL(window_merge_kernel,
                        dim3((unsigned)((local + kWinMergeRows - 1) / kWinMergeRows),
-                            (unsigned)num_seqs),
+                            (unsigned)a.num_seqs),
                        dim3(64 * kWinMergeRows), 0, st, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(window_sum_kernel<T>,
-                     dim3((unsigned)a.chunks, (unsigned)a.hk, (unsigned)num_seqs),
-                     dim3(kWinThreads), 0, st, a);
+  if (a.rows <= kWinRows)
+    hipLaunchKernelGGL((window_sum_kernel<T, kWinRows>), grid(a.hk), dim3(kWinThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((window_sum_kernel<T, 2 * kWinRows>), grid(a.hk), dim3(kWinThreads), 0, st,
+                       a);
   return hipGetLastError();
 }
 
-// Key chunks of a window call, by the most keys of a sequence.
-static int64_t window_chunks(int64_t max_seqlen_k, int block_size, int w) {
+// Tiles of the longest sequence of a window call.
+static int64_t window_tiles(int64_t max_seqlen_k, int block_size, int w) {
   int64_t keys = (int64_t)w * block_size;
   if (max_seqlen_k > 0) keys = std::min(keys, max_seqlen_k);
-  return (keys + kWinKeys - 1) / kWinKeys;
+  return (keys + kWinTile - 1) / kWinTile;
 }
 
 // Most bytes of scores that a tracking decode asks for; past it K is read again
@@ -405,7 +520,7 @@ extern "C" size_t mskv_window_weights_workspace_bytes(int64_t total_q, int64_t m
                                                       int max_blocks_per_seq) {
   if (total_q <= 0 || num_q_heads <= 0 || block_size <= 0 || max_blocks_per_seq <= 0) return 0;
   return mskv::window_bytes(total_q, num_q_heads,
-                            mskv::window_chunks(max_seqlen_k, block_size, max_blocks_per_seq));
+                            mskv::window_tiles(max_seqlen_k, block_size, max_blocks_per_seq));
 }
 
 namespace mskv {
@@ -430,7 +545,10 @@ static int window_checked(
   const int group = num_q_heads / num_kv_heads;
   const int64_t rows = (int64_t)max_seqlen_q * group;
   const int64_t turns = (rows + kWinRows - 1) / kWinRows;
-  if (num_seqs > 65535 || turns * num_kv_heads > 65535 || total_q > 0x7FFFFFFFLL)
+  // (the launches' workgroups, and the sum of the tiles, stay within an int)
+  if (num_seqs > 65535 || total_q > 0x7FFFFFFFLL || rows > 0x7FFFFFFFLL ||
+      (num_seqs + kWinSlots) * turns * num_kv_heads > 0x7FFFFF ||
+      (int64_t)num_seqs * max_blocks_per_seq * block_size / kWinTile > 0x7FFFFFFF)
     return MSKV_EUNSUPPORTED;
   if (num_seqs == 0) return MSKV_OK;
   if (!k_cache || !k_scale_cache || !block_tables || !cu_seqlens_k || !weights)
@@ -438,7 +556,7 @@ static int window_checked(
   if (total_q > 0 && !query) return MSKV_EINVAL;
   if (misaligned({query, k_cache})) return MSKV_EINVAL;
   WindowArgs a = {};
-  a.chunks = (int)window_chunks(max_seqlen_k, block_size, max_blocks_per_seq);
+  a.ranges = (int)window_tiles(max_seqlen_k, block_size, max_blocks_per_seq);
   const size_t need = mskv_window_weights_workspace_bytes(total_q, max_seqlen_k, num_q_heads,
                                                           block_size, max_blocks_per_seq);
   if (need > 0 && (!workspace || workspace_bytes < need)) return MSKV_EWORKSPACE;
@@ -452,10 +570,12 @@ static int window_checked(
   a.start = start;
   a.weights = weights;
   a.part = (float*)workspace;
-  a.lse = a.part + (size_t)total_q * num_q_heads * a.chunks;
+  a.lse = a.part + (size_t)total_q * num_q_heads * a.ranges;
+  a.per = (int*)(a.lse + (size_t)total_q * num_q_heads);
   a.total_q = total_q;
   a.num_blocks = num_blocks;
   a.scale_log2 = softmax_scale * kLog2e;
+  a.num_seqs = num_seqs;
   a.hq = num_q_heads;
   a.hk = num_kv_heads;
   a.group = group;
@@ -465,8 +585,8 @@ static int window_checked(
   a.add = accumulate;
   a.set_new = cu_seqlens_q == nullptr;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return (int)(act_dtype == MSKV_BFLOAT16 ? launch_window<__bf16>(a, num_seqs, s)
-                                          : launch_window<_Float16>(a, num_seqs, s));
+  return (int)(act_dtype == MSKV_BFLOAT16 ? launch_window<__bf16>(a, s)
+                                          : launch_window<_Float16>(a, s));
 }
 
 }  // namespace mskv

@@ -376,9 +376,19 @@ __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh
   for (int t0 = t_begin; t0 < t_end; t0 += kStep, buf ^= 1) {
     const int valid = cur.valid;
     const bool more = t0 + kStep < t_end;
-    if (more)
-      load_step(a, a.bt[(int64_t)b * a.w + (t0 + kStep) / a.bs], kvh, t0 + kStep, t_end, lane,
-                nxt);
+    if (more) {
+      int blk;
+      if constexpr (kTrack) {
+        // (beside stores the compiler reads the table by vector loads, whose
+        // wait is one for every store in flight: the constant address space
+        // keeps it scalar.  64 x 4096 tokens: 129 us by vector loads)
+        typedef const __attribute__((address_space(4))) int32_t* Table;
+        blk = ((Table)reinterpret_cast<uintptr_t>(a.bt))[(int64_t)b * a.w + (t0 + kStep) / a.bs];
+      } else {
+        blk = a.bt[(int64_t)b * a.w + (t0 + kStep) / a.bs];
+      }
+      load_step(a, blk, kvh, t0 + kStep, t_end, lane, nxt);
+    }
 
     // S^T = K . Q^T for tokens [0,16) and [16,32) of the step
     const uint8_t* kt = kv_lds[buf][0];
@@ -413,14 +423,6 @@ __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh
       for (int r = 0; r < 4; ++r) {
         if (!(4 * g + r < valid)) x[r] = -INFINITY;
         if (!(16 + 4 * g + r < valid)) x[4 + r] = -INFINITY;
-      }
-    }
-    if constexpr (kTrack) {
-      if (head_ok) {
-        // (a page is whole steps: the row has room for this one)
-        float* to = scores + t0 + 4 * g;
-        *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4*>(to + 16) = f32x4{x[4], x[5], x[6], x[7]};
       }
     }
     float tmax = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
@@ -466,6 +468,15 @@ __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh
     if (more) {
       stage(nxt, buf ^ 1);
       cur = nxt;
+    }
+    if constexpr (kTrack) {
+      // Behind the wait for the next step's rows, which would be one for these
+      // stores too.  (A page is whole steps: the row has room for this one.)
+      if (head_ok) {
+        float* to = scores + t0 + 4 * g;
+        *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(to + 16) = f32x4{x[4], x[5], x[6], x[7]};
+      }
     }
     wave_lds_sync();
   }
