@@ -579,7 +579,7 @@ int mskv_fp8_shared_prefix_decode_attention(
  * cache_seqlens[b] - 1 (the entry of a reused page needs no clearing).
  * weights starts on 16 bytes.  The workspace holds
  * mskv_decode_weights_workspace_bytes: the split partials and, up to 1 GiB,
- * every score of the step (batch * num_q_heads * max_blocks_per_seq *
+ * every score of the step (about batch * num_q_heads * max_blocks_per_seq *
  * block_size floats); past that K is read again instead, and block_size must
  * be a multiple of 128.
  */

@@ -59,7 +59,7 @@ __global__ __launch_bounds__(kTrackThreads) void track_weights_kernel(TrackArgs 
     if (lane == 0) s_lse[h] = lse;
   }
   __syncthreads();
-  const int64_t cap = (int64_t)a.w * a.bs;
+  const int64_t cap = score_stride(a.w, a.bs);
   const int first = max(t.starts ? t.starts[b] : t.start, 0);
   for (int at = blockIdx.x * kTrackTokens; at < L; at += gridDim.x * kTrackTokens) {
     const int tok = at + 4 * threadIdx.x;
@@ -677,7 +677,7 @@ extern "C" int mskv_fp8_decode_attention_weights(
       hipLaunchKernelGGL(track_weights_kernel<false>, grid, dim3(kTrackThreads), lds, s, t);
     return (int)hipGetLastError();
   };
-  return decode_checked<Fp8Cache, true>(
+  return decode_checked<TrackedFp8Cache>(
       query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens, block_tables, out,
       batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,
       softmax_scale, act_dtype, splits, workspace, workspace_bytes, stream, track);

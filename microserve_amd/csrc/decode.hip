@@ -142,9 +142,16 @@ struct DecodeArgs {
   // the sequences' last ones by length; rule.info[0] of them are valid.
   const int4* items;
   SplitRule rule;
-  // [batch, hq, w * bs] scores of a decode that tracks its weights (else null)
+  // [batch, hq, score_stride(w, bs)] scores of a decode that tracks its weights (else null)
   float* scores;
 };
+
+// Floats from row to row of the scores.  The waves of a step walk their rows side
+// by side: rows a multiple of 4 KB apart would all be written to the same memory
+// channel at once.
+static inline __host__ __device__ int64_t score_stride(int w, int bs) {
+  return (int64_t)w * bs + 32;
+}
 
 // Sum / max over the wave with DPP row shifts and the two cross-row swaps
 // (no LDS round trip).
@@ -278,15 +285,13 @@ __device__ __forceinline__ void load_step(const DecodeArgs& a, int blk, int kvh,
 // un-normalized accumulator O^T, the running max m (log2 units) and the
 // lane's share of the denominator l.  kv_lds / s_lds are this wave's own
 // double-buffered LDS tiles; blk_first is the block of t_begin's page.
-// kTrack: the scores of the lane's tokens, in log2 units (-inf: not a token),
-// are left in `scores`, the row's by position, for track_weights_kernel.
-template <typename T, bool kTrack = false>
+template <typename T>
 __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh, int qh,
                                              bool head_ok, int t_begin, int t_end,
                                              int blk_first, int lane,
                                              uint8_t (&kv_lds)[2][2][kStep * kHeadDim],
                                              float (&s_lds)[2][2 * kStep], f32x4 (&acc)[8],
-                                             float& m, float& l, float* scores = nullptr) {
+                                             float& m, float& l) {
   using A = Act<T>;
   using x8 = typename A::x8;
   const int g = lane >> 4, n = lane & 15;
@@ -376,19 +381,9 @@ __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh
   for (int t0 = t_begin; t0 < t_end; t0 += kStep, buf ^= 1) {
     const int valid = cur.valid;
     const bool more = t0 + kStep < t_end;
-    if (more) {
-      int blk;
-      if constexpr (kTrack) {
-        // (beside stores the compiler reads the table by vector loads, whose
-        // wait is one for every store in flight: the constant address space
-        // keeps it scalar.  64 x 4096 tokens: 129 us by vector loads)
-        typedef const __attribute__((address_space(4))) int32_t* Table;
-        blk = ((Table)reinterpret_cast<uintptr_t>(a.bt))[(int64_t)b * a.w + (t0 + kStep) / a.bs];
-      } else {
-        blk = a.bt[(int64_t)b * a.w + (t0 + kStep) / a.bs];
-      }
-      load_step(a, blk, kvh, t0 + kStep, t_end, lane, nxt);
-    }
+    if (more)
+      load_step(a, a.bt[(int64_t)b * a.w + (t0 + kStep) / a.bs], kvh, t0 + kStep, t_end, lane,
+                nxt);
 
     // S^T = K . Q^T for tokens [0,16) and [16,32) of the step
     const uint8_t* kt = kv_lds[buf][0];
@@ -469,15 +464,6 @@ __device__ __forceinline__ void attend_range(const DecodeArgs& a, int b, int kvh
       stage(nxt, buf ^ 1);
       cur = nxt;
     }
-    if constexpr (kTrack) {
-      // Behind the wait for the next step's rows, which would be one for these
-      // stores too.  (A page is whole steps: the row has room for this one.)
-      if (head_ok) {
-        float* to = scores + t0 + 4 * g;
-        *reinterpret_cast<f32x4*>(to) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4*>(to + 16) = f32x4{x[4], x[5], x[6], x[7]};
-      }
-    }
     wave_lds_sync();
   }
   l = sum_xor32(sum_xor16(l));
@@ -496,6 +482,7 @@ struct Fp8Cache {
   static constexpr int kMaxPages = kMaxPagesPerSplit;
   static constexpr int kMinSteps = kMinSplitSteps;
   static constexpr int kItemWaves = kWavesPerWG;  // of a workgroup that takes work items
+  static constexpr bool kTrack = false;           // no scores are left
   typedef uint8_t Tiles[2][2][kStep * kHeadDim];  // K and V, double-buffered
   typedef float Scales[2][2 * kStep];
   template <typename T>
@@ -512,6 +499,7 @@ struct Fp8Cache {
 }  // namespace mskv
 
 #include "fp4_decode.h"
+#include "track_decode.h"
 
 namespace mskv {
 
@@ -558,9 +546,7 @@ __device__ __forceinline__ void write_partial(float* po, float* plse, const f32x
 // against 124 us.)
 // kFollow: the splits follow the lengths; kFixed: they are the shape's.
 enum DecodeMode { kFixed, kFollow, kItems };
-// kTrack: scores and every split's log-sum-exp are left for track_weights_kernel
-// (the FP8 cache only).
-template <typename T, int W, DecodeMode kMode, typename Cache, bool kTrack = false>
+template <typename T, int W, DecodeMode kMode, typename Cache>
 __device__ __forceinline__ void decode_split(const DecodeArgs& a) {
   // per wave: two buffers of tiles and their scales; step i is read from
   // buffer i&1 while step i+1 is staged into the other one
@@ -638,13 +624,8 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& a) {
 
   f32x4 acc[8];
   float m, l;
-  if constexpr (kTrack)
-    attend_range<T, true>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane,
-                          kv_lds_all[wave], s_lds_all[wave], acc, m, l,
-                          a.scores + ((int64_t)b * a.hq + qh) * a.w * a.bs);
-  else
-    Cache::template attend<T>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane,
-                              kv_lds_all[wave], s_lds_all[wave], acc, m, l);
+  Cache::template attend<T>(a, b, kvh, qh, head_ok, t_begin, t_end, blk_first, lane,
+                            kv_lds_all[wave], s_lds_all[wave], acc, m, l);
 
   // splits that hold tokens of this sequence; a sequence that fits in one
   // split is written here directly
@@ -652,7 +633,7 @@ __device__ __forceinline__ void decode_split(const DecodeArgs& a) {
   if (!head_ok) return;
   if (nvalid == 1) {
     write_output<T>(a.out + ((int64_t)b * a.hq + qh) * kHeadDim, acc, l, g);
-    if (kTrack && g == 0)
+    if (Cache::kTrack && g == 0)  // (the weights' kernel needs it)
       a.part_lse[((int64_t)b * a.hq + qh) * a.splits] = partial_lse(m, l);
     return;
   }
@@ -677,11 +658,11 @@ template <typename T, int W, DecodeMode kMode>
 __global__ __launch_bounds__(64 * W)
 __attribute__((amdgpu_waves_per_eu(2, 8)))
 void decode_track_kernel(DecodeArgs a) {
-  decode_split<T, W, kMode, Fp8Cache, true>(a);
+  decode_split<T, W, kMode, TrackedFp8Cache>(a);
 }
-template <typename T, int W, DecodeMode kMode, typename Cache, bool kTrack>
+template <typename T, int W, DecodeMode kMode, typename Cache>
 static auto split_kernel() {
-  if constexpr (kTrack)
+  if constexpr (Cache::kTrack)
     return decode_track_kernel<T, W, kMode>;
   else if constexpr (std::is_same<Cache, Fp4Cache>::value)
     return decode_fp4_kernel<T, W, kMode>;
@@ -1079,7 +1060,7 @@ static size_t partials_bytes(int batch, int hq, int splits) {
   return (raw + 255) & ~(size_t)255;
 }
 
-template <typename T, typename Cache, bool kTrack = false>
+template <typename T, typename Cache>
 static hipError_t launch_decode(const DecodeArgs& a, int batch, bool joined, hipStream_t stream) {
   // One 8-wave workgroup (128 KB of LDS) fills a CU.  A grid of at most
   // kWideGridMax of those runs in about two rounds; a larger grid runs in
@@ -1115,24 +1096,24 @@ static hipError_t launch_decode(const DecodeArgs& a, int batch, bool joined, hip
       hipLaunchKernelGGL(kernel, grid, dim3(64 * per_wg), 0, stream, a);
     };
     if constexpr (Cache::kItemWaves == kWavesPerWG) {
-      if (wide) run(split_kernel<T, kWavesPerWG, kItems, Cache, kTrack>());
+      if (wide) run(split_kernel<T, kWavesPerWG, kItems, Cache>());
     }
-    if (!wide) run(split_kernel<T, kNarrowWaves, kItems, Cache, kTrack>());
+    if (!wide) run(split_kernel<T, kNarrowWaves, kItems, Cache>());
   } else if (wide_wgs <= kWideGridMax) {
     dim3 grid((unsigned)((units + kWavesPerWG - 1) / kWavesPerWG), (unsigned)a.splits,
               (unsigned)batch);
     if (a.rule.adapt) {
       std::swap(grid.y, grid.z);
-      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFollow, Cache, kTrack>()), grid,
+      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFollow, Cache>()), grid,
                          dim3(64 * kWavesPerWG), 0, stream, a);
     } else {
-      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFixed, Cache, kTrack>()), grid,
+      hipLaunchKernelGGL((split_kernel<T, kWavesPerWG, kFixed, Cache>()), grid,
                          dim3(64 * kWavesPerWG), 0, stream, a);
     }
   } else {
     const dim3 grid((unsigned)((units + kNarrowWaves - 1) / kNarrowWaves), (unsigned)a.splits,
                     (unsigned)batch);
-    hipLaunchKernelGGL((split_kernel<T, kNarrowWaves, kFixed, Cache, kTrack>()), grid,
+    hipLaunchKernelGGL((split_kernel<T, kNarrowWaves, kFixed, Cache>()), grid,
                        dim3(64 * kNarrowWaves), 0, stream, a);
   }
   hipError_t e = hipGetLastError();
@@ -1276,16 +1257,16 @@ static size_t track_scores_at(int batch, int hq, int hk, int splits) {
   return (std::max(items, partials_bytes(batch, hq, splits)) + 255) & ~(size_t)255;
 }
 static size_t track_scores_bytes(int batch, int hq, int w, int block_size) {
-  return (size_t)batch * hq * w * block_size * sizeof(float);
+  return (size_t)batch * hq * score_stride(w, block_size) * sizeof(float);
 }
 
 // Validates a decode call and launches it with `workspace` as the split
 // partials ([batch, hq, splits, 128] outputs, then [batch, hq, splits]
 // lse values); `workspace_bytes` is what the caller's buffer holds.
 //
-// kTrack: the workspace holds partials whatever the splits, then the scores
-// (track_scores_at), and `track` is launched behind the decode.
-template <typename Cache, bool kTrack = false, typename Track = std::nullptr_t>
+// Where the cache is tracked, the workspace holds partials whatever the splits,
+// then the scores (track_scores_at), and `track` is launched behind the decode.
+template <typename Cache, typename Track = std::nullptr_t>
 static int decode_checked(const void* query, const void* k_cache, const void* v_cache,
                           const void* k_scale_cache, const float* v_scale_cache,
                           const int32_t* cache_seqlens, const int32_t* block_tables, void* out,
@@ -1317,9 +1298,10 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
        (((uintptr_t)k_scale_cache | (uintptr_t)v_scale_cache) & 3)))
     return MSKV_EINVAL;
   const size_t need =
-      kTrack ? track_scores_at(batch, num_q_heads, num_kv_heads, num_splits) +
-                   track_scores_bytes(batch, num_q_heads, max_blocks_per_seq, block_size)
-             : mskv_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, num_splits);
+      Cache::kTrack ? track_scores_at(batch, num_q_heads, num_kv_heads, num_splits) +
+                          track_scores_bytes(batch, num_q_heads, max_blocks_per_seq, block_size)
+                    : mskv_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim,
+                                                  num_splits);
   if (need > 0 && (!workspace || workspace_bytes < need)) return MSKV_EWORKSPACE;
 
   DecodeArgs a;
@@ -1381,12 +1363,12 @@ static int decode_checked(const void* query, const void* k_cache, const void* v_
   a.scale_log2 = softmax_scale * kLog2e;
   a.scores = nullptr;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if constexpr (kTrack) {
+  if constexpr (Cache::kTrack) {
     a.scores = (float*)((uint8_t*)workspace +
                         track_scores_at(batch, num_q_heads, num_kv_heads, num_splits));
     const hipError_t e = act_dtype == MSKV_BFLOAT16
-                             ? launch_decode<__bf16, Cache, true>(a, batch, false, s)
-                             : launch_decode<_Float16, Cache, true>(a, batch, false, s);
+                             ? launch_decode<__bf16, Cache>(a, batch, false, s)
+                             : launch_decode<_Float16, Cache>(a, batch, false, s);
     return e != hipSuccess ? (int)e : track(a, s);
   }
   const bool joined = std::is_same<Cache, Fp4Cache>::value &&

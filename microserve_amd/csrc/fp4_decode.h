@@ -41,6 +41,7 @@ struct Fp4Cache {
   // tokens 10.0 us (two steps 11.8), 8 x 1000 10.4 (12.1)
   static constexpr int kMinSteps = 1;
   static constexpr int kItemWaves = kNarrowWaves;
+  static constexpr bool kTrack = false;
   // a token whose bytes (64 a token, 31 bits) lie past the end of any page
   static constexpr uint32_t kPastEnd = (1u << 25) - kUnit;
   typedef uint8_t Tiles[2][kUnit * kFp4Row];  // V, double-buffered

@@ -134,7 +134,7 @@ def test_refused_by_the_c_abi():
 
 def test_workspaces_follow_the_shapes():
     lib = _lib.load()
-    scores = 64 * 32 * 16 * 256 * 4
+    scores = 64 * 32 * (16 * 256 + 32) * 4
     splits = lib.mskv_decode_num_splits(64, 32, 8, 16, 256)
     part = (64 * 32 * splits * 129 * 4 + 255) // 256 * 256
     assert lib.mskv_decode_weights_workspace_bytes(64, 32, 8, 256, 16) == part + scores
