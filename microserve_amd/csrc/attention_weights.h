@@ -19,6 +19,7 @@ struct TrackArgs {
   float* weights;
   const int32_t* starts;
   int start;
+  int merge_blocks, turns;
 };
 
 // The log-sum-exp of a row from those of its first n splits (+inf for a row
@@ -38,21 +39,76 @@ __device__ __forceinline__ float merged_lse(const float* lse, int n, int lane) {
 
 constexpr int kTrackThreads = 256;
 constexpr int kTrackTokens = 4 * kTrackThreads;  // of a workgroup's turn
+constexpr int kTrackFew = 8;                     // splits that are loaded all at once
 
-// grid (turns of a sequence's tokens, kv heads, sequences).  A page is whole
+// One grid: workgroups that merge the splits of four rows each (merge_blocks of
+// them; the decode's own merges, to the same bits), then the weights' ones, (sequence, kv
+// head, turn of its tokens) with the turns varying fastest.  A page is whole
 // steps of 32 tokens, so a thread's four lie in one page.
-template <bool kRule>
+template <typename T, bool kRule>
 __global__ __launch_bounds__(kTrackThreads) void track_weights_kernel(TrackArgs t) {
   const DecodeArgs& a = t.d;
   extern __shared__ float s_lse[];  // of the group's heads
-  const int b = blockIdx.z, kvh = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int own = kRule ? lane_length(a.seqlens, a.rule) : 0;
+  auto valid_splits = [&](int L) {
+    const int split_tokens =
+        kRule ? split_tokens_of<kStep>(own, L, a.seqlens, a.rule) : a.rule.fixed;
+    return L <= 0 ? 0 : min(a.splits, (L + split_tokens - 1) / split_tokens);
+  };
+  if ((int)blockIdx.x < t.merge_blocks) {
+    const int row = blockIdx.x * (kTrackThreads / 64) + wave;
+    if (row >= a.batch * a.hq) return;
+    const float* lse = a.part_lse + (int64_t)row * a.splits;
+    const float* po = a.part_o + (int64_t)row * a.splits * kHeadDim;
+    const int len = min(a.seqlens[row / a.hq], a.w * a.bs);
+    if (a.splits <= kTrackFew) {  // in order, as decode_combine_small_kernel
+      float ls[kTrackFew];
+      float2 pv[kTrackFew];
+#pragma unroll
+      for (int i = 0; i < kTrackFew; ++i) {
+        const int at = min(i, a.splits - 1);
+        ls[i] = lse[at];
+        pv[i] = *reinterpret_cast<const float2*>(po + (int64_t)at * kHeadDim + 2 * lane);
+      }
+      const int nvalid = valid_splits(len);
+      if (nvalid == 1) return;  // written by the split kernel
+      float top = -INFINITY, o0 = 0.0f, o1 = 0.0f, den = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kTrackFew; ++i)
+        if (i < nvalid) top = fmaxf(top, ls[i]);
+#pragma unroll
+      for (int i = 0; i < kTrackFew; ++i) {
+        if (i < nvalid && top != -INFINITY) {
+          const float p = exp2_fast(ls[i] - top);
+          o0 += p * pv[i].x;
+          o1 += p * pv[i].y;
+          den += p;
+        }
+      }
+      const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+      *reinterpret_cast<uint32_t*>(a.out + (int64_t)row * kHeadDim + 2 * lane) =
+          (uint32_t)Act<T>::from_f32(o0 * inv) | ((uint32_t)Act<T>::from_f32(o1 * inv) << 16);
+      return;
+    }
+    const int nvalid = valid_splits(len);
+    if (nvalid == 1) return;  // written by the split kernel
+    const int j = lane >> 5, i = lane & 31;
+    po += 4 * i;
+    float m = -INFINITY, den = 0.0f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int base = 0; base < nvalid; base += 2 * kLoopK)
+      merge_splits<kLoopK>(m, den, o, lse, po, base + j, 2, nvalid);
+    merge_across<true>(m, den, o);
+    if (j == 0) write_merged<T>(a.out + (int64_t)row * kHeadDim + 4 * i, den, o);
+    return;
+  }
+  const int at0 = blockIdx.x - t.merge_blocks;
+  const int turn = at0 % t.turns, pair = at0 / t.turns;
+  const int b = pair / a.hk, kvh = pair - b * a.hk;
   const int L = min(a.seqlens[b], a.w * a.bs);
-  if ((int)blockIdx.x * kTrackTokens >= L) return;
-  const int split_tokens =
-      kRule ? split_tokens_of<kStep>(own, L, a.seqlens, a.rule) : a.rule.fixed;
-  const int nvalid = min(a.splits, (L + split_tokens - 1) / split_tokens);
+  if (turn * kTrackTokens >= L) return;
+  const int nvalid = valid_splits(L);
   const int64_t row0 = (int64_t)b * a.hq + kvh * a.group;
   for (int h = wave; h < a.group; h += kTrackThreads / 64) {
     const float lse = merged_lse(a.part_lse + (row0 + h) * a.splits, nvalid, lane);
@@ -61,7 +117,7 @@ __global__ __launch_bounds__(kTrackThreads) void track_weights_kernel(TrackArgs 
   __syncthreads();
   const int64_t cap = score_stride(a.w, a.bs);
   const int first = max(t.starts ? t.starts[b] : t.start, 0);
-  for (int at = blockIdx.x * kTrackTokens; at < L; at += gridDim.x * kTrackTokens) {
+  for (int at = turn * kTrackTokens; at < L; at += t.turns * kTrackTokens) {
     const int tok = at + 4 * threadIdx.x;
     if (tok >= L || tok + 4 <= first) continue;
     const int page = tok / a.bs;
@@ -642,7 +698,8 @@ extern "C" int mskv_fp8_decode_attention_weights(
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || block_size <= 0 ||
       max_blocks_per_seq <= 0 || start < 0 || num_q_heads % num_kv_heads != 0)
     return MSKV_EINVAL;
-  if (batch > 65535 || num_kv_heads > 65535 || num_q_heads / num_kv_heads > 8192)
+  if (batch > 65535 || num_q_heads / num_kv_heads > 8192 ||
+      (int64_t)batch * num_q_heads > 0x3FFFFFFF / kTrackThreads)
     return MSKV_EUNSUPPORTED;
   if (batch > 0 && (!weights || misaligned({weights}))) return MSKV_EINVAL;
   if (batch > 0 && (!workspace || workspace_bytes < mskv_decode_weights_workspace_bytes(
@@ -664,18 +721,27 @@ extern "C" int mskv_fp8_decode_attention_weights(
                           softmax_scale, act_dtype, workspace, workspace_bytes, stream);
   }
   auto track = [&](const DecodeArgs& d, hipStream_t s) -> int {
-    const TrackArgs t = {d, weights, starts, start};
-    const int64_t turns = ((int64_t)d.w * d.bs + kTrackTokens - 1) / kTrackTokens;
     // (a table's width says little of the lengths: workgroups walk the turns
     // past a grid of 4096)
+    const int64_t turns = ((int64_t)d.w * d.bs + kTrackTokens - 1) / kTrackTokens;
     const int64_t most = std::max<int64_t>(1, 4096 / ((int64_t)d.batch * d.hk));
-    const dim3 grid((unsigned)std::min(turns, most), (unsigned)d.hk, (unsigned)d.batch);
+    const bool merge = d.splits > 1 && d.splits <= kWideThreshold;
+    const int per = kTrackThreads / 64;
+    const TrackArgs t = {d, weights, starts, start,
+                         merge ? (int)(((int64_t)d.batch * d.hq + per - 1) / per) : 0,
+                         (int)std::min(turns, most)};
+    const dim3 grid((unsigned)(t.merge_blocks + (int64_t)t.turns * d.batch * d.hk));
     const unsigned lds = (unsigned)(d.group * sizeof(float));
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(kTrackThreads), lds, s, t);
+      return (int)hipGetLastError();
+    };
+    const bool bf16 = act_dtype == MSKV_BFLOAT16;
     if (d.rule.adapt || d.rule.info)
-      hipLaunchKernelGGL(track_weights_kernel<true>, grid, dim3(kTrackThreads), lds, s, t);
-    else
-      hipLaunchKernelGGL(track_weights_kernel<false>, grid, dim3(kTrackThreads), lds, s, t);
-    return (int)hipGetLastError();
+      return bf16 ? run(track_weights_kernel<__bf16, true>)
+                  : run(track_weights_kernel<_Float16, true>);
+    return bf16 ? run(track_weights_kernel<__bf16, false>)
+                : run(track_weights_kernel<_Float16, false>);
   };
   return decode_checked<TrackedFp8Cache>(
       query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens, block_tables, out,

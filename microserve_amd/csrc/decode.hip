@@ -1118,6 +1118,8 @@ static hipError_t launch_decode(const DecodeArgs& a, int batch, bool joined, hip
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
+  // (track_weights_kernel merges these itself)
+  if (Cache::kTrack && a.splits <= kWideThreshold) return e;
   const bool rule = a.rule.adapt || a.rule.info;
   auto merge = [&](auto kernel, dim3 grid, unsigned threads) {
     hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, a.part_o, a.part_lse, a.seqlens,

@@ -25,6 +25,20 @@
 
 namespace mskv {
 
+// Division of 0 <= x < 2^31 by a constant of the launch.
+struct Divider {
+  uint32_t magic;
+  int d, shift;
+  __device__ __forceinline__ int operator()(int x) const {
+    return (int)((__umulhi(magic, (uint32_t)x) + (uint32_t)x) >> shift);
+  }
+};
+static Divider divider_of(int d) {
+  int shift = 0;
+  while ((1LL << shift) < d) ++shift;
+  return {(uint32_t)(((1ULL << 32) * ((1ULL << shift) - d)) / d + 1), d, shift};
+}
+
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
 constexpr int kSelectBins = 2048;
@@ -35,6 +49,7 @@ struct SelectArgs {
   int32_t *kept, *new_lens;
   int64_t num_blocks;
   int hk, bs, w, start, recent, budget;
+  Divider by_block;
 };
 
 // An integer that orders as the weight does: NaN lowest, -0 as 0.
@@ -103,18 +118,22 @@ __global__ __launch_bounds__(kSelectThreads) void select_kv_tokens_kernel(Select
   const int count = L - last - first;  // tokens that compete: more than quota
 
   const int32_t* table = a.bt + (int64_t)b * a.w;
-  auto read = [&](int i) -> uint32_t {  // the key of the range's token i
-    const int t = first + i, page = t / a.bs;
+  // The key of the range's token i.  Without branches, so that the reads of all
+  // of a thread's keys are in flight at once: a token past the end stands for the
+  // last one, an invalid block for the first.
+  auto read = [&](int i) -> uint32_t {
+    const int t = first + min(i, count - 1), page = a.by_block(t);
     const int blk = table[page];
-    if (blk < 0 || (int64_t)blk >= a.num_blocks) return 0u;
-    return weight_key(a.weights[((int64_t)blk * a.hk + h) * a.bs + (t - page * a.bs)]);
+    const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
+    const float x = a.weights[((int64_t)(ok ? blk : 0) * a.hk + h) * a.bs + (t - page * a.bs)];
+    return ok ? weight_key(x) : 0u;
   };
   uint32_t own[kItems > 0 ? kItems : 1];
   if constexpr (kItems > 0) {
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
       const int i = j * kSelectThreads + tid;
-      own[j] = i < count ? read(i) : 0u;
+      own[j] = read(i);
     }
   }
   auto each = [&](auto&& f) {  // f(token of the range, key)
@@ -211,97 +230,168 @@ __global__ __launch_bounds__(kSelectThreads) void select_kv_tokens_kernel(Select
 #pragma unroll
       for (int j = 0; j < kTurn; ++j) {
         const int i = at + j * kSelectThreads + tid;
-        key[j] = i < count ? read(i) : 0u;
+        key[j] = read(i);
       }
       turn(at, key);
     }
   }
 }
 
-constexpr int kEvictThreads = 1024;
-constexpr int kEvictLoads = 4;  // 16-byte pieces a lane and run
+constexpr int kEvictThreads = 512;
+constexpr int kEvictLoads = 4;  // 16-byte pieces of a lane and run
 
 struct EvictArgs {
   uint8_t *kc, *vc;
   float *ks, *vs, *weights;
   const int32_t *kept, *lens, *bt;
   int64_t num_blocks;
-  int hk, bs, w, budget;
+  int hk, bs, w, budget, scale_heads, scale_units;
+  Divider by_block, by_heads;
 };
 
 // A token's slot (its row among all pages' rows), -1 if it has none.
+// (No branches: a lane's table entries are read all at once.)
 __device__ __forceinline__ int64_t slot_of(const EvictArgs& a, const int32_t* table, int t) {
-  if (t < 0 || t >= a.w * a.bs) return -1;
-  const int page = t / a.bs;
+  const int in = min(max(t, 0), a.w * a.bs - 1);
+  const int page = a.by_block(in);
   const int blk = table[page];
-  return blk < 0 || (int64_t)blk >= a.num_blocks ? -1 : (int64_t)blk * a.bs + (t - page * a.bs);
+  return t != in || blk < 0 || (int64_t)blk >= a.num_blocks
+             ? -1
+             : (int64_t)blk * a.bs + (in - page * a.bs);
 }
 
-// grid (kv head, part, sequence); parts: columns of K's rows, columns of V's
-// rows (kParts pieces of a row each), the scales and weights.
+// A run of places: this lane's pieces of rows, and where they go (-1: nowhere).
+struct EvictRun {
+  u32x4 v[kEvictLoads];
+  int64_t dst[kEvictLoads];
+};
+
+// What a workgroup of a sequence moves: its scales (two tensors, so many heads
+// of a token at a time), its weights, or columns of its rows (kParts pieces of a
+// row each).
+//
+// The rows of the next run are asked for before those of this one are stored,
+// and what they are is known a run earlier still.  Between two runs there is
+// one barrier, behind the arrival of the first one's rows: nobody stores to a
+// run's places before all have read it.
+//
+// A token's scales of all heads are one piece of memory (32 bytes at eight
+// heads): moved head by head, by workgroups on other XCDs, each line is written
+// in parts that memory has to read first (64 x 4096 rows of eight heads: 273 us
+// for the whole call).
 template <int kParts>
 __global__ __launch_bounds__(kEvictThreads) void evict_kv_tokens_kernel(EvictArgs a) {
   const int tid = threadIdx.x;
-  const int h = blockIdx.x, part = blockIdx.y, b = blockIdx.z;
+  const int b = blockIdx.y;
   const int32_t* table = a.bt + (int64_t)b * a.w;
-  const int32_t* kept = a.kept + ((int64_t)b * a.hk + h) * a.budget;
-  const int n = min(a.lens[b], a.budget);
-  if (part < 2 * kParts) {
-    constexpr int kLanes = kHeadDim / 16 / kParts;  // of a piece of a row
-    constexpr int kRows = kEvictThreads / kLanes;
-    uint8_t* rows = (part < kParts ? a.kc : a.vc) + h * kHeadDim +
-                    (part % kParts) * (kHeadDim / kParts) + 16 * (tid % kLanes);
-    const int64_t stride = (int64_t)a.hk * kHeadDim;
-    for (int at = 0; at < n; at += kRows * kEvictLoads) {
-      u32x4 v[kEvictLoads];
-      int64_t dst[kEvictLoads];
+  const int32_t* kept = a.kept + (int64_t)b * a.hk * a.budget;
+  const int n = min(__builtin_amdgcn_readfirstlane(a.lens[b]), a.budget);
+  if (n <= 0) return;
+  int unit = blockIdx.x;
+
+  // Runs of single floats: `of(e)` is element e's (position it comes from,
+  // place, offset of a slot); `count` elements, whose places ascend.
+  auto floats = [&](float* x, int count, auto&& of) {
+    constexpr int kFloats = 4;
+    for (int at = 0; at < count; at += kEvictThreads * kFloats) {
+      float v[kFloats];
+      int64_t dst[kFloats];
 #pragma unroll
-      for (int k = 0; k < kEvictLoads; ++k) {
-        const int i = at + k * kRows + tid / kLanes;
-        const int from = i < n ? kept[i] : i;
-        dst[k] = -1;
-        if (from != i) {
-          const int64_t src = slot_of(a, table, from);
-          if (src >= 0) {
-            dst[k] = slot_of(a, table, i);
-            v[k] = *reinterpret_cast<const u32x4*>(rows + src * stride);
-          }
-        }
+      for (int k = 0; k < kFloats; ++k) {
+        const int e = at + k * kEvictThreads + tid;
+        int64_t src, to;
+        of(min(e, count - 1), src, to);
+        dst[k] = e < count && src != to && src >= 0 ? to : -1;
+        v[k] = x[max(src, (int64_t)0)];
       }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();  // every row of this run is read
 #pragma unroll
-      for (int k = 0; k < kEvictLoads; ++k)
-        if (dst[k] >= 0) *reinterpret_cast<u32x4*>(rows + dst[k] * stride) = v[k];
+      for (int k = 0; k < kFloats; ++k) asm volatile("" ::"v"(v[k]));  // they are here
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int k = 0; k < kFloats; ++k)
+        if (dst[k] >= 0) x[dst[k]] = v[k];
     }
+  };
+  if (unit < 2 * a.scale_units) {  // `scale_heads` heads of K's or V's scales
+    const int h0 = unit % a.scale_units * a.scale_heads;
+    floats(unit < a.scale_units ? a.ks : a.vs, n * a.scale_heads,
+           [&](int e, int64_t& src, int64_t& to) {
+             const int i = a.by_heads(e), h = h0 + e - i * a.scale_heads;
+             const int64_t s = slot_of(a, table, kept[(int64_t)h * a.budget + i]);
+             const int64_t d = slot_of(a, table, i);
+             src = s < 0 ? -1 : s * a.hk + h;
+             to = d < 0 ? -1 : d * a.hk + h;
+           });
     return;
   }
-  for (int at = 0; at < n; at += kEvictThreads) {
-    const int i = at + tid;
-    const int from = i < n ? kept[i] : i;
-    int64_t src = -1, dst = -1;
-    if (from != i) {
-      src = slot_of(a, table, from);
-      dst = src < 0 ? -1 : slot_of(a, table, i);
+  unit -= 2 * a.scale_units;
+  if (a.weights) {
+    if (unit < a.hk) {
+      floats(a.weights, n, [&](int e, int64_t& src, int64_t& to) {
+        // a head's weights of a page are one piece
+        auto place = [&](int64_t slot) {
+          const int64_t page = slot / a.bs;
+          return slot < 0 ? -1 : (page * a.hk + unit) * a.bs + (slot - page * a.bs);
+        };
+        src = place(slot_of(a, table, kept[(int64_t)unit * a.budget + e]));
+        to = place(slot_of(a, table, e));
+      });
+      return;
     }
-    // a weight lies in its page's stretch of the head
-    auto place = [&](int64_t slot) {
-      const int64_t page = slot / a.bs;
-      return (page * a.hk + h) * a.bs + (slot - page * a.bs);
-    };
-    float k = 0.0f, v = 0.0f, x = 0.0f;
-    if (dst >= 0) {
-      k = a.ks[src * a.hk + h];
-      v = a.vs[src * a.hk + h];
-      if (a.weights) x = a.weights[place(src)];
+    unit -= a.hk;
+  }
+  constexpr int kLanes = kHeadDim / 16 / kParts;  // of a piece of a row
+  constexpr int kRows = kEvictThreads / kLanes;
+  constexpr int kRun = kRows * kEvictLoads;
+  const int h = unit % a.hk, part = unit / a.hk;
+  kept += (int64_t)h * a.budget;
+  uint8_t* rows = (part < kParts ? a.kc : a.vc) + h * kHeadDim +
+                  (part % kParts) * (kHeadDim / kParts) + 16 * (tid % kLanes);
+  const int64_t stride = (int64_t)a.hk * kHeadDim;
+  const int own = tid / kLanes;
+  int from[kEvictLoads];  // of the run after the next one to be asked for
+  auto look = [&](int at) {
+#pragma unroll
+    for (int k = 0; k < kEvictLoads; ++k) from[k] = kept[min(at + k * kRows + own, n - 1)];
+  };
+  // asks for the rows of the run at `at`, whose positions `from` holds; a row
+  // that has no page reads its cache's first one
+  auto ask = [&](int at, EvictRun& r) {
+    int64_t src[kEvictLoads];
+#pragma unroll
+    for (int k = 0; k < kEvictLoads; ++k) {
+      const int i = min(at + k * kRows + own, n - 1);
+      src[k] = slot_of(a, table, from[k]);
+      r.dst[k] = slot_of(a, table, i);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (dst >= 0) {
-      a.ks[dst * a.hk + h] = k;
-      a.vs[dst * a.hk + h] = v;
-      if (a.weights) a.weights[place(dst)] = x;
+#pragma unroll
+    for (int k = 0; k < kEvictLoads; ++k) {
+      if (at + k * kRows + own >= n || src[k] == r.dst[k] || src[k] < 0) r.dst[k] = -1;
+      r.v[k] = *reinterpret_cast<const u32x4*>(rows + max(src[k], (int64_t)0) * stride);
     }
+  };
+  auto store = [&](const EvictRun& r) {
+#pragma unroll
+    for (int k = 0; k < kEvictLoads; ++k) asm volatile("" ::"v"(r.v[k]));  // they are here
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < kEvictLoads; ++k)
+      if (r.dst[k] >= 0) *reinterpret_cast<u32x4*>(rows + r.dst[k] * stride) = r.v[k];
+  };
+  EvictRun even, odd;
+  look(0);
+  ask(0, even);
+  look(kRun);
+  for (int at = 0; at < n; at += 2 * kRun) {
+    ask(at + kRun, odd);
+    look(at + 2 * kRun);
+    store(even);
+    if (at + kRun >= n) break;
+    ask(at + 2 * kRun, even);
+    look(at + 3 * kRun);
+    store(odd);
   }
 }
 
@@ -329,10 +419,11 @@ extern "C" int mskv_select_kv_tokens(const float* weights, const int32_t* cache_
   if (status != MSKV_OK) return status;
   if (start < 0 || recent < 0) return MSKV_EINVAL;
   if (batch == 0) return MSKV_OK;
+  if (num_blocks == 0) return MSKV_EINVAL;  // (there are no weights to read)
   if (!weights || !cache_seqlens || !block_tables || !kept || !new_seqlens) return MSKV_EINVAL;
   const SelectArgs a = {weights, cache_seqlens, block_tables,       starts, kept,   new_seqlens,
                         num_blocks, num_kv_heads, block_size, max_blocks_per_seq, start, recent,
-                        budget};
+                        budget, divider_of(block_size)};
   const dim3 grid((unsigned)(batch * num_kv_heads));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   // (by the most tokens that can compete)
@@ -359,17 +450,31 @@ extern "C" int mskv_evict_kv_tokens(void* k_cache, void* v_cache, float* k_scale
                                  budget);
   if (status != MSKV_OK) return status;
   if (head_dim != kHeadDim) return MSKV_EUNSUPPORTED;
-  if (batch == 0) return MSKV_OK;
+  // (a run of one plus a sequence's rows of all heads)
+  if ((int64_t)max_blocks_per_seq * block_size * num_kv_heads > 0x7FFFFFFFLL - (1 << 14))
+    return MSKV_EUNSUPPORTED;
+  if (batch == 0 || num_blocks == 0) return MSKV_OK;
   if (!k_cache || !v_cache || !k_scale_cache || !v_scale_cache || !kept || !new_seqlens ||
       !block_tables || misaligned({k_cache, v_cache}))
     return MSKV_EINVAL;
+  // the heads of a token whose scales one workgroup moves: all of them where the
+  // sequences alone are workgroups enough
+  int scale_heads = (int)std::min<int64_t>(num_kv_heads, (int64_t)batch * num_kv_heads / 32);
+  scale_heads = std::max(1, scale_heads);
+  while (num_kv_heads % scale_heads != 0) --scale_heads;
+  const int scale_units = num_kv_heads / scale_heads;
   const EvictArgs a = {(uint8_t*)k_cache, (uint8_t*)v_cache, k_scale_cache, v_scale_cache, weights,
                        kept, new_seqlens, block_tables, num_blocks, num_kv_heads, block_size,
-                       max_blocks_per_seq, budget};
+                       max_blocks_per_seq, budget, scale_heads, scale_units,
+                       divider_of(block_size), divider_of(scale_heads)};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  constexpr int kParts = 1;
-  hipLaunchKernelGGL(evict_kv_tokens_kernel<kParts>,
-                     dim3((unsigned)num_kv_heads, 2 * kParts + 1, (unsigned)batch),
-                     dim3(kEvictThreads), 0, s, a);
-  return (int)hipGetLastError();
+  auto run = [&](auto kernel, int parts) {
+    const int units = 2 * scale_units + (weights ? num_kv_heads : 0) + 2 * parts * num_kv_heads;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)units, (unsigned)batch), dim3(kEvictThreads), 0, s,
+                       a);
+    return (int)hipGetLastError();
+  };
+  // halves of rows where whole ones are too few workgroups for the chip
+  if ((int64_t)batch * num_kv_heads * 2 >= 512) return run(evict_kv_tokens_kernel<1>, 1);
+  return run(evict_kv_tokens_kernel<2>, 2);
 }
