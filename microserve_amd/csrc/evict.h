@@ -7,7 +7,7 @@
 //    bits of an order-preserving integer form of the weight), each by a
 //    histogram in LDS; one more pass writes the kept positions in ascending
 //    order, of the tokens at the threshold the earliest.  One workgroup a
-//    (sequence, kv head), which holds up to 32 keys a thread in registers.
+//    (sequence, kv head), which holds the keys in registers, up to 32 a thread.
 //  * evict_kv_tokens_kernel: place i of a (sequence, kv head) gets the row of
 //    position kept[i].  The positions ascend, so kept[i] >= i, and a workgroup
 //    that walks the places in order may overwrite what it has read: a run of
@@ -39,8 +39,6 @@ static Divider divider_of(int d) {
   return {(uint32_t)(((1ULL << 32) * ((1ULL << shift) - d)) / d + 1), d, shift};
 }
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWaves = kSelectThreads / 64;
 constexpr int kSelectBins = 2048;
 
 struct SelectArgs {
@@ -66,8 +64,11 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
 }
 
 // The sum of v over the threads before this one, and over all.
+template <int kWaves>
 __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_wave, uint32_t& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (masks kept from scan to scan would spill)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t x = v;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -79,7 +80,7 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_wave, ui
   uint32_t before = x - v;
   all = 0;
 #pragma unroll
-  for (int i = 0; i < kSelectWaves; ++i) {
+  for (int i = 0; i < kWaves; ++i) {
     const uint32_t t = s_wave[i];
     if (i < wave) before += t;
     all += t;
@@ -88,16 +89,19 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_wave, ui
   return before;
 }
 
-// kItems: keys that a thread holds (0: the weights are read again on every
-// pass; thread t's j-th key is that of token j * 1024 + t of the range).
-template <int kItems>
-__global__ __launch_bounds__(kSelectThreads) void select_kv_tokens_kernel(SelectArgs a) {
+// kItems: keys that a thread holds, thread t's j-th key that of token
+// j * kThreads + t of the range; kReread: as many at a time, read again on every
+// pass.
+template <int kThreads, int kItems, bool kReread>
+__global__ __launch_bounds__(kThreads) void select_kv_tokens_kernel(SelectArgs a) {
+  constexpr int kWaves = kThreads / 64;
+  constexpr int kEntries = kItems * kWaves;  // waves' counts of a turn
+  constexpr int kEach = (kEntries + kThreads - 1) / kThreads;
+  constexpr int kBinsEach = kSelectBins / kThreads;
   __shared__ uint32_t s_hist[kSelectBins];
-  __shared__ uint32_t s_wave[kSelectWaves];
+  __shared__ uint32_t s_wave[kWaves];
   __shared__ uint32_t s_found[2];
-  constexpr int kTurn = kItems > 0 && kItems < 8 ? kItems : 8;  // keys of the last pass's turn
-  constexpr int kEntries = kTurn * kSelectWaves;
-  __shared__ uint32_t s_count[kEntries];
+  __shared__ uint32_t s_count[kEach * kThreads];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / a.hk, h = blockIdx.x - b * a.hk;
   const int L = max(0, min(__builtin_amdgcn_readfirstlane(a.seqlens[b]), a.w * a.bs));
@@ -109,10 +113,10 @@ __global__ __launch_bounds__(kSelectThreads) void select_kv_tokens_kernel(Select
   const int last = min(a.recent, n - first);
   // what stays whatever it weighs
   const int fixed_front = n == L ? n : first;
-  for (int i = tid; i < fixed_front; i += kSelectThreads) kept[i] = i;
-  for (int i = n + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+  for (int i = tid; i < fixed_front; i += kThreads) kept[i] = i;
+  for (int i = n + tid; i < a.budget; i += kThreads) kept[i] = -1;
   if (n == L) return;
-  for (int i = tid; i < last; i += kSelectThreads) kept[n - last + i] = L - last + i;
+  for (int i = tid; i < last; i += kThreads) kept[n - last + i] = L - last + i;
   const int quota = n - first - last;
   if (quota == 0) return;
   const int count = L - last - first;  // tokens that compete: more than quota
@@ -128,27 +132,18 @@ __global__ __launch_bounds__(kSelectThreads) void select_kv_tokens_kernel(Select
     const float x = a.weights[((int64_t)(ok ? blk : 0) * a.hk + h) * a.bs + (t - page * a.bs)];
     return ok ? weight_key(x) : 0u;
   };
-  uint32_t own[kItems > 0 ? kItems : 1];
-  if constexpr (kItems > 0) {
+  constexpr int kTurn = kItems * kThreads;
+  uint32_t own[kItems];
+  auto fill = [&](int at) {
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      const int i = j * kSelectThreads + tid;
-      own[j] = read(i);
-    }
-  }
-  auto each = [&](auto&& f) {  // f(token of the range, key)
-    if constexpr (kItems > 0) {
-      // (the compiler would keep a mask a key from pass to pass, and spill them)
-      int n_own = count;
-      asm volatile("" : "+s"(n_own));
+    for (int j = 0; j < kItems; ++j) own[j] = read(at + j * kThreads + tid);
+  };
+  if (!kReread) fill(0);
+  // keys that live past a barrier, seen anew: the compiler would keep masks of
+  // what it knows of each key from pass to pass, and spill them
+  auto anew = [&] {
 #pragma unroll
-      for (int j = 0; j < kItems; ++j) {
-        const int i = j * kSelectThreads + tid;
-        if (i < n_own) f(i, own[j]);
-      }
-    } else {
-      for (int i = tid; i < count; i += kSelectThreads) f(i, read(i));
-    }
+    for (int j = 0; j < kItems; ++j) asm volatile("" : "+v"(own[j]));
   };
 
   // The threshold: the quota-th largest key, digit by digit; `need` of the
@@ -158,86 +153,95 @@ __global__ __launch_bounds__(kSelectThreads) void select_kv_tokens_kernel(Select
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t mask = pass == 2 ? 1023u : 2047u;
-    for (int i = tid; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
+#pragma unroll
+    for (int i = 0; i < kBinsEach; ++i) s_hist[i * kThreads + tid] = 0;
     __syncthreads();
-    each([&](int, uint32_t key) {
-      // (the digits above: all 32 bits on the first pass have none)
-      if (pass == 0 || (key >> (pass == 1 ? 21 : 10)) == digits)
-        atomicAdd(&s_hist[(key >> shift) & mask], 1u);
-    });
+    for (int at = 0; at < count; at += kTurn) {
+      if (kReread) fill(at);
+      int left = count - at;
+      asm volatile("" : "+s"(left));
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        // (the digits above: all 32 bits on the first pass have none)
+        if (j * kThreads + tid < left &&
+            (pass == 0 || (own[j] >> (pass == 1 ? 21 : 10)) == digits))
+          atomicAdd(&s_hist[(own[j] >> shift) & mask], 1u);
+      }
+    }
     __syncthreads();
-    // this thread's two bins, from the highest down
-    const uint32_t hi = s_hist[kSelectBins - 1 - 2 * tid], lo = s_hist[kSelectBins - 2 - 2 * tid];
-    uint32_t all;
-    const uint32_t before = scan_before(hi + lo, s_wave, all);
-    if (before < need && before + hi + lo >= need) {
-      const bool upper = before + hi >= need;
-      s_found[0] = kSelectBins - 1 - 2 * tid - (upper ? 0 : 1);
-      s_found[1] = need - before - (upper ? 0 : hi);
+    // this thread's bins, from the highest down
+    uint32_t bins[kBinsEach], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < kBinsEach; ++i) {
+      bins[i] = s_hist[kSelectBins - 1 - (kBinsEach * tid + i)];
+      sum += bins[i];
+    }
+    uint32_t before = scan_before<kWaves>(sum, s_wave, all);
+    if (before < need && before + sum >= need) {
+#pragma unroll
+      for (int i = 0; i < kBinsEach; ++i) {
+        if (before < need && before + bins[i] >= need) {
+          s_found[0] = kSelectBins - 1 - (kBinsEach * tid + i);
+          s_found[1] = need - before;
+        }
+        before += bins[i];
+      }
     }
     __syncthreads();
     digits = pass == 0 ? s_found[0] : digits << (pass == 1 ? 11 : 10) | s_found[0];
     need = s_found[1];
-    __syncthreads();
+    if (!kReread) anew();
   }
   const uint32_t threshold = digits;
 
   // The kept positions in order: those above the threshold, and the first
   // `need` at it.  A wave's counts of 64 tokens of either, then their running
-  // sums over the workgroup (two counts in a word: at most 2^13 tokens a turn).
+  // sums over the workgroup (two counts in a word: at most 2^15 tokens a turn).
+  static_assert(kTurn <= 1 << 15, "two counts fit a word");
   uint32_t above0 = 0, equal0 = 0;  // before this turn
   int32_t* to = kept + first;
-  auto turn = [&](int at, const uint32_t (&key)[kTurn]) {
+  for (int at = 0; at < count; at += kTurn) {
+    if (kReread) fill(at);
 #pragma unroll
-    for (int j = 0; j < kTurn; ++j) {
-      const bool live = at + j * kSelectThreads + tid < count;
-      const uint64_t above = __ballot(live && key[j] > threshold);
-      const uint64_t equal = __ballot(live && key[j] == threshold);
-      if (lane == 0) s_count[j * kSelectWaves + wave] = __popcll(above) | __popcll(equal) << 16;
+    for (int j = 0; j < kItems; ++j) {
+      const bool live = at + j * kThreads + tid < count;
+      const uint64_t above = __ballot(live && own[j] > threshold);
+      const uint64_t equal = __ballot(live && own[j] == threshold);
+      if (lane == 0) s_count[j * kWaves + wave] = __popcll(above) | __popcll(equal) << 16;
+      __builtin_amdgcn_sched_barrier(0);  // (masks of many keys at once would spill)
+    }
+    anew();
+    __syncthreads();
+    uint32_t c[kEach], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      c[i] = kEach * tid + i < kEntries ? s_count[kEach * tid + i] : 0u;
+      sum += c[i];
+    }
+    uint32_t before = scan_before<kWaves>(sum, s_wave, all);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      s_count[kEach * tid + i] = before;
+      before += c[i];
     }
     __syncthreads();
-    uint32_t all;
-    const uint32_t c = tid < kEntries ? s_count[tid] : 0u;
-    const uint32_t before = scan_before(c, s_wave, all);
-    if (tid < kEntries) s_count[tid] = before;
-    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kTurn; ++j) {
-      const int i = at + j * kSelectThreads + tid;
-      const bool is_above = i < count && key[j] > threshold;
-      const bool is_equal = i < count && key[j] == threshold;
-      const uint32_t base = s_count[j * kSelectWaves + wave];
+    for (int j = 0; j < kItems; ++j) {
+      const int i = at + j * kThreads + tid;
+      const bool is_above = i < count && own[j] > threshold;
+      const bool is_equal = i < count && own[j] == threshold;
+      const uint32_t base = s_count[j * kWaves + wave];
       const uint32_t above = above0 + (base & 0xFFFFu) + lanes_below(__ballot(is_above));
       const uint32_t equal = equal0 + (base >> 16) + lanes_below(__ballot(is_equal));
       if (is_above || (is_equal && equal < need)) to[above + min(equal, need)] = first + i;
+      __builtin_amdgcn_sched_barrier(0);
     }
     above0 += all & 0xFFFFu;
     equal0 += all >> 16;
-    __syncthreads();
-  };
-  if constexpr (kItems > 0) {
-#pragma unroll
-    for (int t = 0; t < kItems / kTurn; ++t) {
-      if (t * kTurn * kSelectThreads >= count) break;
-      uint32_t key[kTurn];
-#pragma unroll
-      for (int j = 0; j < kTurn; ++j) key[j] = own[t * kTurn + j];
-      turn(t * kTurn * kSelectThreads, key);
-    }
-  } else {
-    for (int at = 0; at < count; at += kTurn * kSelectThreads) {
-      uint32_t key[kTurn];
-#pragma unroll
-      for (int j = 0; j < kTurn; ++j) {
-        const int i = at + j * kSelectThreads + tid;
-        key[j] = read(i);
-      }
-      turn(at, key);
-    }
+    if (kReread) __syncthreads();  // (the counts are read before the next turn's)
   }
 }
 
-constexpr int kEvictThreads = 512;
 constexpr int kEvictLoads = 4;  // 16-byte pieces of a lane and run
 
 struct EvictArgs {
@@ -245,8 +249,8 @@ struct EvictArgs {
   float *ks, *vs, *weights;
   const int32_t *kept, *lens, *bt;
   int64_t num_blocks;
-  int hk, bs, w, budget, scale_heads, scale_units;
-  Divider by_block, by_heads;
+  int hk, bs, w, budget, scale_heads, scale_units, row_heads, row_units;
+  Divider by_block, by_heads, by_row_heads;
 };
 
 // A token's slot (its row among all pages' rows), -1 if it has none.
@@ -266,9 +270,8 @@ struct EvictRun {
   int64_t dst[kEvictLoads];
 };
 
-// What a workgroup of a sequence moves: its scales (two tensors, so many heads
-// of a token at a time), its weights, or columns of its rows (kParts pieces of a
-// row each).
+// What a workgroup of a sequence moves: rows of K or of V, scales of either (both
+// of so many heads of a token at a time), or a head's weights.
 //
 // The rows of the next run are asked for before those of this one are stored,
 // and what they are is known a run earlier still.  Between two runs there is
@@ -279,8 +282,8 @@ struct EvictRun {
 // heads): moved head by head, by workgroups on other XCDs, each line is written
 // in parts that memory has to read first (64 x 4096 rows of eight heads: 273 us
 // for the whole call).
-template <int kParts>
-__global__ __launch_bounds__(kEvictThreads) void evict_kv_tokens_kernel(EvictArgs a) {
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void evict_kv_tokens_kernel(EvictArgs a) {
   const int tid = threadIdx.x;
   const int b = blockIdx.y;
   const int32_t* table = a.bt + (int64_t)b * a.w;
@@ -292,13 +295,13 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kv_tokens_kernel(EvictArg
   // Runs of single floats: `of(e)` is element e's (position it comes from,
   // place, offset of a slot); `count` elements, whose places ascend.
   auto floats = [&](float* x, int count, auto&& of) {
-    constexpr int kFloats = 4;
-    for (int at = 0; at < count; at += kEvictThreads * kFloats) {
+    constexpr int kFloats = 8;
+    for (int at = 0; at < count; at += kThreads * kFloats) {
       float v[kFloats];
       int64_t dst[kFloats];
 #pragma unroll
       for (int k = 0; k < kFloats; ++k) {
-        const int e = at + k * kEvictThreads + tid;
+        const int e = at + k * kThreads + tid;
         int64_t src, to;
         of(min(e, count - 1), src, to);
         dst[k] = e < count && src != to && src >= 0 ? to : -1;
@@ -341,35 +344,59 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kv_tokens_kernel(EvictArg
     }
     unit -= a.hk;
   }
-  constexpr int kLanes = kHeadDim / 16 / kParts;  // of a piece of a row
-  constexpr int kRows = kEvictThreads / kLanes;
+  constexpr int kLanes = kHeadDim / 16;  // of a row
+  constexpr int kRows = kThreads / kLanes;
   constexpr int kRun = kRows * kEvictLoads;
-  const int h = unit % a.hk, part = unit / a.hk;
-  kept += (int64_t)h * a.budget;
-  uint8_t* rows = (part < kParts ? a.kc : a.vc) + h * kHeadDim +
-                  (part % kParts) * (kHeadDim / kParts) + 16 * (tid % kLanes);
+  // row r is place r / row_heads of head h0 + r % row_heads
+  const int h0 = unit % a.row_units * a.row_heads;
+  const int count = n * a.row_heads;
+  kept += (int64_t)h0 * a.budget;
+  uint8_t* rows = (unit < a.row_units ? a.kc : a.vc) + h0 * kHeadDim + 16 * (tid % kLanes);
   const int64_t stride = (int64_t)a.hk * kHeadDim;
   const int own = tid / kLanes;
-  int from[kEvictLoads];  // of the run after the next one to be asked for
+  // A run's rows are known in three steps, each a run ahead of the next: the
+  // positions (kept), their blocks (the table), the rows.  A wave's loads come
+  // back in order, so whatever a later run needs first is asked for before the
+  // rows of an earlier one: waiting for it is then no wait for those.
+  int from[kEvictLoads];  // positions
+  int from_blk[kEvictLoads], to_blk[kEvictLoads], from_off[kEvictLoads], to_off[kEvictLoads];
   auto look = [&](int at) {
 #pragma unroll
-    for (int k = 0; k < kEvictLoads; ++k) from[k] = kept[min(at + k * kRows + own, n - 1)];
+    for (int k = 0; k < kEvictLoads; ++k) {
+      const int r = min(at + k * kRows + own, count - 1);
+      const int i = a.by_row_heads(r);
+      from[k] = kept[(int64_t)(r - i * a.row_heads) * a.budget + i];
+    }
   };
-  // asks for the rows of the run at `at`, whose positions `from` holds; a row
-  // that has no page reads its cache's first one
-  auto ask = [&](int at, EvictRun& r) {
-    int64_t src[kEvictLoads];
+  auto find = [&](int at) {
 #pragma unroll
     for (int k = 0; k < kEvictLoads; ++k) {
-      const int i = min(at + k * kRows + own, n - 1);
-      src[k] = slot_of(a, table, from[k]);
-      r.dst[k] = slot_of(a, table, i);
+      const int i = a.by_row_heads(min(at + k * kRows + own, count - 1));
+      const int t = min(max(from[k], 0), a.w * a.bs - 1);
+      const int page = a.by_block(t), to_page = a.by_block(i);
+      // (a row that stays, or whose position is none, goes nowhere: block -1)
+      from_off[k] = at + k * kRows + own < count && t == from[k] && t != i ? t - page * a.bs : -1;
+      to_off[k] = i - to_page * a.bs;
+      from_blk[k] = table[page];
+      to_blk[k] = table[to_page];
     }
+  };
+  int64_t src[kEvictLoads];
+  auto place = [&](int at, EvictRun& run) {
 #pragma unroll
     for (int k = 0; k < kEvictLoads; ++k) {
-      if (at + k * kRows + own >= n || src[k] == r.dst[k] || src[k] < 0) r.dst[k] = -1;
-      r.v[k] = *reinterpret_cast<const u32x4*>(rows + max(src[k], (int64_t)0) * stride);
+      const int r = min(at + k * kRows + own, count - 1);
+      const int64_t head = (r - a.by_row_heads(r) * a.row_heads) * kHeadDim;
+      const bool moves = from_off[k] >= 0 && from_blk[k] >= 0 && from_blk[k] < a.num_blocks &&
+                         to_blk[k] >= 0 && to_blk[k] < a.num_blocks;
+      src[k] = (moves ? (int64_t)from_blk[k] * a.bs + from_off[k] : 0) * stride + head;
+      run.dst[k] = moves ? ((int64_t)to_blk[k] * a.bs + to_off[k]) * stride + head : -1;
     }
+  };
+  auto ask = [&](EvictRun& run) {
+#pragma unroll
+    for (int k = 0; k < kEvictLoads; ++k)
+      run.v[k] = *reinterpret_cast<const u32x4*>(rows + src[k]);
   };
   auto store = [&](const EvictRun& r) {
 #pragma unroll
@@ -378,20 +405,34 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kv_tokens_kernel(EvictArg
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int k = 0; k < kEvictLoads; ++k)
-      if (r.dst[k] >= 0) *reinterpret_cast<u32x4*>(rows + r.dst[k] * stride) = r.v[k];
+      if (r.dst[k] >= 0)
+        __builtin_nontemporal_store(r.v[k], reinterpret_cast<u32x4*>(rows + r.dst[k]));
+  };
+  // the run at `at` is on its way in `now`; `next` takes the one after it, whose
+  // blocks are known, as are the positions of the one after that
+  auto turn = [&](int at, EvictRun& now, EvictRun& next) {
+    place(at + kRun, next);
+    find(at + 2 * kRun);
+    look(at + 3 * kRun);
+    __builtin_amdgcn_sched_barrier(0);
+    ask(next);
+    __builtin_amdgcn_sched_barrier(0);
+    store(now);
+    __builtin_amdgcn_sched_barrier(0);
   };
   EvictRun even, odd;
   look(0);
-  ask(0, even);
+  find(0);
   look(kRun);
-  for (int at = 0; at < n; at += 2 * kRun) {
-    ask(at + kRun, odd);
-    look(at + 2 * kRun);
-    store(even);
-    if (at + kRun >= n) break;
-    ask(at + 2 * kRun, even);
-    look(at + 3 * kRun);
-    store(odd);
+  place(0, even);
+  find(kRun);
+  look(2 * kRun);
+  __builtin_amdgcn_sched_barrier(0);
+  ask(even);
+  for (int at = 0; at < count; at += 2 * kRun) {
+    turn(at, even, odd);
+    if (at + kRun >= count) break;
+    turn(at + kRun, odd, even);
   }
 }
 
@@ -428,15 +469,14 @@ extern "C" int mskv_select_kv_tokens(const float* weights, const int32_t* cache_
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   // (by the most tokens that can compete)
   const int64_t tokens = (int64_t)max_blocks_per_seq * block_size;
-  if (tokens <= 2 * kSelectThreads)
-    hipLaunchKernelGGL(select_kv_tokens_kernel<2>, grid, dim3(kSelectThreads), 0, s, a);
-  else if (tokens <= 8 * kSelectThreads)
-    hipLaunchKernelGGL(select_kv_tokens_kernel<8>, grid, dim3(kSelectThreads), 0, s, a);
-  else if (tokens <= 32 * kSelectThreads)
-    hipLaunchKernelGGL(select_kv_tokens_kernel<32>, grid, dim3(kSelectThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL(select_kv_tokens_kernel<0>, grid, dim3(kSelectThreads), 0, s, a);
-  return (int)hipGetLastError();
+  auto run = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), 0, s, a);
+    return (int)hipGetLastError();
+  };
+  if (tokens <= 2048) return run(select_kv_tokens_kernel<256, 8, false>, 256);
+  if (tokens <= 8192) return run(select_kv_tokens_kernel<512, 16, false>, 512);
+  if (tokens <= 32768) return run(select_kv_tokens_kernel<1024, 32, false>, 1024);
+  return run(select_kv_tokens_kernel<1024, 16, true>, 1024);
 }
 
 extern "C" int mskv_evict_kv_tokens(void* k_cache, void* v_cache, float* k_scale_cache,
@@ -457,24 +497,27 @@ extern "C" int mskv_evict_kv_tokens(void* k_cache, void* v_cache, float* k_scale
   if (!k_cache || !v_cache || !k_scale_cache || !v_scale_cache || !kept || !new_seqlens ||
       !block_tables || misaligned({k_cache, v_cache}))
     return MSKV_EINVAL;
-  // the heads of a token whose scales one workgroup moves: all of them where the
-  // sequences alone are workgroups enough
-  int scale_heads = (int)std::min<int64_t>(num_kv_heads, (int64_t)batch * num_kv_heads / 32);
-  scale_heads = std::max(1, scale_heads);
-  while (num_kv_heads % scale_heads != 0) --scale_heads;
-  const int scale_units = num_kv_heads / scale_heads;
+  // The heads of a token that one workgroup moves, all of them where the
+  // sequences alone are workgroups enough.
+  auto heads_of = [&](int64_t units) {
+    int heads = (int)std::max<int64_t>(1, std::min<int64_t>(num_kv_heads, units));
+    while (num_kv_heads % heads != 0) --heads;
+    return heads;
+  };
+  const int scale_heads = heads_of((int64_t)batch * num_kv_heads / 32);
+  const int row_heads = heads_of((int64_t)batch * 2 * num_kv_heads / 512);
+  const int scale_units = num_kv_heads / scale_heads, row_units = num_kv_heads / row_heads;
   const EvictArgs a = {(uint8_t*)k_cache, (uint8_t*)v_cache, k_scale_cache, v_scale_cache, weights,
                        kept, new_seqlens, block_tables, num_blocks, num_kv_heads, block_size,
-                       max_blocks_per_seq, budget, scale_heads, scale_units,
-                       divider_of(block_size), divider_of(scale_heads)};
+                       max_blocks_per_seq, budget, scale_heads, scale_units, row_heads, row_units,
+                       divider_of(block_size), divider_of(scale_heads), divider_of(row_heads)};
+  const dim3 grid((unsigned)(2 * scale_units + (weights ? num_kv_heads : 0) + 2 * row_units),
+                  (unsigned)batch);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  auto run = [&](auto kernel, int parts) {
-    const int units = 2 * scale_units + (weights ? num_kv_heads : 0) + 2 * parts * num_kv_heads;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)units, (unsigned)batch), dim3(kEvictThreads), 0, s,
-                       a);
-    return (int)hipGetLastError();
-  };
-  // halves of rows where whole ones are too few workgroups for the chip
-  if ((int64_t)batch * num_kv_heads * 2 >= 512) return run(evict_kv_tokens_kernel<1>, 1);
-  return run(evict_kv_tokens_kernel<2>, 2);
+  // (longer runs where the workgroups are too few to fill the chip)
+  if ((int64_t)grid.x * batch > 256)
+    hipLaunchKernelGGL(evict_kv_tokens_kernel<512>, grid, dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL(evict_kv_tokens_kernel<1024>, grid, dim3(1024), 0, s, a);
+  return (int)hipGetLastError();
 }
