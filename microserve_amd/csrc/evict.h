@@ -19,6 +19,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mskv_device.h"
 #include "../../include/mskv.h"
@@ -52,10 +53,9 @@ struct SelectArgs {
 
 // An integer that orders as the weight does: NaN lowest, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float x) {
-  const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
-  if ((u & 0x7FFFFFFFu) == 0u) return 0x80000000u;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(x + 0.0f);  // (-0 + 0 is 0)
+  const uint32_t key = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return x != x ? 0u : key;
 }
 
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
@@ -66,16 +66,17 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
 // The sum of v over the threads before this one, and over all.
 template <int kWaves>
 __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_wave, uint32_t& all) {
-  int lane = threadIdx.x & 63;
-  asm volatile("" : "+v"(lane));  // (masks kept from scan to scan would spill)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the wave's running sum by DPP: shifts within rows of 16 lanes, then the rows'
+  // last lanes to the rows behind them
   uint32_t x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) s_wave[wave] = x;
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xF, 0xF, true);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xF, 0xF, true);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xF, 0xF, true);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xF, 0xF, true);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xA, 0xF, false);  // row_bcast:15, rows 1, 3
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xC, 0xF, false);  // row_bcast:31, rows 2, 3
+  if ((threadIdx.x & 63) == 63) s_wave[wave] = x;
   __syncthreads();
   uint32_t before = x - v;
   all = 0;
@@ -89,19 +90,20 @@ __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_wave, ui
   return before;
 }
 
-// kItems: keys that a thread holds, thread t's j-th key that of token
-// j * kThreads + t of the range; kReread: as many at a time, read again on every
-// pass.
-template <int kThreads, int kItems, bool kReread>
+// kQuads: runs of four tokens that a thread holds the keys of, thread t's j-th
+// run that number j * kThreads + t of the range; kReread: as many at a time, read
+// again on every pass.
+template <int kThreads, int kQuads, bool kReread>
 __global__ __launch_bounds__(kThreads) void select_kv_tokens_kernel(SelectArgs a) {
   constexpr int kWaves = kThreads / 64;
-  constexpr int kEntries = kItems * kWaves;  // waves' counts of a turn
-  constexpr int kEach = (kEntries + kThreads - 1) / kThreads;
+  constexpr int kEntries = kQuads * kWaves;  // waves' counts of a turn
+  static_assert(kEntries <= kThreads, "a thread takes one of the counts");
   constexpr int kBinsEach = kSelectBins / kThreads;
-  __shared__ uint32_t s_hist[kSelectBins];
+  // four copies of the counts, for lanes side by side: weights lie in few bins
+  __shared__ __attribute__((aligned(16))) uint32_t s_hist[kSelectBins][4];
   __shared__ uint32_t s_wave[kWaves];
-  __shared__ uint32_t s_found[2];
-  __shared__ uint32_t s_count[kEach * kThreads];
+  __shared__ uint32_t s_found[3];
+  __shared__ uint32_t s_count[kEntries];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / a.hk, h = blockIdx.x - b * a.hk;
   const int L = max(0, min(__builtin_amdgcn_readfirstlane(a.seqlens[b]), a.w * a.bs));
@@ -119,31 +121,39 @@ __global__ __launch_bounds__(kThreads) void select_kv_tokens_kernel(SelectArgs a
   for (int i = tid; i < last; i += kThreads) kept[n - last + i] = L - last + i;
   const int quota = n - first - last;
   if (quota == 0) return;
-  const int count = L - last - first;  // tokens that compete: more than quota
+  // the tokens that compete, more than quota: [first, end); runs of four of them
+  // start at multiples of four and lie in one page
+  const int end = L - last, base = first & ~3;
+  const int quads = (end - base + 3) / 4;
 
   const int32_t* table = a.bt + (int64_t)b * a.w;
-  // The key of the range's token i.  Without branches, so that the reads of all
-  // of a thread's keys are in flight at once: a token past the end stands for the
-  // last one, an invalid block for the first.
-  auto read = [&](int i) -> uint32_t {
-    const int t = first + min(i, count - 1), page = a.by_block(t);
-    const int blk = table[page];
-    const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
-    const float x = a.weights[((int64_t)(ok ? blk : 0) * a.hk + h) * a.bs + (t - page * a.bs)];
-    return ok ? weight_key(x) : 0u;
-  };
-  constexpr int kTurn = kItems * kThreads;
-  uint32_t own[kItems];
+  uint32_t own[kQuads][4];
+  // The keys of a turn's runs.  Without branches, so that all of a thread's reads
+  // are in flight at once: a run past the end stands for the last one, an invalid
+  // block for the first.  A token that does not compete has key 0, with the
+  // lightest.
   auto fill = [&](int at) {
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) own[j] = read(at + j * kThreads + tid);
+    for (int j = 0; j < kQuads; ++j) {
+      const int t = base + 4 * min(at + j * kThreads + tid, quads - 1), page = a.by_block(t);
+      const int blk = table[page];
+      const bool ok = (uint32_t)blk < (uint32_t)a.num_blocks;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(
+          a.weights + ((int64_t)(ok ? blk : 0) * a.hk + h) * a.bs + (t - page * a.bs));
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        own[j][q] = ok && t + q >= first && t + q < end ? weight_key(x[q]) : 0u;
+    }
   };
+  constexpr int kTurn = kQuads * kThreads;
   if (!kReread) fill(0);
   // keys that live past a barrier, seen anew: the compiler would keep masks of
   // what it knows of each key from pass to pass, and spill them
   auto anew = [&] {
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) asm volatile("" : "+v"(own[j]));
+    for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(own[j][q]));
   };
 
   // The threshold: the quota-th largest key, digit by digit; `need` of the
@@ -154,18 +164,20 @@ __global__ __launch_bounds__(kThreads) void select_kv_tokens_kernel(SelectArgs a
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t mask = pass == 2 ? 1023u : 2047u;
 #pragma unroll
-    for (int i = 0; i < kBinsEach; ++i) s_hist[i * kThreads + tid] = 0;
+    for (int i = 0; i < kBinsEach; ++i)
+      *reinterpret_cast<u32x4*>(s_hist[i * kThreads + tid]) = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
-    for (int at = 0; at < count; at += kTurn) {
+    for (int at = 0; at < quads; at += kTurn) {
       if (kReread) fill(at);
-      int left = count - at;
-      asm volatile("" : "+s"(left));
 #pragma unroll
-      for (int j = 0; j < kItems; ++j) {
-        // (the digits above: all 32 bits on the first pass have none)
-        if (j * kThreads + tid < left &&
-            (pass == 0 || (own[j] >> (pass == 1 ? 21 : 10)) == digits))
-          atomicAdd(&s_hist[(own[j] >> shift) & mask], 1u);
+      for (int j = 0; j < kQuads; ++j) {
+        if (at + j * kThreads + tid < quads) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            // (the digits above: all 32 bits on the first pass have none)
+            if (pass == 0 || (own[j][q] >> (pass == 1 ? 21 : 10)) == digits)
+              atomicAdd(&s_hist[(own[j][q] >> shift) & mask][lane & 3], 1u);
+        }
       }
     }
     __syncthreads();
@@ -173,7 +185,9 @@ __global__ __launch_bounds__(kThreads) void select_kv_tokens_kernel(SelectArgs a
     uint32_t bins[kBinsEach], sum = 0, all;
 #pragma unroll
     for (int i = 0; i < kBinsEach; ++i) {
-      bins[i] = s_hist[kSelectBins - 1 - (kBinsEach * tid + i)];
+      const u32x4 c =
+          *reinterpret_cast<const u32x4*>(s_hist[kSelectBins - 1 - (kBinsEach * tid + i)]);
+      bins[i] = (c[0] + c[1]) + (c[2] + c[3]);
       sum += bins[i];
     }
     uint32_t before = scan_before<kWaves>(sum, s_wave, all);
@@ -183,6 +197,7 @@ __global__ __launch_bounds__(kThreads) void select_kv_tokens_kernel(SelectArgs a
         if (before < need && before + bins[i] >= need) {
           s_found[0] = kSelectBins - 1 - (kBinsEach * tid + i);
           s_found[1] = need - before;
+          s_found[2] = bins[i];
         }
         before += bins[i];
       }
@@ -194,52 +209,73 @@ __global__ __launch_bounds__(kThreads) void select_kv_tokens_kernel(SelectArgs a
   }
   const uint32_t threshold = digits;
 
-  // The kept positions in order: those above the threshold, and the first
-  // `need` at it.  A wave's counts of 64 tokens of either, then their running
-  // sums over the workgroup (two counts in a word: at most 2^15 tokens a turn).
-  static_assert(kTurn <= 1 << 15, "two counts fit a word");
-  uint32_t above0 = 0, equal0 = 0;  // before this turn
+  // The kept positions in order: a wave's counts of 64 runs, their running sums
+  // over the workgroup, then each token's place.  Where every token at the
+  // threshold stays, one comparison decides; else those above it stay and the
+  // first `need` at it, whose counts travel in the upper halves of the words (at
+  // most 2^15 tokens a turn).
+  static_assert(4 * kTurn <= 1 << 15, "two counts fit a word");
   int32_t* to = kept + first;
-  for (int at = 0; at < count; at += kTurn) {
-    if (kReread) fill(at);
+  auto write = [&](auto ties) {
+    constexpr bool kTies = decltype(ties)::value;
+    uint32_t above0 = 0, equal0 = 0;  // before this turn
+    for (int at = 0; at < quads; at += kTurn) {
+      if (kReread) fill(at);
+      auto is_above = [&](int j, int q) {
+        return kTies ? own[j][q] > threshold : own[j][q] >= threshold;
+      };
+      auto is_equal = [&](int j, int q) {  // (a token that does not compete is none)
+        const int t = base + 4 * (at + j * kThreads + tid) + q;
+        return own[j][q] == threshold && t >= first && t < end;
+      };
+      auto live = [&](int j) { return at + j * kThreads + tid < quads; };
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      const bool live = at + j * kThreads + tid < count;
-      const uint64_t above = __ballot(live && own[j] > threshold);
-      const uint64_t equal = __ballot(live && own[j] == threshold);
-      if (lane == 0) s_count[j * kWaves + wave] = __popcll(above) | __popcll(equal) << 16;
-      __builtin_amdgcn_sched_barrier(0);  // (masks of many keys at once would spill)
-    }
-    anew();
-    __syncthreads();
-    uint32_t c[kEach], sum = 0, all;
+      for (int j = 0; j < kQuads; ++j) {
+        uint32_t above = 0, equal = 0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      c[i] = kEach * tid + i < kEntries ? s_count[kEach * tid + i] : 0u;
-      sum += c[i];
-    }
-    uint32_t before = scan_before<kWaves>(sum, s_wave, all);
+        for (int q = 0; q < 4; ++q) {
+          above += __popcll(__ballot(live(j) && is_above(j, q)));
+          if (kTies) equal += __popcll(__ballot(live(j) && is_equal(j, q)));
+        }
+        if (lane == 0) s_count[j * kWaves + wave] = above | equal << 16;
+        __builtin_amdgcn_sched_barrier(0);  // (masks of many keys at once would spill)
+      }
+      anew();
+      __syncthreads();
+      uint32_t all;
+      const uint32_t before =
+          scan_before<kWaves>(tid < kEntries ? s_count[tid] : 0u, s_wave, all);
+      if (tid < kEntries) s_count[tid] = before;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      s_count[kEach * tid + i] = before;
-      before += c[i];
-    }
-    __syncthreads();
+      for (int j = 0; j < kQuads; ++j) {
+        const uint32_t counts = s_count[j * kWaves + wave];
+        uint32_t above = above0 + (counts & 0xFFFFu), equal = equal0 + (counts >> 16);
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      const int i = at + j * kThreads + tid;
-      const bool is_above = i < count && own[j] > threshold;
-      const bool is_equal = i < count && own[j] == threshold;
-      const uint32_t base = s_count[j * kWaves + wave];
-      const uint32_t above = above0 + (base & 0xFFFFu) + lanes_below(__ballot(is_above));
-      const uint32_t equal = equal0 + (base >> 16) + lanes_below(__ballot(is_equal));
-      if (is_above || (is_equal && equal < need)) to[above + min(equal, need)] = first + i;
-      __builtin_amdgcn_sched_barrier(0);
+        for (int q = 0; q < 4; ++q) {
+          above += lanes_below(__ballot(live(j) && is_above(j, q)));
+          if (kTies) equal += lanes_below(__ballot(live(j) && is_equal(j, q)));
+        }
+        const int t = base + 4 * (at + j * kThreads + tid);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const bool up = live(j) && is_above(j, q);
+          const bool tie = kTies && live(j) && is_equal(j, q);
+          if (up || (tie && equal < need)) to[above + (kTies ? min(equal, need) : 0u)] = t + q;
+          above += up;
+          equal += tie;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      above0 += all & 0xFFFFu;
+      equal0 += all >> 16;
+      if (kReread) __syncthreads();  // (the counts are read before the next turn's)
     }
-    above0 += all & 0xFFFFu;
-    equal0 += all >> 16;
-    if (kReread) __syncthreads();  // (the counts are read before the next turn's)
-  }
+  };
+  if (s_found[2] == need)
+    write(std::false_type());
+  else
+    write(std::true_type());
 }
 
 constexpr int kEvictLoads = 4;  // 16-byte pieces of a lane and run
@@ -461,7 +497,10 @@ extern "C" int mskv_select_kv_tokens(const float* weights, const int32_t* cache_
   if (start < 0 || recent < 0) return MSKV_EINVAL;
   if (batch == 0) return MSKV_OK;
   if (num_blocks == 0) return MSKV_EINVAL;  // (there are no weights to read)
-  if (!weights || !cache_seqlens || !block_tables || !kept || !new_seqlens) return MSKV_EINVAL;
+  if (block_size % 4 != 0 || num_blocks > 0x7FFFFFFFLL) return MSKV_EUNSUPPORTED;
+  if (!weights || !cache_seqlens || !block_tables || !kept || !new_seqlens ||
+      misaligned({weights}))
+    return MSKV_EINVAL;
   const SelectArgs a = {weights, cache_seqlens, block_tables,       starts, kept,   new_seqlens,
                         num_blocks, num_kv_heads, block_size, max_blocks_per_seq, start, recent,
                         budget, divider_of(block_size)};
@@ -473,10 +512,10 @@ extern "C" int mskv_select_kv_tokens(const float* weights, const int32_t* cache_
     hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), 0, s, a);
     return (int)hipGetLastError();
   };
-  if (tokens <= 2048) return run(select_kv_tokens_kernel<256, 8, false>, 256);
-  if (tokens <= 8192) return run(select_kv_tokens_kernel<512, 16, false>, 512);
-  if (tokens <= 32768) return run(select_kv_tokens_kernel<1024, 32, false>, 1024);
-  return run(select_kv_tokens_kernel<1024, 16, true>, 1024);
+  if (tokens <= 2048) return run(select_kv_tokens_kernel<512, 1, false>, 512);
+  if (tokens <= 8192) return run(select_kv_tokens_kernel<1024, 2, false>, 1024);
+  if (tokens <= 32768) return run(select_kv_tokens_kernel<1024, 8, false>, 1024);
+  return run(select_kv_tokens_kernel<1024, 4, true>, 1024);
 }
 
 extern "C" int mskv_evict_kv_tokens(void* k_cache, void* v_cache, float* k_scale_cache,
