@@ -197,15 +197,6 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowArgs& a, int s) {
 struct WindowRange {
   int s, index, per;  // the sequence (-1: none), its range, tiles of a range
 };
-__device__ __forceinline__ int wave_scan_i32(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(v, d);
-    if (lane >= d) v += y;
-  }
-  return v;
-}
 __device__ __forceinline__ WindowRange window_range(const WindowArgs& a, int item, int units) {
   const int lane = threadIdx.x & 63;
   auto tiles_of = [&](int s) {

@@ -67,15 +67,7 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
 template <int kWaves>
 __device__ __forceinline__ uint32_t scan_before(uint32_t v, uint32_t* s_wave, uint32_t& all) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // the wave's running sum by DPP: shifts within rows of 16 lanes, then the rows'
-  // last lanes to the rows behind them
-  uint32_t x = v;
-  x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xF, 0xF, true);   // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xF, 0xF, true);   // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xF, 0xF, true);   // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xF, 0xF, true);   // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xA, 0xF, false);  // row_bcast:15, rows 1, 3
-  x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xC, 0xF, false);  // row_bcast:31, rows 2, 3
+  const uint32_t x = (uint32_t)wave_scan_i32((int)v);
   if ((threadIdx.x & 63) == 63) s_wave[wave] = x;
   __syncthreads();
   uint32_t before = x - v;

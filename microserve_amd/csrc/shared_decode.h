@@ -27,6 +27,7 @@ namespace mskv {
 constexpr int kSharedThreads = 256;
 constexpr int kSharedTile = 128;  // keys
 constexpr int kSharedMaxGroups = 1024;
+constexpr int kSharedWorkgroups = 512;  // that run at once: two a CU
 
 struct SharedArgs {
   DecodeArgs d;  // part_o, part_lse: [batch * hq, d.splits]
@@ -34,14 +35,12 @@ struct SharedArgs {
   int* counts;  // partials of each sequence's rows; -1: its rows are written
   int groups, max_prefix;  // max_prefix: whole tiles' tokens
   int gc, tpr;             // heads of a unit, sequences of a 16-row block
-  int slots_a, slots_b;    // items that should run at once
   int sa, sb;              // most ranges of a prefix, of a tail
-  int blocks_a;            // workgroups of prefix items
 };
 
 // What a workgroup is to do.
 struct SharedItem {
-  int kind;         // 0: nothing, else the item exists
+  int kind;         // 0: nothing, 1: of a prefix, 2: of a tail
   int first, size;  // prefix: the group's sequences; tail: the sequence, -
   int row0;         // prefix: first sequence of its 128 rows
   int source;       // prefix: the sequence whose table names the pages
@@ -51,49 +50,30 @@ struct SharedItem {
 
 struct SharedPlan {
   int cu[kSharedMaxGroups + 1], shared[kSharedMaxGroups], source[kSharedMaxGroups];
-  int wave_a[4], wave_b[4], wave_c[4], wave_d[4];
+  int sums[4][4], scans[4][2];
   SharedItem item;
 };
 
-__device__ __forceinline__ void block_sum_max(int& sum, int& most, int* s_sum, int* s_max) {
-  sum = wave_sum_i32(sum);
-  most = wave_max_u31(most);
-  if ((threadIdx.x & 63) == 0) {
-    s_sum[threadIdx.x >> 6] = sum;
-    s_max[threadIdx.x >> 6] = most;
-  }
-  __syncthreads();
-  sum = most = 0;
-#pragma unroll
-  for (int i = 0; i < kSharedThreads / 64; ++i) {
-    sum += s_sum[i];
-    most = max(most, s_max[i]);
-  }
-}
-__device__ __forceinline__ int block_before(int v, int* s_wave) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  if (lane == 63) s_wave[wave] = x;
-  __syncthreads();
-  int before = x - v;
-#pragma unroll
-  for (int i = 0; i < kSharedThreads / 64; ++i)
-    if (i < wave) before += s_wave[i];
-  return before;
-}
+// Time of a prefix item's tile and of a tail item's step beside another
+// workgroup, in the same unit (us): what the ranges are balanced by.
+constexpr float kSharedTileTime = 3.6f, kSharedStepTime = 2.2f;
+
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Fills p.item with item `index` of the workgroup's kind (tail or prefix).
-__device__ __forceinline__ void shared_plan(const SharedArgs& a, bool tail, int index,
-                                            SharedPlan& p) {
-  const int tid = threadIdx.x;
+// Finds workgroup `index`'s item and its unit: items of prefixes first (`units`
+// workgroups each), then those of tails (`tail_units` each), then none.
+//
+// The ranges are as long as lets all of them run at once, a prefix's and a
+// tail's taking about as long: a second round would pay for the plan, the first
+// loads and the last stores again.  (64 sequences over a prefix of 8192 tokens:
+// 44 us in two rounds of ranges sized apart.)
+__device__ __forceinline__ int shared_plan(const SharedArgs& a, int index, int units,
+                                           int tail_units, SharedPlan& p) {
+  const int tid = threadIdx.x, wave = tid >> 6;
   const int batch = a.d.batch;
   const int cap = a.d.w * a.d.bs;
+  // (a thread's first length is read with the groups, and kept)
+  const int own_raw = tid < batch ? a.d.seqlens[tid] : 0;
   if (tid == 0) p.item.kind = 0;
   for (int g = tid; g <= a.groups; g += kSharedThreads)
     p.cu[g] = min(max(a.cu_groups[g], 0), batch);
@@ -115,9 +95,13 @@ __device__ __forceinline__ void shared_plan(const SharedArgs& a, bool tail, int 
     }
     return b < p.cu[lo + 1] ? lo : -1;
   };
-  auto length = [&](int b) { return max(0, min(a.d.seqlens[b], cap)); };
+  auto length = [&](int b) {
+    return max(0, min(b == tid ? own_raw : a.d.seqlens[b], cap));
+  };
+  const int own_group = tid < batch ? group_of(tid) : -1;
+  auto group = [&](int b) { return b == tid ? own_group : group_of(b); };
   for (int b = tid; b < batch; b += kSharedThreads) {
-    const int g = group_of(b), len = length(b);
+    const int g = group(b), len = length(b);
     if (g >= 0 && len > 0) {
       atomicMin(&p.shared[g], len);
       atomicMin(&p.source[g], b);
@@ -130,73 +114,95 @@ __device__ __forceinline__ void shared_plan(const SharedArgs& a, bool tail, int 
   };
   const int rows = 8 * a.tpr;  // sequences of a workgroup's 128 rows
   auto blocks_of = [&](int g) { return ceil_div(max(p.cu[g + 1] - p.cu[g], 0), rows); };
-  int work = 0, longest = 0;
+  auto prefix_of = [&](int b) {  // tiles that a sequence shares
+    const int g = group(b);
+    return g >= 0 && length(b) > 0 ? tiles_of(g) : 0;
+  };
+  auto steps_of = [&](int b) { return ceil_div(length(b) - prefix_of(b) * kSharedTile, kStep); };
+  int work = 0, longest = 0, steps = 0, most = 0;
   for (int g = tid; g < a.groups; g += kSharedThreads) {
     const int t = tiles_of(g);
     work += t * blocks_of(g);
     longest = max(longest, t);
   }
-  block_sum_max(work, longest, p.wave_a, p.wave_b);
-  // tiles of a prefix's range
-  const int per_a = max(max(ceil_div(work, a.slots_a), ceil_div(longest, a.sa)), 1);
-  if (!tail) {
-    const int each = ceil_div(a.groups, kSharedThreads);
-    const int g0 = min(tid * each, a.groups), g1 = min(g0 + each, a.groups);
-    int n = 0;
-    for (int g = g0; g < g1; ++g) n += blocks_of(g) * ceil_div(tiles_of(g), per_a);
-    int at = block_before(n, p.wave_c);
-    if (index >= at && index < at + n) {
-      for (int g = g0; g < g1; ++g) {
-        const int blocks = blocks_of(g), ranges = ceil_div(tiles_of(g), per_a);
-        if (index < at + blocks * ranges) {
-          // (a range's row blocks one after the other: they read the same keys)
-          const int range = (index - at) / blocks, rb = index - at - range * blocks;
-          p.item = SharedItem{1, p.cu[g], p.cu[g + 1] - p.cu[g], rb * rows, p.source[g],
-                              range * per_a * kSharedTile,
-                              min((range + 1) * per_a, tiles_of(g)) * kSharedTile, range, 0};
-          break;
-        }
-        at += blocks * ranges;
+  for (int b = tid; b < batch; b += kSharedThreads) {
+    const int s = steps_of(b);
+    steps += s;
+    most = max(most, s);
+  }
+  work = wave_sum_i32(work), steps = wave_sum_i32(steps);
+  longest = wave_max_u31(longest), most = wave_max_u31(most);
+  if ((tid & 63) == 0) {
+    p.sums[wave][0] = work, p.sums[wave][1] = longest;
+    p.sums[wave][2] = steps, p.sums[wave][3] = most;
+  }
+  __syncthreads();
+  work = longest = steps = most = 0;
+#pragma unroll
+  for (int i = 0; i < kSharedThreads / 64; ++i) {
+    work += p.sums[i][0], longest = max(longest, p.sums[i][1]);
+    steps += p.sums[i][2], most = max(most, p.sums[i][3]);
+  }
+  const float chain = ((float)work * units * kSharedTileTime +
+                       (float)steps * tail_units * kSharedStepTime) / kSharedWorkgroups;
+  // tiles of a prefix's range, steps of a tail's
+  const int per_a = max(max((int)ceilf(chain / kSharedTileTime), ceil_div(longest, a.sa)), 1);
+  const int per_b = max(max((int)ceilf(chain / kSharedStepTime), ceil_div(most, a.sb)),
+                        kMinSplitSteps);
+
+  // each thread's groups and sequences, one after the other, and the items
+  // before them
+  const int each_g = ceil_div(a.groups, kSharedThreads);
+  const int g0 = min(tid * each_g, a.groups), g1 = min(g0 + each_g, a.groups);
+  const int each_b = ceil_div(batch, kSharedThreads);
+  const int b0 = min(tid * each_b, batch), b1 = min(b0 + each_b, batch);
+  int na = 0, nb = 0;
+  for (int g = g0; g < g1; ++g) na += blocks_of(g) * ceil_div(tiles_of(g), per_a);
+  // (a sequence without a tail has an item too, which notes its partials)
+  for (int b = b0; b < b1; ++b) nb += max(1, ceil_div(steps_of(b), per_b));
+  int at_a = wave_scan_i32(na), at_b = wave_scan_i32(nb);
+  if ((tid & 63) == 63) p.scans[wave][0] = at_a, p.scans[wave][1] = at_b;
+  __syncthreads();
+  at_a -= na, at_b -= nb;
+  int items_a = 0;
+#pragma unroll
+  for (int i = 0; i < kSharedThreads / 64; ++i) {
+    if (i < wave) at_a += p.scans[i][0], at_b += p.scans[i][1];
+    items_a += p.scans[i][0];
+  }
+  const bool tail = index >= items_a * units;
+  if (tail) index -= items_a * units;
+  const int item = index / (tail ? tail_units : units);
+  const int unit = index - item * (tail ? tail_units : units);
+  if (!tail && item >= at_a && item < at_a + na) {
+    for (int g = g0; g < g1; ++g) {
+      const int blocks = blocks_of(g), ranges = ceil_div(tiles_of(g), per_a);
+      if (item < at_a + blocks * ranges) {
+        // (a range's row blocks one after the other: they read the same keys)
+        const int range = (item - at_a) / blocks, rb = item - at_a - range * blocks;
+        p.item = SharedItem{1, p.cu[g], p.cu[g + 1] - p.cu[g], rb * rows, p.source[g],
+                            range * per_a * kSharedTile,
+                            min((range + 1) * per_a, tiles_of(g)) * kSharedTile, range, 0};
+        break;
       }
+      at_a += blocks * ranges;
     }
-  } else {
-    auto steps_of = [&](int b, int& g, int& len) {
-      g = group_of(b);
-      len = length(b);
-      const int begin = g >= 0 && len > 0 ? tiles_of(g) * kSharedTile : 0;
-      return ceil_div(len - begin, kStep);
-    };
-    int steps = 0, most = 0, g, len;
-    for (int b = tid; b < batch; b += kSharedThreads) {
-      const int s = steps_of(b, g, len);
-      steps += s;
-      most = max(most, s);
-    }
-    block_sum_max(steps, most, p.wave_c, p.wave_d);
-    const int per_b =
-        max(max(ceil_div(steps, a.slots_b), ceil_div(most, a.sb)), kMinSplitSteps);
-    const int each = ceil_div(batch, kSharedThreads);
-    const int b0 = min(tid * each, batch), b1 = min(b0 + each, batch);
-    // (a sequence without a tail has an item too, which notes its partials)
-    int n = 0;
-    for (int b = b0; b < b1; ++b) n += max(1, ceil_div(steps_of(b, g, len), per_b));
-    int at = block_before(n, p.wave_a);
-    if (index >= at && index < at + n) {
-      for (int b = b0; b < b1; ++b) {
-        const int s = steps_of(b, g, len), ranges = ceil_div(s, per_b), i = index - at;
-        if (i < max(1, ranges)) {
-          const int tiles = g >= 0 && len > 0 ? tiles_of(g) : 0;
-          const int ahead = ceil_div(tiles, per_a);
-          const int begin = tiles * kSharedTile + i * per_b * kStep;
-          p.item = SharedItem{1, b, 0, i, 0, begin, min(begin + per_b * kStep, len), ahead + i,
-                              ahead + ranges};
-          break;
-        }
-        at += max(1, ranges);
+  }
+  if (tail && item >= at_b && item < at_b + nb) {
+    for (int b = b0; b < b1; ++b) {
+      const int ranges = ceil_div(steps_of(b), per_b), i = item - at_b;
+      if (i < max(1, ranges)) {
+        const int tiles = prefix_of(b), ahead = ceil_div(tiles, per_a), len = length(b);
+        const int begin = tiles * kSharedTile + i * per_b * kStep;
+        p.item = SharedItem{2, b, 0, i, 0, begin, min(begin + per_b * kStep, len), ahead + i,
+                            ahead + ranges};
+        break;
       }
+      at_b += max(1, ranges);
     }
   }
   __syncthreads();
+  return unit;
 }
 
 // The LDS of a workgroup: tiles of K and V, double-buffered (separate objects,
@@ -395,14 +401,21 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& s, const SharedI
     }
   }
   const float inv_f = f != 0.0f ? 1.0f / f : 1.0f;  // a power of two: exact
+  // (the arguments read again: held in scalar registers across the loop, they
+  // spill)
+  typedef const __attribute__((address_space(4))) SharedArgs* KernArgs;
+  KernArgs ka = (KernArgs)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(ka));
+  float *part_o = ka->d.part_o, *part_lse = ka->d.part_lse;
+  const int splits = ka->d.splits;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const float den = sum_xor32(sum_xor16(l[k]));
     if (row[k] < 0) continue;
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) acc[k][dt] *= inv_f;
-    const int64_t at = row[k] * a.splits + e.slot;
-    write_partial(a.part_o + at * kHeadDim, a.part_lse + at, acc[k], m[k], den, g);
+    const int64_t at = row[k] * splits + e.slot;
+    write_partial(part_o + at * kHeadDim, part_lse + at, acc[k], m[k], den, g);
   }
 }
 
@@ -449,11 +462,8 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_decode_kernel(Shared
   static_assert(sizeof(SharedTile) == sizeof(Fp8Cache::Tiles), "a wave's tiles fit a tile");
   static_assert(sizeof(SharedPlan) <= sizeof(SharedTile), "the plan fits a tile");
   const int units = a.d.hk * a.d.qgroups;
-  const bool tail = (int)blockIdx.x >= a.blocks_a;
   SharedPlan& plan = *reinterpret_cast<SharedPlan*>(k_lds0);
-  const int at = tail ? (int)blockIdx.x - a.blocks_a : (int)blockIdx.x;
-  const int per_item = tail ? (units + 3) / 4 : units;
-  shared_plan(a, tail, at / per_item, plan);
+  const int own = shared_plan(a, blockIdx.x, units, (units + 3) / 4, plan);
   SharedItem e = plan.item;
   __syncthreads();  // (the tiles take its place)
   // the same for every lane: page resources and table reads stay scalar
@@ -462,12 +472,13 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_decode_kernel(Shared
   for (int i = 0; i < (int)(sizeof(SharedItem) / sizeof(int)); ++i)
     reinterpret_cast<int*>(&e)[i] = __builtin_amdgcn_readfirstlane(reinterpret_cast<int*>(&e)[i]);
   if (!e.kind) return;
-  if (!tail) {
-    shared_prefix<T>(a, e, at % per_item, k_lds0, v_lds0, k_lds1, v_lds1, sc_lds0, sc_lds1);
+  if (e.kind == 1) {
+    shared_prefix<T>(a, e, __builtin_amdgcn_readfirstlane(own), k_lds0, v_lds0, k_lds1, v_lds1,
+                     sc_lds0, sc_lds1);
     return;
   }
   const int wave = threadIdx.x >> 6;
-  const int unit = at % per_item * 4 + wave;
+  const int unit = own * 4 + wave;
   if (unit >= units) return;
   uint8_t* tile = wave == 0 ? k_lds0 : wave == 1 ? v_lds0 : wave == 2 ? k_lds1 : v_lds1;
   float* scales = wave < 2 ? sc_lds0[wave] : sc_lds1[wave - 2];
@@ -496,30 +507,31 @@ __global__ __launch_bounds__(64) void shared_merge_kernel(SharedArgs s) {
 
 // What a shape's launch is made of.
 struct SharedShape {
-  int max_prefix, gc, tpr, slots_a, slots_b, sa, sb;
-  int64_t items_a, items_b;
+  int max_prefix, gc, tpr, sa, sb;
+  int64_t grid;
 };
-constexpr int64_t kSharedWorkgroups = 512;  // that run at once: two a CU
 
 static SharedShape shared_shape(int batch, int groups, int hq, int hk, int w, int bs,
                                 int64_t max_prefix_len) {
   SharedShape s;
-  const int group = hq / hk, units = hk * qgroups_of(group);
+  const int group = hq / hk, units = hk * qgroups_of(group), tail_units = (units + 3) / 4;
   const int64_t cap = (int64_t)w * bs;
-  s.max_prefix = (int)(std::min(cap, max_prefix_len) / kSharedTile * kSharedTile);
+  s.max_prefix = groups > 0 ? (int)(std::min(cap, max_prefix_len) / kSharedTile * kSharedTile) : 0;
   s.gc = group < 16 ? group : 16;
   s.tpr = 16 / s.gc;
-  s.slots_a = (int)std::max<int64_t>(1, kSharedWorkgroups / units);
-  s.sa = std::max(1, std::min(s.max_prefix / kSharedTile, std::min(s.slots_a, 64)));
-  // (a group's last 128 rows may be few; a group needs a sequence)
-  const int64_t blocks = std::min<int64_t>(batch, batch / (8 * s.tpr) + groups);
-  s.items_a = s.max_prefix == 0 || groups == 0 ? 0 : std::min(s.slots_a + blocks, blocks * s.sa);
-  const int64_t per = (units + 3) / 4;
-  s.slots_b = (int)std::max<int64_t>(kSharedWorkgroups / per - batch / 2, 128 / per + 1);
-  const int64_t most = 8 * ((s.slots_b + batch - 1) / batch);
-  s.sb = (int)std::max<int64_t>(
-      1, std::min(std::min<int64_t>(most, s.slots_b), cap / (kMinSplitSteps * kStep)));
-  s.items_b = std::min((int64_t)s.slots_b + batch, (int64_t)batch * s.sb);
+  s.sa = std::max(1, std::min({s.max_prefix / kSharedTile, kSharedWorkgroups / units, 64}));
+  // (many sequences: partials of a few ranges each)
+  const int64_t slots = kSharedWorkgroups / tail_units;
+  const int64_t most = std::max<int64_t>(1, std::min(slots, 8 * ((slots + batch - 1) / batch)));
+  s.sb = (int)std::max<int64_t>(1, std::min(most, cap / (kMinSplitSteps * kStep)));
+  // Items of ranges that all run at once, and of each sequence's and group's
+  // last range (a group's last 128 rows may be few; a group needs a sequence)
+  const int64_t blocks = s.max_prefix == 0 ? 0 : std::min<int64_t>(batch, batch / (8 * s.tpr) + groups);
+  const int64_t least = std::min<int64_t>(blocks * s.sa * units, blocks * units + kSharedWorkgroups) +
+                        std::min<int64_t>((int64_t)batch * s.sb * tail_units,
+                                          (int64_t)batch * tail_units + kSharedWorkgroups);
+  s.grid = std::min<int64_t>(least, (blocks * units + (int64_t)batch * tail_units) +
+                                        kSharedWorkgroups + units + tail_units);
   return s;
 }
 
@@ -529,9 +541,7 @@ static size_t shared_bytes(int batch, int hq, const SharedShape& s) {
 
 template <typename T>
 static hipError_t launch_shared(const SharedArgs& a, const SharedShape& s, hipStream_t st) {
-  const int units = a.d.hk * a.d.qgroups;
-  const int64_t grid = a.blocks_a + s.items_b * ((units + 3) / 4);
-  hipLaunchKernelGGL(shared_decode_kernel<T>, dim3((unsigned)grid), dim3(kSharedThreads), 0, st,
+  hipLaunchKernelGGL(shared_decode_kernel<T>, dim3((unsigned)s.grid), dim3(kSharedThreads), 0, st,
                      a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -573,7 +583,7 @@ extern "C" int mskv_fp8_shared_prefix_decode_attention(
   if ((int64_t)max_blocks_per_seq * block_size >= (1LL << 30)) return MSKV_EUNSUPPORTED;
   // (sums over the batch of 32-token steps, and the merge's grid, stay within
   // an int)
-  if (num_groups > kSharedMaxGroups || (int64_t)batch * num_q_heads > 0x7FFFFFFF / 64 ||
+  if (num_groups > kSharedMaxGroups || batch > 65535 || num_kv_heads > 1024 || (int64_t)batch * num_q_heads > 0x7FFFFFFF / 64 ||
       (int64_t)batch * max_blocks_per_seq * block_size / kStep > 0x3FFFFFFF)
     return MSKV_EUNSUPPORTED;
   if (batch == 0) return MSKV_OK;
@@ -585,6 +595,7 @@ extern "C" int mskv_fp8_shared_prefix_decode_attention(
     return MSKV_EINVAL;
   const SharedShape s = shared_shape(batch, num_groups, num_q_heads, num_kv_heads,
                                      max_blocks_per_seq, block_size, max_prefix_len);
+  if (s.grid > 0x3FFFFF) return MSKV_EUNSUPPORTED;  // (a grid's threads fit 32 bits)
   if (!workspace || workspace_bytes < shared_bytes(batch, num_q_heads, s)) return MSKV_EWORKSPACE;
   SharedArgs a = {};
   a.d.q = (const uint16_t*)query;
@@ -614,11 +625,8 @@ extern "C" int mskv_fp8_shared_prefix_decode_attention(
   a.max_prefix = s.max_prefix;
   a.gc = s.gc;
   a.tpr = s.tpr;
-  a.slots_a = s.slots_a;
-  a.slots_b = s.slots_b;
   a.sa = s.sa;
   a.sb = s.sb;
-  a.blocks_a = (int)(s.items_a * num_kv_heads * a.d.qgroups);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return (int)(act_dtype == MSKV_BFLOAT16 ? launch_shared<__bf16>(a, s, st)
                                           : launch_shared<_Float16>(a, s, st));
