@@ -421,7 +421,7 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& s, const SharedI
 
 template <typename T>
 __device__ __forceinline__ void shared_tail(const SharedArgs& s, const SharedItem& e, int unit,
-                                            Fp8Cache::Tiles& tiles, Fp8Cache::Scales& scales) {
+                                            WalkTiles<false>& tiles, WalkScales& scales) {
   const DecodeArgs& a = s.d;
   const int lane = threadIdx.x & 63;
   const int g = lane >> 4, n = lane & 15;
@@ -444,8 +444,8 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& s, const SharedIte
   f32x4 acc[8];
   float m, l;
   const int blk = a.bt[(int64_t)b * a.w + e.begin / a.bs];
-  attend_range<T>(a, b, kvh, kvh * a.group + hig, head_ok, e.begin, e.end, blk, lane, tiles,
-                  scales, acc, m, l);
+  walk_range<T, false>(a, b, kvh, kvh * a.group + hig, head_ok, e.begin, e.end, blk, lane, tiles,
+                       scales, acc, m, l);
   if (!head_ok) return;
   if (e.count == 1) {
     write_output<T>(a.out + row * kHeadDim, acc, l, g);
@@ -459,7 +459,7 @@ template <typename T>
 __global__ __launch_bounds__(kSharedThreads, 2) void shared_decode_kernel(SharedArgs a) {
   __shared__ __attribute__((aligned(16))) SharedTile k_lds0, v_lds0, k_lds1, v_lds1;
   __shared__ __attribute__((aligned(16))) SharedScales sc_lds0, sc_lds1;
-  static_assert(sizeof(SharedTile) == sizeof(Fp8Cache::Tiles), "a wave's tiles fit a tile");
+  static_assert(sizeof(SharedTile) >= sizeof(WalkTiles<false>), "a wave's tile fits a tile");
   static_assert(sizeof(SharedPlan) <= sizeof(SharedTile), "the plan fits a tile");
   const int units = a.d.hk * a.d.qgroups;
   SharedPlan& plan = *reinterpret_cast<SharedPlan*>(k_lds0);
@@ -482,9 +482,8 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_decode_kernel(Shared
   if (unit >= units) return;
   uint8_t* tile = wave == 0 ? k_lds0 : wave == 1 ? v_lds0 : wave == 2 ? k_lds1 : v_lds1;
   float* scales = wave < 2 ? sc_lds0[wave] : sc_lds1[wave - 2];
-  static_assert(sizeof(Fp8Cache::Scales) == sizeof(float) * kSharedTile, "");
-  shared_tail<T>(a, e, unit, *reinterpret_cast<Fp8Cache::Tiles*>(tile),
-                 *reinterpret_cast<Fp8Cache::Scales*>(scales));
+  shared_tail<T>(a, e, unit, *reinterpret_cast<WalkTiles<false>*>(tile),
+                 *reinterpret_cast<WalkScales*>(scales));
 }
 
 // out = the merge of a row's partials, one wave a row.
