@@ -72,6 +72,10 @@ def fp8_decode_attention_weights(
     pages of new tokens need no clearing.  Pages that two sequences of the batch
     name must lie before ``start``.  The call may be captured in a HIP graph.
     """
+    res = _lib.fast.track(query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens,
+                          block_tables, softmax_scale, weights, start, out)
+    if res is not None:
+        return res
     what = "fp8_decode_attention_weights"
     query = _lib.aligned(query)
     cache_seqlens, block_tables = cache_seqlens.contiguous(), block_tables.contiguous()
@@ -123,6 +127,10 @@ def fp8_window_attention_weights(
     ``max_seqlen_q`` and ``max_seqlen_k`` (default: the tables' width) must be
     at least every sequence's numbers: what lies past them is not counted.
     """
+    res = _lib.fast.window(query, k_cache, k_scale_cache, block_tables, cu_seqlens_q, cu_seqlens_k,
+                           max_seqlen_q, softmax_scale, weights, accumulate, start, max_seqlen_k)
+    if res is not None:
+        return res
     what = "fp8_window_attention_weights"
     query = _lib.aligned(query)
     block_tables = block_tables.contiguous()
@@ -170,6 +178,9 @@ def select_kv_tokens(weights: torch.Tensor, cache_seqlens: torch.Tensor,
     behind them, and int32 ``[B]``, ``n``.  Any fp32 ``[NB, H_kv, BS]`` serves
     as ``weights``.  Nothing is read on the host.
     """
+    res = _lib.fast.choose(weights, cache_seqlens, block_tables, budget, recent, start)
+    if res is not None:
+        return res
     what = "select_kv_tokens"
     assert weights.dim() == 3, f"{what}: weights must be [blocks, kv heads, block size]"
     num_blocks, num_kv_heads, block_size = weights.shape
@@ -211,6 +222,9 @@ def evict_kv_tokens(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale_cache:
     (``copy_kv_blocks``), or keep it before ``start``.  The same rows of several
     layers take a call each.
     """
+    if _lib.fast.evict(k_cache, v_cache, k_scale_cache, v_scale_cache, kept, seqlens, block_tables,
+                       weights):
+        return
     what = "evict_kv_tokens"
     _caches(what, k_cache, v_cache, k_scale_cache, v_scale_cache)
     num_blocks, block_size, num_kv_heads, head_dim = k_cache.shape

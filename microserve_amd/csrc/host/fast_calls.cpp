@@ -43,6 +43,14 @@ struct Api {
   decltype(&mskv_fp4_prefill_attention) prefill4 = nullptr;
   decltype(&mskv_copy_kv_blocks) copy = nullptr;
   decltype(&mskv_compact_kv_blocks) compact = nullptr;
+  decltype(&mskv_shared_decode_workspace_bytes) shared_bytes = nullptr;
+  decltype(&mskv_fp8_shared_prefix_decode_attention) shared = nullptr;
+  decltype(&mskv_decode_weights_workspace_bytes) track_bytes = nullptr;
+  decltype(&mskv_fp8_decode_attention_weights) track = nullptr;
+  decltype(&mskv_window_weights_workspace_bytes) window_bytes = nullptr;
+  decltype(&mskv_fp8_window_attention_weights) window = nullptr;
+  decltype(&mskv_select_kv_tokens) choose = nullptr;
+  decltype(&mskv_evict_kv_tokens) evict = nullptr;
   decltype(&mskv_status_string) text = nullptr;
   bool bound = false;
 } api;
@@ -644,6 +652,8 @@ PyObject* compact_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+#include "cache_calls.h"
+
 // bind({name: address}): the entry points of the loaded library
 PyObject* bind(PyObject*, PyObject* table) {
   auto get = [&](const char* name, auto& fn) {
@@ -666,7 +676,15 @@ PyObject* bind(PyObject*, PyObject* table) {
             get("mskv_fp4_decode_num_splits", f.num_splits4) &&
             get("mskv_fp4_decode_attention", f.decode4) &&
             get("mskv_fp4_prefill_attention", f.prefill4) &&
-            get("mskv_copy_kv_blocks", f.copy) && get("mskv_compact_kv_blocks", f.compact) && get("mskv_status_string", f.text);
+            get("mskv_copy_kv_blocks", f.copy) && get("mskv_compact_kv_blocks", f.compact) &&
+            get("mskv_shared_decode_workspace_bytes", f.shared_bytes) &&
+            get("mskv_fp8_shared_prefix_decode_attention", f.shared) &&
+            get("mskv_decode_weights_workspace_bytes", f.track_bytes) &&
+            get("mskv_fp8_decode_attention_weights", f.track) &&
+            get("mskv_window_weights_workspace_bytes", f.window_bytes) &&
+            get("mskv_fp8_window_attention_weights", f.window) &&
+            get("mskv_select_kv_tokens", f.choose) && get("mskv_evict_kv_tokens", f.evict) &&
+            get("mskv_status_string", f.text);
   if (!f.bound) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "an entry point has no address");
     return nullptr;
@@ -678,7 +696,8 @@ PyObject* bind(PyObject*, PyObject* table) {
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FAST(store), FAST(decode), FAST(prefill), FAST(fresh), FAST(prologue),
                           FAST(store4), FAST(load4), FAST(decode4), FAST(prefill4),
-                          FAST(copy_blocks), FAST(compact_blocks),
+                          FAST(copy_blocks), FAST(compact_blocks), FAST(shared), FAST(track),
+                          FAST(window), FAST(choose), FAST(evict),
                           {"bind", bind, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 

@@ -58,6 +58,11 @@ def fp8_shared_prefix_decode_attention(
     sequence.  The launch depends on shapes and ``max_prefix_len`` alone, so the
     call can be captured in a HIP graph.
     """
+    res = _lib.fast.shared(query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens,
+                           block_tables, softmax_scale, cu_groups, prefix_lens, max_prefix_len,
+                           out)
+    if res is not None:
+        return res
     what = "fp8_shared_prefix_decode_attention"
     query = _lib.aligned(query)
     cache_seqlens, block_tables = cache_seqlens.contiguous(), block_tables.contiguous()

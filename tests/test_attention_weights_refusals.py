@@ -141,5 +141,6 @@ def test_workspaces_follow_the_shapes():
     # the largest tables: no scores in memory
     wide = lib.mskv_decode_weights_workspace_bytes(256, 32, 8, 256, 512)
     assert wide < 256 * 32 * 512 * 256 * 4
-    assert lib.mskv_window_weights_workspace_bytes(32, 1000, 32, 256, 128) == 32 * 32 * 5 * 4
-    assert lib.mskv_window_weights_workspace_bytes(32, 0, 32, 256, 2) == 32 * 32 * 3 * 4
+    # partials of four and of two tiles, the logarithms, and the tiles of a range
+    assert lib.mskv_window_weights_workspace_bytes(32, 1000, 32, 256, 128) == 32 * 32 * 5 * 4 + 4
+    assert lib.mskv_window_weights_workspace_bytes(32, 0, 32, 256, 2) == 32 * 32 * 3 * 4 + 4
