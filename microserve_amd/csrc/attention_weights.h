@@ -300,6 +300,13 @@ __device__ __forceinline__ void window_query(const uint8_t* q_lds, int rb, int l
   }
 }
 
+// A row's place in the partials: a kv head's rows side by side, so that they are
+// read 64 at a time.
+__device__ __forceinline__ int64_t window_row(const WindowArgs& a, const WindowSeq& w, int kvh,
+                                              int row) {
+  return ((int64_t)kvh * a.total_q + w.q_begin) * a.group + row;
+}
+
 // The log-sum-exp of each of 128 rows over the workgroup's range of keys.
 // S^T = K . Q^T: a lane holds 16 keys of one row, for which it keeps a running
 // maximum and sum of its own; they meet at the end.
@@ -353,12 +360,13 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_lse_kernel(WindowArgs a
           window_query<T>(q_lds, rb, lane, qop);
           f32x4 x[4];
 #pragma unroll
-          for (int kg = 0; kg < 4; ++kg) {
-            x[kg] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int kg = 0; kg < 4; ++kg) x[kg] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[kg] = A::mfma(kop[kg][j], qop[j], x[kg]);
-            x[kg] *= ksc[kg];
-          }
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int kg = 0; kg < 4; ++kg) x[kg] = A::mfma(kop[kg][j], qop[j], x[kg]);
+#pragma unroll
+          for (int kg = 0; kg < 4; ++kg) x[kg] *= ksc[kg];
           if (!all) {
             const int lim = min(s_lim[16 * rb + n] - k0, valid);
 #pragma unroll
@@ -403,25 +411,54 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_lse_kernel(WindowArgs a
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) sum += s_l[i][tid] * exp2_fast(s_m[i][tid] - ref);
-  const int row = row0 + tid;
-  const int qi = row / a.group;
-  const int64_t at = (int64_t)(w.q_begin + qi) * a.hq + kvh * a.group + (row - qi * a.group);
-  a.part[at * a.ranges + range.index] = partial_lse(top, sum);
+  a.part[range.index * (a.total_q * a.hq) + window_row(a, w, kvh, row0 + tid)] =
+      partial_lse(top, sum);
 }
 
-// lse[row] from the ranges that hold keys; +inf where no key is seen.
-// One wave a row; grid (rows of the query tensor / 4, sequences)
-constexpr int kWinMergeRows = 4;
-__global__ __launch_bounds__(64 * kWinMergeRows) void window_merge_kernel(WindowArgs a) {
-  const WindowSeq w = window_seq(a, blockIdx.y);
-  const int local = blockIdx.x * kWinMergeRows + (threadIdx.x >> 6);
-  // (row `local` of the sequence: query local / hq, q head local % hq)
-  if (local >= w.rows / a.group * a.hq || w.lk == 0) return;
-  const int64_t at = (int64_t)w.q_begin * a.hq + local;
+// A row's log-sum-exp from the ranges that hold keys, by kThreads neighbouring
+// lanes; +inf where no key is seen.
+template <int kThreads>
+__device__ __forceinline__ float window_row_lse(const WindowArgs& a, const WindowSeq& w, int64_t at,
+                                                int lane) {
+  constexpr int kBatch = 16;  // loads in flight a lane
+  const int64_t stride = a.total_q * a.hq;
   const int keys = *a.per * kWinTile;
   const int n = min(a.ranges, (w.lk + keys - 1) / keys);
-  const float lse = merged_lse(a.part + at * a.ranges, n, threadIdx.x & 63);
-  if ((threadIdx.x & 63) == 0) a.lse[at] = lse;
+  float m = -INFINITY, l = 0.0f;
+  for (int base = lane; base < n; base += kBatch * kThreads) {
+    float x[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) x[i] = a.part[at + min(base + i * kThreads, n - 1) * stride];
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      x[i] = base + i * kThreads < n ? x[i] : -INFINITY;
+      top = fmaxf(top, x[i]);
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    l *= exp2_fast(m - ref);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) l += exp2_fast(x[i] - ref);
+    m = top;
+  }
+#pragma unroll
+  for (int d = 1; d < kThreads; d *= 2) {
+    const float mo = __shfl_xor(m, d), lo = __shfl_xor(l, d);
+    const float top = fmaxf(m, mo), ref = top == -INFINITY ? 0.0f : top;
+    l = l * exp2_fast(m - ref) + lo * exp2_fast(mo - ref);
+    m = top;
+  }
+  return m == -INFINITY ? INFINITY : m + __log2f(l);
+}
+
+// lse[row], where a sequence has more rows than window_sum_kernel holds at once:
+// grid (rows of a kv head / 256 x kv heads, sequences)
+__global__ __launch_bounds__(kWinThreads) void window_merge_kernel(WindowArgs a) {
+  const WindowSeq w = window_seq(a, blockIdx.y);
+  const int kvh = blockIdx.x % a.hk, row = blockIdx.x / a.hk * kWinThreads + threadIdx.x;
+  if (w.rows <= 2 * kWinRows || row >= w.rows || w.lk == 0) return;
+  const int64_t at = window_row(a, w, kvh, row);
+  a.lse[at] = window_row_lse<1>(a, w, at, 0);
 }
 
 // The sums over the rows of 2^(score - lse) at the workgroup's range of keys.
@@ -445,10 +482,15 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
   const int from = max(a.starts ? a.starts[s] : a.start, 0);
   auto rows = [&](int row0) {
     window_rows<kRows>(a, w, kvh, row0, q_lds, s_lim);
-    if (tid < kRows) {
-      const int row = row0 + tid, qi = row / a.group;
-      const int64_t at = (int64_t)(w.q_begin + qi) * a.hq + kvh * a.group + (row - qi * a.group);
-      s_lse[tid] = row < w.rows ? a.lse[at] : INFINITY;
+    if (w.rows > kRows) {
+      const int row = row0 + tid;
+      if (tid < kRows) s_lse[tid] = row < w.rows ? a.lse[window_row(a, w, kvh, row)] : INFINITY;
+    } else {
+      constexpr int kOf = kWinThreads / kRows;
+      const int row = tid / kOf;
+      const float lse = row < w.rows
+          ? window_row_lse<kOf>(a, w, window_row(a, w, kvh, row), tid % kOf) : INFINITY;
+      if (tid % kOf == 0) s_lse[row] = lse;
     }
   };
   const int first = range.index * range.per * kWinTile;
@@ -533,13 +575,14 @@ static hipError_t launch_window(const WindowArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(window_lse_kernel<T>, grid(units), dim3(kWinThreads), 0, st, a, units);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t local = (int64_t)a.rows / a.group * a.hq;
-    hipLaunchKernelGGL(window_merge_kernel,
-                       dim3((unsigned)((local + kWinMergeRows - 1) / kWinMergeRows),
-                            (unsigned)a.num_seqs),
-                       dim3(64 * kWinMergeRows), 0, st, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (a.rows > 2 * kWinRows) {
+      hipLaunchKernelGGL(window_merge_kernel,
+                         dim3((unsigned)((a.rows + kWinThreads - 1) / kWinThreads * a.hk),
+                              (unsigned)a.num_seqs),
+                         dim3(kWinThreads), 0, st, a);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
   }
   if (a.rows <= kWinRows)
     hipLaunchKernelGGL((window_sum_kernel<T, kWinRows>), grid(a.hk), dim3(kWinThreads), 0, st, a);
