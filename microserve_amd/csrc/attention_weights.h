@@ -155,6 +155,7 @@ struct WindowArgs {
   int64_t total_q, num_blocks;
   float scale_log2;
   int num_seqs, hq, hk, group, bs, w, start, ranges, rows;
+  Divider by_group;
   bool add, set_new;
 };
 
@@ -268,25 +269,43 @@ __device__ __forceinline__ void window_operand(const WindowLoads& x,
   }
 }
 
-// Stages kRows rows of a kv head from row0 on into LDS (256-byte rows, 16-byte
-// chunks XOR-swizzled by the row; zeros past the last one), with each row's
-// number of visible keys.
-template <int kRows>
-__device__ __forceinline__ void window_rows(const WindowArgs& a, const WindowSeq& w, int kvh,
-                                            int row0, uint8_t* q_lds, int* s_lim) {
+// 128 rows of a kv head from row0 on, on their way into LDS: all the loads
+// before the first wait (a load and its store row by row took 22 and 31 us of
+// window_32k's two kernels).  In LDS rows of 256 bytes, 16-byte chunks
+// XOR-swizzled by the row, zeros past the last one; and each row's number of
+// visible keys.
+struct WindowRows {
+  static constexpr int kEach = kWinRows * 16 / kWinThreads;
+  u32x4 v[kEach];
+  int lim[kEach];
+  __device__ __forceinline__ void load(const WindowArgs& a, const WindowSeq& w, int kvh, int row0) {
+    const int c = threadIdx.x & 15;
+    const uint16_t* q = a.q + ((int64_t)w.q_begin * a.hq + kvh * a.group) * kHeadDim + 8 * c;
 #pragma unroll
-  for (int i = 0; i < kRows * 16 / kWinThreads; ++i) {
-    const int r = (i * kWinThreads + threadIdx.x) >> 4, c = threadIdx.x & 15;
-    const int row = row0 + r;
-    const int qi = row / a.group, h = row - qi * a.group;
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (row < w.rows)
-      v = *reinterpret_cast<const u32x4*>(
-          a.q + ((int64_t)(w.q_begin + qi) * a.hq + kvh * a.group + h) * kHeadDim + 8 * c);
-    *reinterpret_cast<u32x4*>(q_lds + r * 256 + 16 * (c ^ (r & 15))) = v;
-    if (c == 0) s_lim[r] = row < w.rows ? w.lk - w.lq + qi + 1 : 0;
+    for (int i = 0; i < kEach; ++i) v[i] = u32x4{0u, 0u, 0u, 0u}, lim[i] = 0;
+    if (row0 >= w.rows) return;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int row = min(row0 + ((i * kWinThreads + (int)threadIdx.x) >> 4), w.rows - 1);
+      const int qi = a.by_group(row);
+      v[i] = *reinterpret_cast<const u32x4*>(
+          q + (row + (int64_t)qi * (a.hq - a.group)) * kHeadDim);
+      lim[i] = w.lk - w.lq + qi + 1;
+    }
   }
-}
+  __device__ __forceinline__ void store(const WindowSeq& w, int row0, uint8_t* q_lds,
+                                        int* s_lim) const {
+    const int c = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int r = (i * kWinThreads + threadIdx.x) >> 4;
+      const bool ok = row0 + r < w.rows;
+      *reinterpret_cast<u32x4*>(q_lds + r * 256 + 16 * (c ^ (r & 15))) =
+          ok ? v[i] : u32x4{0u, 0u, 0u, 0u};
+      if (c == 0) s_lim[r] = ok ? lim[i] : 0;
+    }
+  }
+};
 template <typename T>
 __device__ __forceinline__ void window_query(const uint8_t* q_lds, int rb, int lane,
                                              typename Act<T>::x8 (&qop)[4]) {
@@ -331,11 +350,15 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_lse_kernel(WindowArgs a
   if (row0 >= w.rows) return;
   const int first = range.index * range.per * kWinTile;
   const int end = min(w.lk, first + range.per * kWinTile);
+  WindowRows q;
+  q.load(a, w, kvh, row0);
   WindowLoads next;
   window_load(a, s, kvh, first + 64 * wave, w.lk, lane, next);
-  window_rows<kWinRows>(a, w, kvh, row0, q_lds, s_lim);
+  q.store(w, row0, q_lds, s_lim);
   __syncthreads();
   const int blocks = (min(kWinRows, w.rows - row0) + 15) / 16;
+  int index = range.index;
+  asm("" : "+v"(index));  // (kept in a vector register: the scalar ones are short)
   float m[kBlocks], l[kBlocks];
 #pragma unroll
   for (int rb = 0; rb < kBlocks; ++rb) m[rb] = -INFINITY, l[rb] = 0.0f;
@@ -411,7 +434,7 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_lse_kernel(WindowArgs a
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) sum += s_l[i][tid] * exp2_fast(s_m[i][tid] - ref);
-  a.part[range.index * (a.total_q * a.hq) + window_row(a, w, kvh, row0 + tid)] =
+  a.part[index * (a.total_q * a.hq) + window_row(a, w, kvh, row0 + tid)] =
       partial_lse(top, sum);
 }
 
@@ -425,10 +448,14 @@ __device__ __forceinline__ float window_row_lse(const WindowArgs& a, const Windo
   const int keys = *a.per * kWinTile;
   const int n = min(a.ranges, (w.lk + keys - 1) / keys);
   float m = -INFINITY, l = 0.0f;
+  const float* p = a.part + at + min(lane, max(n - 1, 0)) * stride;
   for (int base = lane; base < n; base += kBatch * kThreads) {
     float x[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) x[i] = a.part[at + min(base + i * kThreads, n - 1) * stride];
+    for (int i = 0; i < kBatch; ++i) {
+      x[i] = *p;
+      p += base + (i + 1) * kThreads < n ? kThreads * stride : 0;
+    }
     float top = m;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -480,8 +507,8 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
   const int s = range.s;
   const WindowSeq w = window_seq(a, s);
   const int from = max(a.starts ? a.starts[s] : a.start, 0);
-  auto rows = [&](int row0) {
-    window_rows<kRows>(a, w, kvh, row0, q_lds, s_lim);
+  WindowRows q;
+  auto rows = [&](int row0) {  // into LDS (the first 128 are in q), with their log-sum-exps
     if (w.rows > kRows) {
       const int row = row0 + tid;
       if (tid < kRows) s_lse[tid] = row < w.rows ? a.lse[window_row(a, w, kvh, row)] : INFINITY;
@@ -492,9 +519,16 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
           ? window_row_lse<kOf>(a, w, window_row(a, w, kvh, row), tid % kOf) : INFINITY;
       if (tid % kOf == 0) s_lse[row] = lse;
     }
+    q.store(w, row0, q_lds, s_lim);
+#pragma unroll
+    for (int more = kWinRows; more < kRows; more += kWinRows) {
+      q.load(a, w, kvh, row0 + more);
+      q.store(w, row0 + more, q_lds + 256 * more, s_lim + more);
+    }
   };
   const int first = range.index * range.per * kWinTile;
   const int end = min(w.lk, first + range.per * kWinTile);
+  q.load(a, w, kvh, 0);
   WindowLoads next;
   window_load(a, s, kvh, first + 64 * wave, w.lk, lane, next);
   rows(0);
@@ -514,32 +548,41 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
     const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;  // every row sees every key
     for (int row0 = 0; row0 < w.rows; row0 += kRows) {
       if (w.rows > kRows && (row0 > 0 || t0 > first)) {
+        q.load(a, w, kvh, row0);
         __syncthreads();
         rows(row0);
         __syncthreads();
       }
       if (valid == 0) continue;
       const int blocks = (min(kRows, w.rows - row0) + 15) / 16;
-      for (int rb = 0; rb < blocks; ++rb) {
+      auto add_block = [&](int rb, bool masked) {
         typename A::x8 qop[4];
         window_query<T>(q_lds, rb, lane, qop);
         const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[16 * rb + 4 * g]);
+        f32x4 x[4];
+#pragma unroll
+        for (int kg = 0; kg < 4; ++kg) x[kg] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int kg = 0; kg < 4; ++kg) x[kg] = A::mfma(qop[j], kop[kg][j], x[kg]);
 #pragma unroll
         for (int kg = 0; kg < 4; ++kg) {
-          f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x = A::mfma(qop[j], kop[kg][j], x);
+          const int key = 16 * kg + n;
           f32x4 p;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) p[r] = exp2_fast(fmaf(x[r], ksc[kg], -lse[r]));
-          if (!all) {
-            const int key = 16 * kg + n;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (!(key < valid && k0 + key < s_lim[16 * rb + 4 * g + r])) p[r] = 0.0f;
+          for (int r = 0; r < 4; ++r) {
+            p[r] = exp2_fast(fmaf(x[kg][r], ksc[kg], -lse[r]));
+            if (masked && !(key < valid && k0 + key < s_lim[16 * rb + 4 * g + r])) p[r] = 0.0f;
           }
           sum[kg] += (p[0] + p[1]) + (p[2] + p[3]);
         }
+      };
+      if (all) {
+#pragma unroll 2
+        for (int rb = 0; rb < blocks; ++rb) add_block(rb, false);
+      } else {
+        for (int rb = 0; rb < blocks; ++rb) add_block(rb, true);
       }
     }
 #pragma unroll
@@ -669,6 +712,7 @@ static int window_checked(
   a.hq = num_q_heads;
   a.hk = num_kv_heads;
   a.group = group;
+  a.by_group = divider_of(group);
   a.bs = block_size;
   a.w = max_blocks_per_seq;
   a.rows = total_q > 0 ? (int)std::min<int64_t>(rows, total_q * group) : 0;

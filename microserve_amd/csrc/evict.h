@@ -26,20 +26,6 @@
 
 namespace mskv {
 
-// Division of 0 <= x < 2^31 by a constant of the launch.
-struct Divider {
-  uint32_t magic;
-  int d, shift;
-  __device__ __forceinline__ int operator()(int x) const {
-    return (int)((__umulhi(magic, (uint32_t)x) + (uint32_t)x) >> shift);
-  }
-};
-static Divider divider_of(int d) {
-  int shift = 0;
-  while ((1LL << shift) < d) ++shift;
-  return {(uint32_t)(((1ULL << 32) * ((1ULL << shift) - d)) / d + 1), d, shift};
-}
-
 constexpr int kSelectBins = 2048;
 
 struct SelectArgs {

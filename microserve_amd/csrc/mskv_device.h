@@ -149,6 +149,20 @@ __device__ __forceinline__ f16x8 fp8x8_to_f16(uint32_t w0, uint32_t w1) {
   return r;
 }
 
+// Division of 0 <= x < 2^31 by a constant of the launch.
+struct Divider {
+  uint32_t magic;
+  int d, shift;
+  __device__ __forceinline__ int operator()(int x) const {
+    return (int)((__umulhi(magic, (uint32_t)x) + (uint32_t)x) >> shift);
+  }
+};
+static Divider divider_of(int d) {
+  int shift = 0;
+  while ((1LL << shift) < d) ++shift;
+  return {(uint32_t)(((1ULL << 32) * ((1ULL << shift) - d)) / d + 1), d, shift};
+}
+
 // largest power of two <= x, for a positive normal x
 __device__ __forceinline__ float pow2_floor(float x) {
   return __uint_as_float(__float_as_uint(x) & 0xFF800000u);
