@@ -11,6 +11,13 @@ norms, rotary embedding and the store fused into one launch.
 
 With ``kv_cache_dtype`` ``"fp4_e2m1"`` the injected caches are the 4-bit ones
 (``allocate_fp4_kvcache``) and ``forward`` does the same over them.
+
+Over an FP8 cache a decode step also keeps its tokens' attention weights where
+``attention_weights`` was injected (``allocate_attention_weights``; the tokens
+before ``attention_weights_start`` are left out), and reads prefixes that
+sequences share once where the ``Context`` names groups
+(``fp8_shared_prefix_decode_attention``).  With both the weights go first: they
+are sums over the tokens of each sequence by itself.
 """
 
 from __future__ import annotations
@@ -18,6 +25,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from microserve_amd.attention_weights import fp8_decode_attention_weights
 from microserve_amd.context import AttentionMode, get_context
 from microserve_amd.fp4_attention import fp4_chunk_prefill_attention, fp4_decode_attention
 from microserve_amd.fp4_kv_cache import store_fp4_kvcache
@@ -25,6 +33,7 @@ from microserve_amd.fp8_chunk_prefill_attention import fp8_chunk_prefill_attenti
 from microserve_amd.fp8_decode_attention import fp8_decode_attention
 from microserve_amd.fp8_kv_cache import store_fp8_kvcache
 from microserve_amd.qk_norm_rope import qk_norm_rope_store
+from microserve_amd.shared_prefix import fp8_shared_prefix_decode_attention
 from microserve_amd.varlen_attention import varlen_attention
 
 
@@ -44,6 +53,8 @@ class Attention(nn.Module):
         self.k_cache = self.v_cache = torch.tensor([])
         self.k_scale_cache = self.v_scale_cache = None
         self.kv_cache_dtype = FP8
+        self.attention_weights = None
+        self.attention_weights_start = 0
 
     def _check_cache(self):
         assert self.k_cache.numel(), "k_cache was not injected: allocate the KV cache first"
@@ -84,6 +95,8 @@ class Attention(nn.Module):
         k_cache, v_cache = self.k_cache, self.v_cache
         four = self.kv_cache_dtype == FP4
         if ctx.mode is AttentionMode.DECODE:
+            if self.attention_weights is not None or ctx.cu_groups is not None:
+                return self._attend_more(ctx, q)
             return (fp4_decode_attention if four else fp8_decode_attention)(
                 q, k_cache, v_cache, self.k_scale_cache, self.v_scale_cache,
                 ctx.cache_seqlens, ctx.block_tables, self.scale)
@@ -99,3 +112,18 @@ class Attention(nn.Module):
                 q, k_cache, v_cache, self.k_scale_cache, self.v_scale_cache,
                 ctx.block_tables, ctx.prefix_len, self.scale)
         raise RuntimeError(f"unsupported attention mode: {ctx.mode}")
+
+    def _attend_more(self, ctx, q):
+        """A decode step that keeps weights or reads shared prefixes once."""
+        if self.kv_cache_dtype != FP8:
+            raise NotImplementedError(
+                f"attention weights and shared prefixes need an {FP8} cache, not "
+                f"{self.kv_cache_dtype}")
+        cache = (self.k_cache, self.v_cache, self.k_scale_cache, self.v_scale_cache)
+        if self.attention_weights is not None:
+            return fp8_decode_attention_weights(
+                q, *cache, ctx.cache_seqlens, ctx.block_tables, self.scale,
+                self.attention_weights, self.attention_weights_start)
+        return fp8_shared_prefix_decode_attention(
+            q, *cache, ctx.cache_seqlens, ctx.block_tables, self.scale, ctx.cu_groups,
+            ctx.prefix_lens, ctx.max_prefix_len)

@@ -3,7 +3,9 @@
 The runner builds one ``Context`` per forward pass and installs it globally;
 ``Attention.forward`` reads it (``context.py:8-43``).  Field names and
 defaults are the reference's: ``cache_seqlens`` is the per-sequence context
-length and ``block_tables`` is int32, -1 padded.
+length and ``block_tables`` is int32, -1 padded.  The last three, of a decode
+step whose sequences share prefixes, are this library's own
+(``group_by_prefix``'s results and a bound of the prefixes' lengths).
 """
 
 from __future__ import annotations
@@ -39,6 +41,10 @@ class Context:
     slot_mapping: torch.Tensor | None = None
 
     block_tables: torch.Tensor | None = None
+
+    cu_groups: torch.Tensor | None = None
+    prefix_lens: torch.Tensor | None = None
+    max_prefix_len: int | None = None
 
 
 def get_context() -> Context:
