@@ -302,7 +302,8 @@ __global__ __launch_bounds__(kThreads) void evict_kv_tokens_kernel(EvictArgs a) 
   const int b = blockIdx.y;
   const int32_t* table = a.bt + (int64_t)b * a.w;
   const int32_t* kept = a.kept + (int64_t)b * a.hk * a.budget;
-  const int n = min(__builtin_amdgcn_readfirstlane(a.lens[b]), a.budget);
+  // (places past the table have no slots)
+  const int n = min(min(__builtin_amdgcn_readfirstlane(a.lens[b]), a.budget), a.w * a.bs);
   if (n <= 0) return;
   int unit = blockIdx.x;
 

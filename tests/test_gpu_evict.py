@@ -114,6 +114,32 @@ def test_evict_without_weights_leaves_them_and_invalid_pages_are_skipped():
     _evict(gen, [600, 600, 600], 2, 128, 300, 10, 0, spoil=spoil)
 
 
+def test_evict_of_lengths_past_the_table():
+    """More places than the pages have: those behind the last page are left out."""
+    gen = torch.Generator().manual_seed(9)
+    block, heads, cap = 128, 2, 256
+    host, dev = H.pool(gen, 6, heads, block)
+    tables = H.tables_of(gen, [cap, cap], block, 6)
+    kept = np.full((2, heads, 700), -1, np.int32)
+    kept[0, :, :cap - 3] = np.arange(3, cap)
+    kept[1, :, :600] = np.arange(600)
+    kept[1, 1, 100:cap] = np.minimum(np.arange(100, cap) + 7, cap + 5)
+    M.evict_kv_tokens(*dev, H.gpu(kept), H.gpu([700, 600]), H.gpu(tables))
+    torch.cuda.synchronize()
+    for b in range(2):
+        now = kept[b, :, :cap].copy()
+        now[now >= cap] = -1
+        for h in range(heads):
+            moved = np.flatnonzero((now[h] >= 0) & (now[h] != np.arange(cap)))
+            src, dst = now[h][moved], moved
+            slot = lambda t: tables[b][t // block] * block + t % block
+            for x in host:
+                rows = x.reshape(6 * block, heads, -1)
+                rows[slot(dst), h] = rows[slot(src), h]
+    for got, want in zip(H.to_cpu(dev), host):
+        assert got.tobytes() == want.tobytes()
+
+
 def test_evict_of_rows_past_32_bits_of_bytes():
     """A pool of 4.3 GB a cache, the sequence's pages at its ends."""
     gen = torch.Generator().manual_seed(6)
