@@ -492,7 +492,9 @@ __global__ __launch_bounds__(64) void shared_merge_kernel(SharedArgs s) {
   const DecodeArgs& a = s.d;
   const int row = blockIdx.x;
   const int lane = threadIdx.x, j = lane >> 5, i = lane & 31;
-  const int n = s.counts[row / a.hq];
+  // (boundaries that do not ascend may leave a sequence without an item, and its
+  // count unwritten)
+  const int n = min(s.counts[row / a.hq], a.splits);
   if (n < 0) return;
   const float* lse = a.part_lse + (int64_t)row * a.splits;
   const float* po = a.part_o + (int64_t)row * a.splits * kHeadDim + 4 * i;

@@ -114,6 +114,20 @@ def test_padding_sequences_and_groups():
     _check(gen, [0] * 9, tables, pool, [9], [512], 16, 4, 256, torch.float16)
 
 
+def test_groups_that_do_not_ascend_end():
+    """No result is promised; every read stays inside, and the next call is right."""
+    gen = torch.Generator().manual_seed(21)
+    sizes, prefixes = [3, 4], [256, 512]
+    lens, tables, pool = _batch(gen, sizes, prefixes, range(20, 27), 128)
+    _, args = _check(gen, lens, tables, pool, sizes, prefixes, 8, 2, 128, torch.float16)
+    want = M.fp8_shared_prefix_decode_attention(*args, H.gpu([0, 3, 7]), H.gpu(prefixes))
+    for cu in ([7, 3, 0], [0, 7, 3], [5, 5, 5], [-9, 99, 2], [3, 0, 7]):
+        M.fp8_shared_prefix_decode_attention(*args, H.gpu(cu), H.gpu(prefixes))
+        torch.cuda.synchronize()
+    got = M.fp8_shared_prefix_decode_attention(*args, H.gpu([0, 3, 7]), H.gpu(prefixes))
+    assert torch.equal(got, want)
+
+
 def test_invalid_pages_are_skipped():
     def spoil(tables):
         tables[:3, 1] = -1      # of a prefix
