@@ -6,10 +6,15 @@
 //    leaves each score in memory, 4 bytes a (q head, token), and the splits'
 //    log-sum-exps; this kernel adds 2^(score - lse) over a kv head's q heads.
 //    HBM-bound: the scores are 8 bytes a q head and token (written and read
-//    once), 32 at a group of four, where reading K again for them is 132.
+//    once), 32 at a group of four, where reading K again for them is 132.  64 x
+//    4096 tokens of 32 heads: 50 MB, 14 us.
 //  * The last queries of prompts (window_lse_kernel, window_sum_kernel): many
 //    rows a kv head, whose scores would be more bytes than K.  The scores are
-//    computed twice, first for each row's log-sum-exp, then for the sums.
+//    computed twice, first for each row's log-sum-exp, then for the sums.  32
+//    queries over 32768 tokens at 32 heads over 8 (8.6 GFLOP a pass): 20 and 26
+//    us, a SIMD's vector instructions (exponentials, the running maxima) about
+//    half of it and the matrix products a fifth; the rest is the chain of lengths,
+//    table and first tile at the start and the arrival of K, 33 MB from HBM.
 #pragma once
 
 namespace mskv {
@@ -193,8 +198,8 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowArgs& a, int s) {
 // workgroups that run at once, from the lengths (`units` workgroups take a range:
 // kv heads, turns of rows), and the ranges with keys come first in the grid.
 // (By sequence and chunk, with a grid as wide as the longest one, workgroups
-// without keys leave the others on a fraction of the CUs: 8 sequences of 20 to
-// 8192 tokens 63 us where eight of 8192 take 75.)
+// without keys left the others on a fraction of the CUs: 8 sequences of 20 to
+// 8192 tokens took 63 us where eight of 8192 took 75.)
 struct WindowRange {
   int s, index, per;  // the sequence (-1: none), its range, tiles of a range
 };
@@ -270,8 +275,8 @@ __device__ __forceinline__ void window_operand(const WindowLoads& x,
 }
 
 // 128 rows of a kv head from row0 on, on their way into LDS: all the loads
-// before the first wait (a load and its store row by row took 22 and 31 us of
-// window_32k's two kernels).  In LDS rows of 256 bytes, 16-byte chunks
+// before the first wait (row by row, each load waited for before the next, the
+// two kernels took 22 and 31 us where they take 20 and 26).  In LDS rows of 256 bytes, 16-byte chunks
 // XOR-swizzled by the row, zeros past the last one; and each row's number of
 // visible keys.
 struct WindowRows {

