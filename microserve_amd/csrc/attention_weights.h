@@ -209,10 +209,9 @@ __device__ __forceinline__ WindowRange window_range(const WindowArgs& a, int ite
     return s < a.num_seqs ? (window_keys_of(a, s) + kWinTile - 1) / kWinTile : 0;
   };
   const int own = tiles_of(lane);
-  int64_t total = own;
+  int total = own;  // (the host keeps the sum within an int)
   for (int s = 64 + lane; s < a.num_seqs; s += 64) total += tiles_of(s);
-  int tiles = (int)min(total, (int64_t)1 << 24);
-  tiles = __builtin_amdgcn_readfirstlane(wave_sum_i32(tiles));
+  const int tiles = __builtin_amdgcn_readfirstlane(wave_sum_i32(total));
   WindowRange r = {-1, 0, 0};
   r.per = max(1, (int)(((int64_t)tiles * units + kWinSlots - 1) / kWinSlots));
   for (int base = 0; base < a.num_seqs; base += 64) {
@@ -686,7 +685,7 @@ static int window_checked(
   // (the launches' workgroups, and the sum of the tiles, stay within an int)
   if (num_seqs > 65535 || total_q > 0x7FFFFFFFLL || rows > 0x7FFFFFFFLL ||
       (num_seqs + kWinSlots) * turns * num_kv_heads > 0x7FFFFF ||
-      (int64_t)num_seqs * max_blocks_per_seq * block_size / kWinTile > 0x7FFFFFFF)
+      num_seqs * ((int64_t)max_blocks_per_seq * block_size / kWinTile + 1) > 0x7FFFFFFF)
     return MSKV_EUNSUPPORTED;
   if (num_seqs == 0) return MSKV_OK;
   if (!k_cache || !k_scale_cache || !block_tables || !cu_seqlens_k || !weights)

@@ -163,6 +163,18 @@ def test_window_weights(new, lens, hq, hk, block, width, dtype, accumulate):
     _window_case(sum(lens) + hq, new, lens, hq, hk, block, dtype, accumulate, width)
 
 
+@pytest.mark.parametrize("group", [4, 13])
+def test_window_weights_of_many_sequences(group):
+    """More sequences than a wave has lanes, some without queries, some without
+    tokens; rows of one turn and of several side by side."""
+    rng = np.random.default_rng(group)
+    lens = [int(x) for x in rng.integers(0, 300, 90)]
+    lens[7], lens[70] = 2000, 1300
+    new = [int(rng.integers(0, min(n, 40) + 1)) for n in lens]
+    new[7], new[70] = 33, 1
+    _window_case(group, new, lens, 2 * group, 2, 128, torch.bfloat16, False, 0)
+
+
 def test_window_weights_from_a_start_and_without_a_bound():
     _window_case(3, [8, 8], [600, 300], 8, 2, 256, torch.bfloat16, True, start=290, max_k=False)
     _window_case(4, [8], [600], 8, 2, 256, torch.float16, False, start=10 ** 6)

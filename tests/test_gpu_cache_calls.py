@@ -149,3 +149,86 @@ def test_arguments_of_other_layouts_go_to_the_wrapper():
     assert torch.equal(
         M.fp8_shared_prefix_decode_attention(off, *cache, l2, t2, SCALE, groups, prefix),
         M.fp8_shared_prefix_decode_attention(q, *cache, lens, tables, SCALE, groups, prefix))
+
+
+def test_captured_run_replays():
+    """A turn's window weights, a decode step that keeps weights, the choice and the
+    moving in one graph: each replay, over lengths and caches of its own, is the
+    eager run."""
+    gen = torch.Generator().manual_seed(12)
+    heads, block, scale = 2, 128, 0.1
+    _, pool = H.pool(gen, 16, heads, block)
+    tables = H.gpu(H.tables_of(gen, [512, 640, 384], block, 16))
+    q = torch.randn(3, 8, 128, generator=gen).half().to(H.DEV)
+    qw = torch.randn(24, 8, 128, generator=gen).half().to(H.DEV)
+    cu_q = H.gpu([0, 10, 10, 24])
+    lens, cu_k = H.gpu([1, 1, 1]), H.gpu([0, 1, 2, 3])
+    cache, w = [t.clone() for t in pool], torch.zeros(16, heads, block, device=H.DEV)
+
+    def run(c, x):
+        M.fp8_window_attention_weights(qw, c[0], c[2], tables, cu_q, cu_k, 14, scale, x)
+        out = M.fp8_decode_attention_weights(q, *c, lens, tables, scale, x, 3)
+        kept, n = M.select_kv_tokens(x, lens, tables, 200, 20, 3)
+        M.evict_kv_tokens(*c, kept, n, tables, x)
+        return out, kept, n
+
+    def fill(n):
+        lens.copy_(H.gpu(n))
+        cu_k.copy_(H.gpu(np.cumsum([0, *n])))
+
+    def bytes_of(c):
+        return [t.view(torch.uint8) if t.element_size() == 1 else t for t in c]
+
+    fill([500, 600, 300])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run([t.clone() for t in pool], w.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(cache, w)
+    for n in ([500, 600, 300], [20, 0, 384], [512, 640, 1], [201, 200, 199]):
+        fill(n)
+        for mine, start in zip(bytes_of(cache), bytes_of(pool)):
+            mine.copy_(start)
+        w.fill_(0.25)
+        copy, x = [t.clone() for t in pool], w.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(copy, x)
+        torch.cuda.synchronize()
+        for a, b in zip([*got, w, *bytes_of(cache)], [*want, x, *bytes_of(copy)]):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    """Runs of the operators side by side, each with workspaces of its own."""
+    runs = []
+    for i in range(2):
+        gen = torch.Generator().manual_seed(30 + i)
+        lens = [2000 + 300 * i, 900]
+        _, cache = H.pool(gen, 28, 2, 128)
+        tables = H.gpu(H.tables_of(gen, lens, 128, 28))
+        q = torch.randn(2, 16, 128, generator=gen).to(H.DEV, torch.bfloat16)
+        runs.append((q, cache, H.gpu(lens), tables, H.gpu(np.cumsum([0, *lens])),
+                     torch.rand(28, 2, 128, generator=gen).to(H.DEV)))
+
+    def run(r, x):
+        q, cache, lens, tables, cu_k, _ = r
+        out = M.fp8_decode_attention_weights(q, *cache, lens, tables, SCALE, x)
+        M.fp8_window_attention_weights(q, cache[0], cache[2], tables, H.gpu([0, 1, 2]), cu_k, 1,
+                                       SCALE, x, accumulate=True)
+        return (out, x, *M.select_kv_tokens(x, lens, tables, 300, 7))
+    want = [run(r, r[5].clone()) for r in runs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in runs], [[], []]
+    for _ in range(8):
+        for i, (s, r) in enumerate(zip(streams, runs)):
+            with torch.cuda.stream(s):
+                got[i].append(run(r, r[5].clone()))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        for g in gs:
+            for a, b in zip(w, g):
+                assert torch.equal(a, b)
