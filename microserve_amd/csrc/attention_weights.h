@@ -11,10 +11,10 @@
 //  * The last queries of prompts (window_lse_kernel, window_sum_kernel): many
 //    rows a kv head, whose scores would be more bytes than K.  The scores are
 //    computed twice, first for each row's log-sum-exp, then for the sums.  32
-//    queries over 32768 tokens at 32 heads over 8 (8.6 GFLOP a pass): 20 and 26
-//    us, a SIMD's vector instructions (exponentials, the running maxima) about
-//    half of it and the matrix products a fifth; the rest is the chain of lengths,
-//    table and first tile at the start and the arrival of K, 33 MB from HBM.
+//    queries over 32768 tokens at 32 heads over 8 (8.6 GFLOP a pass): 20 us each.
+//    A workgroup's two tiles take 4 us each, issue-bound (exponentials, running
+//    maxima; the products are a third); 6 to 7 go by before, in the chain of lengths,
+//    table, rows and first tile (17 MB at once), and 3 between the launches.
 #pragma once
 
 namespace mskv {
@@ -275,7 +275,7 @@ __device__ __forceinline__ void window_operand(const WindowLoads& x,
 
 // 128 rows of a kv head from row0 on, on their way into LDS: all the loads
 // before the first wait (row by row, each load waited for before the next, the
-// two kernels took 22 and 31 us where they take 20 and 26).  In LDS rows of 256 bytes, 16-byte chunks
+// two kernels took 22 and 31 us, together 20 and 26).  In LDS rows of 256 bytes, 16-byte chunks
 // XOR-swizzled by the row, zeros past the last one; and each row's number of
 // visible keys.
 struct WindowRows {
@@ -570,14 +570,22 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int kg = 0; kg < 4; ++kg) x[kg] = A::mfma(qop[j], kop[kg][j], x[kg]);
+        // row r sees the keys 16 kg + n with 16 kg < sees[r] (with each limit read and
+        // branched on by itself, the workgroup of a sequence's last keys took 20 us of
+        // its kernel's 28)
+        int sees[4];
+        if (masked) {
+          const u32x4 lim = *reinterpret_cast<const u32x4*>(&s_lim[16 * rb + 4 * g]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sees[r] = min((int)lim[r] - k0, valid) - n;
+        }
 #pragma unroll
         for (int kg = 0; kg < 4; ++kg) {
-          const int key = 16 * kg + n;
           f32x4 p;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             p[r] = exp2_fast(fmaf(x[kg][r], ksc[kg], -lse[r]));
-            if (masked && !(key < valid && k0 + key < s_lim[16 * rb + 4 * g + r])) p[r] = 0.0f;
+            if (masked) p[r] = 16 * kg < sees[r] ? p[r] : 0.0f;
           }
           sum[kg] += (p[0] + p[1]) + (p[2] + p[3]);
         }
@@ -586,6 +594,7 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
 #pragma unroll 2
         for (int rb = 0; rb < blocks; ++rb) add_block(rb, false);
       } else {
+#pragma unroll 2
         for (int rb = 0; rb < blocks; ++rb) add_block(rb, true);
       }
     }
