@@ -671,6 +671,15 @@ extern "C" size_t mskv_window_weights_workspace_bytes(int64_t total_q, int64_t m
 
 namespace mskv {
 
+// (the launches' workgroups, and the sum of the tiles, stay within an int)
+static bool window_fits(int num_seqs, int64_t total_q, int64_t rows, int num_kv_heads,
+                        int block_size, int max_blocks_per_seq) {
+  const int64_t turns = (rows + kWinRows - 1) / kWinRows;
+  return num_seqs <= 65535 && total_q <= 0x7FFFFFFFLL && rows <= 0x7FFFFFFFLL &&
+         (num_seqs + kWinSlots) * turns * num_kv_heads <= 0x7FFFFF &&
+         num_seqs * ((int64_t)max_blocks_per_seq * block_size / kWinTile + 1) <= 0x7FFFFFFF;
+}
+
 // Validates a window call and launches it.  Without cu_seqlens_q: one query a
 // sequence, its length in cu_seqlens_k, the newest token's entry set.
 static int window_checked(
@@ -690,11 +699,7 @@ static int window_checked(
   if ((int64_t)max_blocks_per_seq * block_size >= (1LL << 30)) return MSKV_EUNSUPPORTED;
   const int group = num_q_heads / num_kv_heads;
   const int64_t rows = (int64_t)max_seqlen_q * group;
-  const int64_t turns = (rows + kWinRows - 1) / kWinRows;
-  // (the launches' workgroups, and the sum of the tiles, stay within an int)
-  if (num_seqs > 65535 || total_q > 0x7FFFFFFFLL || rows > 0x7FFFFFFFLL ||
-      (num_seqs + kWinSlots) * turns * num_kv_heads > 0x7FFFFF ||
-      num_seqs * ((int64_t)max_blocks_per_seq * block_size / kWinTile + 1) > 0x7FFFFFFF)
+  if (!window_fits(num_seqs, total_q, rows, num_kv_heads, block_size, max_blocks_per_seq))
     return MSKV_EUNSUPPORTED;
   if (num_seqs == 0) return MSKV_OK;
   if (!k_cache || !k_scale_cache || !block_tables || !cu_seqlens_k || !weights)
@@ -800,7 +805,10 @@ extern "C" int mskv_fp8_decode_attention_weights(
   const int splits = mskv_decode_num_splits(batch, num_q_heads, num_kv_heads, max_blocks_per_seq,
                                             block_size);
   if (!track_scores(batch, num_q_heads, max_blocks_per_seq, block_size)) {
-    if (block_size % 128 != 0) return MSKV_EUNSUPPORTED;
+    // (before the decode is launched)
+    if (block_size % 128 != 0 || !window_fits(batch, batch, num_q_heads / num_kv_heads,
+                                              num_kv_heads, block_size, max_blocks_per_seq))
+      return MSKV_EUNSUPPORTED;
     const int status = decode_checked<Fp8Cache>(
         query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens, block_tables, out,
         batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,

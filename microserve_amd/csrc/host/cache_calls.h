@@ -221,7 +221,8 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     const Dims m = dims_of(*kc);
     const int64_t b = len->numel(), w = bt->size(1), budget = kept->size(2);
-    if (!caches_match(*kc, *vc, *ks, *vs, m.heads, m.d) || !fits({b, m.heads, m.d, m.block, w, budget}) ||
+    if (!caches_match(*kc, *vc, *ks, *vs, m.heads, m.d) ||
+        !fits({b, m.heads, m.d, m.block, w, budget}) ||
         kept->size(0) != b || kept->size(1) != m.heads || bt->size(0) != b ||
         (weights && !weights_of(*weights, m)))
       return nullptr;

@@ -534,10 +534,12 @@ static SharedShape shared_shape(int batch, int groups, int hq, int hk, int w, in
   s.sb = (int)std::max<int64_t>(1, std::min(most, cap / (kMinSplitSteps * kStep)));
   // Items of ranges that all run at once, and of each sequence's and group's
   // last range (a group's last 128 rows may be few; a group needs a sequence)
-  const int64_t blocks = s.max_prefix == 0 ? 0 : std::min<int64_t>(batch, batch / (8 * s.tpr) + groups);
-  const int64_t least = std::min<int64_t>(blocks * s.sa * units, blocks * units + kSharedWorkgroups) +
-                        std::min<int64_t>((int64_t)batch * s.sb * tail_units,
-                                          (int64_t)batch * tail_units + kSharedWorkgroups);
+  const int64_t blocks =
+      s.max_prefix == 0 ? 0 : std::min<int64_t>(batch, batch / (8 * s.tpr) + groups);
+  const int64_t least =
+      std::min<int64_t>(blocks * s.sa * units, blocks * units + kSharedWorkgroups) +
+      std::min<int64_t>((int64_t)batch * s.sb * tail_units,
+                        (int64_t)batch * tail_units + kSharedWorkgroups);
   s.grid = std::min<int64_t>(least, (blocks * units + (int64_t)batch * tail_units) +
                                         kSharedWorkgroups + units + tail_units);
   return s;
@@ -591,7 +593,8 @@ extern "C" int mskv_fp8_shared_prefix_decode_attention(
   if ((int64_t)max_blocks_per_seq * block_size >= (1LL << 30)) return MSKV_EUNSUPPORTED;
   // (sums over the batch of 32-token steps, and the merge's grid, stay within
   // an int)
-  if (num_groups > kSharedMaxGroups || batch > 65535 || num_kv_heads > 1024 || (int64_t)batch * num_q_heads > 0x7FFFFFFF / 64 ||
+  if (num_groups > kSharedMaxGroups || batch > 65535 || num_kv_heads > 1024 ||
+      (int64_t)batch * num_q_heads > 0x7FFFFFFF / 64 ||
       (int64_t)batch * max_blocks_per_seq * block_size / kStep > 0x3FFFFFFF)
     return MSKV_EUNSUPPORTED;
   if (batch == 0) return MSKV_OK;
