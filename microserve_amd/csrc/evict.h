@@ -536,8 +536,12 @@ extern "C" int mskv_evict_kv_tokens(void* k_cache, void* v_cache, float* k_scale
   const dim3 grid((unsigned)(2 * scale_units + (weights ? num_kv_heads : 0) + 2 * row_units),
                   (unsigned)batch);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  // (longer runs where the workgroups are too few to fill the chip)
-  if ((int64_t)grid.x * batch > 256)
+  // Longer runs where the workgroups are too few to fill the chip and the places
+  // are more than four short ones (one to eight sequences at eight heads, 512 / 1024
+  // threads: 256 places 6 / 7.5 us, 1024 9.3 to 10.6 / 9.4 to 10.7, 4096 27 to 37 / 24
+  // to 30).
+  const int64_t places = std::min<int64_t>(budget, (int64_t)max_blocks_per_seq * block_size);
+  if ((int64_t)grid.x * batch > 256 || places <= 1024)
     hipLaunchKernelGGL(evict_kv_tokens_kernel<512>, grid, dim3(512), 0, s, a);
   else
     hipLaunchKernelGGL(evict_kv_tokens_kernel<1024>, grid, dim3(1024), 0, s, a);
