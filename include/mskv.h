@@ -601,8 +601,9 @@ int mskv_fp8_decode_attention_weights(
  * tokens: query i of a sequence with Lq queries and Lk tokens sees positions
  * p < Lk - Lq + i + 1.  The entries of positions [start, Lk) are set, or added
  * to where accumulate is not 0.  max_seqlen_q and max_seqlen_k (0: the tables'
- * width) bound every sequence's queries and tokens: rows past them are not
- * counted.  block_size % 128 == 0, head_dim == 128.
+ * width) bound every sequence's queries and tokens: rows past them, and tokens
+ * past the table, are not counted (Lk above stays the whole length).
+ * block_size % 128 == 0, head_dim == 128.
  */
 size_t mskv_window_weights_workspace_bytes(int64_t total_q,
                                            int64_t max_seqlen_k,

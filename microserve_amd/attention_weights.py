@@ -125,7 +125,8 @@ def fp8_window_attention_weights(
     positions ``< Lk - Lq + i + 1``.  The entries of positions ``start .. Lk``
     are set (with ``accumulate``, added to); returns ``weights``.
     ``max_seqlen_q`` and ``max_seqlen_k`` (default: the tables' width) must be
-    at least every sequence's numbers: what lies past them is not counted.
+    at least every sequence's numbers: what lies past them, or past the table,
+    is not counted (``Lk`` stays the whole length).
     """
     res = _lib.fast.window(query, k_cache, k_scale_cache, block_tables, cu_seqlens_q, cu_seqlens_k,
                            max_seqlen_q, softmax_scale, weights, accumulate, start, max_seqlen_k)

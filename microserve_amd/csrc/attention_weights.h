@@ -160,6 +160,7 @@ struct WindowArgs {
   int64_t total_q, num_blocks;
   float scale_log2;
   int num_seqs, hq, hk, group, bs, w, start, ranges, rows;
+  int most_keys;  // of a sequence: the table's width or the caller's bound
   Divider by_group;
   bool add, set_new;
 };
@@ -170,14 +171,18 @@ constexpr int kWinRows = 128;  // (query, q head of the group) rows of a turn
 // Workgroups that should run at once, two a CU
 constexpr int kWinSlots = 512;
 
-// A sequence's queries and keys, clamped to the tensors.
+// A sequence's queries and keys, clamped to the tensors.  What query 0 sees of
+// the past, lk - lq, follows the whole length: keys past the table or the bound
+// are not counted, but the queries stay where they are.  (Without cu_q the
+// length is the table's at most, as the decode takes it.)
 struct WindowSeq {
-  int q_begin, lq, lk, rows;
+  int q_begin, lq, lk, rows, past;
 };
+__device__ __forceinline__ int window_length(const WindowArgs& a, int s) {
+  return a.cu_q ? a.cu_k[s + 1] - a.cu_k[s] : min(a.cu_k[s], a.w * a.bs);
+}
 __device__ __forceinline__ int window_keys_of(const WindowArgs& a, int s) {
-  const int lk = a.cu_q ? a.cu_k[s + 1] - a.cu_k[s] : a.cu_k[s];
-  // (a bound that is too low drops the keys past it)
-  return max(0, (int)min((int64_t)min(lk, a.w * a.bs), (int64_t)a.ranges * kWinTile));
+  return max(0, min(window_length(a, s), a.most_keys));
 }
 __device__ __forceinline__ WindowSeq window_seq(const WindowArgs& a, int s) {
   WindowSeq w;
@@ -189,7 +194,9 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowArgs& a, int s) {
     w.q_begin = s;
     w.lq = 1;
   }
-  w.lk = window_keys_of(a, s);
+  const int length = window_length(a, s);
+  w.lk = max(0, min(length, a.most_keys));
+  w.past = length - w.lq;
   w.rows = (int)min((int64_t)w.lq * a.group, (int64_t)a.rows);
   return w;
 }
@@ -294,7 +301,7 @@ struct WindowRows {
       const int qi = a.by_group(row);
       v[i] = *reinterpret_cast<const u32x4*>(
           q + (row + (int64_t)qi * (a.hq - a.group)) * kHeadDim);
-      lim[i] = w.lk - w.lq + qi + 1;
+      lim[i] = w.past + qi + 1;
     }
   }
   __device__ __forceinline__ void store(const WindowSeq& w, int row0, uint8_t* q_lds,
@@ -379,7 +386,7 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_lse_kernel(WindowArgs a
       ksc[kg] = *reinterpret_cast<const f32x4*>(&s_scale[wave][16 * kg + 4 * g]);
     if (t0 + kWinTile < end) window_load(a, s, kvh, k0 + kWinTile, w.lk, lane, next);
     if (valid > 0) {
-      const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;  // every row sees every key
+      const bool all = valid == 64 && k0 + 64 <= w.past + 1;  // every row sees every key
 #pragma unroll
       for (int rb = 0; rb < kBlocks; ++rb) {
         if (rb < blocks) {
@@ -549,7 +556,7 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
       sum[kg] = 0.0f;
     }
     if (t0 + kWinTile < end) window_load(a, s, kvh, k0 + kWinTile, w.lk, lane, next);
-    const bool all = valid == 64 && k0 + 64 <= w.lk - w.lq + 1;  // every row sees every key
+    const bool all = valid == 64 && k0 + 64 <= w.past + 1;  // every row sees every key
     for (int row0 = 0; row0 < w.rows; row0 += kRows) {
       if (w.rows > kRows && (row0 > 0 || t0 > first)) {
         q.load(a, w, kvh, row0);
@@ -606,7 +613,7 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
       const int page = k0 / a.bs;
       float* to = a.weights + ((int64_t)a.bt[(int64_t)s * a.w + page] * a.hk + kvh) * a.bs +
                   (tok - page * a.bs);
-      const bool add = a.add && !(a.set_new && tok >= w.lk - w.lq);
+      const bool add = a.add && !(a.set_new && tok >= w.past);
       *to = add ? *to + own : own;
     }
   }
@@ -648,11 +655,13 @@ static hipError_t launch_window(const WindowArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Tiles of the longest sequence of a window call.
+// Keys, and tiles of them, of the longest sequence of a window call.
+static int64_t window_keys(int64_t max_seqlen_k, int block_size, int w) {
+  const int64_t keys = (int64_t)w * block_size;
+  return max_seqlen_k > 0 ? std::min(keys, max_seqlen_k) : keys;
+}
 static int64_t window_tiles(int64_t max_seqlen_k, int block_size, int w) {
-  int64_t keys = (int64_t)w * block_size;
-  if (max_seqlen_k > 0) keys = std::min(keys, max_seqlen_k);
-  return (keys + kWinTile - 1) / kWinTile;
+  return (window_keys(max_seqlen_k, block_size, w) + kWinTile - 1) / kWinTile;
 }
 
 // Most bytes of scores that a tracking decode asks for; past it K is read again
@@ -708,6 +717,7 @@ static int window_checked(
   if (misaligned({query, k_cache})) return MSKV_EINVAL;
   WindowArgs a = {};
   a.ranges = (int)window_tiles(max_seqlen_k, block_size, max_blocks_per_seq);
+  a.most_keys = (int)window_keys(max_seqlen_k, block_size, max_blocks_per_seq);
   const size_t need = mskv_window_weights_workspace_bytes(total_q, max_seqlen_k, num_q_heads,
                                                           block_size, max_blocks_per_seq);
   if (need > 0 && (!workspace || workspace_bytes < need)) return MSKV_EWORKSPACE;
