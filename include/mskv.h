@@ -576,7 +576,7 @@ int mskv_fp8_shared_prefix_decode_attention(
  * mskv_fp8_decode_attention_weights: mskv_fp8_decode_attention, which also
  * adds the step's probabilities to the entries of positions below
  * cache_seqlens[b] - 1 and sets that of the newest token, at
- * cache_seqlens[b] - 1 (the entry of a reused page needs no clearing).
+ * cache_seqlens[b] - 1 (its entry needs no clearing).
  * weights starts on 16 bytes.  The workspace holds
  * mskv_decode_weights_workspace_bytes: the split partials and, up to 1 GiB,
  * every score of the step (about batch * num_q_heads * max_blocks_per_seq *
@@ -600,7 +600,8 @@ int mskv_fp8_decode_attention_weights(
  * sequence, described as in mskv_fp8_prefill_attention) give the sequences'
  * tokens: query i of a sequence with Lq queries and Lk tokens sees positions
  * p < Lk - Lq + i + 1.  The entries of positions [start, Lk) are set, or added
- * to where accumulate is not 0.  max_seqlen_q and max_seqlen_k (0: the tables'
+ * to where accumulate is not 0 (tokens that the cache has newly taken must have
+ * been cleared, see mskv_clear_attention_weights).  max_seqlen_q and max_seqlen_k (0: the tables'
  * width) bound every sequence's queries and tokens: rows past them, and tokens
  * past the table, are not counted (Lk above stays the whole length).
  * block_size % 128 == 0, head_dim == 128.
@@ -618,6 +619,18 @@ int mskv_fp8_window_attention_weights(
     int head_dim, int block_size, int64_t num_blocks, int max_blocks_per_seq,
     float softmax_scale, int act_dtype, void* workspace,
     size_t workspace_bytes, void* stream);
+
+/*
+ * Set the entries of the tokens at slot_mapping (as mskv_store_fp8_kvcache takes
+ * it; slots outside the cache are skipped) to 0, for every kv head: those of a
+ * prompt's or a turn's tokens as they are stored, whose places in reused pages,
+ * or behind an eviction's lengths, hold what was there before.  A window call
+ * that sets entries and the decode's newest token need no clearing.
+ */
+int mskv_clear_attention_weights(float* weights, const void* slot_mapping,
+                                 int slot_dtype, int64_t num_tokens,
+                                 int num_kv_heads, int block_size,
+                                 int64_t num_blocks, void* stream);
 
 /*
  * The tokens that stay of every (sequence, kv head): of L = cache_seqlens[b]

@@ -33,6 +33,6 @@ from microserve_amd.kv_blocks import compact_kv_blocks, copy_kv_blocks  # noqa: 
 from microserve_amd.shared_prefix import (  # noqa: F401
     fp8_shared_prefix_decode_attention, group_by_prefix)
 from microserve_amd.attention_weights import (  # noqa: F401
-    allocate_attention_weights, evict_kv_tokens, fp8_decode_attention_weights,
-    fp8_window_attention_weights, select_kv_tokens)
+    allocate_attention_weights, clear_attention_weights, evict_kv_tokens,
+    fp8_decode_attention_weights, fp8_window_attention_weights, select_kv_tokens)
 from microserve_amd.attention import Attention  # noqa: F401

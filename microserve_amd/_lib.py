@@ -150,6 +150,8 @@ _PROTOS = {
         _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int,
         _c_int, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_int, _c_f32,
         _c_int, _vp, _c_size, _vp]),
+    "mskv_clear_attention_weights": (_c_int, [
+        _vp, _vp, _c_int, _c_i64, _c_int, _c_int, _c_i64, _vp]),
     "mskv_select_kv_tokens": (_c_int, [
         _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp,
         _c_int, _c_int, _c_int, _c_i64, _c_int, _vp]),

@@ -14,7 +14,8 @@ With ``kv_cache_dtype`` ``"fp4_e2m1"`` the injected caches are the 4-bit ones
 
 Over an FP8 cache a decode step also keeps its tokens' attention weights where
 ``attention_weights`` was injected (``allocate_attention_weights``; the tokens
-before ``attention_weights_start`` are left out), and reads prefixes that
+before ``attention_weights_start`` are left out); a prefill sets the entries of
+the tokens that it stores to 0.  A decode step reads prefixes that
 sequences share once where the ``Context`` names groups
 (``fp8_shared_prefix_decode_attention``).  With both the weights go first: they
 are sums over the tokens of each sequence by itself.
@@ -25,7 +26,8 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from microserve_amd.attention_weights import fp8_decode_attention_weights
+from microserve_amd.attention_weights import (
+    clear_attention_weights, fp8_decode_attention_weights)
 from microserve_amd.context import AttentionMode, get_context
 from microserve_amd.fp4_attention import fp4_chunk_prefill_attention, fp4_decode_attention
 from microserve_amd.fp4_kv_cache import store_fp4_kvcache
@@ -70,6 +72,7 @@ class Attention(nn.Module):
         store = store_fp4_kvcache if self.kv_cache_dtype == FP4 else store_fp8_kvcache
         store(k, v, self.k_cache, self.v_cache, self.k_scale_cache, self.v_scale_cache,
               ctx.slot_mapping)
+        self._clear_weights(ctx)
         return self._attend(ctx, q, k, v)
 
     def forward_fused(self, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
@@ -89,7 +92,14 @@ class Attention(nn.Module):
             positions, q, k, v, q_norm_weight, k_norm_weight, eps, cos_cache, sin_cache,
             self.k_cache, self.v_cache, self.k_scale_cache, self.v_scale_cache,
             ctx.slot_mapping, return_k=ctx.mode is AttentionMode.PREFILL)
+        self._clear_weights(ctx)
         return self._attend(ctx, q, k_embed, v)
+
+    def _clear_weights(self, ctx):
+        """The stored tokens' entries (a decode step sets its own)."""
+        if (self.attention_weights is not None and self.kv_cache_dtype == FP8
+                and ctx.mode is not AttentionMode.DECODE):
+            clear_attention_weights(self.attention_weights, ctx.slot_mapping)
 
     def _attend(self, ctx, q, k, v):
         k_cache, v_cache = self.k_cache, self.v_cache

@@ -26,6 +26,31 @@ def allocate_attention_weights(num_blocks: int, block_size: int, num_kv_heads: i
     return torch.zeros(lead + shape, dtype=torch.float32, device=device)
 
 
+def clear_attention_weights(weights: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Set the entries of the tokens at ``slot_mapping`` (the store's: int32 or
+    int64; slots outside the cache, -1 among them, are skipped) to 0.
+
+    For the tokens that a prompt or a turn stores: a reused page, and the places
+    behind ``evict_kv_tokens``'s lengths, hold the entries of what was there
+    before.  ``Attention`` does this in its prefills.  Decode steps set their
+    newest token's entry themselves, and so does a window without ``accumulate``.
+    """
+    what = "clear_attention_weights"
+    assert weights.dim() == 3, f"{what}: weights must be [blocks, kv heads, block size]"
+    _weights(what, weights, *weights.shape)
+    assert slot_mapping.dtype in (torch.int32, torch.int64), (
+        f"{what}: slot_mapping must be int32 or int64")
+    slot_mapping = slot_mapping.contiguous()
+    _lib.on_device(what, weights, slot_mapping)
+    num_blocks, num_kv_heads, block_size = weights.shape
+    with _lib.current(weights):
+        status = _lib.load().mskv_clear_attention_weights(
+            weights.data_ptr(), slot_mapping.data_ptr(),
+            _lib.INT64 if slot_mapping.dtype == torch.int64 else _lib.INT32,
+            slot_mapping.numel(), num_kv_heads, block_size, num_blocks, _lib.stream_of(weights))
+    _lib.check(status, what)
+
+
 def _start(what, start, batch, device):
     """(the int32 tensor or None, the integer)"""
     if isinstance(start, torch.Tensor):
@@ -68,8 +93,8 @@ def fp8_decode_attention_weights(
     """``fp8_decode_attention`` that also keeps its tokens' attention weights.
 
     The step's probabilities are added to the entries of ``weights``; the entry
-    of the newest token, at position ``cache_seqlens - 1``, is set, so that the
-    pages of new tokens need no clearing.  Pages that two sequences of the batch
+    of the newest token, at position ``cache_seqlens - 1``, is set, so that it
+    needs no clearing (a prompt's do: ``clear_attention_weights``).  Pages that two sequences of the batch
     name must lie before ``start``.  The call may be captured in a HIP graph.
     """
     res = _lib.fast.track(query, k_cache, v_cache, k_scale_cache, v_scale_cache, cache_seqlens,
@@ -123,7 +148,9 @@ def fp8_window_attention_weights(
     ``fp8_varlen_prefill_attention``: after a prompt, the last few rows of its
     queries, already stored tokens of the cache.  Query ``i`` of a sequence sees
     positions ``< Lk - Lq + i + 1``.  The entries of positions ``start .. Lk``
-    are set (with ``accumulate``, added to); returns ``weights``.
+    are set (with ``accumulate``, added to: those of tokens that this turn has
+    stored must have been cleared before, ``clear_attention_weights``); returns
+    ``weights``.
     ``max_seqlen_q`` and ``max_seqlen_k`` (default: the tables' width) must be
     at least every sequence's numbers: what lies past them, or past the table,
     is not counted (``Lk`` stays the whole length).

@@ -770,12 +770,49 @@ extern "C" int mskv_fp8_window_attention_weights(
 
 namespace mskv {
 
+// The entries of stored tokens, 0: thread x takes a token of head y (neighbouring
+// tokens' entries of a head lie side by side).
+template <typename SlotT>
+__global__ __launch_bounds__(kWinThreads) void clear_weights_kernel(
+    float* __restrict__ weights, const SlotT* __restrict__ slots, int64_t num_tokens, int hk,
+    int bs, int64_t num_slots) {
+  const int64_t t = (int64_t)blockIdx.x * kWinThreads + threadIdx.x;
+  if (t >= num_tokens) return;
+  const int64_t slot = (int64_t)slots[t];
+  if (slot < 0 || slot >= num_slots) return;
+  const int64_t page = slot / bs;
+  weights[(page * hk + blockIdx.y) * bs + (slot - page * bs)] = 0.0f;
+}
+
 // Whether a tracking decode of this shape leaves its scores in memory.
 static bool track_scores(int batch, int hq, int w, int block_size) {
   return track_scores_bytes(batch, hq, w, block_size) <= kTrackMaxScores;
 }
 
 }  // namespace mskv
+
+extern "C" int mskv_clear_attention_weights(float* weights, const void* slot_mapping,
+                                            int slot_dtype, int64_t num_tokens, int num_kv_heads,
+                                            int block_size, int64_t num_blocks, void* stream) {
+  using namespace mskv;
+  if (num_tokens < 0 || num_kv_heads <= 0 || block_size <= 0 || num_blocks < 0) return MSKV_EINVAL;
+  if (slot_dtype != MSKV_INT32 && slot_dtype != MSKV_INT64) return MSKV_EINVAL;
+  if (num_kv_heads > 65535 || num_blocks > 0x7FFFFFFFLL || num_tokens > 0x7FFFFFFFLL)
+    return MSKV_EUNSUPPORTED;
+  if (num_tokens == 0) return MSKV_OK;
+  if (!weights || !slot_mapping) return MSKV_EINVAL;
+  const dim3 grid((unsigned)((num_tokens + kWinThreads - 1) / kWinThreads),
+                  (unsigned)num_kv_heads);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  auto run = [&](auto* slots) {
+    using SlotT = std::remove_const_t<std::remove_pointer_t<decltype(slots)>>;
+    hipLaunchKernelGGL(clear_weights_kernel<SlotT>, grid, dim3(kWinThreads), 0, s, weights, slots,
+                       num_tokens, num_kv_heads, block_size, num_blocks * block_size);
+    return (int)hipGetLastError();
+  };
+  return slot_dtype == MSKV_INT64 ? run((const int64_t*)slot_mapping)
+                                  : run((const int32_t*)slot_mapping);
+}
 
 extern "C" size_t mskv_decode_weights_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
                                                       int block_size, int max_blocks_per_seq) {
