@@ -543,8 +543,11 @@ int mskv_compact_kv_blocks(int num_pools, void* const* bases,
  * aside) and at max_prefix_len, a bound known to the host that the launch is
  * laid out by; the rest is read sequence by sequence, so that the result is
  * mskv_fp8_decode_attention's in any case.
- * The workspace holds mskv_shared_decode_workspace_bytes: fp32 partials, merged
- * by a second kernel.  It belongs to one call at a time.
+ * The workspace holds mskv_shared_decode_workspace_bytes: fp32 partials of 516
+ * bytes, merged by a second kernel; a row has 64 at most for its prefix and at
+ * most as many for its own tokens as run at once, fewer the larger the batch
+ * (32 heads over 8, prefixes of 8192 tokens: 101 MB at 64 sequences, 203 at 512,
+ * 271 at 1024).  It belongs to one call at a time.
  * Supported: head_dim == 128, block_size % 128 == 0, num_groups <= 1024;
  * query, k_cache, v_cache, out and workspace on 16 bytes (MSKV_EINVAL).
  */

@@ -527,7 +527,14 @@ static SharedShape shared_shape(int batch, int groups, int hq, int hk, int w, in
   s.max_prefix = groups > 0 ? (int)(std::min(cap, max_prefix_len) / kSharedTile * kSharedTile) : 0;
   s.gc = group < 16 ? group : 16;
   s.tpr = 16 / s.gc;
-  s.sa = std::max(1, std::min({s.max_prefix / kSharedTile, kSharedWorkgroups / units, 64}));
+  // Ranges of a prefix: four times as many as run at once where all of the batch
+  // shares it (512 sequences of 32 heads: 16 for 8192 tokens, partials of 203 MB
+  // where 64 took 609), so that a few sequences' long prefix beside many others
+  // is still spread.
+  const int64_t rows = (batch + 8 * s.tpr - 1) / (8 * s.tpr);
+  const int64_t at_once = std::max(1, kSharedWorkgroups / units);
+  s.sa = (int)std::max<int64_t>(1, std::min({(int64_t)s.max_prefix / kSharedTile, at_once,
+                                             (int64_t)64, 4 * ((at_once + rows - 1) / rows)}));
   // (many sequences: partials of a few ranges each)
   const int64_t slots = kSharedWorkgroups / tail_units;
   const int64_t most = std::max<int64_t>(1, std::min(slots, 8 * ((slots + batch - 1) / batch)));

@@ -128,6 +128,31 @@ def test_ranges_of_several_tiles(size, tiles, hq, hk, tails, spoiled, per, dtype
     assert torch.equal(call(), out)  # nothing depends on timing
 
 
+def test_one_long_prefix_in_a_large_batch():
+    """The ranges that a prefix may have shrink with the batch: two sequences over
+    40 tiles, beside 1022 of five tokens in no group."""
+    gen = torch.Generator().manual_seed(1)
+    batch, heads, block, scale, tiles = 1024, 8, 128, 0.05, 40
+    pages = tiles + batch + 1
+    cache = _pool(gen, pages, heads, block)
+    order = torch.randperm(pages, generator=gen).numpy()
+    tables = np.full((batch, tiles + 1), -1, np.int32)
+    tables[:2, :tiles] = order[:tiles]
+    tables[:2, tiles] = order[tiles:tiles + 2]
+    tables[2:, 0] = order[tiles + 2:tiles + batch]
+    lens = [tiles * block + 1] * 2 + [5] * (batch - 2)
+    q = torch.randn(batch, heads, D, generator=gen).half().to(H.DEV)
+    out = M.fp8_shared_prefix_decode_attention(q, *cache, H.gpu(lens), H.gpu(tables), scale,
+                                               H.gpu([0, 2]), H.gpu([tiles * block]))
+    for b in (0, 1, 2, 500, batch - 1):
+        k, ok = _rows(cache[0], cache[2], tables[b], lens[b])
+        v, _ = _rows(cache[1], cache[3], tables[b], lens[b])
+        p = _attend(q[b:b + 1], k, ok, scale, [lens[b]])
+        H.check_out(out[b], torch.bmm(p, v).reshape(heads, D).cpu().numpy(),
+                    torch.bmm(p, v.abs()).reshape(heads, D).cpu().numpy(), _reach(q[b], k, scale),
+                    torch.float16, lens[b], float(cache[3].max()), 1)
+
+
 # ------------------------------------------------------------------- windows --
 
 @pytest.mark.parametrize("accumulate", [False, True])
