@@ -613,6 +613,12 @@ size_t mskv_window_weights_workspace_bytes(int64_t total_q,
                                            int64_t max_seqlen_k,
                                            int num_q_heads, int block_size,
                                            int max_blocks_per_seq);
+/* What a call of these bounds and heads uses of it: at 8 kv heads and up to 128
+ * rows of each 64 partials a row at most, fewer with more rows, where the above
+ * knows of 512. */
+size_t mskv_window_weights_bounded_workspace_bytes(
+    int64_t total_q, int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads,
+    int num_kv_heads, int block_size, int max_blocks_per_seq);
 int mskv_fp8_window_attention_weights(
     const void* query, const void* k_cache, const float* k_scale_cache,
     const int32_t* block_tables, const int32_t* cu_seqlens_q,

@@ -146,6 +146,8 @@ _PROTOS = {
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_int, _c_f32, _c_int,
         _vp, _c_size, _vp]),
     "mskv_window_weights_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_int, _c_int, _c_int]),
+    "mskv_window_weights_bounded_workspace_bytes": (_c_size, [
+        _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int]),
     "mskv_fp8_window_attention_weights": (_c_int, [
         _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int,
         _c_int, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_int, _c_f32,

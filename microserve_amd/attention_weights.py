@@ -178,8 +178,8 @@ def fp8_window_attention_weights(
     starts, start = _start(what, start, num_seqs, query.device)
     bound = 0 if max_seqlen_k is None else max(int(max_seqlen_k), 1)
     lib, width = _lib.load(), block_tables.shape[1]
-    nbytes = lib.mskv_window_weights_workspace_bytes(total_q, bound, num_q_heads, block_size,
-                                                     width)
+    nbytes = lib.mskv_window_weights_bounded_workspace_bytes(
+        total_q, int(max_seqlen_q), bound, num_q_heads, num_kv_heads, block_size, width)
     with _lib.current(query):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
         status = lib.mskv_fp8_window_attention_weights(

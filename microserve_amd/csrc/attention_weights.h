@@ -161,6 +161,7 @@ struct WindowArgs {
   float scale_log2;
   int num_seqs, hq, hk, group, bs, w, start, ranges, rows;
   int most_keys;  // of a sequence: the table's width or the caller's bound
+  int parts;      // most ranges of a sequence in window_lse_kernel
   Divider by_group;
   bool add, set_new;
 };
@@ -457,7 +458,7 @@ __device__ __forceinline__ float window_row_lse(const WindowArgs& a, const Windo
   constexpr int kBatch = 16;  // loads in flight a lane
   const int64_t stride = a.total_q * a.hq;
   const int keys = *a.per * kWinTile;
-  const int n = min(a.ranges, (w.lk + keys - 1) / keys);
+  const int n = min(a.parts, (w.lk + keys - 1) / keys);
   float m = -INFINITY, l = 0.0f;
   const float* p = a.part + at + min(lane, max(n - 1, 0)) * stride;
   for (int base = lane; base < n; base += kBatch * kThreads) {
@@ -619,10 +620,19 @@ __global__ __launch_bounds__(kWinThreads, 2) void window_sum_kernel(WindowArgs a
   }
 }
 
-// [total_q * hq, ranges] partial log-sum-exps, [total_q * hq] final ones, then
+// [parts, total_q * hq] partial log-sum-exps, [total_q * hq] final ones, then
 // the tiles of a range
-static size_t window_bytes(int64_t total_q, int hq, int64_t ranges) {
-  return ((size_t)total_q * hq * (ranges + 1) + 1) * sizeof(float);
+static size_t window_bytes(int64_t total_q, int hq, int64_t parts) {
+  return ((size_t)total_q * hq * (parts + 1) + 1) * sizeof(float);
+}
+
+// Turns of rows of a sequence, and the most ranges that window_lse_kernel makes of
+// its keys: a range holds at least the batch's tiles times the units over the
+// workgroups that run at once (window_range).
+static int64_t window_turns(int64_t rows) { return (rows + kWinRows - 1) / kWinRows; }
+static int64_t window_parts(int64_t tiles, int64_t rows, int hk) {
+  const int64_t units = hk * std::max<int64_t>(1, window_turns(rows));
+  return std::min(tiles, (kWinSlots + units - 1) / units);
 }
 
 template <typename T>
@@ -634,7 +644,7 @@ static hipError_t launch_window(const WindowArgs& a, hipStream_t st) {
     return dim3((unsigned)(std::min(most, (int64_t)a.ranges * a.num_seqs) * units));
   };
   if (a.rows > 0) {  // (without queries there are only zeros to write)
-    const int units = a.hk * ((a.rows + kWinRows - 1) / kWinRows);
+    const int units = a.hk * (int)window_turns(a.rows);
     hipLaunchKernelGGL(window_lse_kernel<T>, grid(units), dim3(kWinThreads), 0, st, a, units);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -673,9 +683,25 @@ constexpr size_t kTrackMaxScores = (size_t)1 << 30;
 extern "C" size_t mskv_window_weights_workspace_bytes(int64_t total_q, int64_t max_seqlen_k,
                                                       int num_q_heads, int block_size,
                                                       int max_blocks_per_seq) {
+  using namespace mskv;
   if (total_q <= 0 || num_q_heads <= 0 || block_size <= 0 || max_blocks_per_seq <= 0) return 0;
-  return mskv::window_bytes(total_q, num_q_heads,
-                            mskv::window_tiles(max_seqlen_k, block_size, max_blocks_per_seq));
+  // (of any number of kv heads and queries)
+  return window_bytes(total_q, num_q_heads,
+                      window_parts(window_tiles(max_seqlen_k, block_size, max_blocks_per_seq), 1,
+                                   1));
+}
+
+extern "C" size_t mskv_window_weights_bounded_workspace_bytes(
+    int64_t total_q, int max_seqlen_q, int64_t max_seqlen_k, int num_q_heads, int num_kv_heads,
+    int block_size, int max_blocks_per_seq) {
+  using namespace mskv;
+  if (total_q <= 0 || max_seqlen_q < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      num_q_heads % num_kv_heads != 0 || block_size <= 0 || max_blocks_per_seq <= 0)
+    return 0;
+  const int64_t rows = std::min<int64_t>(max_seqlen_q, total_q) * (num_q_heads / num_kv_heads);
+  return window_bytes(total_q, num_q_heads,
+                      window_parts(window_tiles(max_seqlen_k, block_size, max_blocks_per_seq),
+                                   rows, num_kv_heads));
 }
 
 namespace mskv {
@@ -683,7 +709,7 @@ namespace mskv {
 // (the launches' workgroups, and the sum of the tiles, stay within an int)
 static bool window_fits(int num_seqs, int64_t total_q, int64_t rows, int num_kv_heads,
                         int block_size, int max_blocks_per_seq) {
-  const int64_t turns = (rows + kWinRows - 1) / kWinRows;
+  const int64_t turns = window_turns(rows);
   return num_seqs <= 65535 && total_q <= 0x7FFFFFFFLL && rows <= 0x7FFFFFFFLL &&
          (num_seqs + kWinSlots) * turns * num_kv_heads <= 0x7FFFFF &&
          num_seqs * ((int64_t)max_blocks_per_seq * block_size / kWinTile + 1) <= 0x7FFFFFFF;
@@ -718,8 +744,9 @@ static int window_checked(
   WindowArgs a = {};
   a.ranges = (int)window_tiles(max_seqlen_k, block_size, max_blocks_per_seq);
   a.most_keys = (int)window_keys(max_seqlen_k, block_size, max_blocks_per_seq);
-  const size_t need = mskv_window_weights_workspace_bytes(total_q, max_seqlen_k, num_q_heads,
-                                                          block_size, max_blocks_per_seq);
+  const size_t need = mskv_window_weights_bounded_workspace_bytes(
+      total_q, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, block_size,
+      max_blocks_per_seq);
   if (need > 0 && (!workspace || workspace_bytes < need)) return MSKV_EWORKSPACE;
   a.q = (const uint16_t*)query;
   a.kc = (const uint8_t*)k_cache;
@@ -731,7 +758,9 @@ static int window_checked(
   a.start = start;
   a.weights = weights;
   a.part = (float*)workspace;
-  a.lse = a.part + (size_t)total_q * num_q_heads * a.ranges;
+  a.rows = total_q > 0 ? (int)std::min<int64_t>(rows, total_q * group) : 0;
+  a.parts = (int)window_parts(a.ranges, a.rows, num_kv_heads);
+  a.lse = a.part + (size_t)total_q * num_q_heads * a.parts;
   a.per = (int*)(a.lse + (size_t)total_q * num_q_heads);
   a.total_q = total_q;
   a.num_blocks = num_blocks;
@@ -743,7 +772,6 @@ static int window_checked(
   a.by_group = divider_of(group);
   a.bs = block_size;
   a.w = max_blocks_per_seq;
-  a.rows = total_q > 0 ? (int)std::min<int64_t>(rows, total_q * group) : 0;
   a.add = accumulate;
   a.set_new = cu_seqlens_q == nullptr;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -827,8 +855,9 @@ extern "C" size_t mskv_decode_weights_workspace_bytes(int batch, int num_q_heads
            track_scores_bytes(batch, num_q_heads, max_blocks_per_seq, block_size);
   // the decode's own workspace, then the window kernels' one
   return std::max(mskv_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, kHeadDim, splits),
-                  mskv_window_weights_workspace_bytes(batch, 0, num_q_heads, block_size,
-                                                      max_blocks_per_seq));
+                  mskv_window_weights_bounded_workspace_bytes(batch, 1, 0, num_q_heads,
+                                                              num_kv_heads, block_size,
+                                                              max_blocks_per_seq));
 }
 
 extern "C" int mskv_fp8_decode_attention_weights(

@@ -151,7 +151,8 @@ PyObject* window(PyObject*, PyObject* const* a, Py_ssize_t n) {
         bt->size(0) != seqs || !weights_of(*weights, m) ||
         !start_of(in, a[10], seqs, start, starts))
       return nullptr;
-    const size_t bytes = api.window_bytes(nq, bound, (int)hq, (int)m.block, (int)w);
+    const size_t bytes =
+        api.window_bytes(nq, max_q, bound, (int)hq, (int)m.heads, (int)m.block, (int)w);
     int status;
     {
       const OnDevice on(in.device);

@@ -47,7 +47,7 @@ struct Api {
   decltype(&mskv_fp8_shared_prefix_decode_attention) shared = nullptr;
   decltype(&mskv_decode_weights_workspace_bytes) track_bytes = nullptr;
   decltype(&mskv_fp8_decode_attention_weights) track = nullptr;
-  decltype(&mskv_window_weights_workspace_bytes) window_bytes = nullptr;
+  decltype(&mskv_window_weights_bounded_workspace_bytes) window_bytes = nullptr;
   decltype(&mskv_fp8_window_attention_weights) window = nullptr;
   decltype(&mskv_select_kv_tokens) choose = nullptr;
   decltype(&mskv_evict_kv_tokens) evict = nullptr;
@@ -681,7 +681,7 @@ PyObject* bind(PyObject*, PyObject* table) {
             get("mskv_fp8_shared_prefix_decode_attention", f.shared) &&
             get("mskv_decode_weights_workspace_bytes", f.track_bytes) &&
             get("mskv_fp8_decode_attention_weights", f.track) &&
-            get("mskv_window_weights_workspace_bytes", f.window_bytes) &&
+            get("mskv_window_weights_bounded_workspace_bytes", f.window_bytes) &&
             get("mskv_fp8_window_attention_weights", f.window) &&
             get("mskv_select_kv_tokens", f.choose) && get("mskv_evict_kv_tokens", f.evict) &&
             get("mskv_status_string", f.text);

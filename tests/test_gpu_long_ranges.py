@@ -278,3 +278,40 @@ def test_heads_that_move_together(batch, heads, scale_heads, row_heads):
     got = [*H.to_cpu(cache), w.permute(0, 2, 1).cpu().numpy()]
     for g, x, name in zip(got, want, ("k", "v", "k_scale", "v_scale", "weights")):
         assert np.ascontiguousarray(g).tobytes() == x.tobytes(), name
+
+
+@pytest.mark.parametrize("new,lens,hq,hk", [
+    ([16, 3], [3000, 700], 32, 32), ([40], [9000], 64, 64), ([130, 1], [5000, 6000], 48, 48)])
+def test_windows_under_tables_wider_than_their_ranges(new, lens, hq, hk):
+    """The partials follow what runs at once, not a table of 64 k tokens; a
+    workspace of just that size is not overrun."""
+    gen = torch.Generator().manual_seed(3)
+    block, scale, width = 256, 0.03, 256
+    pages = sum(-(-n // 256) for n in lens) + 2
+    cache = _pool(gen, pages, hk, block)
+    tables = H.tables_of(gen, lens, block, pages, width)
+    q = torch.randn(sum(new), hq, D, generator=gen).half().to(H.DEV)
+    cu_q, cu_k = (H.gpu(np.cumsum([0, *x])) for x in (new, lens))
+    lib, t, w = _lib.load(), H.gpu(tables), torch.zeros(pages, hk, block, device=H.DEV)
+    need = lib.mskv_window_weights_bounded_workspace_bytes(sum(new), max(new), 0, hq, hk, block,
+                                                           width)
+    turns = -(-max(new) * hq // hk // 128)
+    assert need == sum(new) * hq * (-(-512 // (hk * turns)) + 1) * 4 + 4
+    ws = torch.zeros(need + 4096, dtype=torch.uint8, device=H.DEV)
+    ws[need:] = 77
+    status = lib.mskv_fp8_window_attention_weights(
+        q.data_ptr(), cache[0].data_ptr(), cache[2].data_ptr(), t.data_ptr(), cu_q.data_ptr(),
+        cu_k.data_ptr(), w.data_ptr(), None, 0, 0, len(new), sum(new), max(new), 0, hq, hk, D,
+        block, pages, width, scale, 0, ws.data_ptr(), need, _lib.stream_of(q))
+    torch.cuda.synchronize()
+    assert status == 0 and bool((ws[need:] == 77).all())
+    want, reach = torch.zeros_like(w).double(), 0.0
+    at = np.cumsum([0, *new])
+    for b, (n, lq) in enumerate(zip(lens, new)):
+        k, ok = _rows(cache[0], cache[2], tables[b], n)
+        rows = q[at[b]:at[b + 1]]
+        p = _attend(rows, k, ok, scale, n - lq + 1 + np.arange(lq))
+        _put(want, p.sum(1), tables[b], lambda *a: 0.0)
+        reach = max(reach, _reach(rows, k, scale))
+    H.check_weights(w.cpu().numpy(), want.cpu().numpy(), 0.0, reach, max(lens),
+                    hq // hk * max(new))
