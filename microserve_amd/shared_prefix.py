@@ -11,6 +11,78 @@ from microserve_amd import _lib
 MAX_GROUPS = 1024
 
 
+def _most_saving_groups(tables):
+    """The partition of the sequences whose groups save the most reads of pages: a
+    group of m saves m - 1 reads of each of its common first pages.
+
+    In the tree of common beginnings a sequence belongs to the deepest group that
+    is open above it.  ``best[node][j]``: the most that the sequences below a node
+    save, if the j-th node above it is the nearest group (each member counts its
+    depth, an open group pays its own once); node 0 above all has depth 0.
+    """
+    order = sorted(range(len(tables)), key=lambda i: (tables[i], i))
+    # the nodes, from the common beginnings of neighbours: (depth, children),
+    # children numbers of nodes, or ~i for sequence i
+    nodes, stack = [], [(0, [])]
+
+    def close(depth):
+        while stack[-1][0] > depth:
+            nodes.append(stack.pop())
+            if stack[-1][0] < depth:
+                stack.append((depth, []))
+            stack[-1][1].append(len(nodes) - 1)
+
+    for i, at in zip(order, order[1:] + [None]):
+        if at is None:
+            common = 0
+        else:
+            a, b = tables[i], tables[at]
+            most = min(len(a), len(b))
+            common = most if a[:most] == b[:most] else next(
+                j for j in range(most) if a[j] != b[j])
+        if stack[-1][0] < common:
+            stack.append((common, []))
+        stack[-1][1].append(~i)
+        close(common)
+    nodes.append(stack.pop())  # the root, last; a node comes behind its children
+
+    # each node's depths of the nodes above it, from the root on
+    above = [None] * len(nodes)
+    above[-1] = []
+    for x in range(len(nodes) - 1, -1, -1):
+        for c in nodes[x][1]:
+            if c >= 0:
+                above[c] = above[x] + [x]
+    best, sums = [None] * len(nodes), [None] * len(nodes)
+    for x, (depth, children) in enumerate(nodes):
+        leaves = sum(c < 0 for c in children)
+        sums[x] = [leaves * nodes[y][0] + sum(best[c][j] for c in children if c >= 0)
+                   for j, y in enumerate(above[x] + [x])]
+        opened = sums[x][-1] - depth
+        best[x] = [max(v, opened) for v in sums[x][:-1]]
+    members, nearest = {}, {len(nodes) - 1: 0}  # (the root is a group of depth 0)
+    for x in range(len(nodes) - 1, -1, -1):
+        j = nearest[x]
+        if x < len(nodes) - 1 and sums[x][-1] - nodes[x][0] > sums[x][j]:
+            j = len(above[x])
+        group = (above[x] + [x])[j]
+        for c in nodes[x][1]:
+            if c < 0:
+                members.setdefault(group, []).append(~c)
+            else:
+                nearest[c] = j
+    alone = members.pop(len(nodes) - 1, [])
+    return [sorted(m) for m in members.values()] + [[i] for i in alone]
+
+
+def _common(tables, group):
+    """The pages that all of a group name first (one alone shares none)."""
+    if len(group) == 1:
+        return 0
+    a, b = (f((tables[i] for i in group)) for f in (min, max))
+    return next((j for j, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b)))
+
+
 def group_by_prefix(block_tables, block_size: int):
     """Groups of sequences that name the same first pages.
 
@@ -18,25 +90,18 @@ def group_by_prefix(block_tables, block_size: int):
     Returns ``(order, cu_groups, prefix_lens)``, lists of host integers: the
     order in which the batch must be built so that a group's sequences follow
     one another, the groups' boundaries in it, and the tokens of each group's
-    shared pages.  Sequences that share their first page are one group, and its
-    prefix is what all of them share; a sequence alone has a prefix of 0.
+    shared pages.  The groups are those that save the most reads of pages: a few
+    sequences that share less than the others do not shorten their prefix.  A
+    sequence alone has a prefix of 0.
     """
     tables = [list(t) for t in block_tables]
-    order = sorted(range(len(tables)), key=lambda i: (tables[i][:1], i))
-    cu, prefixes = [0], []
-    for at, i in enumerate(order):
-        first = tables[order[cu[-1]]]
-        if at > cu[-1] and tables[i][:1] == first[:1] and first:
-            same = min(prefixes[-1], len(tables[i]))
-            prefixes[-1] = next((j for j in range(same) if tables[i][j] != first[j]), same)
-            continue
-        if at:
-            cu.append(at)
-        prefixes.append(len(tables[i]))
-    if order:
+    groups = [(m, _common(tables, m)) for m in _most_saving_groups(tables)] if tables else []
+    groups.sort(key=lambda g: (tables[g[0][0]][:1], g[0][0]))
+    order, cu = [], [0]
+    for members, _ in groups:
+        order += members
         cu.append(len(order))
-    alone = [b - a == 1 for a, b in zip(cu, cu[1:])]
-    return order, cu, [0 if one else n * block_size for one, n in zip(alone, prefixes)]
+    return order, cu, [pages * block_size for _, pages in groups]
 
 
 def fp8_shared_prefix_decode_attention(
