@@ -92,11 +92,17 @@ def group_by_prefix(block_tables, block_size: int):
     one another, the groups' boundaries in it, and the tokens of each group's
     shared pages.  The groups are those that save the most reads of pages: a few
     sequences that share less than the others do not shorten their prefix.  A
-    sequence alone has a prefix of 0.
+    sequence alone has a prefix of 0; where there are more than ``MAX_GROUPS``
+    groups, those that save the least are one group, the last, with a prefix of 0.
     """
     tables = [list(t) for t in block_tables]
     groups = [(m, _common(tables, m)) for m in _most_saving_groups(tables)] if tables else []
     groups.sort(key=lambda g: (tables[g[0][0]][:1], g[0][0]))
+    if len(groups) > MAX_GROUPS:
+        first = sorted(groups, key=lambda g: -(len(g[0]) - 1) * g[1])[:MAX_GROUPS - 1]
+        kept = {g[0][0] for g in first}
+        rest = sorted(i for m, _ in groups if m[0] not in kept for i in m)
+        groups = [g for g in groups if g[0][0] in kept] + [(rest, 0)]
     order, cu = [], [0]
     for members, _ in groups:
         order += members

@@ -6,6 +6,7 @@ import time
 import pytest
 
 import microserve_amd as M
+from microserve_amd.shared_prefix import MAX_GROUPS
 
 
 def _saved(tables, groups):
@@ -65,6 +66,19 @@ def test_no_partition_saves_more(seed):
     groups, _ = _groups(tables)
     best = max(_saved(tables, p) for p in _partitions(list(range(len(tables)))))
     assert _saved(tables, groups) == best
+
+
+def test_more_groups_than_a_call_takes():
+    lone = [[i] for i in range(1100)]
+    groups, pages = _groups(lone)
+    assert len(groups) <= MAX_GROUPS and not any(pages)
+    # the pairs that share most stay, whatever lies beside them
+    pairs = [[5000 + i // 2, *range(i // 2 % 7)] for i in range(2400)]
+    groups, pages = _groups(pairs + lone)
+    assert len(groups) == MAX_GROUPS and pages[-1] == 0
+    assert all(len(g) == 2 and p > 0 for g, p in zip(groups[:-1], pages))
+    dropped = {1 + i // 2 % 7 for i in groups[-1] if i < 2400}
+    assert max(dropped) <= min(pages[:-1])
 
 
 def test_nested_prefixes_and_time():
