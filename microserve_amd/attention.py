@@ -16,8 +16,9 @@ Over an FP8 cache a decode step also keeps its tokens' attention weights where
 ``attention_weights`` was injected (``allocate_attention_weights``; the tokens
 before ``attention_weights_start`` are left out); a prefill sets the entries of
 the tokens that it stores to 0.  A decode step reads prefixes that
-sequences share once where the ``Context`` names groups
-(``fp8_shared_prefix_decode_attention``).  With both the weights go first: they
+sequences share once where the ``Context`` names groups, with a ``max_prefix_len``
+other than 0 (``fp8_shared_prefix_decode_attention``; over a 4-bit cache groups
+are refused).  With both the weights go first: they
 are sums over the tokens of each sequence by itself.
 """
 
@@ -105,7 +106,9 @@ class Attention(nn.Module):
         k_cache, v_cache = self.k_cache, self.v_cache
         four = self.kv_cache_dtype == FP4
         if ctx.mode is AttentionMode.DECODE:
-            if self.attention_weights is not None or ctx.cu_groups is not None:
+            # (a bound of 0: no prefix is shared, the plain decode is faster)
+            shares = ctx.cu_groups is not None and ctx.max_prefix_len != 0
+            if self.attention_weights is not None or shares:
                 return self._attend_more(ctx, q)
             return (fp4_decode_attention if four else fp8_decode_attention)(
                 q, k_cache, v_cache, self.k_scale_cache, self.v_scale_cache,

@@ -5,7 +5,8 @@ The runner builds one ``Context`` per forward pass and installs it globally;
 defaults are the reference's: ``cache_seqlens`` is the per-sequence context
 length and ``block_tables`` is int32, -1 padded.  The last three, of a decode
 step whose sequences share prefixes, are this library's own
-(``group_by_prefix``'s results and a bound of the prefixes' lengths).
+(``group_by_prefix``'s results and a bound of the prefixes' lengths; a bound of 0
+says that nothing is shared).
 """
 
 from __future__ import annotations
