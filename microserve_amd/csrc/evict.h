@@ -481,6 +481,8 @@ extern "C" int mskv_select_kv_tokens(const float* weights, const int32_t* cache_
   if (batch == 0) return MSKV_OK;
   if (num_blocks == 0) return MSKV_EINVAL;  // (there are no weights to read)
   if (block_size % 4 != 0 || num_blocks > 0x7FFFFFFFLL) return MSKV_EUNSUPPORTED;
+  // (a grid's threads fit 32 bits)
+  if ((int64_t)batch * num_kv_heads > 0x3FFFFF) return MSKV_EUNSUPPORTED;
   if (!weights || !cache_seqlens || !block_tables || !kept || !new_seqlens ||
       misaligned({weights}))
     return MSKV_EINVAL;
