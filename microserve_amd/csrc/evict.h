@@ -98,7 +98,8 @@ __global__ __launch_bounds__(kThreads) void select_kv_tokens_kernel(SelectArgs a
   // what stays whatever it weighs
   const int fixed_front = n == L ? n : first;
   for (int i = tid; i < fixed_front; i += kThreads) kept[i] = i;
-  for (int i = n + tid; i < a.budget; i += kThreads) kept[i] = -1;
+  // (unsigned: a budget may lie within kThreads of 2^31)
+  for (uint32_t i = n + tid; i < (uint32_t)a.budget; i += kThreads) kept[i] = -1;
   if (n == L) return;
   for (int i = tid; i < last; i += kThreads) kept[n - last + i] = L - last + i;
   const int quota = n - first - last;
