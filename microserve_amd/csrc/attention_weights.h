@@ -221,7 +221,9 @@ __device__ __forceinline__ WindowRange window_range(const WindowArgs& a, int ite
   for (int s = 64 + lane; s < a.num_seqs; s += 64) total += tiles_of(s);
   const int tiles = __builtin_amdgcn_readfirstlane(wave_sum_i32(total));
   WindowRange r = {-1, 0, 0};
-  r.per = max(1, (int)(((int64_t)tiles * units + kWinSlots - 1) / kWinSlots));
+  // (no more than the longest sequence may have: a range's tokens stay an int)
+  r.per = max(1, (int)min(((int64_t)tiles * units + kWinSlots - 1) / kWinSlots,
+                          (int64_t)a.ranges));
   for (int base = 0; base < a.num_seqs; base += 64) {
     const int n = ((base == 0 ? own : tiles_of(base + lane)) + r.per - 1) / r.per;
     const int upto = wave_scan_i32(n);

@@ -51,3 +51,32 @@ def test_limits_follow_the_whole_length(new, lens, pages, bound, dtype, accumula
     assert np.array_equal(got[~touched], old.numpy()[~touched]), "an entry beside the tokens"
     H.check_weights(got, want, np.where(touched, before, want), reach, pages * block,
                     hq // hk * max(new))
+
+
+def test_a_range_of_more_tokens_than_an_int():
+    """One query, a bound of 261632 and 67 million tokens in pages that repeat: by the
+    bound a workgroup's range would hold 2^31 tokens and more."""
+    heads, block, copies, scale = 8, 256, 262700, 0.05
+    bound = 2044 * 128
+    gen = torch.Generator().manual_seed(0)
+    host, dev = H.pool(gen, 4, heads, block)
+    table = torch.zeros(1, copies, dtype=torch.int32)
+    table[0] = torch.arange(copies) % 3  # pages 0 to 2 in turn, then page 3
+    table[0, -1] = 3
+    lk = copies * block
+    assert -(-copies * heads * 2044 // 512) * 256 > 2 ** 31
+    q = torch.zeros(bound, heads, D, device=H.DEV).half()  # (the others are padding)
+    q[0] = torch.randn(heads, D, generator=gen).half()
+    weights = torch.full((4, heads, block), 7.0, device=H.DEV)
+    M.fp8_window_attention_weights(q, dev[0], dev[2], table.to(H.DEV), H.gpu([0, 1]),
+                                   H.gpu([0, lk]), bound, scale, weights, start=lk - block)
+    got = weights.cpu().double().numpy()
+    assert (got[:3] == 7).all()
+    k, _ = W.rows_of(host[0], host[2], range(4), 4 * block, block)
+    s = np.exp(np.einsum("hd,khd->hk", q[0].cpu().double().numpy(), k) * scale)
+    times = np.repeat(np.bincount(table[0].numpy(), minlength=4), block)
+    want = (s / (s * times).sum(-1, keepdims=True))[:, 3 * block:]
+    # a lane adds the sum of 16 probabilities a tile to its running one: a rounding of
+    # 2^-24 a tile, besides weight_bound's (the sum over keys there is this one)
+    tol = H.weight_bound(H.reach_of(q[:1].cpu().double().numpy(), k, scale), copies + 32)
+    assert (np.abs(got[3] - want) <= tol * want).all()
