@@ -152,9 +152,11 @@ __device__ __forceinline__ int shared_plan(const SharedArgs& a, int index, int u
   }
   const float chain = ((float)work * units * kSharedTileTime +
                        (float)steps * tail_units * kSharedStepTime) / kSharedWorkgroups;
-  // tiles of a prefix's range, steps of a tail's
-  const int per_a = max(max((int)ceilf(chain / kSharedTileTime), ceil_div(longest, a.sa)), 1);
-  const int per_b = max(max((int)ceilf(chain / kSharedStepTime), ceil_div(most, a.sb)),
+  // tiles of a prefix's range, steps of a tail's (no more than the longest has, so
+  // that a range's tokens stay an int)
+  const int per_a =
+      max(min(max((int)ceilf(chain / kSharedTileTime), ceil_div(longest, a.sa)), longest), 1);
+  const int per_b = max(min(max((int)ceilf(chain / kSharedStepTime), ceil_div(most, a.sb)), most),
                         kMinSplitSteps);
 
   // each thread's groups and sequences, one after the other, and the items
