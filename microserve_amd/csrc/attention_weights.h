@@ -11,10 +11,13 @@
 //  * The last queries of prompts (window_lse_kernel, window_sum_kernel): many
 //    rows a kv head, whose scores would be more bytes than K.  The scores are
 //    computed twice, first for each row's log-sum-exp, then for the sums.  32
-//    queries over 32768 tokens at 32 heads over 8 (8.6 GFLOP a pass): 20 us each.
-//    A workgroup's two tiles take 4 us each, issue-bound (exponentials, running
-//    maxima; the products are a third); 6 to 7 go by before, in the chain of lengths,
-//    table, rows and first tile (17 MB at once), and 3 between the launches.
+//    queries over 32768 tokens at 32 heads over 8 (8.6 GFLOP a pass): 37 us in all;
+//    under the profiler, which times a kernel from its dispatch, 20 each.  A
+//    workgroup's two tiles take 4 us each, issue-bound (a SIMD issues vector
+//    instructions 20 k cycles of about 40 k and multiplies 8 k; waves wait 30% of
+//    theirs for memory, 30 to 35% for the issue slot); 6 to 7 us go by before, in the
+//    chain of lengths, table, rows and first tile (17 MB at once), and 3 between the
+//    launches.  8 x 20 to 8192 tokens, 64 queries: 33 us.
 #pragma once
 
 namespace mskv {

@@ -24,9 +24,9 @@
 // Bound by what a SIMD issues: a prefix tile's conversions, exponentials and
 // products take about 5750 cycles of its wave, a tail's step 2500; the plan takes
 // 4 us of every workgroup.  64 sequences over a prefix of 8192 tokens with 512
-// each of their own, 32 heads over 8: 32 us and 5 of the merge (the decode reads
-// 64 x 8704 tokens for them); 128 in eight groups over 512 to 6144 tokens, 16 to
-// 2048 of their own: 52 and 5.
+// each of their own, 32 heads over 8: 32 us and 5 of the merge, 35 in all (the
+// decode, which reads 64 x 8704 tokens for them, 120); 128 in eight groups over 512
+// to 6144 tokens, 16 to 2048 of their own: 54 in all.
 #pragma once
 
 namespace mskv {
